@@ -49,7 +49,7 @@
 extern "C" {
 #endif
 
-#define TTT_AMD_ABI_VERSION 11
+#define TTT_AMD_ABI_VERSION 12
 
 enum ttt_dtype { TTT_DTYPE_F32 = 0, TTT_DTYPE_BF16 = 1, TTT_DTYPE_F16 = 2 };
 
@@ -392,6 +392,92 @@ int ttt_post_norm_fwd(const void* XQW, const float* gamma, const float* beta, in
 int ttt_post_norm_bwd(const void* XQW, const float* gamma, const float* stats, const void* dout,
                       int B, int L, int H, int K, int F, int dtype, void* dXQW, float* partial,
                       size_t partial_bytes, void* stream);
+
+/* ---- the selective state-space layer: short causal convolution, scan, layer norm ----
+ * Activations in `dtype`, parameters and scan states fp32.  Activations that are
+ * read come as rows `ld` elements apart (row b*L + t for token t of sequence b),
+ * so that they may be columns of a wider matrix; what is written is contiguous.
+ * No counterpart in the reference, whose layer types are TTT-Linear and TTT-MLP;
+ * these are a third one's. */
+
+enum ttt_activation { TTT_ACT_NONE = 0, TTT_ACT_SILU = 1 };
+
+/* y[t][c] = act(bias[c] + sum_k weight[c][k] s[t+k][c]) with s the W-1 inputs
+ * before the first token followed by x; W in {2, 3, 4}.
+ *   x       [B*L][ldx], any alignment      state [B][W-1][C] dtype, or NULL for zeros
+ *   weight  [C][W] fp32                    bias  [C] fp32, or NULL
+ *   y       [B][L][C]                      state_out [B][W-1][C]: the last W-1 inputs, or NULL */
+int ttt_causal_conv_fwd(const void* x, long long ldx, const void* state, const float* weight, const float* bias,
+                        int B, int L, int C, int W, int activation, int dtype, void* y, void* state_out,
+                        void* stream);
+
+/* Its gradients: dx [B][L][C], dstate [B][W-1][C] (or NULL), dweight [C][W], dbias
+ * [C] (or NULL) from dy [B][L][C] and dstate_out [B][W-1][C] (each may be NULL: zeros).
+ * `partial` holds the workgroups' sums for the two parameters, at least
+ * ttt_causal_conv_partial_bytes. */
+size_t ttt_causal_conv_partial_bytes(int B, int L, int C, int W);
+int ttt_causal_conv_bwd(const void* x, long long ldx, const void* state, const float* weight, const float* bias,
+                        const void* dy, const void* dstate_out, int B, int L, int C, int W, int activation,
+                        int dtype, void* dx, void* dstate, float* dweight, float* dbias, float* partial,
+                        size_t partial_bytes, void* stream);
+
+/* One token of every sequence: x [B][ldx] -> y [B][C], and state [B][W-1][C]
+ * moved up by one in place. */
+int ttt_causal_conv_step(const void* x, long long ldx, void* state, const float* weight, const float* bias,
+                         int B, int C, int W, int activation, int dtype, void* y, void* stream);
+
+/* h_t = exp(d_t A) h_{t-1} + d_t x_t (x) B_t,  y_t = h_t C_t + D x_t  per sequence
+ * and head, h [P][N], with d = softplus(dt + dt_bias) (or dt + dt_bias).
+ *   x       [B*L][ldx]: H heads of P (32 or 64) features
+ *   dt      [B*L][lddt]: H steps, in `dt_dtype` (dtype or TTT_DTYPE_F32)
+ *   Bm, Cm  [B*L][ldb], [B*L][ldc]: G groups of N values (a multiple of 16 up to
+ *           128); head h uses group h / (H/G)
+ *   A       [H], the decay's rate, < 0     D, dt_bias [H], or NULL for zeros
+ *   h0      [B][H][P][N], or NULL for zeros
+ *   y       [B][L][H][P]                   h_last [B][H][P][N], or NULL
+ *   states  NULL, or ttt_scan_states_bytes: what ttt_scan_bwd needs of the forward
+ *   workspace  ttt_scan_workspace_bytes (NULL where that is 0)
+ * x, Bm and Cm and their rows start on 16 bytes. */
+size_t ttt_scan_states_bytes(int B, int L, int H, int P, int N, int dtype);
+size_t ttt_scan_workspace_bytes(int B, int L, int H, int P, int N, int dtype);
+int ttt_scan_fwd(const void* x, long long ldx, const void* dt, long long lddt, const float* A, const void* Bm,
+                 long long ldb, const void* Cm, long long ldc, const float* D, const float* dt_bias, const float* h0,
+                 int B, int L, int H, int P, int G, int N, int dtype, int dt_dtype, int softplus, void* y,
+                 float* h_last, void* states, size_t states_bytes, void* workspace, size_t workspace_bytes,
+                 void* stream);
+
+/* Its gradients from dy [B*L][ldy] and dh_last (NULL: zeros), given the `states`
+ * that ttt_scan_fwd wrote for the same inputs: dx [B][L][H][P], ddt [B][L][H] in
+ * dt_dtype, dB, dC [B][L][G][N], dA [H], dD, ddt_bias [H] (or NULL), dh0
+ * [B][H][P][N] (or NULL). */
+size_t ttt_scan_bwd_workspace_bytes(int B, int L, int H, int P, int G, int N, int dtype);
+int ttt_scan_bwd(const void* x, long long ldx, const void* dt, long long lddt, const float* A, const void* Bm,
+                 long long ldb, const void* Cm, long long ldc, const float* D, const float* dt_bias, const void* dy,
+                 long long ldy, const float* dh_last, const void* states, size_t states_bytes, int B, int L, int H,
+                 int P, int G, int N, int dtype, int dt_dtype, int softplus, void* dx, void* ddt, float* dA,
+                 void* dB, void* dC, float* dD, float* ddt_bias, float* dh0, void* workspace,
+                 size_t workspace_bytes, void* stream);
+
+/* One token of every sequence: rows of x, dt, Bm, Cm as above with one a sequence,
+ * h [B][H][P][N] updated in place, y [B][H][P]. */
+int ttt_scan_step(const void* x, long long ldx, const void* dt, long long lddt, const float* A, const void* Bm,
+                  long long ldb, const void* Cm, long long ldc, const float* D, const float* dt_bias, float* h,
+                  int B, int H, int P, int G, int N, int dtype, int dt_dtype, int softplus, void* y, void* stream);
+
+/* y = (v - mean v) / sqrt(var v + eps) * weight + bias over rows of D values (up to
+ * 16384), v = x, or x * gate * sigmoid(gate) where a gate is given.
+ *   x [R][ldx], gate [R][ldg] or NULL, any alignment; weight, bias [D] fp32 (both or neither)
+ *   y [R][D];  stats [R][2] fp32 for the backward, or NULL */
+int ttt_layer_norm_fwd(const void* x, long long ldx, const void* gate, long long ldg, const float* weight,
+                       const float* bias, long long R, int D, float eps, int dtype, void* y, float* stats,
+                       void* stream);
+
+/* Its gradients from dy [R][D]: dx, dgate (where there is a gate) [R][D], dweight
+ * and dbias [D] (or both NULL; else `partial` of ttt_layer_norm_partial_bytes). */
+size_t ttt_layer_norm_partial_bytes(long long R, int D);
+int ttt_layer_norm_bwd(const void* x, long long ldx, const void* gate, long long ldg, const float* weight,
+                       const float* stats, const void* dy, long long R, int D, int dtype, void* dx, void* dgate,
+                       float* dweight, float* dbias, float* partial, size_t partial_bytes, void* stream);
 
 /* Bytes of the static device scratch of ttt_mlp_bwd_noalloc (per GPU). */
 #define TTT_MLP_BWD_NOALLOC_SCRATCH_BYTES (64u << 20)

@@ -1,0 +1,327 @@
+// Shared device code of the selective scan's kernels (ttt_scan_walk.hip,
+// ttt_scan_bwd.hip): the mathematics of a chunk, operands in planes, LDS layouts.
+//
+// Per sequence and head, with decay a_t = d_t A (A < 0) and state h [P][N]:
+//   h_t = e^{a_t} h_{t-1} + d_t x_t (x) B_t,      y_t = h_t C_t + D x_t
+// Over a chunk of Q tokens, with the decays' running sum c_t = a_1 + .. + a_t and
+// the state H entering it, this is three matrix products:
+//   y_i  = sum_{j<=i} e^{c_i - c_j} d_j (C_i . B_j) x_j + e^{c_i} H C_i + D x_i
+//   H'   = e^{c_Q} H + sum_j e^{c_Q - c_j} d_j x_j (x) B_j
+// Every exponent is <= 0.  c is summed in 64 bits and kept as two floats: tokens
+// that follow a strong decay have differences c_i - c_j far smaller than the sums,
+// and the factors they give would otherwise lose what the sums have rounded away.
+//
+// Matrix operands are bf16 planes whose sum is the value: an input is one plane in
+// bf16, two in fp16 and three in fp32, exact in each (8 bits a plane), so a single
+// matrix instruction (v_mfma_f32_16x16x32_bf16) and one range serve all types.
+// Values formed on the way are fp32 and split into planes where they are
+// multiplied.  What leads to fp32 results (states, the gradients of states and
+// parameters) takes three planes and all products p q with p + q < 3, 2^-24 of the
+// value: such results of 16-bit calls are as exact as those of fp32 ones.  What
+// leads to 16-bit results alone takes two, 2^-17, which leaves the rounding at the
+// store as the error.
+#pragma once
+
+#include "ttt_ssm.h"
+
+namespace ttt {
+
+struct ScanParams {
+  const void *x, *dt, *Bm, *Cm;      // [B*L][ldx], [B*L][lddt], [B*L][ldb], [B*L][ldc]
+  const float *A, *D, *dt_bias;      // [H] (D, dt_bias may be null)
+  const float* h0;                   // [B][H][P][N] (may be null: zeros)
+  void* y;                           // [B][L][H][P]
+  float* h_last;                     // [B][H][P][N] (may be null)
+  float* states;                     // [B*H][NC][NP][P]: the states entering the chunks, or walking back the
+                                     // gradients of those leaving them (may be null)
+  float *seg, *seg_decay;            // [B*H][S][P][NP] and [B*H][S]: per segment of the sequence
+  long long ldx, lddt, ldb, ldc;
+  int B, L, H, G, N;
+  int S, per;                        // segments, and chunks in one
+  bool softplus, dt_f32;
+  // backward
+  const void* dy;                    // [B*L][ldy]
+  long long ldy;
+  const float* gstates;              // the gradients of the states leaving the chunks
+  void *dx, *ddt, *dB, *dC;          // [B][L][H][P], [B][L][H], [B][L][G][N]
+  float *dBp, *dCp;                  // [splits][B*L][G][N] where a group's heads are split, else null
+  float* partial;                    // [3][H][B*NC]: dA, dD, ddt_bias of each chunk
+  float *dA, *dD, *ddt_bias;         // [H]
+  int splits;
+};
+
+hipError_t launch_scan_fwd(const ScanParams& p, int P, int dtype, hipStream_t stream);
+// walks back from the last state's gradient (p.h0): the gradients of x (into p.dx), of the states leaving the
+// chunks (p.states) and of the initial one (p.h_last)
+hipError_t launch_scan_walk_back(const ScanParams& p, int P, int dtype, hipStream_t stream);
+hipError_t launch_scan_bwd(const ScanParams& p, int P, int dtype, hipStream_t stream);
+struct ScanStepParams {
+  const void *x, *dt, *Bm, *Cm;   // [B][ldx], [B][lddt], [B][ldb], [B][ldc]
+  const float *A, *D, *dt_bias;   // [H]
+  float* h;                       // [B][H][P][N], read and written
+  void* y;                        // [B][H][P]
+  long long ldx, lddt, ldb, ldc;
+  int B, H, P, G, N;
+  bool softplus, dt_f32;
+};
+hipError_t launch_scan_step(const ScanStepParams& p, int dtype, hipStream_t stream);
+constexpr int scan_padded(int N) { return N <= 32 ? 32 : N <= 64 ? 64 : 128; }
+
+template <typename T> struct ScanType;
+// planes of an input, and of a formed value that leads to results of this type alone
+template <> struct ScanType<__bf16> { static constexpr int IN = 1, MID = 2; };
+template <> struct ScanType<_Float16> { static constexpr int IN = 2, MID = 2; };
+template <> struct ScanType<float> { static constexpr int IN = 3, MID = 3; };
+constexpr int kFull = 3;  // planes of a formed value that leads to fp32 results
+// tokens of a chunk: 64, or 32 where the backward's planes would not fit in LDS
+constexpr int scan_chunk(int dtype, int NP) {
+  return dtype == TTT_DTYPE_F32 || (dtype == TTT_DTYPE_F16 && NP == 128) ? 32 : 64;
+}
+template <typename T, int NP> constexpr int chunk_of() {
+  return scan_chunk(ScanType<T>::IN == 3 ? TTT_DTYPE_F32 : ScanType<T>::IN == 2 ? TTT_DTYPE_F16 : TTT_DTYPE_BF16, NP);
+}
+
+// The wave's number as a scalar: matrix instructions take no notice of the lanes'
+// execution mask, so what decides whether one runs has to be a scalar branch.
+__device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+
+// ---------------------------------------------------------------- planes
+template <int PL> struct Op {  // one operand of a 32-deep product
+  bf8 v[PL];
+};
+template <int PL> __device__ __forceinline__ void split1(float x, __bf16 (&o)[PL]) {
+#pragma unroll
+  for (int q = 0; q < PL; ++q) {
+    o[q] = (__bf16)x;
+    if (q + 1 < PL) x -= (float)o[q];
+  }
+}
+template <int PL> __device__ __forceinline__ Op<PL> split8(const float (&x)[8]) {
+  Op<PL> r;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    __bf16 o[PL];
+    split1<PL>(x[e], o);
+#pragma unroll
+    for (int q = 0; q < PL; ++q) r.v[q][e] = o[q];
+  }
+  return r;
+}
+template <int A, int B> __device__ __forceinline__ Op<A> first(const Op<B>& p) {
+  Op<A> r;
+#pragma unroll
+  for (int q = 0; q < A; ++q) r.v[q] = p.v[q];
+  return r;
+}
+template <int PL> __device__ __forceinline__ float join(const Op<PL>& a, int e) {
+  float s = (float)a.v[PL - 1][e];
+#pragma unroll
+  for (int q = PL - 2; q >= 0; --q) s += (float)a.v[q][e];
+  return s;
+}
+// acc[m][n] += sum_k p[m][k] q[n][k], products of planes a and b with a + b < ORDER
+template <int ORDER, int PA, int PB> __device__ __forceinline__ void mma(f4& acc, const Op<PA>& p, const Op<PB>& q) {
+#pragma unroll
+  for (int a = PA - 1; a >= 0; --a)
+#pragma unroll
+    for (int b = PB - 1; b >= 0; --b)
+      if (a + b < ORDER) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(p.v[a], q.v[b], acc, 0, 0, 0);
+}
+
+// ---------------------------------------------------------------- planes in LDS
+// ROWS x COLS values as PL planes of rows, 16 bytes of padding to a row: the 16
+// rows of a 16-byte read fall into different banks for COLS = 32, 64 and 128.
+typedef short s4v __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s4v lds_s4v;
+__device__ __forceinline__ bf4 read_tr(const __bf16* p) {
+  return __builtin_bit_cast(bf4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4v*)(const_cast<__bf16*>(p))));
+}
+__device__ __forceinline__ bf8 cat(bf4 a, bf4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
+
+template <int PL, int ROWS, int COLS> struct Planes {
+  static constexpr int LD = COLS + 8;
+  __bf16 d[PL][ROWS][LD];
+  // free index: row; contraction: columns k0 + 8g + e
+  __device__ __forceinline__ Op<PL> rows(int r0, int k0) const {
+    const int l = lane_id(), g = l >> 4, r = l & 15;
+    Op<PL> o;
+#pragma unroll
+    for (int q = 0; q < PL; ++q) o.v[q] = *reinterpret_cast<const bf8*>(&d[q][r0 + r][k0 + 8 * g]);
+    return o;
+  }
+  // free index r: column c0 + r, or with NAT8 c0 + 8 (r >> 2) + (r & 3);
+  // contraction: rows k0 + 4g + e and k0 + 16 + 4g + e (e < 4), or with KROW8 k0 + 8g + e.
+  // (the transposing read: lane 4k + q of a group names row k's columns 4q..4q+3
+  // and lane i receives column i of the group's 16 for its four rows)
+  template <bool NAT8 = false, bool KROW8 = false> __device__ __forceinline__ Op<PL> cols(int k0, int c0) const {
+    const int l = lane_id(), g = l >> 4, k = (l & 15) >> 2, c = (l & 3) * (NAT8 ? 8 : 4);
+    const int ra = k0 + (KROW8 ? 8 : 4) * g + k, rb = ra + (KROW8 ? 4 : 16);
+    Op<PL> o;
+#pragma unroll
+    for (int q = 0; q < PL; ++q) o.v[q] = cat(read_tr(&d[q][ra][c0 + c]), read_tr(&d[q][rb][c0 + c]));
+    return o;
+  }
+  // four values of row r from column c on
+  __device__ __forceinline__ f4 quad(int r, int c) const {
+    f4 s = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int q = PL - 1; q >= 0; --q) {
+      const bf4 v = *reinterpret_cast<const bf4*>(&d[q][r][c]);
+      s += f4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
+    }
+    return s;
+  }
+};
+
+// ROWS x COLS values of T on their way from a matrix of rows to planes
+template <typename T, int ROWS, int COLS, int NT> struct Stage {
+  static constexpr int VE = 16 / (int)sizeof(T), PER = COLS / VE, CNT = ROWS * PER / NT;
+  static_assert(ROWS * PER % NT == 0, "whole rounds");
+  u4v v[CNT];
+  // rows from `p` on, `rows` of them and `cols` columns; zeros elsewhere
+  __device__ __forceinline__ void load(const T* __restrict__ p, long long ld, int rows, int cols) {
+#pragma unroll
+    for (int i = 0; i < CNT; ++i) {
+      const int id = i * NT + threadIdx.x, r = id / PER, c = (id - r * PER) * VE;
+      v[i] = u4v{0, 0, 0, 0};
+      if (r < rows && c < cols) v[i] = *reinterpret_cast<const u4v*>(p + (long long)r * ld + c);
+    }
+  }
+  template <int PL> __device__ __forceinline__ void store(Planes<PL, ROWS, COLS>& m) const {
+#pragma unroll
+    for (int i = 0; i < CNT; ++i) {
+      const int id = i * NT + threadIdx.x, r = id / PER, c = (id - r * PER) * VE;
+      if constexpr (sizeof(T) == 4) {
+        const f4 x = __builtin_bit_cast(f4, v[i]);
+        bf4 o[PL];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          __bf16 s[PL];
+          split1<PL>(x[e], s);
+#pragma unroll
+          for (int q = 0; q < PL; ++q) o[q][e] = s[q];
+        }
+#pragma unroll
+        for (int q = 0; q < PL; ++q) *reinterpret_cast<bf4*>(&m.d[q][r][c]) = o[q];
+      } else if constexpr (PL == 1) {
+        *reinterpret_cast<u4v*>(&m.d[0][r][c]) = v[i];
+      } else {
+        const h8 x = __builtin_bit_cast(h8, v[i]);
+        float f[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = (float)x[e];
+        const Op<PL> o = split8<PL>(f);
+#pragma unroll
+        for (int q = 0; q < PL; ++q) *reinterpret_cast<bf8*>(&m.d[q][r][c]) = o.v[q];
+      }
+    }
+  }
+};
+
+// ---------------------------------------------------------------- a chunk's decays
+// The sum of v over lanes 0..l, by DPP moves: within rows of 16 lanes, then each
+// row's total into the rows behind it.
+template <int CTRL, int ROWS> __device__ __forceinline__ double dpp_add(double v) {
+  const unsigned long long u = __builtin_bit_cast(unsigned long long, v);
+  const unsigned lo = __builtin_amdgcn_update_dpp(0, (unsigned)u, CTRL, ROWS, 0xF, false);
+  const unsigned hi = __builtin_amdgcn_update_dpp(0, (unsigned)(u >> 32), CTRL, ROWS, 0xF, false);
+  return v + __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
+}
+__device__ __forceinline__ double lane_sums(double v) {
+  v = dpp_add<0x111, 0xF>(v);  // row_shr:1, 2, 4, 8
+  v = dpp_add<0x112, 0xF>(v);
+  v = dpp_add<0x114, 0xF>(v);
+  v = dpp_add<0x118, 0xF>(v);
+  v = dpp_add<0x142, 0xA>(v);  // row_bcast:15 into rows 1 and 3
+  return dpp_add<0x143, 0xC>(v);  // row_bcast:31 into rows 2 and 3
+}
+__device__ __forceinline__ double lane_value(double v, int l) {
+  const unsigned long long u = __builtin_bit_cast(unsigned long long, v);
+  const unsigned lo = __builtin_amdgcn_readlane((unsigned)u, l), hi = __builtin_amdgcn_readlane((unsigned)(u >> 32), l);
+  return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
+}
+
+// d_t, the running sum c_t of log2(e) d_t A over the chunk in two floats, and its
+// factors from the chunk's start, 2^c_t, and to its end, 2^(c_Q - c_t)
+template <int Q> struct Decays {
+  float hi[Q], lo[Q], d[Q];
+  float head[Q], tail[Q];
+  float end;  // 2^c_Q
+  float total;  // c_Q
+  // one wave, lane t (< Q) with token t's d
+  __device__ __forceinline__ void fill(float dt, float A) {
+    const int l = lane_id();
+    const double c = lane_sums(l < Q ? (double)dt * ((double)A * 1.4426950408889634074) : 0.0);
+    const double last = lane_value(c, 63);
+    if (l < Q) {
+      const float h = (float)c;
+      hi[l] = h;
+      lo[l] = (float)(c - (double)h);
+      d[l] = dt;
+      head[l] = __builtin_amdgcn_exp2f(h);
+      tail[l] = __builtin_amdgcn_exp2f((float)(last - c));
+    }
+    if (l == 0) {
+      total = (float)last;
+      end = __builtin_amdgcn_exp2f((float)last);
+    }
+  }
+  __device__ __forceinline__ static f4 four(const float* a, int t) { return *reinterpret_cast<const f4*>(a + t); }
+};
+// log(1 + e^v), v itself from 20 on (within 2e-9 of it)
+__device__ __forceinline__ float softplus_f(float v) { return v > 20.f ? v : log1pf(expf(v)); }
+template <typename T> __device__ __forceinline__ float load_dt(const ScanParams& p, long long row, int h) {
+  const long long o = row * p.lddt + h;
+  const float v = p.dt_f32 ? static_cast<const float*>(p.dt)[o] : (float)static_cast<const T*>(p.dt)[o];
+  return p.dt_bias != nullptr ? v + p.dt_bias[h] : v;
+}
+template <typename T> __device__ __forceinline__ float token_step(const ScanParams& p, long long row, int h) {
+  const float v = load_dt<T>(p, row, h);
+  return p.softplus ? softplus_f(v) : v;
+}
+
+// ---------------------------------------------------------------- the state in registers
+// Wave w holds h[n][p] of its 16 features p = 16w + r as tiles of 16 x 16 (rows n):
+// tile 2c + o, row 4g + e is n = 32c + 8g + 4o + e, so that two tiles are an operand
+// whose contraction runs over n = 32c + 8g + (0..7), as rows of B and C are read.
+template <int NP> struct StateTiles {
+  static constexpr int NB = NP / 16, NC2 = NP / 32;
+  f4 t[NB];
+  __device__ __forceinline__ static int col(int c) { return 32 * c + 8 * (lane_id() >> 4); }
+  __device__ __forceinline__ void load(const float* __restrict__ s, int ld, int N, int w) {
+    const int r = 16 * w + (lane_id() & 15);
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      const int n = col(i >> 1) + 4 * (i & 1);
+      t[i] = f4{0.f, 0.f, 0.f, 0.f};
+      if (s != nullptr && n < N) t[i] = *reinterpret_cast<const f4*>(s + (long long)r * ld + n);
+    }
+  }
+  __device__ __forceinline__ void store(float* __restrict__ s, int ld, int N, int w) const {
+    const int r = 16 * w + (lane_id() & 15);
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      const int n = col(i >> 1) + 4 * (i & 1);
+      if (n < N) *reinterpret_cast<f4*>(s + (long long)r * ld + n) = t[i];
+    }
+  }
+  // as [NP][P]: what the backward reads as operands with contraction over p
+  __device__ __forceinline__ void keep(float* __restrict__ s, int P, int w) const {
+    const int l = lane_id();
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[(col(i >> 1) + 4 * (i & 1) + e) * P + 16 * w + (l & 15)] = t[i][e];
+  }
+  template <int PL> __device__ __forceinline__ Op<PL> op(int c) const {
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = t[2 * c + (e >> 2)][e & 3];
+    return split8<PL>(x);
+  }
+};
+// the tiles (ib, jb), jb <= ib, of a lower triangle of blocks, row by row
+__device__ __forceinline__ int tri(int ib, int jb) { return ib * (ib + 1) / 2 + jb; }
+__device__ __forceinline__ int tri_row(int t) { return t >= 6 ? 3 : t >= 3 ? 2 : t >= 1 ? 1 : 0; }
+
+}  // namespace ttt

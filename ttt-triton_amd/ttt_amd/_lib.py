@@ -16,7 +16,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 # TTT_AMD_LIB names another build of the same library (e.g. the host-ASan
 # checking build of build_lib.py --asan)
 LIB_PATH = os.environ.get("TTT_AMD_LIB") or os.path.join(_HERE, "libttt_amd.so")
-ABI_VERSION = 11
+ABI_VERSION = 12
 
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
@@ -33,6 +33,8 @@ STATE_SHARED = 0x200  # (forward): initial states [H,...], one for every sequenc
 SAVED_SLOTS = 0x400  # `saved` without the place of the backward's handoff (slot_saved below)
 ETA_RULES = {"dense": ETA_DENSE, "layer": ETA_LAYER, "causal": ETA_CAUSAL}
 
+ACTIVATIONS = {None: 0, "silu": 1}  # enum ttt_activation
+
 # process-wide options (enum ttt_option)
 OPT_MLP_BWD_POLL_LIMIT = 1
 OPT_MLP_BWD_FUSED = 2
@@ -46,6 +48,7 @@ _P = ctypes.c_void_p
 _I = ctypes.c_int
 _F = ctypes.c_float
 _S = ctypes.c_size_t
+_L = ctypes.c_longlong
 
 # name -> (restype, argtypes); mirrors include/ttt_amd.h
 SIGNATURES = {
@@ -78,6 +81,20 @@ SIGNATURES = {
     "ttt_mlp_memo_combine_keep": (_I, [_P] * 10 + [_I] * 8 + [_F] + [_P, _P, _S, _P, _S, _P]),
     "ttt_mlp_memo_combine_bwd_kept": (_I, [_P] * 6 + [_I] * 7 + [_P, _S, _P, _S] + [_P] * 4),
     "ttt_mlp_memo_combine_bwd": (_I, [_P] * 10 + [_I] * 8 + [_F] + [_P, _S, _P, _P, _P, _P]),
+    "ttt_causal_conv_fwd": (_I, [_P, _L] + [_P] * 3 + [_I] * 6 + [_P] * 3),
+    "ttt_causal_conv_partial_bytes": (_S, [_I] * 4),
+    "ttt_causal_conv_bwd": (_I, [_P, _L] + [_P] * 5 + [_I] * 6 + [_P] * 5 + [_S, _P]),
+    "ttt_causal_conv_step": (_I, [_P, _L] + [_P] * 3 + [_I] * 5 + [_P, _P]),
+    "ttt_scan_states_bytes": (_S, [_I] * 6),
+    "ttt_scan_workspace_bytes": (_S, [_I] * 6),
+    "ttt_scan_fwd": (_I, [_P, _L] * 2 + [_P] + [_P, _L] * 2 + [_P] * 3 + [_I] * 9 + [_P, _P] + [_P, _S] * 2 + [_P]),
+    "ttt_scan_bwd_workspace_bytes": (_S, [_I] * 7),
+    "ttt_scan_bwd": (_I, [_P, _L] * 2 + [_P] + [_P, _L] * 2 + [_P] * 2 + [_P, _L, _P, _P, _S] + [_I] * 9 + [_P] * 8
+                     + [_P, _S, _P]),
+    "ttt_scan_step": (_I, [_P, _L] * 2 + [_P] + [_P, _L] * 2 + [_P] * 3 + [_I] * 8 + [_P, _P]),
+    "ttt_layer_norm_fwd": (_I, [_P, _L] * 2 + [_P] * 2 + [_L, _I, _F, _I] + [_P] * 3),
+    "ttt_layer_norm_partial_bytes": (_S, [_L, _I]),
+    "ttt_layer_norm_bwd": (_I, [_P, _L] * 2 + [_P] * 3 + [_L, _I, _I] + [_P] * 5 + [_S, _P]),
 }
 
 _lock = threading.Lock()

@@ -1,0 +1,100 @@
+"""Layer norm over the last axis on the HIP path (ttt_layer_norm_* in
+include/ttt_amd.h), plain or of a gated input, with its backward.
+
+PostNormFunction (layer_io.py) norms the inner loop's [B,H,NC,K,F] output; this
+one takes rows as they are."""
+
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from ._common import check_device, dtype_code, on_device, ptr, stream_of
+from .ssm import _opt, _param, _rows, _wants_grad
+
+LAYER_NORM_EPS = 1e-6
+MAX_WIDTH = 16384
+
+
+def _norm_forward(x, weight, bias, gate, eps, train):
+    """(y, what the backward reads)"""
+    D = x.shape[-1] if x.dim() else 0
+    if not 1 <= D <= MAX_WIDTH:
+        raise ValueError(f"layer_norm takes rows of 1 to {MAX_WIDTH} values, got {list(x.shape)}")
+    if (weight is None) != (bias is None):
+        raise ValueError("layer_norm takes weight and bias, or neither")
+    if gate is not None and (gate.shape != x.shape or gate.dtype != x.dtype):
+        raise ValueError(f"gate must be as x, {list(x.shape)} in {x.dtype}, got {list(gate.shape)} in {gate.dtype}")
+    if not 0.0 < eps <= 1.0:
+        raise ValueError(f"eps must be in (0, 1], got {eps}")
+    dev = check_device(x, *(t for t in (weight, bias, gate) if t is not None))
+    code = dtype_code(x.dtype)
+    w, b = _param(weight, (D,), "weight"), _param(bias, (D,), "bias")
+    lead, es = x.dim() - 1, x.element_size()
+    xr, ldx = _rows(x, x.dtype, lead, es)
+    gr, ldg = (None, 0) if gate is None else _rows(gate, x.dtype, lead, es)
+    y = torch.empty(x.shape, device=dev, dtype=x.dtype)
+    R = y.numel() // D
+    if R >= 1 << 31:
+        raise ValueError(f"layer_norm takes fewer than 2^31 rows, got {R}")
+    stats = torch.empty((R, 2), device=dev, dtype=torch.float32) if train else None
+    with on_device(dev):
+        st = _lib.load().ttt_layer_norm_fwd(ptr(xr), ldx, _opt(gr), ldg, _opt(w), _opt(b), R, D, float(eps), code,
+                                            ptr(y), _opt(stats), stream_of(dev))
+    _lib.check(st, "ttt_layer_norm_fwd")
+    return y, (xr, ldx, gr, ldg, w, stats)
+
+
+class LayerNormFunction(torch.autograd.Function):
+    """apply(x, weight, bias, gate, eps) -> y; differentiable wrt all four tensors."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, gate, eps):
+        y, (xr, ldx, gr, ldg, w, stats) = _norm_forward(x, weight, bias, gate, eps, True)
+        ctx.save_for_backward(xr, gr, w, stats)
+        ctx.lds = ldx, ldg
+        ctx.dtypes = None if weight is None else (weight.dtype, bias.dtype)
+        ctx.shape = x.shape
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, gate, w, stats = ctx.saved_tensors
+        dev, dt = x.device, x.dtype
+        D = ctx.shape[-1]
+        R = stats.shape[0]
+        dy = dy.to(dt).contiguous()
+        dx = torch.empty(ctx.shape, device=dev, dtype=dt)
+        dg = torch.empty(ctx.shape, device=dev, dtype=dt) if gate is not None else None
+        lib = _lib.load()
+        dw = db = part = None
+        n = 0
+        if w is not None and (ctx.needs_input_grad[1] or ctx.needs_input_grad[2]):
+            dw, db = torch.empty((2, D), device=dev, dtype=torch.float32)
+            n = lib.ttt_layer_norm_partial_bytes(R, D)
+            part = torch.empty(n // 4, device=dev, dtype=torch.float32)
+        with on_device(dev):
+            st = lib.ttt_layer_norm_bwd(ptr(x), ctx.lds[0], _opt(gate), ctx.lds[1], _opt(w), ptr(stats), ptr(dy), R, D,
+                                        dtype_code(dt), ptr(dx), _opt(dg), _opt(dw), _opt(db), _opt(part), n,
+                                        stream_of(dev))
+        _lib.check(st, "ttt_layer_norm_bwd")
+        if dw is not None:
+            dw, db = dw.to(ctx.dtypes[0]), db.to(ctx.dtypes[1])
+        return dx, dw, db, dg, None
+
+
+def layer_norm(x, weight=None, bias=None, gate=None, eps: float = LAYER_NORM_EPS):
+    """(v - mean v) / sqrt(var v + eps) * weight + bias over the last axis (up to
+    16,384 values) of v = x, or of v = x * silu(gate) where a gate of x's shape and
+    dtype is given.  weight and bias [D], both or neither; the variance is the biased
+    one.  x and gate may be columns of a wider matrix."""
+    if x.dim() and x.numel() == 0 and x.shape[-1]:
+        return x.clone()
+    if _wants_grad(x, weight, bias, gate):
+        return LayerNormFunction.apply(x, weight, bias, gate, eps)
+    return _norm_forward(x, weight, bias, gate, eps, False)[0]
+
+
+__all__ = ["layer_norm", "LayerNormFunction", "LAYER_NORM_EPS"]

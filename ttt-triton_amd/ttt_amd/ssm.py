@@ -1,0 +1,369 @@
+"""The selective state-space operators on the HIP path (ttt_causal_conv_* and
+ttt_scan_* in include/ttt_amd.h): the short causal convolution and the scan,
+over whole sequences with gradients, and one token at a time on a state.
+
+causal_conv     y[t,c] = act(bias[c] + sum_k weight[c,k] s[t+k,c]) over x [B,L,C], s
+                being the W-1 inputs before the first token followed by x
+selective_scan  h_t = exp(d_t A) h_{t-1} + d_t x_t (x) B_t,  y_t = h_t C_t + D x_t
+                with d = softplus(dt + dt_bias): one decay a head, x [B,L,H,P], B and
+                C [B,L,G,N] shared by the H/G heads of a group, h [B,H,P,N] fp32
+
+Activations share one dtype (fp32, bf16 or fp16; dt may be fp32 beside a 16-bit
+x); parameters and scan states are fp32.  x, dt, Bm and Cm may be columns of a
+wider contiguous matrix of rows: they are read in place where x, Bm and Cm start
+on 16 bytes in every row, and from a copy elsewhere.  Results do not depend on
+which; nothing of a call depends on another sequence of its batch, but its
+rounding may: the length is cut up by the number of sequences and heads.
+
+A token that is not finite reaches the outputs and states of its own sequence from
+that token on, and no earlier output.  In the backward it may reach every gradient
+of its sequence."""
+
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from ._common import check_device, dtype_code, f32c, on_device, ptr, stream_of
+
+HEAD_DIMS = (32, 64)
+MAX_STATE = 128
+CONV_WIDTHS = (2, 3, 4)
+
+
+def _rows(t: torch.Tensor, dt: torch.dtype, lead: int, align: int):
+    """(t, row stride) with t's first `lead` axes as rows a fixed stride apart and
+    the rest contiguous inside a row, `align` bytes of alignment; a contiguous
+    copy where t is not laid out so."""
+    if t.dtype == dt:
+        ld = width = 1
+        for n, st in zip(reversed(t.shape[lead:]), reversed(t.stride()[lead:])):
+            if n != 1 and st != width:
+                break
+            width *= n
+        else:
+            # the innermost leading axis that is more than one row gives the stride
+            ld, step = None, 0
+            for n, st in zip(reversed(t.shape[:lead]), reversed(t.stride()[:lead])):
+                if n == 1:
+                    continue
+                if ld is None:
+                    ld, step = st, st * n
+                elif st != step:
+                    ld = -1
+                    break
+                else:
+                    step *= n
+            ld = width if ld is None else ld
+            if ld >= width and (t.data_ptr() | ld * t.element_size()) % align == 0:
+                return t, ld
+    t = t.detach().to(dt).contiguous()
+    return t, t[(0,) * lead].numel()
+
+
+def _opt(t):
+    return None if t is None else t.data_ptr()
+
+
+def _param(t, shape, name):
+    if t is None:
+        return None
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
+    return f32c(t)
+
+
+def _wants_grad(*ts) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+
+
+def _no_grad_through(what, *ts):
+    if _wants_grad(*ts):
+        raise ValueError(f"{what} updates its state in place and has no gradient: call it under torch.no_grad()")
+
+
+def _sizes(*ns):
+    if max(ns) >= 1 << 31:
+        raise ValueError(f"sizes must be below 2^31, got {ns}")
+
+
+def _state_in_place(state, shape, dt, dev, what):
+    if tuple(state.shape) != shape or state.dtype != dt or not state.is_contiguous() or state.device != dev:
+        raise ValueError(f"{what}: the state must be contiguous, {list(shape)} in {dt} on {dev}, got "
+                         f"{list(state.shape)} in {state.dtype} on {state.device}")
+
+
+# ---------------------------------------------------------------------------
+# short causal convolution
+# ---------------------------------------------------------------------------
+
+def _conv_args(x, weight, bias, state, activation, lead):
+    if x.dim() != lead + 1:
+        raise ValueError(f"x must be [{'B,L,C' if lead == 2 else 'B,C'}], got {list(x.shape)}")
+    C = x.shape[-1]
+    if weight.dim() != 2 or weight.shape[0] != C or weight.shape[1] not in CONV_WIDTHS:
+        raise ValueError(f"weight must be [C,W]=[{C},W] with W in {CONV_WIDTHS}, got {list(weight.shape)}")
+    if activation not in _lib.ACTIVATIONS:
+        raise ValueError(f"unknown activation {activation!r} (None or 'silu')")
+    dev = check_device(x, weight, *(t for t in (bias, state) if t is not None))
+    W = weight.shape[1]
+    _sizes(*x.shape)
+    return dev, dtype_code(x.dtype), C, W, f32c(weight), _param(bias, (C,), "bias")
+
+
+def _conv_state(state, shape, dt):
+    if state is None:
+        return None
+    if tuple(state.shape) != shape:
+        raise ValueError(f"initial_state must be [B,W-1,C]={list(shape)}, got {list(state.shape)}")
+    return state.detach().to(dt).contiguous()
+
+
+def _conv_forward(x, weight, bias, state, activation, want_last):
+    """(y, last state or None, what the backward reads)"""
+    dev, code, C, W, w, b = _conv_args(x, weight, bias, state, activation, 2)
+    B, L = x.shape[:2]
+    xr, ldx = _rows(x, x.dtype, 2, x.element_size())
+    s0 = _conv_state(state, (B, W - 1, C), x.dtype)
+    y = torch.empty((B, L, C), device=dev, dtype=x.dtype)
+    last = torch.empty((B, W - 1, C), device=dev, dtype=x.dtype) if want_last else None
+    with on_device(dev):
+        st = _lib.load().ttt_causal_conv_fwd(ptr(xr), ldx, _opt(s0), ptr(w), _opt(b), B, L, C, W,
+                                             _lib.ACTIVATIONS[activation], code, ptr(y), _opt(last), stream_of(dev))
+    _lib.check(st, "ttt_causal_conv_fwd")
+    return y, last, (xr, ldx, s0, w, b)
+
+
+class CausalConvFunction(torch.autograd.Function):
+    """apply(x, weight, bias, initial_state, activation, want_last) -> (y, last
+    state or None); differentiable wrt x, weight, bias and initial_state."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, state, activation, want_last):
+        y, last, (xr, ctx.ldx, s0, w, b) = _conv_forward(x, weight, bias, state, activation, want_last)
+        ctx.save_for_backward(xr, s0, w, b)
+        ctx.activation = activation
+        ctx.dtypes = weight.dtype, None if bias is None else bias.dtype, None if state is None else state.dtype
+        ctx.shape = (*x.shape, weight.shape[1])
+        ctx.set_materialize_grads(False)
+        return y, last
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dlast):
+        x, s0, w, b = ctx.saved_tensors
+        B, L, C, W = ctx.shape
+        dev = x.device
+        dt = x.dtype
+        dy, dlast = (None if g is None else g.to(dt).contiguous() for g in (dy, dlast))
+        dx = torch.empty((B, L, C), device=dev, dtype=dt)
+        ds = torch.empty((B, W - 1, C), device=dev, dtype=dt) if ctx.needs_input_grad[3] else None
+        dw = torch.empty((C, W), device=dev, dtype=torch.float32)
+        db = torch.empty(C, device=dev, dtype=torch.float32) if ctx.dtypes[1] is not None else None
+        lib = _lib.load()
+        part = torch.empty(lib.ttt_causal_conv_partial_bytes(B, L, C, W) // 4, device=dev, dtype=torch.float32)
+        with on_device(dev):
+            st = lib.ttt_causal_conv_bwd(ptr(x), ctx.ldx, _opt(s0), ptr(w), _opt(b), _opt(dy), _opt(dlast), B, L, C, W,
+                                         _lib.ACTIVATIONS[ctx.activation], dtype_code(dt), ptr(dx), _opt(ds), ptr(dw),
+                                         _opt(db), ptr(part), part.numel() * 4, stream_of(dev))
+        _lib.check(st, "ttt_causal_conv_bwd")
+        wt, bt, sd = ctx.dtypes
+        return (dx, dw.to(wt), None if db is None else db.to(bt), None if ds is None else ds.to(sd), None, None)
+
+
+def causal_conv(x, weight, bias=None, initial_state=None, activation=None, return_final_state: bool = False):
+    """The causal convolution of every channel over x [B,L,C] with weight [C,W],
+    W in 2..4, from zeros or initial_state [B,W-1,C] (the inputs before the first
+    token, oldest first).  activation: None or "silu".  Returns y [B,L,C], and with
+    return_final_state the last W-1 inputs [B,W-1,C] as well: the state that
+    causal_conv_step and a later call go on from."""
+    if x.dim() == 3 and x.numel() == 0:
+        W = weight.shape[-1]
+        first = x.new_zeros(x.shape[0], W - 1, x.shape[2]) if initial_state is None else initial_state.to(x.dtype)
+        return (x.clone(), first.clone()) if return_final_state else x.clone()
+    if _wants_grad(x, weight, bias, initial_state):
+        y, last = CausalConvFunction.apply(x, weight, bias, initial_state, activation, return_final_state)
+    else:
+        y, last, _ = _conv_forward(x, weight, bias, initial_state, activation, return_final_state)
+    return (y, last) if return_final_state else y
+
+
+def causal_conv_step(x, state, weight, bias=None, activation=None):
+    """One token x [B,C] of every sequence: returns y [B,C] and moves state
+    [B,W-1,C] (contiguous, in x's dtype) up by one in place.  No gradient."""
+    _no_grad_through("causal_conv_step", x, state, weight, bias)
+    dev, code, C, W, w, b = _conv_args(x, weight, bias, state, activation, 1)
+    B = x.shape[0]
+    _state_in_place(state, (B, W - 1, C), x.dtype, dev, "causal_conv_step")
+    y = torch.empty((B, C), device=dev, dtype=x.dtype)
+    if B == 0:
+        return y
+    xr, ldx = _rows(x, x.dtype, 1, x.element_size())
+    with on_device(dev):
+        st = _lib.load().ttt_causal_conv_step(ptr(xr), ldx, ptr(state), ptr(w), _opt(b), B, C, W,
+                                              _lib.ACTIVATIONS[activation], code, ptr(y), stream_of(dev))
+    _lib.check(st, "ttt_causal_conv_step")
+    torch.autograd.graph.increment_version(state)
+    return y
+
+
+# ---------------------------------------------------------------------------
+# selective scan
+# ---------------------------------------------------------------------------
+
+def _scan_args(x, dt, A, Bm, Cm, D, dt_bias, state, lead):
+    """(device, (B, L, H, P, G, N), code of x, code of dt, A, D, dt_bias)"""
+    if x.dim() != lead + 2:
+        raise ValueError(f"x must be [{'B,L,H,P' if lead == 2 else 'B,H,P'}], got {list(x.shape)}")
+    rows = tuple(x.shape[:lead])
+    H, P = x.shape[lead:]
+    if Bm.dim() != lead + 2 or tuple(Bm.shape[:lead]) != rows or Bm.shape != Cm.shape:
+        raise ValueError(f"Bm and Cm must be {[*rows, 'G', 'N']}, got {list(Bm.shape)} and {list(Cm.shape)}")
+    G, N = Bm.shape[lead:]
+    if P not in HEAD_DIMS:
+        raise ValueError(f"the head dim P must be one of {HEAD_DIMS}, got {P}")
+    if N % 16 or not 16 <= N <= MAX_STATE:
+        raise ValueError(f"the state's width N must be a multiple of 16 up to {MAX_STATE}, got {N}")
+    if G < 1 or H % G:
+        raise ValueError(f"the {G} groups of Bm and Cm must divide the {H} heads")
+    if tuple(dt.shape) != (*rows, H):
+        raise ValueError(f"dt must be {[*rows, H]}, got {list(dt.shape)}")
+    for name, t in (("Bm", Bm), ("Cm", Cm)):
+        if t.dtype != x.dtype:
+            raise ValueError(f"{name} must have x's dtype {x.dtype}, got {t.dtype}")
+    if dt.dtype not in (x.dtype, torch.float32):
+        raise ValueError(f"dt must be in {x.dtype} or float32, got {dt.dtype}")
+    dev = check_device(x, dt, A, Bm, Cm, *(t for t in (D, dt_bias, state) if t is not None))
+    _sizes(*x.shape)
+    a = _param(A, (H,), "A")
+    if a is None:
+        raise ValueError("A is needed")
+    return (dev, (rows[0], rows[1] if lead == 2 else 1, H, P, G, N), dtype_code(x.dtype), dtype_code(dt.dtype), a,
+            _param(D, (H,), "D"), _param(dt_bias, (H,), "dt_bias"))
+
+
+def _scan_rows(x, dt, Bm, Cm, lead, align):
+    """The four inputs and their row strides as the kernels take them."""
+    out = []
+    for t, al in ((x, align), (dt, dt.element_size()), (Bm, align), (Cm, align)):
+        out += _rows(t, t.dtype, lead, al)
+    return out
+
+
+def _scan_forward(x, dt, A, Bm, Cm, D, dt_bias, h0, softplus, want_last, train):
+    """(y, last state or None, what the backward reads)"""
+    dev, (B, L, H, P, G, N), code, dcode, a, d, bias = _scan_args(x, dt, A, Bm, Cm, D, dt_bias, h0, 2)
+    if h0 is not None:
+        if tuple(h0.shape) != (B, H, P, N):
+            raise ValueError(f"initial_state must be [B,H,P,N]={[B, H, P, N]}, got {list(h0.shape)}")
+        h0 = f32c(h0)
+    rows = _scan_rows(x, dt, Bm, Cm, 2, 16)
+    xr, ldx, dr, ldd, br, ldb, cr, ldc = rows
+    y = torch.empty((B, L, H, P), device=dev, dtype=x.dtype)
+    last = torch.empty((B, H, P, N), device=dev, dtype=torch.float32) if want_last else None
+    lib = _lib.load()
+    nst = lib.ttt_scan_states_bytes(B, L, H, P, N, code) if train else 0
+    nws = lib.ttt_scan_workspace_bytes(B, L, H, P, N, code)
+    states = torch.empty(nst, device=dev, dtype=torch.uint8) if train else None
+    ws = torch.empty(nws, device=dev, dtype=torch.uint8) if nws else None
+    with on_device(dev):
+        st = lib.ttt_scan_fwd(ptr(xr), ldx, ptr(dr), ldd, ptr(a), ptr(br), ldb, ptr(cr), ldc, _opt(d), _opt(bias),
+                              _opt(h0), B, L, H, P, G, N, code, dcode, int(softplus), ptr(y), _opt(last), _opt(states),
+                              nst, _opt(ws), nws, stream_of(dev))
+    _lib.check(st, "ttt_scan_fwd")
+    return y, last, (rows, a, d, bias, states)
+
+
+class SelectiveScanFunction(torch.autograd.Function):
+    """apply(x, dt, A, Bm, Cm, D, dt_bias, initial_state, dt_softplus, want_last) ->
+    (y, last state or None); differentiable wrt all tensors.  The forward keeps the
+    states entering its chunks of 64 tokens (32 in fp32, and in fp16 for N > 64)."""
+
+    @staticmethod
+    def forward(ctx, x, dt, A, Bm, Cm, D, dt_bias, h0, softplus, want_last):
+        y, last, (rows, a, d, bias, states) = _scan_forward(x, dt, A, Bm, Cm, D, dt_bias, h0, softplus, want_last, True)
+        xr, ldx, dr, ldd, br, ldb, cr, ldc = rows
+        ctx.save_for_backward(xr, dr, br, cr, a, d, bias, states)
+        ctx.lds, ctx.softplus = (ldx, ldd, ldb, ldc), softplus
+        ctx.shape = (*x.shape, *Bm.shape[2:])
+        ctx.dtypes = tuple(None if t is None else t.dtype for t in (A, D, dt_bias, h0))
+        ctx.set_materialize_grads(False)
+        return y, last
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dlast):
+        x, dt, Bm, Cm, a, d, bias, states = ctx.saved_tensors
+        B, L, H, P, G, N = ctx.shape
+        ldx, ldd, ldb, ldc = ctx.lds
+        dev, act = x.device, x.dtype
+        code = dtype_code(act)
+        dy = torch.zeros((B, L, H, P), device=dev, dtype=act) if dy is None else dy
+        dyr, ldy = _rows(dy, act, 2, 16)
+        dlast = None if dlast is None else f32c(dlast)
+        f32 = dict(device=dev, dtype=torch.float32)
+        dx = torch.empty((B, L, H, P), device=dev, dtype=act)
+        ddt = torch.empty((B, L, H), device=dev, dtype=dt.dtype)
+        dB, dC = (torch.empty((B, L, G, N), device=dev, dtype=act) for _ in range(2))
+        dA = torch.empty(H, **f32)
+        dD, dbias = (None if t is None else torch.empty(H, **f32) for t in (d, bias))
+        dh0 = torch.empty((B, H, P, N), **f32) if ctx.needs_input_grad[7] else None
+        lib = _lib.load()
+        nws = lib.ttt_scan_bwd_workspace_bytes(B, L, H, P, G, N, code)
+        ws = torch.empty(nws, device=dev, dtype=torch.uint8)
+        with on_device(dev):
+            st = lib.ttt_scan_bwd(ptr(x), ldx, ptr(dt), ldd, ptr(a), ptr(Bm), ldb, ptr(Cm), ldc, _opt(d), _opt(bias),
+                                  ptr(dyr), ldy, _opt(dlast), ptr(states), states.numel(), B, L, H, P, G, N, code,
+                                  dtype_code(dt.dtype), int(ctx.softplus), ptr(dx), ptr(ddt), ptr(dA), ptr(dB), ptr(dC),
+                                  _opt(dD), _opt(dbias), _opt(dh0), ptr(ws), nws, stream_of(dev))
+        _lib.check(st, "ttt_scan_bwd")
+        dts = ctx.dtypes
+        dD, dbias, dh0 = (None if g is None else g.to(t) for g, t in zip((dD, dbias, dh0), dts[1:]))
+        return dx, ddt, dA.to(dts[0]), dB, dC, dD, dbias, dh0, None, None
+
+
+def selective_scan(x, dt, A, Bm, Cm, D=None, dt_bias=None, initial_state=None, dt_softplus: bool = True,
+                   return_final_state: bool = False):
+    """The scan of x [B,L,H,P] with steps dt [B,L,H] (softplus(dt + dt_bias), or with
+    dt_softplus=False dt + dt_bias itself, >= 0), rates A [H] < 0, Bm and Cm [B,L,G,N]
+    and the skip D [H], from zeros or initial_state [B,H,P,N] fp32.  P is 32 or 64,
+    N a multiple of 16 up to 128.  Returns y [B,L,H,P] in x's dtype, and with
+    return_final_state the last state [B,H,P,N] fp32 as well, which
+    selective_scan_step and a later call go on from.  A step of 0 (dt = -inf under
+    the softplus) leaves the state as it is."""
+    if x.dim() == 4 and x.numel() == 0:
+        B, _, H, P = x.shape
+        N = Bm.shape[-1]
+        first = torch.zeros(B, H, P, N, device=x.device) if initial_state is None else initial_state.float()
+        return (x.clone(), first.clone()) if return_final_state else x.clone()
+    if _wants_grad(x, dt, A, Bm, Cm, D, dt_bias, initial_state):
+        y, last = SelectiveScanFunction.apply(x, dt, A, Bm, Cm, D, dt_bias, initial_state, bool(dt_softplus),
+                                              return_final_state)
+    else:
+        y, last, _ = _scan_forward(x, dt, A, Bm, Cm, D, dt_bias, initial_state, bool(dt_softplus), return_final_state,
+                                   False)
+    return (y, last) if return_final_state else y
+
+
+def selective_scan_step(x, dt, A, Bm, Cm, state, D=None, dt_bias=None, dt_softplus: bool = True):
+    """One token of every sequence: x [B,H,P], dt [B,H], Bm and Cm [B,G,N].  Updates
+    state [B,H,P,N] (fp32, contiguous) in place and returns y [B,H,P].  No gradient."""
+    _no_grad_through("selective_scan_step", x, dt, A, Bm, Cm, state, D, dt_bias)
+    dev, (B, _, H, P, G, N), code, dcode, a, d, bias = _scan_args(x, dt, A, Bm, Cm, D, dt_bias, state, 1)
+    _state_in_place(state, (B, H, P, N), torch.float32, dev, "selective_scan_step")
+    y = torch.empty((B, H, P), device=dev, dtype=x.dtype)
+    if B == 0:
+        return y
+    xr, ldx, dr, ldd, br, ldb, cr, ldc = _scan_rows(x, dt, Bm, Cm, 1, 4 * x.element_size())
+    with on_device(dev):
+        st = _lib.load().ttt_scan_step(ptr(xr), ldx, ptr(dr), ldd, ptr(a), ptr(br), ldb, ptr(cr), ldc, _opt(d),
+                                       _opt(bias), ptr(state), B, H, P, G, N, code, dcode, int(dt_softplus), ptr(y),
+                                       stream_of(dev))
+    _lib.check(st, "ttt_scan_step")
+    torch.autograd.graph.increment_version(state)
+    return y
+
+
+__all__ = ["causal_conv", "causal_conv_step", "selective_scan", "selective_scan_step", "CausalConvFunction",
+           "SelectiveScanFunction"]
