@@ -49,10 +49,13 @@ COMMON = [
 # their MFMA accumulators in VGPRs (both convert W or dW into operand frags every
 # mini-batch; forward + backward at B16 H12 T2048 F64 bf16 467 -> 439 us with the
 # backward's, while the MLP's kernels, which need more than 256 registers, lose:
-# forward 640 -> 690, forward + backward 1,944 -> 2,128)
+# forward 640 -> 690, forward + backward 1,944 -> 2,128); the selective scan's state
+# is scaled every chunk, its walks and chunk pass save the moves and a wave of registers
 PER_FILE = {
     "ttt_linear_fwd_rows.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"],
     "ttt_linear_bwd.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"],
+    "ttt_scan_walk.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"],
+    "ttt_scan_bwd.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"],
 }
 
 

@@ -47,12 +47,14 @@ int check_scan(int B, int L, int H, int P, int G, int N, int dtype, int dt_dtype
 int check_row(long long ld, long long least, int dtype) {
   return ld < least || ld * size_of(dtype) % 16 != 0 ? TTT_ERR_SHAPE : TTT_OK;
 }
+constexpr int kSelfJoined = 8;  // segments whose states the walk's workgroups join themselves
 struct ScanPlan {
   int Q, NC, NP, S, per, splits;
   size_t states, seg, decay, partial, split;
 };
-// How a scan is cut up.  Segments: a workgroup walks a sequence and head; below 512
-// of them (two a compute unit) the tokens are shared out as well, whole chunks each.
+// How a scan is cut up.  Segments: a workgroup walks a sequence and head; below 768
+// of them (three a compute unit, of 64 features; twice as many of 32) the tokens are
+// shared out as well, whole chunks each, to at most that many.
 // Splits: the backward's workgroups have a chunk and go over a group's heads; below
 // 512 of them the heads are shared out.
 ScanPlan plan(int B, int L, int H, int P, int G, int N, int dtype) {
@@ -61,7 +63,7 @@ ScanPlan plan(int B, int L, int H, int P, int G, int N, int dtype) {
   s.Q = ttt::scan_chunk(dtype, s.NP);
   s.NC = (L + s.Q - 1) / s.Q;
   const long long chains = (long long)B * H;
-  const long long want = chains >= 256 ? 1 : std::min<long long>(s.NC, (512 + chains - 1) / chains);
+  const long long want = std::max(1LL, std::min<long long>(s.NC, (P == 64 ? 768 : 1536) / chains));
   s.per = (int)((s.NC + want - 1) / want);
   s.S = (s.NC + s.per - 1) / s.per;
   const long long groups = (long long)B * s.NC * G;
@@ -261,6 +263,7 @@ int ttt_scan_fwd(const void* x, long long ldx, const void* dt, long long lddt, c
   p.states = static_cast<float*>(states);
   p.S = s.S;
   p.per = s.per;
+  p.joined = s.S > kSelfJoined;
   if (s.S > 1) {
     p.seg = static_cast<float*>(workspace);
     p.seg_decay = reinterpret_cast<float*>(static_cast<char*>(workspace) + s.seg);
@@ -327,6 +330,7 @@ int ttt_scan_bwd(const void* x, long long ldx, const void* dt, long long lddt, c
   p.dt_f32 = dt_dtype == TTT_DTYPE_F32;
   p.S = s.S;
   p.per = s.per;
+  p.joined = s.S > kSelfJoined;
   p.splits = s.splits;
   char* ws = static_cast<char*>(workspace);
   float* gstates = reinterpret_cast<float*>(ws);

@@ -38,6 +38,7 @@ struct ScanParams {
   long long ldx, lddt, ldb, ldc;
   int B, L, H, G, N;
   int S, per;                        // segments, and chunks in one
+  bool joined;                       // the states in `seg` are those entering the segments
   bool softplus, dt_f32;
   // backward
   const void* dy;                    // [B*L][ldy]
@@ -85,38 +86,63 @@ template <typename T, int NP> constexpr int chunk_of() {
 // execution mask, so what decides whether one runs has to be a scalar branch.
 __device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
+// Workgroups go to the 8 dies in turn, and each die has an L2 of its own: the place of
+// workgroup `id` of n such that each die has a run of neighbours, which share rows.
+__device__ __forceinline__ unsigned on_xcd(unsigned id, unsigned n) {
+  const unsigned die = id & 7, per = n >> 3, rest = n & 7;
+  return die * per + min(die, rest) + (id >> 3);
+}
+
 // ---------------------------------------------------------------- planes
 template <int PL> struct Op {  // one operand of a 32-deep product
   bf8 v[PL];
 };
-template <int PL> __device__ __forceinline__ void split1(float x, __bf16 (&o)[PL]) {
+// two values at a time: one conversion instruction a plane, and what it leaves
+template <int PL> __device__ __forceinline__ void split2(f2 x, bf2 (&o)[PL]) {
 #pragma unroll
   for (int q = 0; q < PL; ++q) {
-    o[q] = (__bf16)x;
-    if (q + 1 < PL) x -= (float)o[q];
+    o[q] = __builtin_convertvector(x, bf2);
+    if (q + 1 < PL) {
+      const unsigned u = __builtin_bit_cast(unsigned, o[q]);
+      x[0] -= __builtin_bit_cast(float, u << 16);
+      x[1] -= __builtin_bit_cast(float, u & 0xffff0000u);
+    }
   }
 }
-template <int PL> __device__ __forceinline__ Op<PL> split8(const float (&x)[8]) {
+template <int PL> __device__ __forceinline__ void split4(f4 x, bf4 (&o)[PL]) {
+  bf2 a[PL], b[PL];
+  split2<PL>(f2{x[0], x[1]}, a);
+  split2<PL>(f2{x[2], x[3]}, b);
+#pragma unroll
+  for (int q = 0; q < PL; ++q) o[q] = __builtin_shufflevector(a[q], b[q], 0, 1, 2, 3);
+}
+template <int PL> __device__ __forceinline__ Op<PL> split8(f4 x, f4 y) {
+  bf4 a[PL], b[PL];
+  split4<PL>(x, a);
+  split4<PL>(y, b);
   Op<PL> r;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    __bf16 o[PL];
-    split1<PL>(x[e], o);
+  for (int q = 0; q < PL; ++q) r.v[q] = __builtin_shufflevector(a[q], b[q], 0, 1, 2, 3, 4, 5, 6, 7);
+  return r;
+}
+// 0 where `keep` is false, without a branch around what x comes from
+__device__ __forceinline__ float only_if(bool keep, float x) {
+  asm("" : "+v"(x));
+  return keep ? x : 0.f;
+}
+// values 4o..4o+3 of an operand
+template <int PL> __device__ __forceinline__ f4 join4(const Op<PL>& a, int o) {
+  typedef unsigned u2 __attribute__((ext_vector_type(2)));
+  f4 s = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int q = 0; q < PL; ++q) r.v[q][e] = o[q];
+  for (int q = PL - 1; q >= 0; --q) {
+    const bf8 v = a.v[q];
+    const bf4 h = o == 0 ? __builtin_shufflevector(v, v, 0, 1, 2, 3) : __builtin_shufflevector(v, v, 4, 5, 6, 7);
+    const u2 u = __builtin_bit_cast(u2, h);
+    const f4 x = f4{__builtin_bit_cast(float, u[0] << 16), __builtin_bit_cast(float, u[0] & 0xffff0000u),
+                    __builtin_bit_cast(float, u[1] << 16), __builtin_bit_cast(float, u[1] & 0xffff0000u)};
+    s = q == PL - 1 ? x : s + x;
   }
-  return r;
-}
-template <int A, int B> __device__ __forceinline__ Op<A> first(const Op<B>& p) {
-  Op<A> r;
-#pragma unroll
-  for (int q = 0; q < A; ++q) r.v[q] = p.v[q];
-  return r;
-}
-template <int PL> __device__ __forceinline__ float join(const Op<PL>& a, int e) {
-  float s = (float)a.v[PL - 1][e];
-#pragma unroll
-  for (int q = PL - 2; q >= 0; --q) s += (float)a.v[q][e];
   return s;
 }
 // acc[m][n] += sum_k p[m][k] q[n][k], products of planes a and b with a + b < ORDER
@@ -163,54 +189,72 @@ template <int PL, int ROWS, int COLS> struct Planes {
   }
   // four values of row r from column c on
   __device__ __forceinline__ f4 quad(int r, int c) const {
-    f4 s = f4{0.f, 0.f, 0.f, 0.f};
+    Op<PL> o;
 #pragma unroll
-    for (int q = PL - 1; q >= 0; --q) {
+    for (int q = 0; q < PL; ++q) {
       const bf4 v = *reinterpret_cast<const bf4*>(&d[q][r][c]);
-      s += f4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
+      o.v[q] = cat(v, v);
     }
-    return s;
+    return join4(o, 0);
   }
 };
 
-// ROWS x COLS values of T on their way from a matrix of rows to planes
+// ROWS x COLS values of T on their way from a matrix of rows to planes.  A thread's
+// places are the same in every chunk: their offsets are formed once.
 template <typename T, int ROWS, int COLS, int NT> struct Stage {
-  static constexpr int VE = 16 / (int)sizeof(T), PER = COLS / VE, CNT = ROWS * PER / NT;
-  static_assert(ROWS * PER % NT == 0, "whole rounds");
+  static constexpr int VE = 16 / (int)sizeof(T), PER = COLS / VE, ALL = ROWS * PER, CNT = (ALL + NT - 1) / NT;
+  static_assert(ALL % NT == 0 || CNT == 1, "whole rounds, or some threads without a place");
   u4v v[CNT];
-  // rows from `p` on, `rows` of them and `cols` columns; zeros elsewhere
-  __device__ __forceinline__ void load(const T* __restrict__ p, long long ld, int rows, int cols) {
+  unsigned off[CNT];  // bytes
+  int cols;
+  __device__ __forceinline__ static int row(int i) { return (i * NT + (int)threadIdx.x) / PER; }
+  __device__ __forceinline__ static int col(int i) { return (i * NT + (int)threadIdx.x) % PER * VE; }
+  // rows `ld` apart (ROWS of them within 4 GiB), `cols` columns
+  __device__ __forceinline__ void place(long long ld, int n) {
+    cols = n;
 #pragma unroll
-    for (int i = 0; i < CNT; ++i) {
-      const int id = i * NT + threadIdx.x, r = id / PER, c = (id - r * PER) * VE;
-      v[i] = u4v{0, 0, 0, 0};
-      if (r < rows && c < cols) v[i] = *reinterpret_cast<const u4v*>(p + (long long)r * ld + c);
+    for (int i = 0; i < CNT; ++i) off[i] = (unsigned)(row(i) * (int)ld + col(i)) * (unsigned)sizeof(T);
+  }
+  __device__ __forceinline__ static bool has() { return ALL % NT == 0 || (int)threadIdx.x < ALL; }
+  __device__ __forceinline__ static u4v get(const char* q, unsigned o) {
+    asm volatile("" : "+v"(o));  // 32 bits beside a scalar base: not widened ahead of the loop
+    return *reinterpret_cast<const u4v*>(q + o);
+  }
+  // rows from `p` on, `rows` of them; zeros elsewhere
+  __device__ __forceinline__ void load(const T* __restrict__ p, int rows) {
+    const char* q = reinterpret_cast<const char*>(p);
+    if (rows == ROWS && cols == COLS && ALL % NT == 0) {
+#pragma unroll
+      for (int i = 0; i < CNT; ++i) v[i] = get(q, off[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < CNT; ++i) {
+        v[i] = u4v{0, 0, 0, 0};
+        if (has() && col(i) < cols && row(i) < rows) v[i] = get(q, off[i]);
+      }
     }
   }
+  // the loads are done
+  __device__ __forceinline__ void settle() {
+#pragma unroll
+    for (int i = 0; i < CNT; ++i) asm volatile("" : "+v"(v[i]));
+  }
   template <int PL> __device__ __forceinline__ void store(Planes<PL, ROWS, COLS>& m) const {
+    if (!has()) return;
 #pragma unroll
     for (int i = 0; i < CNT; ++i) {
-      const int id = i * NT + threadIdx.x, r = id / PER, c = (id - r * PER) * VE;
+      const int r = row(i), c = col(i);
       if constexpr (sizeof(T) == 4) {
-        const f4 x = __builtin_bit_cast(f4, v[i]);
         bf4 o[PL];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          __bf16 s[PL];
-          split1<PL>(x[e], s);
-#pragma unroll
-          for (int q = 0; q < PL; ++q) o[q][e] = s[q];
-        }
+        split4<PL>(__builtin_bit_cast(f4, v[i]), o);
 #pragma unroll
         for (int q = 0; q < PL; ++q) *reinterpret_cast<bf4*>(&m.d[q][r][c]) = o[q];
       } else if constexpr (PL == 1) {
         *reinterpret_cast<u4v*>(&m.d[0][r][c]) = v[i];
       } else {
         const h8 x = __builtin_bit_cast(h8, v[i]);
-        float f[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = (float)x[e];
-        const Op<PL> o = split8<PL>(f);
+        const Op<PL> o = split8<PL>(f4{(float)x[0], (float)x[1], (float)x[2], (float)x[3]},
+                                    f4{(float)x[4], (float)x[5], (float)x[6], (float)x[7]});
 #pragma unroll
         for (int q = 0; q < PL; ++q) *reinterpret_cast<bf8*>(&m.d[q][r][c]) = o.v[q];
       }
@@ -243,9 +287,10 @@ __device__ __forceinline__ double lane_value(double v, int l) {
 
 // d_t, the running sum c_t of log2(e) d_t A over the chunk in two floats, and its
 // factors from the chunk's start, 2^c_t, and to its end, 2^(c_Q - c_t)
-template <int Q> struct Decays {
+template <int Q, bool WALK = false> struct Decays {
   float hi[Q], lo[Q], d[Q];
   float head[Q], tail[Q];
+  float in[WALK ? Q : 4];  // d_t 2^(c_Q - c_t): what token t adds to the state
   float end;  // 2^c_Q
   float total;  // c_Q
   // one wave, lane t (< Q) with token t's d
@@ -259,7 +304,9 @@ template <int Q> struct Decays {
       lo[l] = (float)(c - (double)h);
       d[l] = dt;
       head[l] = __builtin_amdgcn_exp2f(h);
-      tail[l] = __builtin_amdgcn_exp2f((float)(last - c));
+      const float t = __builtin_amdgcn_exp2f((float)(last - c));
+      tail[l] = t;
+      if (WALK) in[l] = t * dt;
     }
     if (l == 0) {
       total = (float)last;
@@ -270,14 +317,16 @@ template <int Q> struct Decays {
 };
 // log(1 + e^v), v itself from 20 on (within 2e-9 of it)
 __device__ __forceinline__ float softplus_f(float v) { return v > 20.f ? v : log1pf(expf(v)); }
-template <typename T> __device__ __forceinline__ float load_dt(const ScanParams& p, long long row, int h) {
+// a step's bits as they are in memory: nothing waits for them until they are decoded
+template <typename T> __device__ __forceinline__ unsigned dt_bits(const ScanParams& p, long long row, int h) {
   const long long o = row * p.lddt + h;
-  const float v = p.dt_f32 ? static_cast<const float*>(p.dt)[o] : (float)static_cast<const T*>(p.dt)[o];
-  return p.dt_bias != nullptr ? v + p.dt_bias[h] : v;
+  return sizeof(T) == 4 || p.dt_f32 ? static_cast<const unsigned*>(p.dt)[o] : static_cast<const unsigned short*>(p.dt)[o];
 }
-template <typename T> __device__ __forceinline__ float token_step(const ScanParams& p, long long row, int h) {
-  const float v = load_dt<T>(p, row, h);
-  return p.softplus ? softplus_f(v) : v;
+template <typename T> __device__ __forceinline__ float dt_value(const ScanParams& p, unsigned u, float bias) {
+  if constexpr (sizeof(T) == 4)
+    return __builtin_bit_cast(float, u) + bias;
+  else
+    return (p.dt_f32 ? __builtin_bit_cast(float, u) : (float)__builtin_bit_cast(T, (unsigned short)u)) + bias;
 }
 
 // ---------------------------------------------------------------- the state in registers
@@ -314,10 +363,7 @@ template <int NP> struct StateTiles {
       for (int e = 0; e < 4; ++e) s[(col(i >> 1) + 4 * (i & 1) + e) * P + 16 * w + (l & 15)] = t[i][e];
   }
   template <int PL> __device__ __forceinline__ Op<PL> op(int c) const {
-    float x[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = t[2 * c + (e >> 2)][e & 3];
-    return split8<PL>(x);
+    return split8<PL>(t[2 * c], t[2 * c + 1]);
   }
 };
 // the tiles (ib, jb), jb <= ib, of a lower triangle of blocks, row by row

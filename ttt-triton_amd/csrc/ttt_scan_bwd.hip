@@ -25,18 +25,26 @@ namespace ttt {
 
 namespace {
 
+// waves for 16 features: two in fp32, whose chunks of 32 tokens give one little to do
+// (measured at 16,384 tokens, 4 heads of 32, N 32: 27 us with one, 20 with two; bf16 at 32,768
+// tokens, 12 heads of 64, N 64 the other way round: 106 and 127)
+template <typename T> constexpr int kRoles = ScanType<T>::IN == 3 ? 2 : 1;
+
 template <typename T, int P, int NP> struct BwdShared {
   static constexpr int IN = ScanType<T>::IN, MID = ScanType<T>::MID, Q = chunk_of<T, NP>(), TB = Q / 16;
   static constexpr int W = P / 16, TILES = TB * (TB + 1) / 2, NB = NP / 16;
   Planes<IN, Q, P> x, dy;
   Planes<IN, Q, NP> b, c;
   bf4 wv[MID][TILES][64];  // W, tile rows i, columns j
-  Decays<Q> dec;
-  float row[TILES][16], col[TILES][16];  // sums of W (C . B), and of its d_j-th part, off the diagonal
-  float cross[Q];                        // what crosses t inside its own block
-  float diag[Q];                         // F (x . dy) (C . B) on the diagonal
-  float u[NB][Q], v[NB][Q];              // shares of u_i and of v_j / d_j by 16 columns
-  float dD[W], gh[W];
+  Decays<Q> dec[3];        // of the head before, this one and the next
+  // What is left of a head for the gradient of its steps: of W (C . B) by tiles the sums of
+  // the columns, before d_j, and of the rows (of a block that meets itself what crosses its
+  // tokens), and shares of u_i and of v_j / d_j by 16 columns
+  struct Head {
+    float row[TILES][16], col[TILES][16];
+    float u[NB][Q], v[NB][Q];
+    float dD[W * kRoles<T>], gh[W];
+  } head[2];
 };
 
 // Columns n = 16 nb + r of a state [NP][P] in memory, all P values of them: lane (g, r)
@@ -52,10 +60,7 @@ template <int P> struct StateColumns {
       for (int o = 0; o < 2; ++o) v[k][o] = *reinterpret_cast<const f4*>(s + (16 * nb + r) * P + 32 * k + 8 * g + 4 * o);
   }
   __device__ __forceinline__ Op<kFull> op(int k) const {
-    float x[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = v[k][e >> 2][e & 3];
-    return split8<kFull>(x);
+    return split8<kFull>(v[k][0], v[k][1]);
   }
   __device__ __forceinline__ float dot(const StateColumns& o) const {
     f4 s = f4{0.f, 0.f, 0.f, 0.f};
@@ -92,19 +97,85 @@ template <typename T> __device__ __forceinline__ void put_dt(const ScanParams& p
     static_cast<T*>(p.ddt)[o] = (T)v;
 }
 
+// A head's steps, from its sums in LDS, by one wave (lane t with token t): the gradients
+// of dt, and the chunk's part of those of A, D and dt_bias
 template <typename T, int P, int NP>
-__global__ __launch_bounds__(4 * P) void scan_bwd_kernel(ScanParams p) {
+__device__ __forceinline__ void steps_grad(const ScanParams& p, const BwdShared<T, P, NP>& sh, unsigned bits, int h,
+                                           long long row0, int left, long long chunk) {
   using Sh = BwdShared<T, P, NP>;
-  constexpr int IN = Sh::IN, MID = Sh::MID, Q = Sh::Q, TB = Sh::TB, W = Sh::W, NB = Sh::NB, NT = 4 * P, NC2 = NP / 32;
-  constexpr int TILES = Sh::TILES, OWN = (TILES + W - 1) / W;
-  // A wave's part of dB and dC: with as many blocks of 16 columns as waves, or more, all
-  // tokens of its blocks; else one block and every SHARE-th 16 tokens
+  constexpr int Q = Sh::Q, TB = Sh::TB, NB = Sh::NB, W = Sh::W;
+  const typename Sh::Head& s = sh.head[h & 1];
+  const Decays<Q>& dec = sh.dec[h % 3];
+  const int l = lane_id();
+  const bool in = l < Q;
+  const int t = in ? l : 0, tb = t >> 4, tr = t & 15;
+  float u = 0.f, v = 0.f, dir = 0.f, gh = 0.f, dsum = 0.f, before = 0.f, past = 0.f, over = 0.f;
+  if (in) {
+    for (int k = tb + 1; k < TB; ++k) before += s.col[tri(k, tb)][tr];
+#pragma unroll
+    for (int k = 0; k < NB; ++k) {
+      u += s.u[k][t];
+      v += s.v[k][t];
+    }
+    past = s.row[tri(tb, tb)][tr];
+    dir = (s.col[tri(tb, tb)][tr] + before) + v;
+  }
+#pragma unroll
+  for (int k = 0; k < W; ++k) {
+    if (k < NB) gh += s.gh[k];  // (waves that share a block of columns count it once)
+  }
+#pragma unroll
+  for (int k = 0; k < W * kRoles<T>; ++k) dsum += s.dD[k];
+  // rows from t on of the blocks left of t's, and whole blocks left of and below it
+  const float d = in ? dec.d[t] : 0.f;
+#pragma unroll
+  for (int jb = 0; jb + 1 < TB; ++jb) {
+    float rows = in && jb < tb ? s.row[tri(tb, jb)][tr] : 0.f;
+    rows = row_from(rows);  // the row's lanes from this one on
+    past += rows;
+#pragma unroll
+    for (int ib = jb + 2; ib < TB; ++ib) {
+      const float all = lane_read(rows, 16 * ib);
+      if (tb > jb && tb < ib) over += all;
+    }
+  }
+  before *= d;
+  past += row_upto(dpp0<0x111>(before)) + over;
+  v *= d;
+  const double run = lane_sums(u), all = lane_value(run, 63);
+  const float da = past + (float)(all - run + (double)u) + (float)(lane_sums(v) - (double)v) + dec.end * gh;
+  float dr = 0.f;
+  if (in && t < left) {
+    const float raw = dt_value<T>(p, bits, p.dt_bias != nullptr ? p.dt_bias[h] : 0.f);
+    dr = (dir + p.A[h] * da) * (p.softplus ? sigmoid_f(raw) : 1.0f);
+    put_dt<T>(p, (row0 + t) * p.H + h, dr);
+  }
+  const float sa = sum_wave(in && t < left ? d * da : 0.f), sr = sum_wave(dr);
+  if (l == 0) {
+    const long long n = (long long)p.B * ((p.L + Q - 1) / Q), o = (long long)h * n + chunk;
+    p.partial[o] = sa;
+    p.partial[(long long)p.H * n + o] = dsum;
+    p.partial[2LL * p.H * n + o] = sr;
+  }
+}
+
+// A wave for every 16 features has dB and dC of its columns; with ROLES = 2 there are two,
+// the first P/16 waves with dB and the others with dC
+template <typename T, int P, int NP, int ROLES>
+__global__ __launch_bounds__(4 * P * ROLES) void scan_bwd_kernel(ScanParams p) {
+  using Sh = BwdShared<T, P, NP>;
+  constexpr int IN = Sh::IN, MID = Sh::MID, Q = Sh::Q, TB = Sh::TB, W = Sh::W, NB = Sh::NB, NC2 = NP / 32;
+  constexpr int WAVES = W * ROLES, NT = 64 * WAVES, BOTH = 3 - ROLES;
+  constexpr int TILES = Sh::TILES, OWN = (TILES + WAVES - 1) / WAVES;
+  // A wave's part of dB or dC: with as many blocks of 16 columns as waves for it, or more,
+  // all tokens of its blocks; else one block and every SHARE-th 16 tokens
   constexpr int COLS = NB >= W ? NB / W : 1, SHARE = NB >= W ? 1 : W / NB, TOK = TB / SHARE;
   static_assert(COLS * W * TOK == NB * TB, "whole shares");
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   Sh& sh = *reinterpret_cast<Sh*>(smem);
   const int w = wave_id(), l = lane_id(), g = l >> 4, r = l & 15;
-  const int nb0 = w % NB, tb0 = w / NB;  // (tb0 = 0 with NB >= W)
+  const int wr = ROLES == 2 && w >= W ? w - W : w, nb0 = SHARE == 1 ? wr : wr % NB, tb0 = SHARE == 1 ? 0 : wr / NB;
+  const bool hasB = w < W, hasC = ROLES == 1 || !hasB;
   const int NC = (p.L + Q - 1) / Q, HG = p.H / p.G, per = (HG + p.splits - 1) / p.splits;
   int id = blockIdx.x;
   const int split = id % p.splits;
@@ -112,63 +183,106 @@ __global__ __launch_bounds__(4 * P) void scan_bwd_kernel(ScanParams p) {
   const int grp = id % p.G;
   id /= p.G;
   const int c = id % NC, b = id / NC;
-  const int t0 = c * Q, left = p.L - t0;
-  const long long row0 = (long long)b * p.L + t0;
+  const int t0 = c * Q, left = min(Q, p.L - t0);
+  const long long row0 = (long long)b * p.L + t0, chunk = (long long)b * NC + c;
   const int h0 = grp * HG + split * per, h1 = min(grp * HG + HG, h0 + per);
 
   Stage<T, Q, P, NT> sx, sdy;
-  StateColumns<P> gam[COLS], hin[COLS];
-  float dt = 0.f;
-  const auto fetch = [&](int h) {
-    sx.load(static_cast<const T*>(p.x) + row0 * p.ldx + h * P, p.ldx, left, P);
-    sdy.load(static_cast<const T*>(p.dy) + row0 * p.ldy + h * P, p.ldy, left, P);
-    const long long st = (((long long)b * p.H + h) * NC + c) * (long long)(P * NP);
-#pragma unroll
-    for (int q = 0; q < COLS; ++q) {
-      gam[q].load(p.gstates + st, nb0 + W * q);
-      hin[q].load(p.states + st, nb0 + W * q);
-    }
-    if (w == 0) dt = l < Q && l < left ? load_dt<T>(p, row0 + l, h) : 0.f;
+  StateColumns<P> st[BOTH][COLS];  // Gam and H, or the role's
+  sx.place(p.ldx, P);
+  sdy.place(p.ldy, P);
+  const T* xp = static_cast<const T*>(p.x) + row0 * p.ldx;
+  const T* dyp = static_cast<const T*>(p.dy) + row0 * p.ldy;
+  const auto tokens = [&](int h) {
+    sx.load(xp + h * P, left);
+    sdy.load(dyp + h * P, left);
   };
-  {
+  const auto state_of = [&](int h) { return (((long long)b * p.H + h) * NC + c) * (long long)(P * NP); };
+  const auto states = [&](int h, int which) {
+#pragma unroll
+    for (int q = 0; q < COLS; ++q)
+      st[BOTH == 1 ? 0 : which][q].load((which == 0 ? p.gstates : p.states) + state_of(h), nb0 + W * q);
+  };
+  // Steps are read two heads ahead and decays formed one ahead, while the tiles are; the
+  // wave that forms them and the one that finishes the head before have the fewest tiles
+  const bool fills = w == WAVES - 2, ends = w == WAVES - 1;
+  const auto bits_of = [&](int h) {
+    return (fills || ends) && h < h1 && l < left ? dt_bits<T>(p, row0 + l, h) : 0u;
+  };
+  const auto decays = [&](int h, unsigned bits) {
+    const float raw = dt_value<T>(p, bits, p.dt_bias != nullptr ? p.dt_bias[h] : 0.f);
+    sh.dec[h % 3].fill(l < left ? (p.softplus ? softplus_f(raw) : raw) : 0.f, p.A[h]);
+  };
+  unsigned bits0 = 0, bits1 = 0, bits2 = 0;  // of the head before, this one and the next
+  if (h0 < h1) {
+    bits1 = bits_of(h0);
+    bits2 = bits_of(h0 + 1);
     Stage<T, Q, NP, NT> sb, sc;
-    sb.load(static_cast<const T*>(p.Bm) + row0 * p.ldb + grp * p.N, p.ldb, left, p.N);
-    sc.load(static_cast<const T*>(p.Cm) + row0 * p.ldc + grp * p.N, p.ldc, left, p.N);
-    if (h0 < h1) fetch(h0);
+    sb.place(p.ldb, p.N);
+    sc.place(p.ldc, p.N);
+    sb.load(static_cast<const T*>(p.Bm) + row0 * p.ldb + grp * p.N, left);
+    sc.load(static_cast<const T*>(p.Cm) + row0 * p.ldc + grp * p.N, left);
+    tokens(h0);
+    if (hasB) states(h0, 0);
+    if (hasC) states(h0, 1);
     sb.store(sh.b);
     sc.store(sh.c);
+    if (fills) decays(h0, bits1);
   }
   __syncthreads();
   f4 cb[OWN];  // C_i . B_j, rows i
 #pragma unroll
   for (int k = 0; k < OWN; ++k) {
-    const int t = w + W * k, ib = tri_row(t), jb = t - tri(ib, 0);
+    const int t = w + WAVES * k, ib = tri_row(t), jb = t - tri(ib, 0);
     cb[k] = f4{0.f, 0.f, 0.f, 0.f};
     if (t < TILES) {
 #pragma unroll
       for (int q = 0; q < NC2; ++q) mma<kFull>(cb[k], sh.c.rows(16 * ib, 32 * q), sh.b.rows(16 * jb, 32 * q));
     }
   }
-  f4 dB[COLS][TOK], dC[COLS][TOK];
+  f4 sum[BOTH][COLS][TOK];  // dB and dC, or the role's
 #pragma unroll
-  for (int q = 0; q < COLS; ++q)
+  for (int z = 0; z < BOTH; ++z)
 #pragma unroll
-    for (int s = 0; s < TOK; ++s) dB[q][s] = dC[q][s] = f4{0.f, 0.f, 0.f, 0.f};
+    for (int q = 0; q < COLS; ++q)
+#pragma unroll
+      for (int s = 0; s < TOK; ++s) sum[z][q][s] = f4{0.f, 0.f, 0.f, 0.f};
   const bf4 zero = {(__bf16)0.f, (__bf16)0.f, (__bf16)0.f, (__bf16)0.f};
 
   for (int h = h0; h < h1; ++h) {
-    const float A = p.A[h];
+    typename Sh::Head& hd = sh.head[h & 1];
+    const Decays<Q>& dec = sh.dec[h % 3];
     sx.store(sh.x);
     sdy.store(sh.dy);
-    const float raw = dt;
-    if (w == 0) sh.dec.fill(l < Q && l < left ? (p.softplus ? softplus_f(raw) : raw) : 0.f, A);
     __syncthreads();
-    const Decays<Q>& dec = sh.dec;
+    if (h + 1 < h1) {
+      if (fills) decays(h + 1, bits2);
+      tokens(h + 1);
+    }
+    if (ends && h > h0) steps_grad<T, P, NP>(p, sh, bits0, h - 1, row0, left, chunk);
+    bits0 = bits1;
+    bits1 = bits2;
+    bits2 = bits_of(h + 2);
+    if (hasC && tb0 == 0) {  // <Gam, H>
+      float s = 0.f;
+#pragma unroll
+      for (int q = 0; q < COLS; ++q) {
+        if constexpr (BOTH == 2) {
+          s += st[0][q].dot(st[1][q]);
+        } else {
+          StateColumns<P> gam;
+          gam.load(p.gstates + state_of(h), nb0 + W * q);
+          s += gam.dot(st[0][q]);
+        }
+      }
+      s = sum_wave(s);
+      if (l == 0) hd.gh[wr] = s;
+    }
 
     float dd = 0.f;
 #pragma unroll
     for (int k = 0; k < OWN; ++k) {
-      const int t = w + W * k, ib = tri_row(t), jb = t - tri(ib, 0);
+      const int t = w + WAVES * k, ib = tri_row(t), jb = t - tri(ib, 0);
       if (t < TILES) {
         f4 xy = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -176,27 +290,23 @@ __global__ __launch_bounds__(4 * P) void scan_bwd_kernel(ScanParams p) {
         const int j = 16 * jb + r, i0 = 16 * ib + 4 * g;
         const float jh = dec.hi[j], jl = dec.lo[j], d = dec.d[j];
         const f4 ih = dec.four(dec.hi, i0), il = dec.four(dec.lo, i0);
-        f4 pass;
-        bf4 ow[MID];
+        f4 wv;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int i = i0 + e;
-          const float f = __builtin_amdgcn_exp2f((ih[e] - jh) + (il[e] - jl));
-          const float wv = i >= j ? f * xy[e] : 0.f, pv = wv * cb[k][e];
-          pass[e] = i > j ? pv : 0.f;
-          if (i == j) {
-            dd += xy[e];
-            sh.diag[j] = pv;
+        for (int e = 0; e < 4; ++e) wv[e] = __builtin_amdgcn_exp2f((ih[e] - jh) + (il[e] - jl)) * xy[e];
+        if (ib == jb) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            wv[e] = only_if(4 * g + e >= r, wv[e]);
+            if (4 * g + e == r) dd += xy[e];
           }
-          __bf16 q[MID];
-          split1<MID>(wv * d, q);
-#pragma unroll
-          for (int a = 0; a < MID; ++a) ow[a][e] = q[a];
         }
+        f4 pass = wv * cb[k];
+        bf4 ow[MID];
+        split4<MID>(wv * d, ow);
 #pragma unroll
         for (int a = 0; a < MID; ++a) sh.wv[a][t][l] = ow[a];
         const float cs = sum_col4((pass[0] + pass[1]) + (pass[2] + pass[3]));
-        if (g == 0) sh.col[t][r] = cs;
+        if (g == 0) hd.col[t][r] = cs;
         pass *= d;
         if (ib == jb) {  // from row 4g + e on, by columns, then the columns before it
           pass[2] += pass[3];
@@ -204,169 +314,120 @@ __global__ __launch_bounds__(4 * P) void scan_bwd_kernel(ScanParams p) {
           pass[0] += pass[1];
           const float b1 = __shfl_down(pass[0], 16), b2 = __shfl_down(pass[0], 32), b3 = __shfl_down(pass[0], 48);
           pass += (g < 3 ? b1 : 0.f) + (g < 2 ? b2 : 0.f) + (g < 1 ? b3 : 0.f);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) pass[e] = r < 4 * g + e ? pass[e] : 0.f;
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float rs = sum_row16(ib != jb || r < 4 * g + e ? pass[e] : 0.f);
-          if (r == 0) (ib == jb ? sh.cross + 16 * ib : sh.row[t])[4 * g + e] = rs;
-        }
+        for (int e = 0; e < 4; ++e) pass[e] = sum_row16(pass[e]);
+        if (r == 0) *reinterpret_cast<f4*>(&hd.row[t][4 * g]) = pass;
       }
     }
     dd = sum_wave(dd);
-    if (l == 0) sh.dD[w] = dd;
-    {  // (a block of columns that several waves share counts once)
-      float s = 0.f;
-#pragma unroll
-      for (int q = 0; q < COLS; ++q) s += gam[q].dot(hin[q]);
-      s = sum_wave(s);
-      if (l == 0) sh.gh[w] = tb0 == 0 ? s : 0.f;
-    }
+    if (l == 0) hd.dD[w] = dd;
     __syncthreads();
 
-    // dB: rows are columns n of B, columns tokens j
+    if (hasB) {  // rows are columns n of B, columns tokens j
+      Op<kFull> s[COLS][P / 32];
 #pragma unroll
-    for (int q = 0; q < COLS; ++q) {
-      const int n0 = 16 * (nb0 + W * q);
-      Op<kFull> s[P / 32];
+      for (int q = 0; q < COLS; ++q)
 #pragma unroll
-      for (int k = 0; k < P / 32; ++k) s[k] = gam[q].op(k);
-      Op<IN> ct[Q / 32];
+        for (int k = 0; k < P / 32; ++k) s[q][k] = st[0][q].op(k);
+      if (h + 1 < h1) states(h + 1, 0);
 #pragma unroll
-      for (int k = 0; k < Q / 32; ++k) ct[k] = sh.c.template cols<>(32 * k, n0);
+      for (int q = 0; q < COLS; ++q) {
+        const int n0 = 16 * (nb0 + W * q);
+        Op<IN> ct[Q / 32];
 #pragma unroll
-      for (int o = 0; o < TOK; ++o) {
-        const int jb = SHARE * o + tb0, j = 16 * jb + r;
-        f4 acc = f4{0.f, 0.f, 0.f, 0.f};
+        for (int k = 0; k < Q / 32; ++k) ct[k] = sh.c.template cols<>(32 * k, n0);
 #pragma unroll
-        for (int k = 0; k < P / 32; ++k) mma<kFull>(acc, s[k], sh.x.rows(16 * jb, 32 * k));
-        acc *= dec.tail[j];
-        const f4 vv = acc * sh.b.quad(j, n0 + 4 * g);
-        const float sv = sum_col4((vv[0] + vv[1]) + (vv[2] + vv[3]));
-        if (g == 0) sh.v[nb0 + W * q][j] = sv;
-        dB[q][o] += acc * dec.d[j];
+        for (int o = 0; o < TOK; ++o) {
+          const int jb = SHARE * o + tb0, j = 16 * jb + r;
+          f4 acc = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int k = 0; k < Q / 32; ++k) {
-          if (2 * k + 1 < jb) continue;
-          const bool one = 2 * k >= jb;
-          Op<MID> m;
+          for (int k = 0; k < P / 32; ++k) mma<kFull>(acc, s[q][k], sh.x.rows(16 * jb, 32 * k));
+          acc *= dec.tail[j];
+          const f4 vv = acc * sh.b.quad(j, n0 + 4 * g);
+          const float sv = sum_col4((vv[0] + vv[1]) + (vv[2] + vv[3]));
+          if (g == 0) hd.v[nb0 + W * q][j] = sv;
+          sum[0][q][o] += acc * dec.d[j];
 #pragma unroll
-          for (int a = 0; a < MID; ++a)
-            m.v[a] = cat(one ? sh.wv[a][one ? tri(2 * k, jb) : 0][l] : zero, sh.wv[a][tri(2 * k + 1, jb)][l]);
-          mma<MID>(dB[q][o], ct[k], m);
-        }
-      }
-    }
-    // dC: rows are columns n of C, columns tokens i
+          for (int k = 0; k < Q / 32; ++k) {
+            if (2 * k + 1 < jb) continue;
+            const bool one = 2 * k >= jb;
+            Op<MID> m;
 #pragma unroll
-    for (int q = 0; q < COLS; ++q) {
-      const int n0 = 16 * (nb0 + W * q);
-      Op<kFull> s[P / 32];
-#pragma unroll
-      for (int k = 0; k < P / 32; ++k) s[k] = hin[q].op(k);
-      Op<IN> bt[Q / 32];
-#pragma unroll
-      for (int k = 0; k < Q / 32; ++k) bt[k] = sh.b.template cols<>(32 * k, n0);
-#pragma unroll
-      for (int o = 0; o < TOK; ++o) {
-        const int ib = SHARE * o + tb0, i = 16 * ib + r;
-        f4 acc = f4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int k = 0; k < P / 32; ++k) mma<kFull>(acc, s[k], sh.dy.rows(16 * ib, 32 * k));
-        acc *= dec.head[i];
-        const f4 uu = acc * sh.c.quad(i, n0 + 4 * g);
-        const float su = sum_col4((uu[0] + uu[1]) + (uu[2] + uu[3]));
-        if (g == 0) sh.u[nb0 + W * q][i] = su;
-        dC[q][o] += acc;
-        // W as an operand with free i and contraction j: the transposing read of its tiles,
-        // whose lane 16 a + j holds rows 4a..4a+3 of column j
-        const int slot = 16 * (l & 3) + 4 * g + (r >> 2);
-#pragma unroll
-        for (int k = 0; k < Q / 32; ++k) {
-          if (2 * k > ib) continue;
-          const bool two = 2 * k + 1 <= ib;
-          Op<MID> m;
-#pragma unroll
-          for (int a = 0; a < MID; ++a) {
-            const bf4 lo = read_tr(reinterpret_cast<const __bf16*>(&sh.wv[a][tri(ib, 2 * k)][slot]));
-            const bf4 hi = read_tr(reinterpret_cast<const __bf16*>(&sh.wv[a][two ? tri(ib, 2 * k + 1) : 0][slot]));
-            m.v[a] = cat(lo, two ? hi : zero);
+            for (int a = 0; a < MID; ++a)
+              m.v[a] = cat(one ? sh.wv[a][one ? tri(2 * k, jb) : 0][l] : zero, sh.wv[a][tri(2 * k + 1, jb)][l]);
+            mma<MID>(sum[0][q][o], ct[k], m);
           }
-          mma<MID>(dC[q][o], bt[k], m);
         }
       }
     }
-    if (h + 1 < h1) fetch(h + 1);
+    if (hasC) {  // rows are columns n of C, columns tokens i
+      constexpr int Z = BOTH - 1;
+      Op<kFull> s[COLS][P / 32];
+#pragma unroll
+      for (int q = 0; q < COLS; ++q)
+#pragma unroll
+        for (int k = 0; k < P / 32; ++k) s[q][k] = st[Z][q].op(k);
+      if (h + 1 < h1) states(h + 1, 1);
+#pragma unroll
+      for (int q = 0; q < COLS; ++q) {
+        const int n0 = 16 * (nb0 + W * q);
+        Op<IN> bt[Q / 32];
+#pragma unroll
+        for (int k = 0; k < Q / 32; ++k) bt[k] = sh.b.template cols<>(32 * k, n0);
+#pragma unroll
+        for (int o = 0; o < TOK; ++o) {
+          const int ib = SHARE * o + tb0, i = 16 * ib + r;
+          f4 acc = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int k = 0; k < P / 32; ++k) mma<kFull>(acc, s[q][k], sh.dy.rows(16 * ib, 32 * k));
+          acc *= dec.head[i];
+          const f4 uu = acc * sh.c.quad(i, n0 + 4 * g);
+          const float su = sum_col4((uu[0] + uu[1]) + (uu[2] + uu[3]));
+          if (g == 0) hd.u[nb0 + W * q][i] = su;
+          sum[Z][q][o] += acc;
+          // W as an operand with free i and contraction j: the transposing read of its tiles,
+          // whose lane 16 a + j holds rows 4a..4a+3 of column j
+          const int slot = 16 * (l & 3) + 4 * g + (r >> 2);
+#pragma unroll
+          for (int k = 0; k < Q / 32; ++k) {
+            if (2 * k > ib) continue;
+            const bool two = 2 * k + 1 <= ib;
+            Op<MID> m;
+#pragma unroll
+            for (int a = 0; a < MID; ++a) {
+              const bf4 lo = read_tr(reinterpret_cast<const __bf16*>(&sh.wv[a][tri(ib, 2 * k)][slot]));
+              const bf4 hi = read_tr(reinterpret_cast<const __bf16*>(&sh.wv[a][two ? tri(ib, 2 * k + 1) : 0][slot]));
+              m.v[a] = cat(lo, two ? hi : zero);
+            }
+            mma<MID>(sum[Z][q][o], bt[k], m);
+          }
+        }
+      }
+    }
     __syncthreads();
-    if (w == 0) {
-      const bool in = l < Q;
-      const int t = in ? l : 0, tb = t >> 4, tr = t & 15;
-      float u = 0.f, v = 0.f, dir = 0.f, gh = 0.f, dsum = 0.f, before = 0.f, past = 0.f, over = 0.f;
-      if (in) {
-        for (int k = tb + 1; k < TB; ++k) before += sh.col[tri(k, tb)][tr];
-#pragma unroll
-        for (int k = 0; k < NB; ++k) {
-          u += sh.u[k][t];
-          v += sh.v[k][t];
-        }
-        past = sh.cross[t];
-        dir = ((sh.diag[t] + sh.col[tri(tb, tb)][tr]) + before) + v;
-      }
-#pragma unroll
-      for (int k = 0; k < W; ++k) {
-        gh += sh.gh[k];
-        dsum += sh.dD[k];
-      }
-      // rows from t on of the blocks left of t's, and whole blocks left of and below it
-      const float d = in ? dec.d[t] : 0.f;
-#pragma unroll
-      for (int jb = 0; jb + 1 < TB; ++jb) {
-        float rows = in && jb < tb ? sh.row[tri(tb, jb)][tr] : 0.f;
-        rows = row_from(rows);  // the row's lanes from this one on
-        past += rows;
-#pragma unroll
-        for (int ib = jb + 2; ib < TB; ++ib) {
-          const float all = lane_read(rows, 16 * ib);
-          if (tb > jb && tb < ib) over += all;
-        }
-      }
-      before *= d;
-      past += row_upto(dpp0<0x111>(before)) + over;
-      v *= d;
-      const double run = lane_sums(u), all = lane_value(run, 63);
-      const float da = past + (float)(all - run + (double)u) + (float)(lane_sums(v) - (double)v) + dec.end * gh;
-      float dr = 0.f;
-      if (in && t < left) {
-        dr = (dir + A * da) * (p.softplus ? sigmoid_f(raw) : 1.0f);
-        put_dt<T>(p, (row0 + t) * p.H + h, dr);
-      }
-      const float sa = sum_wave(in && t < left ? d * da : 0.f), sr = sum_wave(dr);
-      if (l == 0) {
-        const long long n = (long long)p.B * NC, o = (long long)h * n + (long long)b * NC + c;
-        p.partial[o] = sa;
-        p.partial[(long long)p.H * n + o] = dsum;
-        p.partial[2LL * p.H * n + o] = sr;
-      }
-    }
-    if (h + 1 < h1) __syncthreads();
   }
+  if (ends && h0 < h1) steps_grad<T, P, NP>(p, sh, bits0, h1 - 1, row0, left, chunk);
 
 #pragma unroll
-  for (int q = 0; q < COLS; ++q)
+  for (int z = 0; z < BOTH; ++z)
 #pragma unroll
-    for (int s = 0; s < TOK; ++s) {
-      const int n = 16 * (nb0 + W * q) + 4 * g, j = 16 * (SHARE * s + tb0) + r;
-      if (n < p.N && t0 + j < p.L) {
-        const long long o = ((row0 + j) * p.G + grp) * p.N + n;
-        if (p.dBp != nullptr) {
-          const long long all = (long long)p.B * p.L * p.G * p.N;
-          *reinterpret_cast<f4*>(p.dBp + split * all + o) = dB[q][s];
-          *reinterpret_cast<f4*>(p.dCp + split * all + o) = dC[q][s];
-        } else {
-          store4(static_cast<T*>(p.dB) + o, dB[q][s]);
-          store4(static_cast<T*>(p.dC) + o, dC[q][s]);
+    for (int q = 0; q < COLS; ++q)
+#pragma unroll
+      for (int s = 0; s < TOK; ++s) {
+        const int n = 16 * (nb0 + W * q) + 4 * g, j = 16 * (SHARE * s + tb0) + r;
+        const bool ofB = BOTH == 2 ? z == 0 : hasB;
+        if (n < p.N && t0 + j < p.L) {
+          const long long o = ((row0 + j) * p.G + grp) * p.N + n;
+          float* part = ofB ? p.dBp : p.dCp;
+          if (part != nullptr)
+            *reinterpret_cast<f4*>(part + split * ((long long)p.B * p.L * p.G * p.N) + o) = sum[z][q][s];
+          else
+            store4(static_cast<T*>(ofB ? p.dB : p.dC) + o, sum[z][q][s]);
         }
       }
-    }
 }
 
 // dB and dC of a group whose heads were split over workgroups
@@ -402,11 +463,11 @@ template <typename T, int P, int NP> hipError_t bwd_t(const ScanParams& p, hipSt
   constexpr int Q = chunk_of<T, NP>();
   const int NC = (p.L + Q - 1) / Q;
   if (lds > 65536) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(scan_bwd_kernel<T, P, NP>),
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(scan_bwd_kernel<T, P, NP, kRoles<T>>),
                                              hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL((scan_bwd_kernel<T, P, NP>), dim3((unsigned)((long long)p.B * NC * p.G * p.splits)), dim3(4 * P), lds,
+  hipLaunchKernelGGL((scan_bwd_kernel<T, P, NP, kRoles<T>>), dim3((unsigned)((long long)p.B * NC * p.G * p.splits)), dim3(4 * P * kRoles<T>), lds,
                      stream, p);
   if (p.dBp != nullptr) {
     const long long quads = (long long)p.B * p.L * p.G * p.N / 4;
