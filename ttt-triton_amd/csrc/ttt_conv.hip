@@ -7,7 +7,7 @@
 //   dw[c][k] = sum_t dz[t] s[t+k],   dbias = sum_t dz[t]
 // ds[u] is the state's gradient for u < W-1 and that of token u-W+1 behind it.
 //
-// Everything is bound by HBM.  A thread owns 8 channels (16 bytes of a 16-bit
+// Everything is bound by HBM.  A thread owns V channels (kV: 8 bytes of a 16-bit
 // row) and walks a run of tokens with the window in registers, so that a row is
 // read once and W-1 rows again per run; z is formed again in the backward, which
 // costs W multiply-adds instead of a stored row.
@@ -21,14 +21,16 @@ namespace ttt {
 
 namespace {
 
+constexpr int kV = 4;
 constexpr int kRun = 16;     // tokens of a thread's run in the forward
-constexpr int kLanes = 16;   // backward: channel groups (of 8) per workgroup
+constexpr int kLanes = 32;   // backward: channel groups (of V) per workgroup
+constexpr int kSubs = 256 / kLanes;  // and runs
 constexpr int kRunBwd = 32;  // and tokens of a run
 
 // row u of s, n of its channels from c on; zeros outside
 template <typename T>
-__device__ __forceinline__ Raw8<T> seen_row(const ConvParams& p, long long b, int u, int c, int n) {
-  Raw8<T> r;
+__device__ __forceinline__ Raw<T, kV> seen_row(const ConvParams& p, long long b, int u, int c, int n) {
+  Raw<T, kV> r;
   const int W1 = p.W - 1;
   if (u < 0 || u >= p.L + W1) {
     r.zero();
@@ -44,10 +46,10 @@ __device__ __forceinline__ Raw8<T> seen_row(const ConvParams& p, long long b, in
 }
 
 template <int W> struct Taps {
-  float w[8][W], bias[8];
+  float w[kV][W], bias[kV];
   __device__ __forceinline__ void load(const ConvParams& p, int c, int n) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
+    for (int e = 0; e < kV; ++e) {
 #pragma unroll
       for (int k = 0; k < W; ++k) w[e][k] = e < n ? p.w[(long long)(c + e) * W + k] : 0.f;
       bias[e] = e < n && p.bias != nullptr ? p.bias[c + e] : 0.f;
@@ -63,11 +65,11 @@ __global__ __launch_bounds__(256) void conv_fwd_kernel(ConvParams p, int groups,
   const long long br = id / groups;
   const int run = (int)(br % runs);
   const long long b = br / runs;
-  const int c = 8 * cg, n = min(8, p.C - c);
+  const int c = kV * cg, n = min(kV, p.C - c);
   Taps<W> tp;
   tp.load(p, c, n);
   const int u0 = run * kRun, last = p.L + W - 1;
-  Raw8<T> win[W];
+  Raw<T, kV> win[W];
 #pragma unroll
   for (int k = 0; k < W - 1; ++k) win[k + 1] = seen_row<T>(p, b, u0 - (W - 1) + k, c, n);
 #pragma unroll
@@ -78,51 +80,51 @@ __global__ __launch_bounds__(256) void conv_fwd_kernel(ConvParams p, int groups,
       for (int k = 0; k < W - 1; ++k) win[k] = win[k + 1];
       win[W - 1] = seen_row<T>(p, b, u, c, n);
       if (u >= W - 1) {
-        float o[8];
+        float o[kV];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
+        for (int e = 0; e < kV; ++e) {
           float z = tp.bias[e];
 #pragma unroll
           for (int k = 0; k < W; ++k) z = __builtin_fmaf(tp.w[e][k], win[k].f(e), z);
           o[e] = ACT ? z * sigmoid_f(z) : z;
         }
-        store8(static_cast<T*>(p.y) + (b * p.L + (u - W + 1)) * p.C + c, n, o);
+        store_row<T, kV>(static_cast<T*>(p.y) + (b * p.L + (u - W + 1)) * p.C + c, n, o);
       }
       if (u >= p.L && p.last != nullptr)
-        store8(static_cast<T*>(p.last) + (b * (W - 1) + (u - p.L)) * p.C + c, n, win[W - 1]);
+        win[W - 1].store(static_cast<T*>(p.last) + (b * (W - 1) + (u - p.L)) * p.C + c, n);
     }
   }
 }
 
-// A workgroup: kLanes channel groups x 16 runs of kRunBwd tokens, then the next
-// 16 runs of the rows `step` further.  A lane's sums of dw and dbias go over its
+// A workgroup: kLanes channel groups x kSubs runs of kRunBwd tokens, then the next
+// kSubs runs of the rows `step` further.  A lane's sums of dw and dbias go over its
 // runs, then over the runs of its workgroup in a fixed order.
 template <typename T, int W, bool ACT>
 __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvParams p, int groups, int runs, long long jobs) {
   const int lane = threadIdx.x & (kLanes - 1), sub = threadIdx.x / kLanes;
   const int cg = blockIdx.y * kLanes + lane;
   const bool act = cg < groups;
-  const int c = 8 * cg, n = act ? min(8, p.C - c) : 0;
+  const int c = kV * cg, n = act ? min(kV, p.C - c) : 0;
   Taps<W> tp;
   tp.load(p, c, n);
-  float dw[W][8], dbias[8];
+  float dw[W][kV], dbias[kV];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
+  for (int e = 0; e < kV; ++e) {
     dbias[e] = 0.f;
 #pragma unroll
     for (int k = 0; k < W; ++k) dw[k][e] = 0.f;
   }
   const int last = p.L + W - 1;
-  for (long long job = (long long)blockIdx.x * 16 + sub; act && job < jobs; job += (long long)gridDim.x * 16) {
+  for (long long job = (long long)blockIdx.x * kSubs + sub; act && job < jobs; job += (long long)gridDim.x * kSubs) {
     const int run = (int)(job % runs);
     const long long b = job / runs;
     const int u0 = run * kRunBwd;
     // Step m handles token t = u0 - (W-1) + m, in groups of W steps whose rows are
     // loaded a group ahead.  Row s[t + W-1] has place m % W, dz[t] too, so that
     // s[t + k] is at (m + 1 + k) % W and dz[t - k] at (m - k) % W.
-    Raw8<T> win[W], nx[W], ng[W];
-    float dz[W][8];
-    const auto fetch = [&](int m, Raw8<T>& x, Raw8<T>& g) {
+    Raw<T, kV> win[W], nx[W], ng[W];
+    float dz[W][kV];
+    const auto fetch = [&](int m, Raw<T, kV>& x, Raw<T, kV>& g) {
       const int t = u0 - (W - 1) + m;
       x = seen_row<T>(p, b, t + W - 1, c, n);
       if (t >= 0 && t < p.L && p.dy != nullptr)
@@ -134,11 +136,11 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvParams p, int groups,
     for (int k = 0; k < W; ++k) {
       if (k < W - 1) win[(k + 1) % W] = seen_row<T>(p, b, u0 - (W - 1) + k, c, n);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) dz[k][e] = 0.f;
+      for (int e = 0; e < kV; ++e) dz[k][e] = 0.f;
       fetch(k, nx[k], ng[k]);
     }
     for (int m0 = 0; m0 < kRunBwd + W - 1; m0 += W) {
-      Raw8<T> cx[W], cg[W];
+      Raw<T, kV> cx[W], cg[W];
 #pragma unroll
       for (int k = 0; k < W; ++k) {
         cx[k] = nx[k];
@@ -153,7 +155,7 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvParams p, int groups,
         const int m = m0 + q, t = u0 - (W - 1) + m;
         win[q] = cx[q];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
+        for (int e = 0; e < kV; ++e) {
           float d = cg[q].f(e);
           if (ACT) {
             float z = tp.bias[e];
@@ -165,9 +167,9 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvParams p, int groups,
           dz[q][e] = t >= 0 && t < p.L ? d : 0.f;
         }
         if (m < W - 1 || m >= kRunBwd + W - 1 || t >= last) continue;
-        float o[8];
+        float o[kV];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
+        for (int e = 0; e < kV; ++e) {
           dbias[e] += dz[q][e];
           o[e] = 0.f;
 #pragma unroll
@@ -178,52 +180,45 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvParams p, int groups,
           }
         }
         if (t >= p.L && p.dlast != nullptr) {
-          Raw8<T> r;
+          Raw<T, kV> r;
           r.load(static_cast<const T*>(p.dlast) + (b * (W - 1) + (t - p.L)) * p.C + c, n);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) o[e] += r.f(e);
+          for (int e = 0; e < kV; ++e) o[e] += r.f(e);
         }
         if (t >= W - 1)
-          store8(static_cast<T*>(p.dx) + (b * p.L + (t - W + 1)) * p.C + c, n, o);
+          store_row<T, kV>(static_cast<T*>(p.dx) + (b * p.L + (t - W + 1)) * p.C + c, n, o);
         else if (p.dstate != nullptr)
-          store8(static_cast<T*>(p.dstate) + (b * (W - 1) + t) * p.C + c, n, o);
+          store_row<T, kV>(static_cast<T*>(p.dstate) + (b * (W - 1) + t) * p.C + c, n, o);
       }
     }
   }
-  // lanes l, l ^ 16, l ^ 32, l ^ 48 hold the same channels; then the four waves
-  __shared__ float red[4][W + 1][kLanes * 8];
+  // lanes l and l ^ 32 hold the same channels; then the four waves
+  static_assert(kLanes == 32, "half a wave");
+  __shared__ float red[4][W + 1][kLanes * kV];
   const int wave = threadIdx.x >> 6;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
+  for (int e = 0; e < kV; ++e) {
 #pragma unroll
     for (int k = 0; k <= W; ++k) {
-      const float s = sum_col4(k < W ? dw[k < W ? k : 0][e] : dbias[e]);
-      if ((threadIdx.x & 63) < kLanes) red[wave][k][8 * lane + e] = s;
+      const float v = k < W ? dw[k < W ? k : 0][e] : dbias[e], s = v + __shfl_xor(v, 32);
+      if ((threadIdx.x & 63) < kLanes) red[wave][k][kV * lane + e] = s;
     }
   }
   __syncthreads();
-  const int c0 = blockIdx.y * kLanes * 8;
-  for (int i = threadIdx.x; i < (W + 1) * kLanes * 8; i += 256) {
-    const int k = i / (kLanes * 8), j = i - k * kLanes * 8;
+  const int c0 = blockIdx.y * kLanes * kV;
+  for (int i = threadIdx.x; i < (W + 1) * kLanes * kV; i += 256) {
+    const int k = i / (kLanes * kV), j = i - k * kLanes * kV;
     if (c0 + j < p.C)
       p.partial[((long long)blockIdx.x * (W + 1) + k) * p.C + c0 + j] =
           ((red[0][k][j] + red[1][k][j]) + red[2][k][j]) + red[3][k][j];
   }
 }
 
-// dw, dbias: the sum over the workgroups' partial sums, four lanes to a channel and tap
+// dw, dbias: the sum over the workgroups' partial sums, 16 lanes to a channel and tap
 __global__ __launch_bounds__(256) void conv_param_grads_kernel(ConvParams p, int parts) {
-  const int wave = threadIdx.x >> 6, l = threadIdx.x & 63;
-  const long long i = (long long)blockIdx.x * 64 + l;
-  const long long n = (long long)(p.W + 1) * p.C;
-  __shared__ float red[4][64];
-  float s = 0.f;
-  if (i < n)
-    for (int q = wave; q < parts; q += 4) s += p.partial[q * n + i];
-  red[wave][l] = s;
-  __syncthreads();
-  if (wave == 0 && i < n) {
-    s = ((red[0][l] + red[1][l]) + red[2][l]) + red[3][l];
+  const long long n = (long long)(p.W + 1) * p.C, i = (long long)blockIdx.x * 16 + (threadIdx.x & 15);
+  const float s = sum_parts(p.partial, n, i, parts);
+  if (threadIdx.x < 16 && i < n) {
     const int k = (int)(i / p.C);
     const long long c = i - (long long)k * p.C;
     if (k < p.W)
@@ -239,45 +234,45 @@ __global__ __launch_bounds__(256) void conv_step_kernel(ConvParams p, int groups
   const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
   if (id >= threads) return;
   const long long b = id / groups;
-  const int c = 8 * (int)(id % groups), n = min(8, p.C - c);
+  const int c = kV * (int)(id % groups), n = min(kV, p.C - c);
   T* st = static_cast<T*>(p.last) + b * (W - 1) * p.C + c;
-  Raw8<T> win[W];
+  Raw<T, kV> win[W];
 #pragma unroll
   for (int k = 0; k < W - 1; ++k) win[k].load(st + (long long)k * p.C, n);
   win[W - 1].load(static_cast<const T*>(p.x) + b * p.ldx + c, n);
   Taps<W> tp;
   tp.load(p, c, n);
-  float o[8];
+  float o[kV];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
+  for (int e = 0; e < kV; ++e) {
     float z = tp.bias[e];
 #pragma unroll
     for (int k = 0; k < W; ++k) z = __builtin_fmaf(tp.w[e][k], win[k].f(e), z);
     o[e] = ACT ? z * sigmoid_f(z) : z;
   }
-  store8(static_cast<T*>(p.y) + b * p.C + c, n, o);
+  store_row<T, kV>(static_cast<T*>(p.y) + b * p.C + c, n, o);
 #pragma unroll
-  for (int k = 0; k < W - 1; ++k) store8(st + (long long)k * p.C, n, win[k + 1]);
+  for (int k = 0; k < W - 1; ++k) win[k + 1].store(st + (long long)k * p.C, n);
 }
 
 template <typename T, int W, bool ACT> hipError_t fwd_t(const ConvParams& p, hipStream_t stream) {
-  const int groups = (p.C + 7) / 8, runs = (p.L + W - 1 + kRun - 1) / kRun;
+  const int groups = (p.C + kV - 1) / kV, runs = (p.L + W - 1 + kRun - 1) / kRun;
   const long long threads = (long long)p.B * runs * groups;
   hipLaunchKernelGGL((conv_fwd_kernel<T, W, ACT>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, stream, p,
                      groups, runs, threads);
   return hipGetLastError();
 }
 template <typename T, int W, bool ACT> hipError_t bwd_t(const ConvParams& p, hipStream_t stream) {
-  const int groups = (p.C + 7) / 8, runs = (p.L + W - 1 + kRunBwd - 1) / kRunBwd;
+  const int groups = (p.C + kV - 1) / kV, runs = (p.L + W - 1 + kRunBwd - 1) / kRunBwd;
   const int parts = conv_bwd_parts(p.B, p.L, p.C);
   hipLaunchKernelGGL((conv_bwd_kernel<T, W, ACT>), dim3(parts, (groups + kLanes - 1) / kLanes), dim3(256), 0, stream, p,
                      groups, runs, (long long)p.B * runs);
   const long long n = (long long)(W + 1) * p.C;
-  hipLaunchKernelGGL(conv_param_grads_kernel, dim3((unsigned)((n + 63) / 64)), dim3(256), 0, stream, p, parts);
+  hipLaunchKernelGGL(conv_param_grads_kernel, dim3((unsigned)((n + 15) / 16)), dim3(256), 0, stream, p, parts);
   return hipGetLastError();
 }
 template <typename T, int W, bool ACT> hipError_t step_t(const ConvParams& p, hipStream_t stream) {
-  const int groups = (p.C + 7) / 8;
+  const int groups = (p.C + kV - 1) / kV;
   const long long threads = (long long)p.B * groups;
   hipLaunchKernelGGL((conv_step_kernel<T, W, ACT>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, stream, p,
                      groups, threads);
@@ -306,8 +301,8 @@ hipError_t launch(const ConvParams& p, int dtype, ConvPass q, hipStream_t s) {
 // unit over all channels, and no more than there are runs
 int conv_bwd_parts(int B, int L, int C) {
   const long long jobs = (long long)B * ((L + 3 + kRunBwd - 1) / kRunBwd);
-  const int by = (C + 8 * kLanes - 1) / (8 * kLanes);
-  return (int)std::max(1LL, std::min((jobs + 15) / 16, (2048LL + by - 1) / by));
+  const int by = (C + kV * kLanes - 1) / (kV * kLanes);
+  return (int)std::max(1LL, std::min((jobs + kSubs - 1) / kSubs, (2048LL + by - 1) / by));
 }
 hipError_t launch_conv_fwd(const ConvParams& p, int dtype, hipStream_t s) { return launch(p, dtype, ConvPass::Fwd, s); }
 hipError_t launch_conv_bwd(const ConvParams& p, int dtype, hipStream_t s) { return launch(p, dtype, ConvPass::Bwd, s); }

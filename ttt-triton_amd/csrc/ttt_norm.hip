@@ -8,9 +8,10 @@
 //   dx = dv z sigma(z),   dz = dv x sigma(z) (1 + z (1 - sigma(z)))
 //
 // Both are bound by HBM: a row is read once and held in registers over its two
-// reductions (the variance is that of the centred values).  Rows up to 1,024
-// values have a wave each, longer ones a workgroup of four.  The backward's
-// workgroups walk rows with the sums of dw and db in registers and write one
+// reductions (the variance is that of the centred values).  A row has 1, 4, 8 or 16
+// waves and a lane 4, 8, 12 or 16 of its values, in groups of 4 or 8 that one load
+// brings.  The backward's workgroups walk rows,
+// the next one on its way (not with 16 waves, which have 128 registers), with the sums of dw and db in registers, and write one
 // partial sum each, added up by a second launch in a fixed order.
 #include <math.h>
 
@@ -22,6 +23,8 @@ namespace ttt {
 
 namespace {
 
+constexpr int threads_of(int NW) { return NW == 1 ? 256 : 64 * NW; }
+
 // the sum over the lanes that share a row, in every one of them
 template <int NW> __device__ __forceinline__ float row_sum(float s, float* red) {
   s = sum_wave(s);
@@ -31,43 +34,52 @@ template <int NW> __device__ __forceinline__ float row_sum(float s, float* red) 
     __syncthreads();  // the last sum's readers are done
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
     __syncthreads();
-    return ((red[0] + red[1]) + red[2]) + red[3];
+    float v = 0.f;
+#pragma unroll
+    for (int k = 0; k < NW; ++k) v += red[k];
+    return v;
   }
 }
 
-// NW waves to a row, NCH x 8 values to a lane
-template <typename T, int NW, int NCH, bool GATE>
-__global__ __launch_bounds__(256) void norm_fwd_kernel(NormParams p) {
+// NW waves to a row, NCH groups of V values to a lane
+template <typename T, int NW, int V, int NCH, bool GATE>
+__global__ __launch_bounds__(threads_of(NW)) void norm_fwd_kernel(NormParams p) {
   constexpr int LANES = 64 * NW;
   const int l = threadIdx.x & (LANES - 1);
   const long long row = NW == 1 ? (long long)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
-  __shared__ float red[4];
-  if (row >= p.R) return;  // a whole wave of a one-wave row; never with NW = 4
+  __shared__ float red[16];
+  if (row >= p.R) return;  // a whole wave of a one-wave row; never with more waves
   const int D = p.D;
-  float v[NCH][8];
+  float v[NCH][V];
   float s = 0.f;
+  {
+    Raw<T, V> x[NCH], z[NCH];
 #pragma unroll
-  for (int i = 0; i < NCH; ++i) {
-    const int c = 8 * (LANES * i + l), n = D - c;
-    Raw8<T> x, z;
-    if (n > 0) {
-      x.load(static_cast<const T*>(p.x) + row * p.ldx + c, n);
-      if (GATE) z.load(static_cast<const T*>(p.gate) + row * p.ldg + c, n);
+    for (int i = 0; i < NCH; ++i) {
+      const int c = V * (LANES * i + l), n = D - c;
+      x[i].zero();
+      if (GATE) z[i].zero();
+      if (n > 0) {
+        x[i].load(static_cast<const T*>(p.x) + row * p.ldx + c, n);
+        if (GATE) z[i].load(static_cast<const T*>(p.gate) + row * p.ldg + c, n);
+      }
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      v[i][e] = e < n ? x.f(e) : 0.f;
-      if (GATE && e < n) v[i][e] *= z.f(e) * sigmoid_f(z.f(e));
-      s += v[i][e];
-    }
+    for (int i = 0; i < NCH; ++i)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        v[i][e] = x[i].f(e);
+        if (GATE) v[i][e] *= z[i].f(e) * sigmoid_f(z[i].f(e));
+        s += v[i][e];
+      }
   }
   const float mean = row_sum<NW>(s, red) / (float)D;
   s = 0.f;
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
-    const int n = D - 8 * (LANES * i + l);
+    const int n = D - V * (LANES * i + l);
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
+    for (int e = 0; e < V; ++e)
       if (e < n) {
         const float d = v[i][e] - mean;
         s = __builtin_fmaf(d, d, s);
@@ -76,20 +88,20 @@ __global__ __launch_bounds__(256) void norm_fwd_kernel(NormParams p) {
   const float rstd = 1.0f / sqrtf(row_sum<NW>(s, red) / (float)D + p.eps);
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
-    const int c = 8 * (LANES * i + l), n = D - c;
+    const int c = V * (LANES * i + l), n = D - c;
     if (n > 0) {
-      float o[8];
-      Raw8<float> w, b;
+      float o[V];
+      Raw<float, V> w, b;
       if (p.w != nullptr) {
         w.load(p.w + c, n);
         b.load(p.b + c, n);
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
+      for (int e = 0; e < V; ++e) {
         o[e] = (v[i][e] - mean) * rstd;
         if (p.w != nullptr) o[e] = __builtin_fmaf(o[e], w.v[e], b.v[e]);
       }
-      store8(static_cast<T*>(p.y) + row * D + c, n, o);
+      store_row<T, V>(static_cast<T*>(p.y) + row * D + c, n, o);
     }
   }
   if (l == 0 && p.stats != nullptr) {
@@ -98,83 +110,106 @@ __global__ __launch_bounds__(256) void norm_fwd_kernel(NormParams p) {
   }
 }
 
-template <typename T, int NW, int NCH, bool GATE>
-__global__ __launch_bounds__(256) void norm_bwd_kernel(NormParams p) {
-  constexpr int LANES = 64 * NW, ROWS = 4 / NW;
+template <typename T, int NW, int V, int NCH, bool GATE>
+__global__ __launch_bounds__(threads_of(NW)) void norm_bwd_kernel(NormParams p) {
+  constexpr int LANES = 64 * NW, ROWS = NW == 1 ? 4 : 1;
+  constexpr bool AHEAD = NW < 16;
   const int l = threadIdx.x & (LANES - 1);
-  __shared__ float red[4];
+  __shared__ float red[16];
   const int D = p.D;
-  float dw[NCH][8], db[NCH][8];
+  float dw[NCH][V], db[NCH][V];
+  Raw<T, V> nx[NCH], nz[NCH], ny[NCH];  // the next row
 #pragma unroll
-  for (int i = 0; i < NCH; ++i)
+  for (int i = 0; i < NCH; ++i) {
+    nx[i].zero();
+    nz[i].zero();
+    ny[i].zero();
 #pragma unroll
-    for (int e = 0; e < 8; ++e) dw[i][e] = db[i][e] = 0.f;
-  // (rows of one wave: each wave ends by itself; of four: together)
-  for (long long row = (long long)blockIdx.x * ROWS + (NW == 1 ? threadIdx.x >> 6 : 0); row < p.R;
-       row += (long long)gridDim.x * ROWS) {
-    const float mean = p.stats[2 * row], rstd = p.stats[2 * row + 1];
-    float u[NCH][8], g[NCH][8];
-    Raw8<T> x[NCH], z[NCH];
+    for (int e = 0; e < V; ++e) dw[i][e] = db[i][e] = 0.f;
+  }
+  float nmean = 0.f, nrstd = 0.f;
+  const auto fetch = [&](long long row) {
+    nmean = p.stats[2 * row];
+    nrstd = p.stats[2 * row + 1];
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      const int c = V * (LANES * i + l), n = D - c;
+      if (n > 0) {
+        nx[i].load(static_cast<const T*>(p.x) + row * p.ldx + c, n);
+        if (GATE) nz[i].load(static_cast<const T*>(p.gate) + row * p.ldg + c, n);
+        ny[i].load(static_cast<const T*>(p.dy) + row * D + c, n);
+      }
+    }
+  };
+  const long long step = (long long)gridDim.x * ROWS;
+  // (rows of one wave: each wave ends by itself; of more: together)
+  long long row = (long long)blockIdx.x * ROWS + (NW == 1 ? threadIdx.x >> 6 : 0);
+  if (AHEAD && row < p.R) fetch(row);
+  for (; row < p.R; row += step) {
+    if (!AHEAD) fetch(row);
+    const float mean = nmean, rstd = nrstd;
+    float u[NCH][V], g[NCH][V], sx[NCH][V], sz[NCH][V];  // (sx, sz: what dv is multiplied with)
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const int c = 8 * (LANES * i + l), n = D - c;
-      Raw8<T> dy;
-      Raw8<float> w;
-      if (n > 0) {
-        x[i].load(static_cast<const T*>(p.x) + row * p.ldx + c, n);
-        dy.load(static_cast<const T*>(p.dy) + row * D + c, n);
-        if (GATE) z[i].load(static_cast<const T*>(p.gate) + row * p.ldg + c, n);
-        if (p.w != nullptr) w.load(p.w + c, n);
-      }
+      const int c = V * (LANES * i + l), n = D - c;
+      Raw<float, V> w;
+      if (p.w != nullptr && n > 0) w.load(p.w + c, n);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        u[i][e] = g[i][e] = 0.f;
-        if (e < n) {
-          float v = x[i].f(e);
-          if (GATE) v *= z[i].f(e) * sigmoid_f(z[i].f(e));
-          u[i][e] = (v - mean) * rstd;
-          g[i][e] = p.w != nullptr ? dy.f(e) * w.v[e] : dy.f(e);
-          dw[i][e] = __builtin_fmaf(dy.f(e), u[i][e], dw[i][e]);
-          db[i][e] += dy.f(e);
-          s1 += g[i][e];
-          s2 = __builtin_fmaf(g[i][e], u[i][e], s2);
+      for (int e = 0; e < V; ++e) {
+        const float x = nx[i].f(e), dy = ny[i].f(e);
+        float v = x;
+        if (GATE) {
+          const float z = nz[i].f(e), sg = sigmoid_f(z);
+          v *= z * sg;
+          if (AHEAD) {
+            sx[i][e] = z * sg;
+            sz[i][e] = x * sg * __builtin_fmaf(z, 1.0f - sg, 1.0f);
+          }
         }
+        u[i][e] = e < n ? (v - mean) * rstd : 0.f;
+        g[i][e] = p.w != nullptr && e < n ? dy * w.v[e] : dy;
+        dw[i][e] = __builtin_fmaf(dy, u[i][e], dw[i][e]);
+        db[i][e] += dy;
+        s1 += g[i][e];
+        s2 = __builtin_fmaf(g[i][e], u[i][e], s2);
       }
     }
+    if (AHEAD && row + step < p.R) fetch(row + step);
     const float m1 = row_sum<NW>(s1, red) / (float)D, m2 = row_sum<NW>(s2, red) / (float)D;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const int c = 8 * (LANES * i + l), n = D - c;
-      if (n > 0) {
-        float dx[8], dz[8];
+      const int c = V * (LANES * i + l), n = D - c;
+      float dx[V], dz[V];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float dv = (g[i][e] - m1 - u[i][e] * m2) * rstd;
-          dx[e] = dv;
-          if (GATE) {
-            const float zz = z[i].f(e), sg = sigmoid_f(zz);
-            dx[e] = dv * zz * sg;
-            dz[e] = dv * x[i].f(e) * sg * __builtin_fmaf(zz, 1.0f - sg, 1.0f);
-          }
+      for (int e = 0; e < V; ++e) {
+        const float dv = (g[i][e] - m1 - u[i][e] * m2) * rstd;
+        if (GATE && !AHEAD) {
+          const float z = nz[i].f(e), sg = sigmoid_f(z);
+          sx[i][e] = z * sg;
+          sz[i][e] = nx[i].f(e) * sg * __builtin_fmaf(z, 1.0f - sg, 1.0f);
         }
-        store8(static_cast<T*>(p.dx) + row * D + c, n, dx);
-        if (GATE) store8(static_cast<T*>(p.dgate) + row * D + c, n, dz);
+        dx[e] = GATE ? dv * sx[i][e] : dv;
+        if (GATE) dz[e] = dv * sz[i][e];
+      }
+      if (n > 0) {
+        store_row<T, V>(static_cast<T*>(p.dx) + row * D + c, n, dx);
+        if (GATE) store_row<T, V>(static_cast<T*>(p.dgate) + row * D + c, n, dz);
       }
     }
   }
   if (p.partial == nullptr) return;
   float* part = p.partial + (long long)blockIdx.x * 2 * D;
   if constexpr (NW == 1) {  // the four waves' sums, one after the other
-    __shared__ float acc[2][64 * 8 * NCH];
+    __shared__ float acc[2][64 * V * NCH];
 #pragma unroll 1
     for (int q = 0; q < 4; ++q) {
       if ((threadIdx.x >> 6) == q) {
 #pragma unroll
         for (int i = 0; i < NCH; ++i)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int j = 64 * (8 * i + e) + l;  // lane-major: no two lanes share a bank
+          for (int e = 0; e < V; ++e) {
+            const int j = 64 * (V * i + e) + l;  // lane-major: no two lanes share a bank
             acc[0][j] = q == 0 ? dw[i][e] : acc[0][j] + dw[i][e];
             acc[1][j] = q == 0 ? db[i][e] : acc[1][j] + db[i][e];
           }
@@ -182,19 +217,19 @@ __global__ __launch_bounds__(256) void norm_bwd_kernel(NormParams p) {
       __syncthreads();
     }
     for (int k = threadIdx.x >> 6; k < 2 * NCH; k += 4) {
-      const int which = k / NCH, i = k - which * NCH, c = 8 * (64 * i + l), n = D - c;
-      float o[8];
+      const int which = k / NCH, i = k - which * NCH, c = V * (64 * i + l), n = D - c;
+      float o[V];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) o[e] = acc[which][64 * (8 * i + e) + l];
-      if (n > 0) store8(part + (long long)which * D + c, n, o);
+      for (int e = 0; e < V; ++e) o[e] = acc[which][64 * (V * i + e) + l];
+      if (n > 0) store_row<float, V>(part + (long long)which * D + c, n, o);
     }
   } else {
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const int c = 8 * (LANES * i + l), n = D - c;
+      const int c = V * (LANES * i + l), n = D - c;
       if (n > 0) {
-        store8(part + c, n, dw[i]);
-        store8(part + D + c, n, db[i]);
+        store_row<float, V>(part + c, n, dw[i]);
+        store_row<float, V>(part + D + c, n, db[i]);
       }
     }
   }
@@ -202,59 +237,55 @@ __global__ __launch_bounds__(256) void norm_bwd_kernel(NormParams p) {
 
 // dw, db: the sum over the workgroups' partial sums
 __global__ __launch_bounds__(256) void norm_param_grads_kernel(NormParams p, int parts) {
-  const int wave = threadIdx.x >> 6, l = threadIdx.x & 63;
-  const long long n = 2LL * p.D, i = (long long)blockIdx.x * 64 + l;
-  __shared__ float red[4][64];
-  float s = 0.f;
-  if (i < n)
-    for (int q = wave; q < parts; q += 4) s += p.partial[q * n + i];
-  red[wave][l] = s;
-  __syncthreads();
-  if (wave == 0 && i < n) {
-    s = ((red[0][l] + red[1][l]) + red[2][l]) + red[3][l];
-    if (i < p.D)
-      p.dw[i] = s;
-    else
-      p.db[i - p.D] = s;
-  }
+  const long long n = 2LL * p.D, i = (long long)blockIdx.x * 16 + (threadIdx.x & 15);
+  const float s = sum_parts(p.partial, n, i, parts);
+  if (threadIdx.x < 16 && i < n) (i < p.D ? p.dw[i] : p.db[i - p.D]) = s;
 }
 
-template <typename T, int NW, int NCH, bool GATE>
+template <typename T, int NW, int V, int NCH, bool GATE>
 hipError_t run_t(const NormParams& p, bool bwd, hipStream_t stream) {
   if (!bwd) {
     const long long blocks = NW == 1 ? (p.R + 3) / 4 : p.R;
-    hipLaunchKernelGGL((norm_fwd_kernel<T, NW, NCH, GATE>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((norm_fwd_kernel<T, NW, V, NCH, GATE>), dim3((unsigned)blocks), dim3(threads_of(NW)), 0, stream, p);
     return hipGetLastError();
   }
   const int parts = norm_bwd_parts(p.R, p.D);
-  hipLaunchKernelGGL((norm_bwd_kernel<T, NW, NCH, GATE>), dim3(parts), dim3(256), 0, stream, p);
+  hipLaunchKernelGGL((norm_bwd_kernel<T, NW, V, NCH, GATE>), dim3(parts), dim3(threads_of(NW)), 0, stream, p);
   if (p.partial != nullptr)
-    hipLaunchKernelGGL(norm_param_grads_kernel, dim3((2 * p.D + 63) / 64), dim3(256), 0, stream, p, parts);
+    hipLaunchKernelGGL(norm_param_grads_kernel, dim3((2 * p.D + 15) / 16), dim3(256), 0, stream, p, parts);
   return hipGetLastError();
 }
-template <typename T, int NW, int NCH> hipError_t gate_t(const NormParams& p, bool bwd, hipStream_t s) {
-  return p.gate != nullptr ? run_t<T, NW, NCH, true>(p, bwd, s) : run_t<T, NW, NCH, false>(p, bwd, s);
+template <typename T, int NW, int V, int NCH> hipError_t gate_t(const NormParams& p, bool bwd, hipStream_t s) {
+  return p.gate != nullptr ? run_t<T, NW, V, NCH, true>(p, bwd, s) : run_t<T, NW, V, NCH, false>(p, bwd, s);
 }
-template <typename T> hipError_t size_t_(const NormParams& p, bool bwd, hipStream_t s) {
-  if (p.D <= 512) return gate_t<T, 1, 1>(p, bwd, s);
-  if (p.D <= 1024) return gate_t<T, 1, 2>(p, bwd, s);
-  if (p.D <= 2048) return gate_t<T, 4, 1>(p, bwd, s);
-  if (p.D <= 4096) return gate_t<T, 4, 2>(p, bwd, s);
-  if (p.D <= 8192) return gate_t<T, 4, 4>(p, bwd, s);
-  return gate_t<T, 4, 8>(p, bwd, s);
+// Waves to a row and values to a lane, so that few lanes' places are empty and no more than
+// 128 registers are needed with 16 waves
+template <typename T, int NW> hipError_t lanes_t(const NormParams& p, bool bwd, hipStream_t s) {
+  const int four = (p.D + 256 * NW - 1) / (256 * NW);  // values to a lane, in fours
+  if constexpr (NW <= 4) {
+    if (four == 1) return gate_t<T, NW, 4, 1>(p, bwd, s);
+    if (four == 2) return gate_t<T, NW, 8, 1>(p, bwd, s);
+  }
+  return four == 3 ? gate_t<T, NW, 4, 3>(p, bwd, s) : gate_t<T, NW, 8, 2>(p, bwd, s);
+}
+template <typename T> hipError_t waves_t(const NormParams& p, bool bwd, hipStream_t s) {
+  return p.D <= 1024   ? lanes_t<T, 1>(p, bwd, s)
+         : p.D <= 4096 ? lanes_t<T, 4>(p, bwd, s)
+         : p.D <= 8192 ? lanes_t<T, 8>(p, bwd, s)
+                       : lanes_t<T, 16>(p, bwd, s);
 }
 hipError_t launch(const NormParams& p, int dtype, bool bwd, hipStream_t s) {
   if (p.D < 1 || p.D > kNormMaxD) return hipErrorInvalidValue;
-  return dtype == TTT_DTYPE_BF16 ? size_t_<__bf16>(p, bwd, s)
-         : dtype == TTT_DTYPE_F16 ? size_t_<_Float16>(p, bwd, s) : size_t_<float>(p, bwd, s);
+  return dtype == TTT_DTYPE_BF16 ? waves_t<__bf16>(p, bwd, s)
+         : dtype == TTT_DTYPE_F16 ? waves_t<_Float16>(p, bwd, s) : waves_t<float>(p, bwd, s);
 }
 
 }  // namespace
 
-// workgroups of the backward: up to 4 a compute unit
+// workgroups of the backward: as many as are there at once, 12 waves to a compute unit (16 of longer rows)
 int norm_bwd_parts(long long R, int D) {
-  const long long rows = D <= 1024 ? (R + 3) / 4 : R;
-  return (int)std::max(1LL, std::min(rows, 1024LL));
+  const long long rows = D <= 1024 ? (R + 3) / 4 : R, most = D <= 4096 ? 768 : D <= 8192 ? 512 : 256;
+  return (int)std::max(1LL, std::min(rows, most));
 }
 hipError_t launch_norm_fwd(const NormParams& p, int dtype, hipStream_t s) { return launch(p, dtype, false, s); }
 hipError_t launch_norm_bwd(const NormParams& p, int dtype, hipStream_t s) { return launch(p, dtype, true, s); }

@@ -199,6 +199,7 @@ template <int PL, int ROWS, int COLS> struct Planes {
   }
 };
 
+typedef unsigned u4v __attribute__((ext_vector_type(4)));
 // ROWS x COLS values of T on their way from a matrix of rows to planes.  A thread's
 // places are the same in every chunk: their offsets are formed once.
 template <typename T, int ROWS, int COLS, int NT> struct Stage {

@@ -41,73 +41,82 @@ struct NormParams {
   int D;
   float eps;
 };
-constexpr int kNormMaxD = 16384;
+constexpr int kNormMaxD = 16384;  // 16 values to each of a row's 1,024 lanes
 hipError_t launch_norm_fwd(const NormParams& p, int dtype, hipStream_t stream);
 hipError_t launch_norm_bwd(const NormParams& p, int dtype, hipStream_t stream);
 int norm_bwd_parts(long long R, int D);
 
 // ---------------------------------------------------------------- rows of any alignment
-// Eight consecutive elements of a row, 16 bytes a load where all eight are
-// there.  Rows of odd length start at any multiple of the element's size: the
-// loads and stores are declared so aligned, which the vector memory takes.
-typedef unsigned u4v __attribute__((ext_vector_type(4)));
-template <typename T> struct RowVec;
-template <> struct RowVec<__bf16> {
-  typedef __bf16 v8 __attribute__((ext_vector_type(8), aligned(2)));
+// V (4 or 8) consecutive elements of a row, one load where all are there.  Rows of odd
+// length start at any multiple of the element's size: the loads and stores are declared
+// so aligned, which the vector memory takes.
+template <typename T, int V> struct RowVec {
+  typedef T type __attribute__((ext_vector_type(V), aligned(sizeof(T))));
 };
-template <> struct RowVec<_Float16> {
-  typedef _Float16 v8 __attribute__((ext_vector_type(8), aligned(2)));
-};
-template <> struct RowVec<float> {
-  typedef float v8 __attribute__((ext_vector_type(8), aligned(4)));
-};
-
 // raw elements of the row's columns [0, n) from p, zeros behind them
-template <typename T> struct Raw8 {
-  T v[8];
+template <typename T, int V> struct Raw {
+  typename RowVec<T, V>::type v;
   __device__ __forceinline__ void load(const T* __restrict__ p, int n) {
-    if (n >= 8) {
-      const typename RowVec<T>::v8 x = *reinterpret_cast<const typename RowVec<T>::v8*>(p);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = x[e];
+    if (n >= V) {
+      v = *reinterpret_cast<const typename RowVec<T, V>::type*>(p);
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = e < n ? p[e] : (T)0.0f;
+      for (int e = 0; e < V; ++e) v[e] = e < n ? p[e] : (T)0.0f;
     }
   }
   __device__ __forceinline__ void zero() {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = (T)0.0f;
+    for (int e = 0; e < V; ++e) v[e] = (T)0.0f;
   }
   __device__ __forceinline__ float f(int e) const { return (float)v[e]; }
+  __device__ __forceinline__ void store(T* __restrict__ p, int n) const {
+    if (n >= V) {
+      *reinterpret_cast<typename RowVec<T, V>::type*>(p) = v;
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (e < n) p[e] = v[e];
+    }
+  }
 };
-template <typename T> __device__ __forceinline__ void store8(T* __restrict__ p, int n, const float (&v)[8]) {
-  const auto a = to_frag<T>(f4{v[0], v[1], v[2], v[3]}).v, b = to_frag<T>(f4{v[4], v[5], v[6], v[7]}).v;
-  if (n >= 8) {
-    typename RowVec<T>::v8 x = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
-    *reinterpret_cast<typename RowVec<T>::v8*>(p) = x;
-  } else {
+// V values, rounded to T
+template <typename T, int V> __device__ __forceinline__ void store_row(T* __restrict__ p, int n, const float (&v)[V]) {
+  Raw<T, V> r;
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (e < n) p[e] = e < 4 ? a[e] : b[e - 4];
+  for (int q = 0; q < V; q += 4) {
+    const auto a = to_frag<T>(f4{v[q], v[q + 1], v[q + 2], v[q + 3]}).v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r.v[q + e] = a[e];
   }
-}
-template <typename T> __device__ __forceinline__ void store8(T* __restrict__ p, int n, const Raw8<T>& r) {
-  if (n >= 8) {
-    typename RowVec<T>::v8 x;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = r.v[e];
-    *reinterpret_cast<typename RowVec<T>::v8*>(p) = x;
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (e < n) p[e] = r.v[e];
-  }
+  r.store(p, n);
 }
 
 // 1 / (1 + e^-z): e^-z overflows to inf for z < -88, whose reciprocal is the 0 that is meant
 __device__ __forceinline__ float sigmoid_f(float z) {
   return rcp_f(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * z));
+}
+
+// A workgroup of 256 sums `parts` rows of n partial sums: thread t has column i, shared by
+// the threads t, t + 16, .., and every 16th row; threads 0..15 return the sums, which
+// do not depend on anything but their order here.
+__device__ __forceinline__ float sum_parts(const float* __restrict__ part, long long n, long long i, int parts) {
+  __shared__ float red[16][17];
+  const int g = threadIdx.x >> 4, c = threadIdx.x & 15;
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
+  if (i < n) {
+    int q = g;
+    for (; q + 48 < parts; q += 64)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) s[k] += part[(long long)(q + 16 * k) * n + i];
+    for (; q < parts; q += 16) s[0] += part[(long long)q * n + i];
+  }
+  red[g][c] = (s[0] + s[1]) + (s[2] + s[3]);
+  __syncthreads();
+  float v = 0.f;
+  if (threadIdx.x < 16)
+#pragma unroll
+    for (int k = 0; k < 16; ++k) v += red[k][c];
+  return v;
 }
 
 }  // namespace ttt

@@ -10,8 +10,8 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._common import check_device, dtype_code, on_device, ptr, stream_of
-from .ssm import _opt, _param, _rows, _wants_grad
+from ._common import check_device, dtype_code, on_device
+from .ssm import _as, _bytes, _opt, _param, _rows, _stream, _wants_grad
 
 LAYER_NORM_EPS = 1e-6
 MAX_WIDTH = 16384
@@ -32,16 +32,16 @@ def _norm_forward(x, weight, bias, gate, eps, train):
     code = dtype_code(x.dtype)
     w, b = _param(weight, (D,), "weight"), _param(bias, (D,), "bias")
     lead, es = x.dim() - 1, x.element_size()
-    xr, ldx = _rows(x, x.dtype, lead, es)
-    gr, ldg = (None, 0) if gate is None else _rows(gate, x.dtype, lead, es)
+    xr, ldx = _rows(x, lead, es)
+    gr, ldg = (None, 0) if gate is None else _rows(gate, lead, es)
     y = torch.empty(x.shape, device=dev, dtype=x.dtype)
     R = y.numel() // D
     if R >= 1 << 31:
         raise ValueError(f"layer_norm takes fewer than 2^31 rows, got {R}")
     stats = torch.empty((R, 2), device=dev, dtype=torch.float32) if train else None
     with on_device(dev):
-        st = _lib.load().ttt_layer_norm_fwd(ptr(xr), ldx, _opt(gr), ldg, _opt(w), _opt(b), R, D, float(eps), code,
-                                            ptr(y), _opt(stats), stream_of(dev))
+        st = _lib.load().ttt_layer_norm_fwd(xr.data_ptr(), ldx, _opt(gr), ldg, _opt(w), _opt(b), R, D, float(eps), code,
+                                            y.data_ptr(), _opt(stats), _stream(dev))
     _lib.check(st, "ttt_layer_norm_fwd")
     return y, (xr, ldx, gr, ldg, w, stats)
 
@@ -73,15 +73,15 @@ class LayerNormFunction(torch.autograd.Function):
         n = 0
         if w is not None and (ctx.needs_input_grad[1] or ctx.needs_input_grad[2]):
             dw, db = torch.empty((2, D), device=dev, dtype=torch.float32)
-            n = lib.ttt_layer_norm_partial_bytes(R, D)
+            n = _bytes("ttt_layer_norm_partial_bytes", R, D)
             part = torch.empty(n // 4, device=dev, dtype=torch.float32)
         with on_device(dev):
-            st = lib.ttt_layer_norm_bwd(ptr(x), ctx.lds[0], _opt(gate), ctx.lds[1], _opt(w), ptr(stats), ptr(dy), R, D,
-                                        dtype_code(dt), ptr(dx), _opt(dg), _opt(dw), _opt(db), _opt(part), n,
-                                        stream_of(dev))
+            st = lib.ttt_layer_norm_bwd(x.data_ptr(), ctx.lds[0], _opt(gate), ctx.lds[1], _opt(w), stats.data_ptr(), dy.data_ptr(), R, D,
+                                        dtype_code(dt), dx.data_ptr(), _opt(dg), _opt(dw), _opt(db), _opt(part), n,
+                                        _stream(dev))
         _lib.check(st, "ttt_layer_norm_bwd")
         if dw is not None:
-            dw, db = dw.to(ctx.dtypes[0]), db.to(ctx.dtypes[1])
+            dw, db = _as(dw, ctx.dtypes[0]), _as(db, ctx.dtypes[1])
         return dx, dw, db, dg, None
 
 

@@ -21,45 +21,65 @@ of its sequence."""
 
 from __future__ import annotations
 
+import functools
+
 import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._common import check_device, dtype_code, f32c, on_device, ptr, stream_of
+from ._common import check_device, dtype_code, f32c, on_device
 
 HEAD_DIMS = (32, 64)
 MAX_STATE = 128
 CONV_WIDTHS = (2, 3, 4)
 
 
-def _rows(t: torch.Tensor, dt: torch.dtype, lead: int, align: int):
+def _rows(t: torch.Tensor, lead: int, align: int):
     """(t, row stride) with t's first `lead` axes as rows a fixed stride apart and
     the rest contiguous inside a row, `align` bytes of alignment; a contiguous
     copy where t is not laid out so."""
-    if t.dtype == dt:
-        ld = width = 1
-        for n, st in zip(reversed(t.shape[lead:]), reversed(t.stride()[lead:])):
-            if n != 1 and st != width:
+    shape = t.shape
+    width = 1
+    for n in shape[lead:]:
+        width *= n
+    if t.is_contiguous():
+        if (t.data_ptr() | width * t.element_size()) % align == 0:
+            return t, width
+        return t.clone(), width  # (fresh memory starts on more than any of them)
+    strides = t.stride()
+    inner, ld, step = 1, None, 0
+    for i in range(t.dim() - 1, -1, -1):
+        n, st = shape[i], strides[i]
+        if i >= lead:
+            if n != 1 and st != inner:
                 break
-            width *= n
-        else:
-            # the innermost leading axis that is more than one row gives the stride
-            ld, step = None, 0
-            for n, st in zip(reversed(t.shape[:lead]), reversed(t.stride()[:lead])):
-                if n == 1:
-                    continue
-                if ld is None:
-                    ld, step = st, st * n
-                elif st != step:
-                    ld = -1
-                    break
-                else:
-                    step *= n
-            ld = width if ld is None else ld
-            if ld >= width and (t.data_ptr() | ld * t.element_size()) % align == 0:
-                return t, ld
-    t = t.detach().to(dt).contiguous()
-    return t, t[(0,) * lead].numel()
+            inner *= n
+        elif n != 1:
+            if ld is None:  # the innermost leading axis of more than one row gives the stride
+                ld = step = st
+            elif st != step:
+                break
+            step *= n
+    else:
+        ld = width if ld is None else ld
+        if ld >= width and (t.data_ptr() | ld * t.element_size()) % align == 0:
+            return t, ld
+    return t.detach().contiguous(), width
+
+
+def _stream(dev: torch.device) -> int:
+    return torch._C._cuda_getCurrentRawStream(dev.index)
+
+
+@functools.lru_cache(maxsize=4096)
+def _bytes(name: str, *sizes: int) -> int:
+    """What a size function of the library says for these sizes."""
+    return getattr(_lib.load(), name)(*sizes)
+
+
+def _as(g, dt):
+    """A gradient in its input's type."""
+    return g if g is None or g.dtype == dt else g.to(dt)
 
 
 def _opt(t):
@@ -69,9 +89,9 @@ def _opt(t):
 def _param(t, shape, name):
     if t is None:
         return None
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
-    return f32c(t)
+    return t if t.dtype == torch.float32 and t.is_contiguous() else f32c(t)
 
 
 def _wants_grad(*ts) -> bool:
@@ -89,7 +109,7 @@ def _sizes(*ns):
 
 
 def _state_in_place(state, shape, dt, dev, what):
-    if tuple(state.shape) != shape or state.dtype != dt or not state.is_contiguous() or state.device != dev:
+    if state.shape != shape or state.dtype != dt or not state.is_contiguous() or state.device != dev:
         raise ValueError(f"{what}: the state must be contiguous, {list(shape)} in {dt} on {dev}, got "
                          f"{list(state.shape)} in {state.dtype} on {state.device}")
 
@@ -124,13 +144,13 @@ def _conv_forward(x, weight, bias, state, activation, want_last):
     """(y, last state or None, what the backward reads)"""
     dev, code, C, W, w, b = _conv_args(x, weight, bias, state, activation, 2)
     B, L = x.shape[:2]
-    xr, ldx = _rows(x, x.dtype, 2, x.element_size())
+    xr, ldx = _rows(x, 2, x.element_size())
     s0 = _conv_state(state, (B, W - 1, C), x.dtype)
     y = torch.empty((B, L, C), device=dev, dtype=x.dtype)
     last = torch.empty((B, W - 1, C), device=dev, dtype=x.dtype) if want_last else None
     with on_device(dev):
-        st = _lib.load().ttt_causal_conv_fwd(ptr(xr), ldx, _opt(s0), ptr(w), _opt(b), B, L, C, W,
-                                             _lib.ACTIVATIONS[activation], code, ptr(y), _opt(last), stream_of(dev))
+        st = _lib.load().ttt_causal_conv_fwd(xr.data_ptr(), ldx, _opt(s0), w.data_ptr(), _opt(b), B, L, C, W,
+                                             _lib.ACTIVATIONS[activation], code, y.data_ptr(), _opt(last), _stream(dev))
     _lib.check(st, "ttt_causal_conv_fwd")
     return y, last, (xr, ldx, s0, w, b)
 
@@ -162,14 +182,14 @@ class CausalConvFunction(torch.autograd.Function):
         dw = torch.empty((C, W), device=dev, dtype=torch.float32)
         db = torch.empty(C, device=dev, dtype=torch.float32) if ctx.dtypes[1] is not None else None
         lib = _lib.load()
-        part = torch.empty(lib.ttt_causal_conv_partial_bytes(B, L, C, W) // 4, device=dev, dtype=torch.float32)
+        part = torch.empty(_bytes("ttt_causal_conv_partial_bytes", B, L, C, W) // 4, device=dev, dtype=torch.float32)
         with on_device(dev):
-            st = lib.ttt_causal_conv_bwd(ptr(x), ctx.ldx, _opt(s0), ptr(w), _opt(b), _opt(dy), _opt(dlast), B, L, C, W,
-                                         _lib.ACTIVATIONS[ctx.activation], dtype_code(dt), ptr(dx), _opt(ds), ptr(dw),
-                                         _opt(db), ptr(part), part.numel() * 4, stream_of(dev))
+            st = lib.ttt_causal_conv_bwd(x.data_ptr(), ctx.ldx, _opt(s0), w.data_ptr(), _opt(b), _opt(dy), _opt(dlast), B, L, C, W,
+                                         _lib.ACTIVATIONS[ctx.activation], dtype_code(dt), dx.data_ptr(), _opt(ds), dw.data_ptr(),
+                                         _opt(db), part.data_ptr(), part.numel() * 4, _stream(dev))
         _lib.check(st, "ttt_causal_conv_bwd")
         wt, bt, sd = ctx.dtypes
-        return (dx, dw.to(wt), None if db is None else db.to(bt), None if ds is None else ds.to(sd), None, None)
+        return dx, _as(dw, wt), _as(db, bt), _as(ds, sd), None, None
 
 
 def causal_conv(x, weight, bias=None, initial_state=None, activation=None, return_final_state: bool = False):
@@ -199,10 +219,10 @@ def causal_conv_step(x, state, weight, bias=None, activation=None):
     y = torch.empty((B, C), device=dev, dtype=x.dtype)
     if B == 0:
         return y
-    xr, ldx = _rows(x, x.dtype, 1, x.element_size())
+    xr, ldx = _rows(x, 1, x.element_size())
     with on_device(dev):
-        st = _lib.load().ttt_causal_conv_step(ptr(xr), ldx, ptr(state), ptr(w), _opt(b), B, C, W,
-                                              _lib.ACTIVATIONS[activation], code, ptr(y), stream_of(dev))
+        st = _lib.load().ttt_causal_conv_step(xr.data_ptr(), ldx, state.data_ptr(), w.data_ptr(), _opt(b), B, C, W,
+                                              _lib.ACTIVATIONS[activation], code, y.data_ptr(), _stream(dev))
     _lib.check(st, "ttt_causal_conv_step")
     torch.autograd.graph.increment_version(state)
     return y
@@ -216,9 +236,9 @@ def _scan_args(x, dt, A, Bm, Cm, D, dt_bias, state, lead):
     """(device, (B, L, H, P, G, N), code of x, code of dt, A, D, dt_bias)"""
     if x.dim() != lead + 2:
         raise ValueError(f"x must be [{'B,L,H,P' if lead == 2 else 'B,H,P'}], got {list(x.shape)}")
-    rows = tuple(x.shape[:lead])
+    rows = x.shape[:lead]
     H, P = x.shape[lead:]
-    if Bm.dim() != lead + 2 or tuple(Bm.shape[:lead]) != rows or Bm.shape != Cm.shape:
+    if Bm.dim() != lead + 2 or Bm.shape[:lead] != rows or Bm.shape != Cm.shape:
         raise ValueError(f"Bm and Cm must be {[*rows, 'G', 'N']}, got {list(Bm.shape)} and {list(Cm.shape)}")
     G, N = Bm.shape[lead:]
     if P not in HEAD_DIMS:
@@ -227,18 +247,18 @@ def _scan_args(x, dt, A, Bm, Cm, D, dt_bias, state, lead):
         raise ValueError(f"the state's width N must be a multiple of 16 up to {MAX_STATE}, got {N}")
     if G < 1 or H % G:
         raise ValueError(f"the {G} groups of Bm and Cm must divide the {H} heads")
-    if tuple(dt.shape) != (*rows, H):
+    if dt.shape != (*rows, H):
         raise ValueError(f"dt must be {[*rows, H]}, got {list(dt.shape)}")
     for name, t in (("Bm", Bm), ("Cm", Cm)):
         if t.dtype != x.dtype:
             raise ValueError(f"{name} must have x's dtype {x.dtype}, got {t.dtype}")
     if dt.dtype not in (x.dtype, torch.float32):
         raise ValueError(f"dt must be in {x.dtype} or float32, got {dt.dtype}")
+    if A is None:
+        raise ValueError("A is needed")
     dev = check_device(x, dt, A, Bm, Cm, *(t for t in (D, dt_bias, state) if t is not None))
     _sizes(*x.shape)
     a = _param(A, (H,), "A")
-    if a is None:
-        raise ValueError("A is needed")
     return (dev, (rows[0], rows[1] if lead == 2 else 1, H, P, G, N), dtype_code(x.dtype), dtype_code(dt.dtype), a,
             _param(D, (H,), "D"), _param(dt_bias, (H,), "dt_bias"))
 
@@ -247,7 +267,7 @@ def _scan_rows(x, dt, Bm, Cm, lead, align):
     """The four inputs and their row strides as the kernels take them."""
     out = []
     for t, al in ((x, align), (dt, dt.element_size()), (Bm, align), (Cm, align)):
-        out += _rows(t, t.dtype, lead, al)
+        out += _rows(t, lead, al)
     return out
 
 
@@ -263,14 +283,14 @@ def _scan_forward(x, dt, A, Bm, Cm, D, dt_bias, h0, softplus, want_last, train):
     y = torch.empty((B, L, H, P), device=dev, dtype=x.dtype)
     last = torch.empty((B, H, P, N), device=dev, dtype=torch.float32) if want_last else None
     lib = _lib.load()
-    nst = lib.ttt_scan_states_bytes(B, L, H, P, N, code) if train else 0
-    nws = lib.ttt_scan_workspace_bytes(B, L, H, P, N, code)
+    nst = _bytes("ttt_scan_states_bytes", B, L, H, P, N, code) if train else 0
+    nws = _bytes("ttt_scan_workspace_bytes", B, L, H, P, N, code)
     states = torch.empty(nst, device=dev, dtype=torch.uint8) if train else None
     ws = torch.empty(nws, device=dev, dtype=torch.uint8) if nws else None
     with on_device(dev):
-        st = lib.ttt_scan_fwd(ptr(xr), ldx, ptr(dr), ldd, ptr(a), ptr(br), ldb, ptr(cr), ldc, _opt(d), _opt(bias),
-                              _opt(h0), B, L, H, P, G, N, code, dcode, int(softplus), ptr(y), _opt(last), _opt(states),
-                              nst, _opt(ws), nws, stream_of(dev))
+        st = lib.ttt_scan_fwd(xr.data_ptr(), ldx, dr.data_ptr(), ldd, a.data_ptr(), br.data_ptr(), ldb, cr.data_ptr(), ldc, _opt(d), _opt(bias),
+                              _opt(h0), B, L, H, P, G, N, code, dcode, int(softplus), y.data_ptr(), _opt(last), _opt(states),
+                              nst, _opt(ws), nws, _stream(dev))
     _lib.check(st, "ttt_scan_fwd")
     return y, last, (rows, a, d, bias, states)
 
@@ -300,27 +320,26 @@ class SelectiveScanFunction(torch.autograd.Function):
         dev, act = x.device, x.dtype
         code = dtype_code(act)
         dy = torch.zeros((B, L, H, P), device=dev, dtype=act) if dy is None else dy
-        dyr, ldy = _rows(dy, act, 2, 16)
+        dyr, ldy = _rows(dy if dy.dtype == act else dy.to(act), 2, 16)
         dlast = None if dlast is None else f32c(dlast)
         f32 = dict(device=dev, dtype=torch.float32)
         dx = torch.empty((B, L, H, P), device=dev, dtype=act)
         ddt = torch.empty((B, L, H), device=dev, dtype=dt.dtype)
         dB, dC = (torch.empty((B, L, G, N), device=dev, dtype=act) for _ in range(2))
-        dA = torch.empty(H, **f32)
-        dD, dbias = (None if t is None else torch.empty(H, **f32) for t in (d, bias))
+        dA, dD, dbias = torch.empty((3, H), **f32).unbind()
         dh0 = torch.empty((B, H, P, N), **f32) if ctx.needs_input_grad[7] else None
         lib = _lib.load()
-        nws = lib.ttt_scan_bwd_workspace_bytes(B, L, H, P, G, N, code)
+        nws = _bytes("ttt_scan_bwd_workspace_bytes", B, L, H, P, G, N, code)
         ws = torch.empty(nws, device=dev, dtype=torch.uint8)
         with on_device(dev):
-            st = lib.ttt_scan_bwd(ptr(x), ldx, ptr(dt), ldd, ptr(a), ptr(Bm), ldb, ptr(Cm), ldc, _opt(d), _opt(bias),
-                                  ptr(dyr), ldy, _opt(dlast), ptr(states), states.numel(), B, L, H, P, G, N, code,
-                                  dtype_code(dt.dtype), int(ctx.softplus), ptr(dx), ptr(ddt), ptr(dA), ptr(dB), ptr(dC),
-                                  _opt(dD), _opt(dbias), _opt(dh0), ptr(ws), nws, stream_of(dev))
+            st = lib.ttt_scan_bwd(x.data_ptr(), ldx, dt.data_ptr(), ldd, a.data_ptr(), Bm.data_ptr(), ldb, Cm.data_ptr(), ldc, _opt(d), _opt(bias),
+                                  dyr.data_ptr(), ldy, _opt(dlast), states.data_ptr(), states.numel(), B, L, H, P, G, N, code,
+                                  dtype_code(dt.dtype), int(ctx.softplus), dx.data_ptr(), ddt.data_ptr(), dA.data_ptr(), dB.data_ptr(), dC.data_ptr(),
+                                  _opt(None if d is None else dD), _opt(None if bias is None else dbias), _opt(dh0), ws.data_ptr(), nws, _stream(dev))
         _lib.check(st, "ttt_scan_bwd")
         dts = ctx.dtypes
-        dD, dbias, dh0 = (None if g is None else g.to(t) for g, t in zip((dD, dbias, dh0), dts[1:]))
-        return dx, ddt, dA.to(dts[0]), dB, dC, dD, dbias, dh0, None, None
+        return (dx, ddt, _as(dA, dts[0]), dB, dC, None if d is None else _as(dD, dts[1]),
+                None if bias is None else _as(dbias, dts[2]), _as(dh0, dts[3]), None, None)
 
 
 def selective_scan(x, dt, A, Bm, Cm, D=None, dt_bias=None, initial_state=None, dt_softplus: bool = True,
@@ -357,9 +376,9 @@ def selective_scan_step(x, dt, A, Bm, Cm, state, D=None, dt_bias=None, dt_softpl
         return y
     xr, ldx, dr, ldd, br, ldb, cr, ldc = _scan_rows(x, dt, Bm, Cm, 1, 4 * x.element_size())
     with on_device(dev):
-        st = _lib.load().ttt_scan_step(ptr(xr), ldx, ptr(dr), ldd, ptr(a), ptr(br), ldb, ptr(cr), ldc, _opt(d),
-                                       _opt(bias), ptr(state), B, H, P, G, N, code, dcode, int(dt_softplus), ptr(y),
-                                       stream_of(dev))
+        st = _lib.load().ttt_scan_step(xr.data_ptr(), ldx, dr.data_ptr(), ldd, a.data_ptr(), br.data_ptr(), ldb, cr.data_ptr(), ldc, _opt(d),
+                                       _opt(bias), state.data_ptr(), B, H, P, G, N, code, dcode, int(dt_softplus), y.data_ptr(),
+                                       _stream(dev))
     _lib.check(st, "ttt_scan_step")
     torch.autograd.graph.increment_version(state)
     return y
