@@ -362,3 +362,55 @@ def test_empty(lib):
     assert y.shape == (2, 0, 2, 32) and torch.equal(s, d["state"])
     y, s = causal_conv(torch.empty(2, 0, 5, device="cuda"), torch.ones(5, 3, device="cuda"), return_final_state=True)
     assert y.shape == (2, 0, 5) and s.shape == (2, 2, 5) and (s == 0).all()
+
+
+def test_empty_gradients(lib):
+    """No tokens: no gradient of the parameters, and the state's passes through."""
+    from ttt_amd.norm import layer_norm
+    from ttt_amd.ssm import causal_conv, selective_scan
+    d = T.dev(T.scan_inputs(2, 3, 2, 32, 1, 16, BF16, seed=1))
+    a, s0 = (d[k].clone().requires_grad_(True) for k in ("A", "state"))
+    y, s = selective_scan(d["x"][:, :0], d["dt"][:, :0], a, d["Bm"][:, :0], d["Cm"][:, :0], initial_state=s0,
+                          return_final_state=True)
+    ga, gs = torch.autograd.grad(y.sum() + 2 * s.sum(), [a, s0])
+    assert (ga == 0).all() and (gs == 2).all()
+    w = torch.ones(5, 3, device="cuda", requires_grad=True)
+    y = causal_conv(torch.empty(2, 0, 5, device="cuda"), w)
+    assert (torch.autograd.grad(y.sum(), w)[0] == 0).all()
+    w, b = (torch.ones(5, device="cuda", requires_grad=True) for _ in range(2))
+    y = layer_norm(torch.empty(0, 5, device="cuda"), w, b)
+    assert all((g == 0).all() for g in torch.autograd.grad(y.sum(), [w, b]))
+    with pytest.raises(ValueError, match="weight"):
+        causal_conv(torch.empty(2, 0, 5, device="cuda"), torch.ones(4, 3, device="cuda"))
+    with pytest.raises(ValueError, match="initial_state"):
+        selective_scan(d["x"][:, :0], d["dt"][:, :0], d["A"], d["Bm"][:, :0], d["Cm"][:, :0],
+                       initial_state=d["state"][:1])
+
+
+@pytest.mark.parametrize("L", [1, 2])
+def test_scan_of_rows_far_apart(lib, L):
+    """Rows 64 MiB apart: of different sequences where they are tokens alone, and of one."""
+    from ttt_amd.ssm import selective_scan
+    B = 3 - L
+    d = T.dev(T.scan_inputs(B, L, 2, 32, 1, 16, BF16, seed=2))
+    wide = torch.empty(B * L, (1 << 25) + 8, device="cuda", dtype=BF16)
+    x = wide[:, :64].view(B, L, 2, 32)
+    x.copy_(d["x"])
+    a = [d[k].clone().requires_grad_(True) if k == "A" else d[k] for k in ("dt", "A", "Bm", "Cm")]
+    g = wide[:, 64:128].view(B, L, 2, 32)
+    g.copy_(d["x"])
+    want, y = selective_scan(d["x"].contiguous(), *a), selective_scan(x, *a)
+    assert torch.equal(y, want)
+    assert torch.equal(*(torch.autograd.grad(o, a[1], t)[0] for o, t in ((y, g), (want, d["x"].contiguous()))))
+
+
+@pytest.mark.parametrize("dt", T.DTYPES)
+def test_conv_of_a_large_batch(lib, dt):
+    """A thread's run is longer in a large batch: a sequence's values are the same bits alone."""
+    from ttt_amd.ssm import causal_conv
+    torch.manual_seed(3)
+    x, w = torch.randn(33, 1031, 521, device="cuda").to(dt), torch.randn(521, 4, device="cuda")
+    y, last = causal_conv(x, w, None, None, "silu", True)
+    for b in (0, 17, 32):
+        y1, last1 = causal_conv(x[b:b + 1], w, None, None, "silu", True)
+        assert torch.equal(y[b:b + 1], y1) and torch.equal(last[b:b + 1], last1)

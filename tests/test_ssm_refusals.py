@@ -50,6 +50,9 @@ def test_conv(lib):
         assert g(x=None) == E_NULL and g(w=None) == E_NULL and g(x=P + 1) == E_ALIGN and g(w=P + 2) == E_ALIGN
     assert f(L=0) == E_SHAPE and f(L=0x7fffffff) == E_SHAPE and f(y=None) == E_NULL
     assert s(state=None) == E_NULL
+    for g in (f, b, s):
+        assert g(C=(1 << 22) + 1, ldx=1 << 23) == E_SHAPE
+    assert f(B=1 << 20, L=1 << 20) == E_SHAPE and b(B=1 << 20, L=1 << 20) == E_SHAPE
     need = lib.ttt_causal_conv_partial_bytes(2, 9, 64, 4)
     assert need > 0 and lib.ttt_causal_conv_partial_bytes(2, 9, 64, 5) == 0
     assert b(bytes=need - 1) == E_WS and b(part=None) == E_WS and b(part=Q) == E_ALIGN and b(dx=None) == E_NULL
@@ -68,6 +71,12 @@ def test_scan(lib):
     for g in (f, b):
         assert g(L=0) == E_SHAPE and g(ldx=260) == E_SHAPE  # rows off 16 bytes
         assert g(x=Q) == E_ALIGN and g(b=Q) == E_ALIGN
+        # rows of a chunk beyond 32-bit offsets, where there is more than one
+        assert g(ldx=1 << 25) == E_SHAPE and g(ldb=1 << 25) == E_SHAPE and g(ldc=1 << 25) == E_SHAPE
+        assert g(ldx=1 << 25, L=1, A=None) == E_NULL
+        assert g(H=1 << 18, ldx=1 << 24) == E_SHAPE and g(B=1 << 24) == E_SHAPE  # too many for a grid
+    assert b(ldy=1 << 25) == E_SHAPE
+    assert s(B=1 << 23) == E_SHAPE
     assert s(b=P + 4) == E_ALIGN and s(ldb=130) == E_SHAPE and s(h=None) == E_NULL and s(h=Q) == E_ALIGN
     assert f(y=None) == E_NULL and f(h0=Q) == E_ALIGN
     need = lib.ttt_scan_states_bytes(2, 99, 4, 64, 64, BF16)

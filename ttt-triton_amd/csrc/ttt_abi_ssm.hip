@@ -26,12 +26,15 @@ size_t up256(size_t n) { return (n + 255) / 256 * 256; }
   } while (0)
 
 constexpr long long kMaxGrid = 0x7fffffffLL;
+constexpr long long kMaxThreads = 0xffffffffLL;  // of a launch
 
 // ---- convolution
 int check_conv(int B, int L, int C, int W, int act, int dtype) {
   if (!dtype_ok(dtype)) return TTT_ERR_DTYPE;
   if (B <= 0 || L <= 0 || C <= 0 || W < 2 || W > 4) return TTT_ERR_SHAPE;
-  if (L > 0x7fffff00 || (long long)B * ((L + 18) / 16) * ((C + 7) / 8) > kMaxGrid) return TTT_ERR_SHAPE;
+  // (the kernels' threads have four channels each and 16 tokens or, where that makes fewer
+  // threads than this by far, 8)
+  if (L > 0x7fffff00 || C > 1 << 22 || (long long)((L + 18) / 16) * ((C + 3) / 4) > kMaxThreads / B) return TTT_ERR_SHAPE;
   if (act != TTT_ACT_NONE && act != TTT_ACT_SILU) return TTT_ERR_ARG;
   return TTT_OK;
 }
@@ -41,11 +44,13 @@ int check_scan(int B, int L, int H, int P, int G, int N, int dtype, int dt_dtype
   if (!dtype_ok(dtype) || (dt_dtype != dtype && dt_dtype != TTT_DTYPE_F32)) return TTT_ERR_DTYPE;
   if (B <= 0 || L <= 0 || H <= 0 || G <= 0 || H % G != 0) return TTT_ERR_SHAPE;
   if ((P != 32 && P != 64) || N < 16 || N > 128 || N % 16 != 0) return TTT_ERR_SHAPE;
-  if (L > 0x7fffff00 || (long long)B * H > kMaxGrid) return TTT_ERR_SHAPE;
+  if (L > 0x7fffff00 || (long long)B * H > kMaxGrid || H > (1 << 23) / P || G > (1 << 23) / N) return TTT_ERR_SHAPE;
   return TTT_OK;
 }
-int check_row(long long ld, long long least, int dtype) {
-  return ld < least || ld * size_of(dtype) % 16 != 0 ? TTT_ERR_SHAPE : TTT_OK;
+// a chunk's rows, up to 64, are reached by 32-bit offsets
+int check_row(long long ld, long long least, int L, int dtype) {
+  if (ld < least || ld * size_of(dtype) % 16 != 0) return TTT_ERR_SHAPE;
+  return L > 1 && ld >= (1LL << 26) / size_of(dtype) ? TTT_ERR_SHAPE : TTT_OK;
 }
 constexpr int kSelfJoined = 8;  // segments whose states the walk's workgroups join themselves
 struct ScanPlan {
@@ -75,9 +80,10 @@ ScanPlan plan(int B, int L, int H, int P, int G, int N, int dtype) {
   s.split = s.splits > 1 ? (size_t)s.splits * B * L * G * N * 4 : 0;
   return s;
 }
+// (the backward's workgroups have up to 8 P threads)
 bool grid_ok(const ScanPlan& s, int B, int H, int P, int G) {
-  return (long long)B * H * s.S <= kMaxGrid && (long long)B * s.NC * G * s.splits <= kMaxGrid &&
-         (long long)B * s.NC <= kMaxGrid && (long long)B * H * P * s.NP / 1024 <= kMaxGrid && 3LL * H <= kMaxGrid;
+  return (long long)B * H * s.S <= kMaxThreads / (4 * P) && (long long)B * s.NC <= kMaxGrid &&
+         (long long)B * s.NC * G <= kMaxThreads / (8 * P) / s.splits;
 }
 bool plan_ok(int B, int L, int H, int P, int G, int N, int dtype, ScanPlan& s) {
   if (check_scan(B, L, H, P, G, N, dtype, dtype) != TTT_OK) return false;
@@ -221,9 +227,9 @@ int ttt_scan_fwd(const void* x, long long ldx, const void* dt, long long lddt, c
   const ScanPlan s = plan(B, L, H, P, G, N, dtype);
   if (!grid_ok(s, B, H, P, G)) return TTT_ERR_SHAPE;
   if (lddt < H) return TTT_ERR_SHAPE;
-  if ((st = check_row(ldx, (long long)H * P, dtype)) != TTT_OK) return st;
-  if ((st = check_row(ldb, (long long)G * N, dtype)) != TTT_OK) return st;
-  if ((st = check_row(ldc, (long long)G * N, dtype)) != TTT_OK) return st;
+  if ((st = check_row(ldx, (long long)H * P, L, dtype)) != TTT_OK) return st;
+  if ((st = check_row(ldb, (long long)G * N, L, dtype)) != TTT_OK) return st;
+  if ((st = check_row(ldc, (long long)G * N, L, dtype)) != TTT_OK) return st;
   REQUIRE(x, 16);
   REQUIRE(dt, size_of(dt_dtype));
   REQUIRE(A, 4);
@@ -282,10 +288,10 @@ int ttt_scan_bwd(const void* x, long long ldx, const void* dt, long long lddt, c
   const ScanPlan s = plan(B, L, H, P, G, N, dtype);
   if (!grid_ok(s, B, H, P, G)) return TTT_ERR_SHAPE;
   if (lddt < H) return TTT_ERR_SHAPE;
-  if ((st = check_row(ldx, (long long)H * P, dtype)) != TTT_OK) return st;
-  if ((st = check_row(ldy, (long long)H * P, dtype)) != TTT_OK) return st;
-  if ((st = check_row(ldb, (long long)G * N, dtype)) != TTT_OK) return st;
-  if ((st = check_row(ldc, (long long)G * N, dtype)) != TTT_OK) return st;
+  if ((st = check_row(ldx, (long long)H * P, L, dtype)) != TTT_OK) return st;
+  if ((st = check_row(ldy, (long long)H * P, L, dtype)) != TTT_OK) return st;
+  if ((st = check_row(ldb, (long long)G * N, L, dtype)) != TTT_OK) return st;
+  if ((st = check_row(ldc, (long long)G * N, L, dtype)) != TTT_OK) return st;
   REQUIRE(x, 16);
   REQUIRE(dt, size_of(dt_dtype));
   REQUIRE(A, 4);
@@ -370,7 +376,7 @@ int ttt_scan_step(const void* x, long long ldx, const void* dt, long long lddt, 
   const int st = check_scan(B, 1, H, P, G, N, dtype, dt_dtype);
   if (st != TTT_OK) return st;
   if (lddt < H || ldx < (long long)H * P || ldb < (long long)G * N || ldc < (long long)G * N) return TTT_ERR_SHAPE;
-  if ((long long)B * H * P / 8 > kMaxGrid) return TTT_ERR_SHAPE;
+  if ((long long)B * H * P > kMaxThreads / 32) return TTT_ERR_SHAPE;
   const size_t n = size_of(dtype);
   if (ldb * n % (4 * n) != 0 || ldc * n % (4 * n) != 0) return TTT_ERR_SHAPE;  // four values at a time
   REQUIRE(x, n);

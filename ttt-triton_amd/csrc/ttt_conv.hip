@@ -22,10 +22,10 @@ namespace ttt {
 namespace {
 
 constexpr int kV = 4;
-constexpr int kRun = 16;     // tokens of a thread's run in the forward
 constexpr int kLanes = 32;   // backward: channel groups (of V) per workgroup
 constexpr int kSubs = 256 / kLanes;  // and runs
-constexpr int kRunBwd = 32;  // and tokens of a run
+constexpr int kRunBwd = 32;  // and tokens of a run (32,768 x 896 in bf16: 61 us with 16, 59 with 32, 57 with 64,
+                             // which would halve the workgroups of short batches)
 
 // row u of s, n of its channels from c on; zeros outside
 template <typename T>
@@ -57,7 +57,10 @@ template <int W> struct Taps {
   }
 };
 
-template <typename T, int W, bool ACT>
+// RUN tokens to a thread: 16, or 8 where those are not enough threads for 16 waves to a
+// compute unit (1,021 x 3 tokens of 999 channels in fp32: 11 and 18 us; 32,768 of 896 in
+// bf16: 33 and 31)
+template <typename T, int W, bool ACT, int RUN>
 __global__ __launch_bounds__(256) void conv_fwd_kernel(ConvParams p, int groups, int runs, long long threads) {
   const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
   if (id >= threads) return;
@@ -68,12 +71,12 @@ __global__ __launch_bounds__(256) void conv_fwd_kernel(ConvParams p, int groups,
   const int c = kV * cg, n = min(kV, p.C - c);
   Taps<W> tp;
   tp.load(p, c, n);
-  const int u0 = run * kRun, last = p.L + W - 1;
+  const int u0 = run * RUN, last = p.L + W - 1;
   Raw<T, kV> win[W];
 #pragma unroll
   for (int k = 0; k < W - 1; ++k) win[k + 1] = seen_row<T>(p, b, u0 - (W - 1) + k, c, n);
 #pragma unroll
-  for (int i = 0; i < kRun; ++i) {
+  for (int i = 0; i < RUN; ++i) {
     const int u = u0 + i;
     if (u < last) {
 #pragma unroll
@@ -255,12 +258,16 @@ __global__ __launch_bounds__(256) void conv_step_kernel(ConvParams p, int groups
   for (int k = 0; k < W - 1; ++k) win[k + 1].store(st + (long long)k * p.C, n);
 }
 
-template <typename T, int W, bool ACT> hipError_t fwd_t(const ConvParams& p, hipStream_t stream) {
-  const int groups = (p.C + kV - 1) / kV, runs = (p.L + W - 1 + kRun - 1) / kRun;
+template <typename T, int W, bool ACT, int RUN> hipError_t fwd_run(const ConvParams& p, hipStream_t stream) {
+  const int groups = (p.C + kV - 1) / kV, runs = (p.L + W - 1 + RUN - 1) / RUN;
   const long long threads = (long long)p.B * runs * groups;
-  hipLaunchKernelGGL((conv_fwd_kernel<T, W, ACT>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, stream, p,
+  hipLaunchKernelGGL((conv_fwd_kernel<T, W, ACT, RUN>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, stream, p,
                      groups, runs, threads);
   return hipGetLastError();
+}
+template <typename T, int W, bool ACT> hipError_t fwd_t(const ConvParams& p, hipStream_t stream) {
+  const long long threads = (long long)p.B * ((p.L + 18) / 16) * ((p.C + kV - 1) / kV);
+  return threads >= 256 * 16 * 64 ? fwd_run<T, W, ACT, 16>(p, stream) : fwd_run<T, W, ACT, 8>(p, stream);
 }
 template <typename T, int W, bool ACT> hipError_t bwd_t(const ConvParams& p, hipStream_t stream) {
   const int groups = (p.C + kV - 1) / kV, runs = (p.L + W - 1 + kRunBwd - 1) / kRunBwd;

@@ -245,8 +245,17 @@ __global__ __launch_bounds__(256) void norm_param_grads_kernel(NormParams p, int
 template <typename T, int NW, int V, int NCH, bool GATE>
 hipError_t run_t(const NormParams& p, bool bwd, hipStream_t stream) {
   if (!bwd) {
-    const long long blocks = NW == 1 ? (p.R + 3) / 4 : p.R;
-    hipLaunchKernelGGL((norm_fwd_kernel<T, NW, V, NCH, GATE>), dim3((unsigned)blocks), dim3(threads_of(NW)), 0, stream, p);
+    constexpr long long kRows = 0xffffffffLL / (64 * NW) / 4 * 4;  // of a launch: 2^32 threads
+    for (long long r0 = 0; r0 < p.R; r0 += kRows) {
+      NormParams q = p;
+      q.R = std::min(kRows, p.R - r0);
+      q.x = static_cast<const T*>(p.x) + r0 * p.ldx;
+      q.gate = static_cast<const T*>(p.gate) + (GATE ? r0 * p.ldg : 0);
+      q.y = static_cast<T*>(p.y) + r0 * p.D;
+      q.stats = p.stats != nullptr ? p.stats + 2 * r0 : nullptr;
+      const long long blocks = NW == 1 ? (q.R + 3) / 4 : q.R;
+      hipLaunchKernelGGL((norm_fwd_kernel<T, NW, V, NCH, GATE>), dim3((unsigned)blocks), dim3(threads_of(NW)), 0, stream, q);
+    }
     return hipGetLastError();
   }
   const int parts = norm_bwd_parts(p.R, p.D);

@@ -214,7 +214,7 @@ template <typename T, int ROWS, int COLS, int NT> struct Stage {
   __device__ __forceinline__ void place(long long ld, int n) {
     cols = n;
 #pragma unroll
-    for (int i = 0; i < CNT; ++i) off[i] = (unsigned)(row(i) * (int)ld + col(i)) * (unsigned)sizeof(T);
+    for (int i = 0; i < CNT; ++i) off[i] = ((unsigned)row(i) * (unsigned)ld + (unsigned)col(i)) * (unsigned)sizeof(T);
   }
   __device__ __forceinline__ static bool has() { return ALL % NT == 0 || (int)threadIdx.x < ALL; }
   __device__ __forceinline__ static u4v get(const char* q, unsigned o) {

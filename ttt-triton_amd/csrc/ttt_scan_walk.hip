@@ -117,8 +117,8 @@ __global__ __launch_bounds__(4 * P, NP == 128 || ScanType<T>::IN > 1 ? 1 : 3) vo
   const T *xp = X + t00 * ldx, *kp = Key + t00 * ldk, *qp = Query + t00 * ldq;
   char* yp = reinterpret_cast<char*>(Y + (t00 * p.H + h) * P);
   const long long xstep = dir * ldx, kstep = dir * ldk, qstep = dir * ldq, ystep = dir * p.H * P * (int)sizeof(T);
-  const unsigned ylane = (unsigned)((r * p.H * P + 16 * w + 4 * g) * (int)sizeof(T));  // in the rows of y
-  const unsigned yblock = (unsigned)(16 * p.H * P * (int)sizeof(T));
+  const unsigned ylane = (unsigned)(r * p.H * P + 16 * w + 4 * g) * (unsigned)sizeof(T);  // in the rows of y
+  const unsigned yblock = (unsigned)(16 * p.H * P) * (unsigned)sizeof(T);
   const auto fetch = [&](int k, Stage<T, Q, P, NT>& x, Stage<T, Q, NP, NT>& key) {
     const int left = min(Q, p.L - chunk(k) * Q);
     x.load(xp, left);

@@ -11,14 +11,14 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._common import check_device, dtype_code, on_device
-from .ssm import _as, _bytes, _opt, _param, _rows, _stream, _wants_grad
+from .ssm import _as, _bytes, _empty, _opt, _param, _rows, _stream, _wants_grad
 
 LAYER_NORM_EPS = 1e-6
 MAX_WIDTH = 16384
 
 
-def _norm_forward(x, weight, bias, gate, eps, train):
-    """(y, what the backward reads)"""
+def _norm_args(x, weight, bias, gate, eps):
+    """(device, code of x, weight, bias)"""
     D = x.shape[-1] if x.dim() else 0
     if not 1 <= D <= MAX_WIDTH:
         raise ValueError(f"layer_norm takes rows of 1 to {MAX_WIDTH} values, got {list(x.shape)}")
@@ -29,8 +29,13 @@ def _norm_forward(x, weight, bias, gate, eps, train):
     if not 0.0 < eps <= 1.0:
         raise ValueError(f"eps must be in (0, 1], got {eps}")
     dev = check_device(x, *(t for t in (weight, bias, gate) if t is not None))
-    code = dtype_code(x.dtype)
-    w, b = _param(weight, (D,), "weight"), _param(bias, (D,), "bias")
+    return dev, dtype_code(x.dtype), _param(weight, (D,), "weight"), _param(bias, (D,), "bias")
+
+
+def _norm_forward(x, weight, bias, gate, eps, train):
+    """(y, what the backward reads)"""
+    dev, code, w, b = _norm_args(x, weight, bias, gate, eps)
+    D = x.shape[-1]
     lead, es = x.dim() - 1, x.element_size()
     xr, ldx = _rows(x, lead, es)
     gr, ldg = (None, 0) if gate is None else _rows(gate, lead, es)
@@ -91,7 +96,8 @@ def layer_norm(x, weight=None, bias=None, gate=None, eps: float = LAYER_NORM_EPS
     dtype is given.  weight and bias [D], both or neither; the variance is the biased
     one.  x and gate may be columns of a wider matrix."""
     if x.dim() and x.numel() == 0 and x.shape[-1]:
-        return x.clone()
+        _norm_args(x, weight, bias, gate, eps)
+        return _empty(x, weight, bias, gate)
     if _wants_grad(x, weight, bias, gate):
         return LayerNormFunction.apply(x, weight, bias, gate, eps)
     return _norm_forward(x, weight, bias, gate, eps, False)[0]

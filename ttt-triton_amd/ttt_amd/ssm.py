@@ -94,6 +94,15 @@ def _param(t, shape, name):
     return t if t.dtype == torch.float32 and t.is_contiguous() else f32c(t)
 
 
+def _empty(x, *params):
+    """The result over no tokens or values, of x's shape; the parameters' gradients are 0."""
+    y = x.clone()
+    for t in params:
+        if t is not None and t.requires_grad:
+            y = y + (t.sum() * 0).to(y.dtype)
+    return y
+
+
 def _wants_grad(*ts) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
 
@@ -199,9 +208,12 @@ def causal_conv(x, weight, bias=None, initial_state=None, activation=None, retur
     return_final_state the last W-1 inputs [B,W-1,C] as well: the state that
     causal_conv_step and a later call go on from."""
     if x.dim() == 3 and x.numel() == 0:
-        W = weight.shape[-1]
-        first = x.new_zeros(x.shape[0], W - 1, x.shape[2]) if initial_state is None else initial_state.to(x.dtype)
-        return (x.clone(), first.clone()) if return_final_state else x.clone()
+        _, _, C, W, _, _ = _conv_args(x, weight, bias, initial_state, activation, 2)
+        shape = (x.shape[0], W - 1, C)
+        _conv_state(initial_state, shape, x.dtype)
+        first = x.new_zeros(shape) if initial_state is None else initial_state.to(x.dtype).clone()
+        y = _empty(x, weight, bias)
+        return (y, first) if return_final_state else y
     if _wants_grad(x, weight, bias, initial_state):
         y, last = CausalConvFunction.apply(x, weight, bias, initial_state, activation, return_final_state)
     else:
@@ -263,21 +275,32 @@ def _scan_args(x, dt, A, Bm, Cm, D, dt_bias, state, lead):
             _param(D, (H,), "D"), _param(dt_bias, (H,), "dt_bias"))
 
 
+def _scan_state(h0, shape):
+    if h0 is None:
+        return None
+    if tuple(h0.shape) != shape:
+        raise ValueError(f"initial_state must be [B,H,P,N]={list(shape)}, got {list(h0.shape)}")
+    return f32c(h0)
+
+
 def _scan_rows(x, dt, Bm, Cm, lead, align):
     """The four inputs and their row strides as the kernels take them."""
     out = []
     for t, al in ((x, align), (dt, dt.element_size()), (Bm, align), (Cm, align)):
-        out += _rows(t, lead, al)
+        out += _rows(t, lead, al) if t is dt or lead == 1 else _near_rows(t, al)
     return out
+
+
+def _near_rows(t, align):
+    """_rows of [B,L,..], copied too where the rows of a chunk are out of a 32-bit offset's reach"""
+    r, ld = _rows(t, 2, align)
+    return _rows(t.detach().contiguous(), 2, align) if ld * t.element_size() >= 1 << 26 and t.shape[1] > 1 else (r, ld)
 
 
 def _scan_forward(x, dt, A, Bm, Cm, D, dt_bias, h0, softplus, want_last, train):
     """(y, last state or None, what the backward reads)"""
     dev, (B, L, H, P, G, N), code, dcode, a, d, bias = _scan_args(x, dt, A, Bm, Cm, D, dt_bias, h0, 2)
-    if h0 is not None:
-        if tuple(h0.shape) != (B, H, P, N):
-            raise ValueError(f"initial_state must be [B,H,P,N]={[B, H, P, N]}, got {list(h0.shape)}")
-        h0 = f32c(h0)
+    h0 = _scan_state(h0, (B, H, P, N))
     rows = _scan_rows(x, dt, Bm, Cm, 2, 16)
     xr, ldx, dr, ldd, br, ldb, cr, ldc = rows
     y = torch.empty((B, L, H, P), device=dev, dtype=x.dtype)
@@ -320,7 +343,7 @@ class SelectiveScanFunction(torch.autograd.Function):
         dev, act = x.device, x.dtype
         code = dtype_code(act)
         dy = torch.zeros((B, L, H, P), device=dev, dtype=act) if dy is None else dy
-        dyr, ldy = _rows(dy if dy.dtype == act else dy.to(act), 2, 16)
+        dyr, ldy = _near_rows(dy.to(act), 16)
         dlast = None if dlast is None else f32c(dlast)
         f32 = dict(device=dev, dtype=torch.float32)
         dx = torch.empty((B, L, H, P), device=dev, dtype=act)
@@ -352,10 +375,11 @@ def selective_scan(x, dt, A, Bm, Cm, D=None, dt_bias=None, initial_state=None, d
     selective_scan_step and a later call go on from.  A step of 0 (dt = -inf under
     the softplus) leaves the state as it is."""
     if x.dim() == 4 and x.numel() == 0:
-        B, _, H, P = x.shape
-        N = Bm.shape[-1]
-        first = torch.zeros(B, H, P, N, device=x.device) if initial_state is None else initial_state.float()
-        return (x.clone(), first.clone()) if return_final_state else x.clone()
+        dev, (B, _, H, P, _, N), *_ = _scan_args(x, dt, A, Bm, Cm, D, dt_bias, initial_state, 2)
+        _scan_state(initial_state, (B, H, P, N))
+        first = torch.zeros(B, H, P, N, device=dev) if initial_state is None else initial_state.float().clone()
+        y = _empty(x, dt, A, Bm, Cm, D, dt_bias)
+        return (y, first) if return_final_state else y
     if _wants_grad(x, dt, A, Bm, Cm, D, dt_bias, initial_state):
         y, last = SelectiveScanFunction.apply(x, dt, A, Bm, Cm, D, dt_bias, initial_state, bool(dt_softplus),
                                               return_final_state)
