@@ -19,7 +19,11 @@ Per layer call, for hidden states x [B, L, D] (D = H*F):
      gives that token's output and every gradient unchanged (the other rows'
      outputs are never read, so their gradients are exact zeros).
 
-Parameter names and shapes are the reference's (wq ... wu, wo,
+SelectiveSSM is a third layer type beside them, a selective state-space layer on the
+same projection GEMM and heads: short causal convolution, scan and gated norm (ssm.py,
+norm.py), with a form for single tokens that goes on from a prompt's state.
+
+Parameter names and shapes of the TTT layers are the reference's (wq ... wu, wo,
 learnable_ttt_lr_weight [H,1,D], learnable_ttt_lr_bias [H,1],
 ttt_norm_weight/bias [H,F], post_norm, W1/b1/W2/b2), so a reference state
 dict loads unchanged.  Shapes the layer takes (ModelConfig raises ValueError
@@ -44,6 +48,8 @@ from .layer_io import POST_NORM_EPS, RECON_EPS, PostNormFunction, ProducerFuncti
 from .linear import TTTLinearFunction
 from .memo import mlp_memo_combine
 from .mlp import LN_EPS, TTTMLPFunction
+from .norm import layer_norm
+from .ssm import CONV_WIDTHS, MAX_STATE, causal_conv, causal_conv_step, selective_scan, selective_scan_step
 
 MAX_MODEL_DIM = 1024  # H * F, the widest row the producer / post-norm kernels take
 
@@ -119,6 +125,11 @@ class ModelConfig:
     latent_width: int = 1
     theta: float = 10000.0
     compressed_num_frames: Optional[int] = None
+    # ssm_layer "selective_scan": the state's width, the groups of heads that share B
+    # and C, and the convolution's width
+    state_dim: int = 64
+    num_groups: int = 1
+    conv_width: int = 4
 
     def __post_init__(self):
         if self.compressed_num_frames is None:
@@ -139,6 +150,13 @@ class ModelConfig:
             raise ValueError(f"model_dim {self.model_dim} > {MAX_MODEL_DIM}, the widest the layer kernels take")
         if self.mini_batch_size % 16 or not 16 <= self.mini_batch_size <= 64:
             raise ValueError(f"mini_batch_size {self.mini_batch_size}: a multiple of 16 from 16 to 64 is needed")
+        if self.ssm_layer == "selective_scan":
+            if self.state_dim % 16 or not 16 <= self.state_dim <= MAX_STATE:
+                raise ValueError(f"state_dim {self.state_dim}: a multiple of 16 up to {MAX_STATE} is needed")
+            if self.num_groups < 1 or self.num_heads % self.num_groups:
+                raise ValueError(f"num_groups {self.num_groups} must divide the {self.num_heads} heads")
+            if self.conv_width not in CONV_WIDTHS:
+                raise ValueError(f"conv_width {self.conv_width}: one of {CONV_WIDTHS} is needed")
 
 
 class TTTLayerBase(nn.Module):
@@ -271,8 +289,117 @@ class TTTMLP(TTTLayerBase):
         return out
 
 
+@dataclass
+class SSMCache:
+    """What a prompt leaves behind for the next token: the convolution's last inputs
+    [B, W-1, C] and the scan's states [B,H,F,N] fp32.  SelectiveSSM.step updates
+    both in place."""
+    conv: torch.Tensor
+    state: torch.Tensor
+
+
+class SelectiveSSM(nn.Module):
+    """A selective state-space layer: per token one projection to z | x | B | C | dt,
+    a short causal convolution with SiLU over x | B | C, the scan with one decay a
+    head, LayerNorm of y silu(z), and the output projection.
+
+    forward takes any sequence length; prompt also returns the cache that step goes
+    on from, one token a call.  (`rope` is the other layers' and is not read: the
+    scan's decays carry the order.)"""
+
+    def __init__(self, config: ModelConfig):
+        super().__init__()
+        self.config = config
+        self.width, self.num_heads = config.model_dim, config.num_heads
+        self.head_dim = config.model_dim // config.num_heads
+        self.groups, self.state_dim = config.num_groups, config.state_dim
+        D, H = self.width, self.num_heads
+        self.conv_channels = D + 2 * self.groups * self.state_dim
+        self.in_proj = nn.Linear(D, D + self.conv_channels + H, bias=True)
+        self.conv_weight = nn.Parameter(torch.empty(self.conv_channels, config.conv_width))
+        self.conv_bias = nn.Parameter(torch.zeros(self.conv_channels))
+        self.A_log = nn.Parameter(torch.empty(H))
+        self.D = nn.Parameter(torch.ones(H))
+        self.dt_bias = nn.Parameter(torch.empty(H))
+        self.post_norm = nn.LayerNorm(D, eps=POST_NORM_EPS)
+        self.wo = nn.Linear(D, D, bias=True)
+        pad = _padded_width(self.in_proj.out_features) - self.in_proj.out_features
+        self.register_buffer("_proj_pad_w", torch.zeros(pad, D), persistent=False)
+        self.register_buffer("_proj_pad_b", torch.zeros(pad), persistent=False)
+        self.init_weights()
+
+    def init_weights(self):
+        """Rates of 1 to 16, and steps of 0.001 to 0.1 (spread over the logarithm) where the
+        projection gives 0: heads that forget within ten tokens to within a thousand."""
+        for lin in (self.in_proj, self.wo):
+            nn.init.normal_(lin.weight, mean=0.0, std=0.02)
+            nn.init.zeros_(lin.bias)
+        bound = self.config.conv_width ** -0.5
+        nn.init.uniform_(self.conv_weight, -bound, bound)
+        nn.init.zeros_(self.conv_bias)
+        nn.init.ones_(self.D)
+        self.post_norm.reset_parameters()
+        with torch.no_grad():
+            self.A_log.copy_(torch.log(torch.empty_like(self.A_log).uniform_(1.0, 16.0)))
+            step = torch.exp(torch.empty_like(self.dt_bias).uniform_(math.log(1e-3), math.log(0.1)))
+            self.dt_bias.copy_(torch.log(torch.expm1(step)))
+
+    def _project(self, x: torch.Tensor):
+        """(z [.., D], x | B | C [.., C], dt [.., H]): columns of one projection"""
+        D, C = self.width, self.conv_channels
+        w, b = self.in_proj.weight, self.in_proj.bias
+        if self._proj_pad_w.shape[0]:
+            w = torch.cat([w, self._proj_pad_w.to(w.dtype)])
+            b = torch.cat([b, self._proj_pad_b.to(b.dtype)])
+        p = projection(x, w, b)
+        return p[..., :D], p[..., D:D + C], p[..., D + C:D + C + self.num_heads]
+
+    def _heads(self, xbc: torch.Tensor):
+        """x [.., H, F], B and C [.., G, N]"""
+        D, n = self.width, self.groups * self.state_dim
+        x, b, c = xbc[..., :D], xbc[..., D:D + n], xbc[..., D + n:]
+        return (x.unflatten(-1, (self.num_heads, self.head_dim)),
+                *(t.unflatten(-1, (self.groups, self.state_dim)) for t in (b, c)))
+
+    def _rates(self):
+        return -torch.exp(self.A_log.float())
+
+    def _out(self, y: torch.Tensor, z: torch.Tensor):
+        h = layer_norm(y.flatten(-2), self.post_norm.weight, self.post_norm.bias, gate=z, eps=POST_NORM_EPS)
+        return self.wo(h)
+
+    def _run(self, x: torch.Tensor, cache: Optional[SSMCache], keep: bool, last_only: bool):
+        z, xbc, dt = self._project(x)
+        first = (None, None) if cache is None else (cache.conv, cache.state)
+        xbc, conv = causal_conv(xbc, self.conv_weight, self.conv_bias, first[0], "silu", True)
+        xs, b, c = self._heads(xbc)
+        y, state = selective_scan(xs, dt, self._rates(), b, c, self.D, self.dt_bias, first[1], True, True)
+        if last_only:  # the norm and the output projection are by tokens
+            y, z = y[:, -1], z[:, -1]
+        return self._out(y, z), SSMCache(conv, state) if keep else None
+
+    def forward(self, x: torch.Tensor, rope: Optional[torch.Tensor] = None, last_only: bool = False):
+        """[B, L, D], or with last_only the last token's output [B, D]."""
+        return self._run(x, None, False, last_only)[0]
+
+    def prompt(self, x: torch.Tensor, cache: Optional[SSMCache] = None, last_only: bool = False):
+        """(forward's output, the cache behind x), from an empty cache or a given one (which
+        is left as it is)."""
+        return self._run(x, cache, True, last_only)
+
+    @torch.no_grad()
+    def step(self, x: torch.Tensor, cache: SSMCache):
+        """One token x [B, D] of every sequence: its output [B, D], the cache moved on in place."""
+        z, xbc, dt = self._project(x)
+        xbc = causal_conv_step(xbc, cache.conv, self.conv_weight, self.conv_bias, "silu")
+        xs, b, c = self._heads(xbc)
+        y = selective_scan_step(xs, dt, self._rates(), b, c, cache.state, self.D, self.dt_bias)
+        return self._out(y, z)
+
+
 class TTTWrapper(nn.Module):
-    """ttt_layer.py:20-57: the layer and its rotary table."""
+    """ttt_layer.py:20-57: the layer and its rotary table.  ssm_layer "selective_scan" is a
+    SelectiveSSM in the same place."""
 
     def __init__(self, config: ModelConfig):
         super().__init__()
@@ -281,6 +408,8 @@ class TTTWrapper(nn.Module):
             self.ttt = TTTLinear(config)
         elif config.ssm_layer == "ttt_mlp":
             self.ttt = TTTMLP(config)
+        elif config.ssm_layer == "selective_scan":
+            self.ttt = SelectiveSSM(config)
         else:
             raise TypeError(f"no ttt layer of type {config.ssm_layer}")
         self.register_buffer("rope", self._rope(), persistent=False)
@@ -311,8 +440,29 @@ class TTTForecaster(nn.Module):
     def forward(self, seq_x: torch.Tensor) -> torch.Tensor:
         h = projection(seq_x, self.in_proj.weight, self.in_proj.bias)  # self.in_proj(seq_x)
         h = self.ttt(h, last_only=True)  # the head reads h[:, -1] only
-        out = self.head(h)
-        return out.view(seq_x.size(0), self.pred_len, self.d_out)
+        return self._forecast(h)
+
+    def _forecast(self, h: torch.Tensor) -> torch.Tensor:
+        return self.head(h).view(h.size(0), self.pred_len, self.d_out)
+
+    def _ssm(self) -> SelectiveSSM:
+        layer = self.ttt.ttt
+        if not isinstance(layer, SelectiveSSM):
+            raise TypeError("a forecast that goes on token by token needs ssm_layer 'selective_scan'")
+        return layer
+
+    def prompt(self, seq_x: torch.Tensor, cache: Optional[SSMCache] = None):
+        """(forward's forecast [B, pred_len, d_out] behind seq_x [B, L, d_in], the cache that
+        step goes on from); ssm_layer "selective_scan" only."""
+        layer = self._ssm()
+        h, cache = layer.prompt(projection(seq_x, self.in_proj.weight, self.in_proj.bias), cache, last_only=True)
+        return self._forecast(h), cache
+
+    @torch.no_grad()
+    def step(self, x: torch.Tensor, cache: SSMCache):
+        """The forecast behind one more observation x [B, d_in] of every series."""
+        layer = self._ssm()
+        return self._forecast(layer.step(projection(x, self.in_proj.weight, self.in_proj.bias), cache))
 
 
-__all__ = ["ModelConfig", "TTTLinear", "TTTMLP", "TTTWrapper", "TTTForecaster"]
+__all__ = ["ModelConfig", "TTTLinear", "TTTMLP", "SelectiveSSM", "SSMCache", "TTTWrapper", "TTTForecaster"]
