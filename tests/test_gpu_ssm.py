@@ -414,3 +414,21 @@ def test_conv_of_a_large_batch(lib, dt):
     for b in (0, 17, 32):
         y1, last1 = causal_conv(x[b:b + 1], w, None, None, "silu", True)
         assert torch.equal(y[b:b + 1], y1) and torch.equal(last[b:b + 1], last1)
+
+
+@pytest.mark.parametrize("dt", T.DTYPES)
+def test_skip_gradient_over_many_tokens(lib, dt):
+    """dD is a sum of 131,072 products a head.  In steps rounded to nearest its error is that of
+    sums of 1,024 of them, 15 roundings of half a step of 2^-24 each: relative to the root of
+    the sum of the squares, the root of 15 half steps, and no more for more tokens; twice the
+    root is 8."""
+    from ttt_amd.ssm import selective_scan
+    torch.manual_seed(5)
+    B, L, H, P, N = 8, 512, 8, 32, 32
+    x, dy = (torch.randn(B, L, H, P, device="cuda").to(dt) for _ in range(2))
+    b, c = (torch.randn(B, L, 1, N, device="cuda").to(dt) for _ in range(2))
+    D = torch.ones(H, device="cuda", requires_grad=True)
+    y = selective_scan(x, torch.zeros(B, L, H, device="cuda").to(dt), -torch.ones(H, device="cuda"), b, c, D)
+    (got,) = torch.autograd.grad(y, D, dy)
+    terms = (x.double() * dy.double()).permute(2, 0, 1, 3).flatten(1)
+    assert ((got.double() - terms.sum(1)).abs() <= 8 * 2.0 ** -24 * terms.square().sum(1).sqrt()).all()

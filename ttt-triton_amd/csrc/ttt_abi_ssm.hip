@@ -57,9 +57,19 @@ struct ScanPlan {
   int Q, NC, NP, S, per, splits;
   size_t states, seg, decay, partial, split;
 };
-// How a scan is cut up.  Segments: a workgroup walks a sequence and head; below 768
-// of them (three a compute unit, of 64 features; twice as many of 32) the tokens are
-// shared out as well, whole chunks each, to at most that many.
+// Workgroups of the walk that a compute unit holds, by its registers and LDS
+int walk_resident(int P, int NP, int dtype) {
+  constexpr signed char t[2][3][3] = {{{5, 3, 5}, {4, 2, 3}, {2, 3, 2}}, {{3, 3, 4}, {3, 2, 3}, {2, 2, 2}}};
+  return t[P == 64][NP == 32 ? 0 : NP == 64 ? 1 : 2][dtype == TTT_DTYPE_BF16 ? 0 : dtype == TTT_DTYPE_F16 ? 1 : 2];
+}
+// How a scan is cut up.  Segments: a workgroup walks a sequence and head; where that
+// makes too few of them, the tokens are shared out as well, whole chunks each, to at
+// most the full rounds of the card nearest above three workgroups of 64 features or
+// five of 32 a compute unit.  (Forward and backward of 32,768 tokens: 768 at once, 12 heads of
+// 64 x 64 in bf16: 322, 296 and 318 us with 3, 4 and 6 segments; 512 at once, in fp16: 480,
+// 449, 422, 435 with 3, 4, 5, 6; 1,024 at once, 24 heads of 32 x 64: 484, 463, 430, 447 with
+// 3, 4, 5, 8.)  More segments than a workgroup joins by itself cost two launches: not where 8
+// fill three quarters of the card (128 chains of 32 x 64: 166 us with 8 and 189 with 11).
 // Splits: the backward's workgroups have a chunk and go over a group's heads; below
 // 512 of them the heads are shared out.
 ScanPlan plan(int B, int L, int H, int P, int G, int N, int dtype) {
@@ -68,7 +78,10 @@ ScanPlan plan(int B, int L, int H, int P, int G, int N, int dtype) {
   s.Q = ttt::scan_chunk(dtype, s.NP);
   s.NC = (L + s.Q - 1) / s.Q;
   const long long chains = (long long)B * H;
-  const long long want = std::max(1LL, std::min<long long>(s.NC, (P == 64 ? 768 : 1536) / chains));
+  const int at_once = 256 * walk_resident(P, s.NP, dtype), least = P == 64 ? 768 : 1280;
+  const int most = (least + at_once - 1) / at_once * at_once;
+  long long want = std::max(1LL, std::min<long long>(s.NC, most / chains));
+  if (want > kSelfJoined && 4 * kSelfJoined * chains >= 3 * at_once) want = kSelfJoined;
   s.per = (int)((s.NC + want - 1) / want);
   s.S = (s.NC + s.per - 1) / s.per;
   const long long groups = (long long)B * s.NC * G;

@@ -240,6 +240,19 @@ template <typename T, int ROWS, int COLS, int NT> struct Stage {
 #pragma unroll
     for (int i = 0; i < CNT; ++i) asm volatile("" : "+v"(v[i]));
   }
+  // the sum of a thread's values times those of another
+  __device__ __forceinline__ float dot(const Stage& o) const {
+    float s = 0.f;
+    if (!has()) return s;
+    typedef T tv __attribute__((ext_vector_type(VE)));
+#pragma unroll
+    for (int i = 0; i < CNT; ++i) {
+      const tv a = __builtin_bit_cast(tv, v[i]), b = __builtin_bit_cast(tv, o.v[i]);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) s = __builtin_fmaf((float)a[e], (float)b[e], s);
+    }
+    return s;
+  }
   template <int PL> __device__ __forceinline__ void store(Planes<PL, ROWS, COLS>& m) const {
     if (!has()) return;
 #pragma unroll

@@ -25,10 +25,19 @@ namespace ttt {
 
 namespace {
 
-// waves for 16 features: two in fp32, whose chunks of 32 tokens give one little to do
-// (measured at 16,384 tokens, 4 heads of 32, N 32: 27 us with one, 20 with two; bf16 at 32,768
-// tokens, 12 heads of 64, N 64 the other way round: 106 and 127)
-template <typename T> constexpr int kRoles = ScanType<T>::IN == 3 ? 2 : 1;
+// Waves for 16 features, one or two: two where a workgroup has two waves for its features
+// and the state of each is small, and where one would hold two planes of everything.
+// us with one and with two, 32,768 tokens (fp32 16,384), 12 heads of 64 or 24 of 32:
+//              N 32        64        128
+//   P 32 bf16  165 125   192 234   150 181 (16,384 tokens)
+//        fp16  185 134   221 266
+//        fp32  128 108   170 139   217 280
+//   P 64 bf16   85 117   106 127   204 536
+//        fp16  101 138   206 169   244 322
+//        fp32   75 102    95 130   184 188
+template <typename T, int P, int NP>
+constexpr int kRoles = P == 32 ? (NP == 32 || (NP == 64 && ScanType<T>::IN == 3) ? 2 : 1)
+                               : (NP == 64 && ScanType<T>::IN == 2 ? 2 : 1);
 
 template <typename T, int P, int NP> struct BwdShared {
   static constexpr int IN = ScanType<T>::IN, MID = ScanType<T>::MID, Q = chunk_of<T, NP>(), TB = Q / 16;
@@ -43,7 +52,7 @@ template <typename T, int P, int NP> struct BwdShared {
   struct Head {
     float row[TILES][16], col[TILES][16];
     float u[NB][Q], v[NB][Q];
-    float dD[W * kRoles<T>], gh[W];
+    float dD[W * kRoles<T, P, NP>], gh[W];
   } head[2];
 };
 
@@ -125,7 +134,7 @@ __device__ __forceinline__ void steps_grad(const ScanParams& p, const BwdShared<
     if (k < NB) gh += s.gh[k];  // (waves that share a block of columns count it once)
   }
 #pragma unroll
-  for (int k = 0; k < W * kRoles<T>; ++k) dsum += s.dD[k];
+  for (int k = 0; k < W * kRoles<T, P, NP>; ++k) dsum += s.dD[k];
   // rows from t on of the blocks left of t's, and whole blocks left of and below it
   const float d = in ? dec.d[t] : 0.f;
 #pragma unroll
@@ -254,6 +263,10 @@ __global__ __launch_bounds__(4 * P * ROLES) void scan_bwd_kernel(ScanParams p) {
     const Decays<Q>& dec = sh.dec[h % 3];
     sx.store(sh.x);
     sdy.store(sh.dy);
+    // The sum of x dy, for dD: not from the diagonal of the tiles below.  The matrix
+    // instruction's sums are cut off rather than rounded, which adds up over the tokens of
+    // all sequences: 1.0e-6 off that way at 16,384 tokens, 4 heads of 32
+    float xdy = sx.dot(sdy);
     __syncthreads();
     if (h + 1 < h1) {
       if (fills) decays(h + 1, bits2);
@@ -279,7 +292,6 @@ __global__ __launch_bounds__(4 * P * ROLES) void scan_bwd_kernel(ScanParams p) {
       if (l == 0) hd.gh[wr] = s;
     }
 
-    float dd = 0.f;
 #pragma unroll
     for (int k = 0; k < OWN; ++k) {
       const int t = w + WAVES * k, ib = tri_row(t), jb = t - tri(ib, 0);
@@ -295,10 +307,7 @@ __global__ __launch_bounds__(4 * P * ROLES) void scan_bwd_kernel(ScanParams p) {
         for (int e = 0; e < 4; ++e) wv[e] = __builtin_amdgcn_exp2f((ih[e] - jh) + (il[e] - jl)) * xy[e];
         if (ib == jb) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            wv[e] = only_if(4 * g + e >= r, wv[e]);
-            if (4 * g + e == r) dd += xy[e];
-          }
+          for (int e = 0; e < 4; ++e) wv[e] = only_if(4 * g + e >= r, wv[e]);
         }
         f4 pass = wv * cb[k];
         bf4 ow[MID];
@@ -322,8 +331,8 @@ __global__ __launch_bounds__(4 * P * ROLES) void scan_bwd_kernel(ScanParams p) {
         if (r == 0) *reinterpret_cast<f4*>(&hd.row[t][4 * g]) = pass;
       }
     }
-    dd = sum_wave(dd);
-    if (l == 0) hd.dD[w] = dd;
+    xdy = sum_wave(xdy);
+    if (l == 0) hd.dD[w] = xdy;
     __syncthreads();
 
     if (hasB) {  // rows are columns n of B, columns tokens j
@@ -448,13 +457,14 @@ __global__ __launch_bounds__(256) void scan_param_grads_kernel(ScanParams p, int
   float* out = k == 0 ? p.dA : k == 1 ? p.dD : p.ddt_bias;
   if (out == nullptr) return;
   const float* s = p.partial + (long long)blockIdx.x * n;
-  float v = 0.f;
-  for (int i = threadIdx.x; i < n; i += 256) v += s[i];
-  v = sum_wave(v);
-  __shared__ float red[4];
+  double v = 0.0;  // (chunks' sums cancel, those of dA and the bias above all)
+  for (int i = threadIdx.x; i < n; i += 256) v += (double)s[i];
+#pragma unroll
+  for (int k = 32; k > 0; k /= 2) v += __shfl_xor(v, k);
+  __shared__ double red[4];
   if (lane_id() == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
-  if (threadIdx.x == 0) out[h] = ((red[0] + red[1]) + red[2]) + red[3];
+  if (threadIdx.x == 0) out[h] = (float)(((red[0] + red[1]) + red[2]) + red[3]);
 }
 
 template <typename T, int P, int NP> hipError_t bwd_t(const ScanParams& p, hipStream_t stream) {
@@ -463,11 +473,11 @@ template <typename T, int P, int NP> hipError_t bwd_t(const ScanParams& p, hipSt
   constexpr int Q = chunk_of<T, NP>();
   const int NC = (p.L + Q - 1) / Q;
   if (lds > 65536) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(scan_bwd_kernel<T, P, NP, kRoles<T>>),
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(scan_bwd_kernel<T, P, NP, kRoles<T, P, NP>>),
                                              hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL((scan_bwd_kernel<T, P, NP, kRoles<T>>), dim3((unsigned)((long long)p.B * NC * p.G * p.splits)), dim3(4 * P * kRoles<T>), lds,
+  hipLaunchKernelGGL((scan_bwd_kernel<T, P, NP, kRoles<T, P, NP>>), dim3((unsigned)((long long)p.B * NC * p.G * p.splits)), dim3(4 * P * kRoles<T, P, NP>), lds,
                      stream, p);
   if (p.dBp != nullptr) {
     const long long quads = (long long)p.B * p.L * p.G * p.N / 4;

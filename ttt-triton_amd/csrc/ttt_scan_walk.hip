@@ -56,9 +56,14 @@ template <int N, int PL> __device__ __forceinline__ bool any_not_finite(const Op
   return __ballot(m[0] == 0x7f80 || m[1] == 0x7f80) != 0;
 }
 
+// Waves to a SIMD that the registers are cut to: three in bf16 (164 registers), but where
+// that would spill (P = 32, N = 64, 32,768 tokens of 24 heads: 190 us so, 117 without)
+template <typename T, int P, int NP>
+constexpr int kWaves = NP == 128 || ScanType<T>::IN > 1 || (P == 32 && NP == 64) ? 1 : 3;
+
 // OUT: outputs too; else the segments' end states and decays alone
 template <typename T, int P, int NP, Walk WALK, bool OUT>
-__global__ __launch_bounds__(4 * P, NP == 128 || ScanType<T>::IN > 1 ? 1 : 3) void scan_walk_kernel(ScanParams p) {
+__global__ __launch_bounds__(4 * P, (kWaves<T, P, NP>)) void scan_walk_kernel(ScanParams p) {
   using Sh = WalkShared<T, P, NP, OUT>;
   constexpr bool BACK = WALK == Walk::Back;
   constexpr int IN = Sh::IN, MID = Sh::MID, Q = Sh::Q, TB = Sh::TB, W = P / 16, NT = 4 * P, NC2 = NP / 32;
