@@ -7,10 +7,13 @@
 //   dw[c][k] = sum_t dz[t] s[t+k],   dbias = sum_t dz[t]
 // ds[u] is the state's gradient for u < W-1 and that of token u-W+1 behind it.
 //
-// Everything is bound by HBM.  A thread owns V channels (kV: 8 bytes of a 16-bit
+// Everything is bound by HBM.  A thread owns four channels (kV: 8 bytes of a 16-bit
 // row) and walks a run of tokens with the window in registers, so that a row is
 // read once and W-1 rows again per run; z is formed again in the backward, which
-// costs W multiply-adds instead of a stored row.
+// costs W multiply-adds instead of a stored row.  Eight channels a thread need twice the
+// registers for the rows on their way: 176 us for forward and backward of 32,768 tokens of
+// 896 bf16 channels, 94 with four (31 forward, 117 MB: 3.8 TB/s; 59 backward, 176 MB: 3.0;
+// a device copy runs at 5.2).  One token of 64 sequences: 4 us, a launch.
 #include <math.h>
 
 #include <algorithm>

@@ -10,9 +10,12 @@
 // Both are bound by HBM: a row is read once and held in registers over its two
 // reductions (the variance is that of the centred values).  A row has 1, 4, 8 or 16
 // waves and a lane 4, 8, 12 or 16 of its values, in groups of 4 or 8 that one load
-// brings.  The backward's workgroups walk rows,
-// the next one on its way (not with 16 waves, which have 128 registers), with the sums of dw and db in registers, and write one
+// brings.  The backward's workgroups walk rows, the next one on its way (not with 16
+// waves, which have 128 registers), with the sums of dw and db in registers, and write one
 // partial sum each, added up by a second launch in a fixed order.
+// 32,768 gated rows of 768 in bf16: forward 28 us (151 MB, 5.4 TB/s), backward 53 (252 MB,
+// 4.8 TB/s) and 6 for the partial sums; 4,099 rows of 5,001 in fp16, whose rows begin on odd
+// addresses: 26, 38 and 9 (82 and 123 MB, 3.2 TB/s).  A device copy runs at 5.2 TB/s.
 #include <math.h>
 
 #include <algorithm>

@@ -18,6 +18,14 @@
 // end states from a zero start (the same walk without outputs), then all segments at
 // once.  Up to 8 of them, a workgroup joins those before its own by itself; more are
 // joined beforehand (scan_join_kernel).
+//
+// What bounds it, at 32,768 tokens of 12 heads of 64 features and 64 states in bf16 (4
+// segments of 192 chains, three workgroups a compute unit): 69 us for the outputs with the
+// states kept for the backward, 210 MB of which 101 are those states, 3.0 TB/s; the loads
+// and stores alone take 60, the arithmetic alone 49 to 56 (exponentials, masks and planes
+// of the products more than the matrix instructions), with three workgroups to cover one
+// another.  27 us more for the end states of three segments: 8 chunks one after the other,
+// latency.  Walking back the same.
 #include <math.h>
 
 #include <type_traits>

@@ -346,18 +346,20 @@ class SelectiveSSM(nn.Module):
 
     def _project(self, x: torch.Tensor):
         """(z [.., D], x | B | C [.., C], dt [.., H]): columns of one projection"""
-        D, C = self.width, self.conv_channels
         w, b = self.in_proj.weight, self.in_proj.bias
         if self._proj_pad_w.shape[0]:
             w = torch.cat([w, self._proj_pad_w.to(w.dtype)])
             b = torch.cat([b, self._proj_pad_b.to(b.dtype)])
-        p = projection(x, w, b)
-        return p[..., :D], p[..., D:D + C], p[..., D + C:D + C + self.num_heads]
+        return self._columns(projection(x, w, b))
+
+    def _columns(self, p: torch.Tensor):
+        D, C, H = self.width, self.conv_channels, self.num_heads
+        return p.split([D, C, H, p.shape[-1] - D - C - H], -1)[:3]
 
     def _heads(self, xbc: torch.Tensor):
         """x [.., H, F], B and C [.., G, N]"""
         D, n = self.width, self.groups * self.state_dim
-        x, b, c = xbc[..., :D], xbc[..., D:D + n], xbc[..., D + n:]
+        x, b, c = xbc.split([D, n, n], -1)
         return (x.unflatten(-1, (self.num_heads, self.head_dim)),
                 *(t.unflatten(-1, (self.groups, self.state_dim)) for t in (b, c)))
 
@@ -390,7 +392,7 @@ class SelectiveSSM(nn.Module):
     @torch.no_grad()
     def step(self, x: torch.Tensor, cache: SSMCache):
         """One token x [B, D] of every sequence: its output [B, D], the cache moved on in place."""
-        z, xbc, dt = self._project(x)
+        z, xbc, dt = self._columns(self.in_proj(x))
         xbc = causal_conv_step(xbc, cache.conv, self.conv_weight, self.conv_bias, "silu")
         xs, b, c = self._heads(xbc)
         y = selective_scan_step(xs, dt, self._rates(), b, c, cache.state, self.D, self.dt_bias)
