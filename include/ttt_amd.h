@@ -396,7 +396,9 @@ int ttt_post_norm_bwd(const void* XQW, const float* gamma, const float* stats, c
 /* ---- the selective state-space layer: short causal convolution, scan, layer norm ----
  * Activations in `dtype`, parameters and scan states fp32.  Activations that are
  * read come as rows `ld` elements apart (row b*L + t for token t of sequence b),
- * so that they may be columns of a wider matrix; what is written is contiguous.
+ * so that they may be columns of a wider matrix; what is written is contiguous, and
+ * overlaps nothing else that the call reads or writes (states that a step updates in
+ * place aside).  Calls of 2^32 threads a launch or more are refused.
  * No counterpart in the reference, whose layer types are TTT-Linear and TTT-MLP;
  * these are a third one's. */
 
@@ -437,7 +439,8 @@ int ttt_causal_conv_step(const void* x, long long ldx, void* state, const float*
  *   y       [B][L][H][P]                   h_last [B][H][P][N], or NULL
  *   states  NULL, or ttt_scan_states_bytes: what ttt_scan_bwd needs of the forward
  *   workspace  ttt_scan_workspace_bytes (NULL where that is 0)
- * x, Bm and Cm and their rows start on 16 bytes. */
+ * x, Bm and Cm and their rows start on 16 bytes; where there are more tokens than
+ * one, rows of x, Bm, Cm (and dy) are less than 64 MiB apart. */
 size_t ttt_scan_states_bytes(int B, int L, int H, int P, int N, int dtype);
 size_t ttt_scan_workspace_bytes(int B, int L, int H, int P, int N, int dtype);
 int ttt_scan_fwd(const void* x, long long ldx, const void* dt, long long lddt, const float* A, const void* Bm,

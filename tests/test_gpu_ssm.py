@@ -432,3 +432,73 @@ def test_skip_gradient_over_many_tokens(lib, dt):
     (got,) = torch.autograd.grad(y, D, dy)
     terms = (x.double() * dy.double()).permute(2, 0, 1, 3).flatten(1)
     assert ((got.double() - terms.sum(1)).abs() <= 8 * 2.0 ** -24 * terms.square().sum(1).sqrt()).all()
+
+
+def test_offsets_past_32_bits(lib):
+    """Rows of a matrix of more than 4 GiB: the same bits as from rows of their own."""
+    from ttt_amd.norm import layer_norm
+    from ttt_amd.ssm import causal_conv, selective_scan
+    B, L, ld = 2, 70000, 16400
+    wide = torch.empty(B, L, ld, device="cuda", dtype=BF16)
+    assert wide.numel() * 2 > 1 << 32
+    xbc = wide[..., 8:8 + 96]
+    xbc.copy_(torch.randn(B, L, 96, device="cuda"))
+    own = xbc.contiguous()
+    w = torch.randn(96, 4, device="cuda")
+    conv = [causal_conv(t, w, None, None, "silu", True) for t in (xbc, own)]
+    assert all(torch.equal(a, b) for a, b in zip(*conv))
+    norm = [layer_norm(t, gate=t) for t in (xbc, own)]
+    assert torch.equal(*norm)
+    A = -torch.ones(2, device="cuda")
+
+    def scan(t):
+        x = t.detach().requires_grad_(True)
+        y = selective_scan(x[..., :64].unflatten(-1, (2, 32)), x[..., 64:66], A, x[..., 64:80].unflatten(-1, (1, 16)),
+                           x[..., 80:].unflatten(-1, (1, 16)))
+        return y, torch.autograd.grad(y, x, y.detach())[0]
+
+    for a, b in zip(scan(xbc), scan(own)):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("P,N,dt", [(64, 128, F32), (32, 128, F16), (64, 128, BF16)])
+def test_graph_of_large_workgroups(lib, P, N, dt):
+    """Kernels of more than 64 KB of LDS and of many segments, in a graph."""
+    d = T.dev(T.scan_inputs(1, 1500, 2, P, 1, N, dt, seed=40))
+    want = T.scan_run(d)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        T.scan_run(d)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = T.scan_run(d)
+    for _ in range(3):
+        for v in got.values():
+            v.zero_()
+        graph.replay()
+        again = T.scan_run(d)
+        torch.cuda.synchronize()
+        for k in want:
+            assert torch.equal(got[k], want[k]) and torch.equal(again[k], want[k]), k
+
+
+def test_inference_mode(lib):
+    from ttt_amd.ssm import causal_conv, causal_conv_step, selective_scan, selective_scan_step
+    d = T.dev(T.scan_inputs(2, 9, 2, 32, 1, 16, BF16, seed=41))
+    w = torch.randn(64, 4, device="cuda")
+
+    def run():
+        x, s = causal_conv(d["x"].flatten(2), w, None, None, "silu", True)
+        _, h = selective_scan(x.unflatten(-1, (2, 32)), d["dt"], d["A"], d["Bm"], d["Cm"], return_final_state=True)
+        x = causal_conv_step(d["x"][:, 0].flatten(1), s, w, None, "silu")
+        y = selective_scan_step(x.unflatten(-1, (2, 32)), d["dt"][:, 0], d["A"], d["Bm"][:, 0], d["Cm"][:, 0], h)
+        return y, s, h
+
+    with torch.no_grad():
+        want = run()
+    with torch.inference_mode():
+        got = run()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)

@@ -373,9 +373,11 @@ class SelectiveSSM(nn.Module):
     def _run(self, x: torch.Tensor, cache: Optional[SSMCache], keep: bool, last_only: bool):
         z, xbc, dt = self._project(x)
         first = (None, None) if cache is None else (cache.conv, cache.state)
-        xbc, conv = causal_conv(xbc, self.conv_weight, self.conv_bias, first[0], "silu", True)
+        xbc = causal_conv(xbc, self.conv_weight, self.conv_bias, first[0], "silu", keep)
+        xbc, conv = xbc if keep else (xbc, None)
         xs, b, c = self._heads(xbc)
-        y, state = selective_scan(xs, dt, self._rates(), b, c, self.D, self.dt_bias, first[1], True, True)
+        y = selective_scan(xs, dt, self._rates(), b, c, self.D, self.dt_bias, first[1], True, keep)
+        y, state = y if keep else (y, None)
         if last_only:  # the norm and the output projection are by tokens
             y, z = y[:, -1], z[:, -1]
         return self._out(y, z), SSMCache(conv, state) if keep else None
