@@ -19,27 +19,28 @@ MAX_WIDTH = 16384
 
 def _norm_args(x, weight, bias, gate, eps):
     """(device, code of x, weight, bias)"""
-    D = x.shape[-1] if x.dim() else 0
+    shape, act = x.shape, x.dtype
+    D = shape[-1] if shape else 0
     if not 1 <= D <= MAX_WIDTH:
-        raise ValueError(f"layer_norm takes rows of 1 to {MAX_WIDTH} values, got {list(x.shape)}")
+        raise ValueError(f"layer_norm takes rows of 1 to {MAX_WIDTH} values, got {list(shape)}")
     if (weight is None) != (bias is None):
         raise ValueError("layer_norm takes weight and bias, or neither")
-    if gate is not None and (gate.shape != x.shape or gate.dtype != x.dtype):
-        raise ValueError(f"gate must be as x, {list(x.shape)} in {x.dtype}, got {list(gate.shape)} in {gate.dtype}")
+    if gate is not None and (gate.shape != shape or gate.dtype != act):
+        raise ValueError(f"gate must be as x, {list(shape)} in {act}, got {list(gate.shape)} in {gate.dtype}")
     if not 0.0 < eps <= 1.0:
         raise ValueError(f"eps must be in (0, 1], got {eps}")
-    dev = check_device(x, *(t for t in (weight, bias, gate) if t is not None))
-    return dev, dtype_code(x.dtype), _param(weight, (D,), "weight"), _param(bias, (D,), "bias")
+    dev = check_device(x, *[t for t in (weight, bias, gate) if t is not None])
+    return dev, dtype_code(act), _param(weight, (D,), "weight"), _param(bias, (D,), "bias")
 
 
 def _norm_forward(x, weight, bias, gate, eps, train):
     """(y, what the backward reads)"""
     dev, code, w, b = _norm_args(x, weight, bias, gate, eps)
-    D = x.shape[-1]
-    lead, es = x.dim() - 1, x.element_size()
-    xr, ldx = _rows(x, lead, es)
-    gr, ldg = (None, 0) if gate is None else _rows(gate, lead, es)
-    y = torch.empty(x.shape, device=dev, dtype=x.dtype)
+    shape, es = x.shape, x.element_size()
+    D, lead = shape[-1], len(shape) - 1
+    xr, ldx = _rows(x, lead, es, D)
+    gr, ldg = (None, 0) if gate is None else _rows(gate, lead, es, D)
+    y = x.new_empty(shape)
     R = y.numel() // D
     if R >= 1 << 31:
         raise ValueError(f"layer_norm takes fewer than 2^31 rows, got {R}")
@@ -71,8 +72,8 @@ class LayerNormFunction(torch.autograd.Function):
         D = ctx.shape[-1]
         R = stats.shape[0]
         dy = dy.to(dt).contiguous()
-        dx = torch.empty(ctx.shape, device=dev, dtype=dt)
-        dg = torch.empty(ctx.shape, device=dev, dtype=dt) if gate is not None else None
+        dx = x.new_empty(ctx.shape)
+        dg = x.new_empty(ctx.shape) if gate is not None else None
         lib = _lib.load()
         dw = db = part = None
         n = 0

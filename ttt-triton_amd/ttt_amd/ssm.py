@@ -34,19 +34,15 @@ MAX_STATE = 128
 CONV_WIDTHS = (2, 3, 4)
 
 
-def _rows(t: torch.Tensor, lead: int, align: int):
+def _rows(t: torch.Tensor, lead: int, align: int, width: int):
     """(t, row stride) with t's first `lead` axes as rows a fixed stride apart and
-    the rest contiguous inside a row, `align` bytes of alignment; a contiguous
-    copy where t is not laid out so."""
-    shape = t.shape
-    width = 1
-    for n in shape[lead:]:
-        width *= n
+    the rest, `width` values, contiguous inside a row, `align` bytes of alignment; a
+    contiguous copy where t is not laid out so."""
     if t.is_contiguous():
         if (t.data_ptr() | width * t.element_size()) % align == 0:
             return t, width
         return t.clone(), width  # (fresh memory starts on more than any of them)
-    strides = t.stride()
+    shape, strides = t.shape, t.stride()
     inner, ld, step = 1, None, 0
     for i in range(t.dim() - 1, -1, -1):
         n, st = shape[i], strides[i]
@@ -128,17 +124,17 @@ def _state_in_place(state, shape, dt, dev, what):
 # ---------------------------------------------------------------------------
 
 def _conv_args(x, weight, bias, state, activation, lead):
-    if x.dim() != lead + 1:
-        raise ValueError(f"x must be [{'B,L,C' if lead == 2 else 'B,C'}], got {list(x.shape)}")
-    C = x.shape[-1]
-    if weight.dim() != 2 or weight.shape[0] != C or weight.shape[1] not in CONV_WIDTHS:
-        raise ValueError(f"weight must be [C,W]=[{C},W] with W in {CONV_WIDTHS}, got {list(weight.shape)}")
+    shape, of_w = x.shape, weight.shape
+    if len(shape) != lead + 1:
+        raise ValueError(f"x must be [{'B,L,C' if lead == 2 else 'B,C'}], got {list(shape)}")
+    C = shape[-1]
+    if len(of_w) != 2 or of_w[0] != C or of_w[1] not in CONV_WIDTHS:
+        raise ValueError(f"weight must be [C,W]=[{C},W] with W in {CONV_WIDTHS}, got {list(of_w)}")
     if activation not in _lib.ACTIVATIONS:
         raise ValueError(f"unknown activation {activation!r} (None or 'silu')")
-    dev = check_device(x, weight, *(t for t in (bias, state) if t is not None))
-    W = weight.shape[1]
-    _sizes(*x.shape)
-    return dev, dtype_code(x.dtype), C, W, f32c(weight), _param(bias, (C,), "bias")
+    dev = check_device(x, weight, *[t for t in (bias, state) if t is not None])
+    _sizes(*shape)
+    return dev, dtype_code(x.dtype), C, of_w[1], f32c(weight), _param(bias, (C,), "bias")
 
 
 def _conv_state(state, shape, dt):
@@ -153,10 +149,10 @@ def _conv_forward(x, weight, bias, state, activation, want_last):
     """(y, last state or None, what the backward reads)"""
     dev, code, C, W, w, b = _conv_args(x, weight, bias, state, activation, 2)
     B, L = x.shape[:2]
-    xr, ldx = _rows(x, 2, x.element_size())
+    xr, ldx = _rows(x, 2, x.element_size(), C)
     s0 = _conv_state(state, (B, W - 1, C), x.dtype)
-    y = torch.empty((B, L, C), device=dev, dtype=x.dtype)
-    last = torch.empty((B, W - 1, C), device=dev, dtype=x.dtype) if want_last else None
+    y = x.new_empty((B, L, C))
+    last = x.new_empty((B, W - 1, C)) if want_last else None
     with on_device(dev):
         st = _lib.load().ttt_causal_conv_fwd(xr.data_ptr(), ldx, _opt(s0), w.data_ptr(), _opt(b), B, L, C, W,
                                              _lib.ACTIVATIONS[activation], code, y.data_ptr(), _opt(last), _stream(dev))
@@ -186,12 +182,12 @@ class CausalConvFunction(torch.autograd.Function):
         dev = x.device
         dt = x.dtype
         dy, dlast = (None if g is None else g.to(dt).contiguous() for g in (dy, dlast))
-        dx = torch.empty((B, L, C), device=dev, dtype=dt)
-        ds = torch.empty((B, W - 1, C), device=dev, dtype=dt) if ctx.needs_input_grad[3] else None
-        dw = torch.empty((C, W), device=dev, dtype=torch.float32)
-        db = torch.empty(C, device=dev, dtype=torch.float32) if ctx.dtypes[1] is not None else None
+        dx = x.new_empty((B, L, C))
+        ds = x.new_empty((B, W - 1, C)) if ctx.needs_input_grad[3] else None
+        dw = w.new_empty((C, W))
+        db = w.new_empty(C) if ctx.dtypes[1] is not None else None
         lib = _lib.load()
-        part = torch.empty(_bytes("ttt_causal_conv_partial_bytes", B, L, C, W) // 4, device=dev, dtype=torch.float32)
+        part = w.new_empty(_bytes("ttt_causal_conv_partial_bytes", B, L, C, W) // 4)
         with on_device(dev):
             st = lib.ttt_causal_conv_bwd(x.data_ptr(), ctx.ldx, _opt(s0), w.data_ptr(), _opt(b), _opt(dy), _opt(dlast), B, L, C, W,
                                          _lib.ACTIVATIONS[ctx.activation], dtype_code(dt), dx.data_ptr(), _opt(ds), dw.data_ptr(),
@@ -228,10 +224,10 @@ def causal_conv_step(x, state, weight, bias=None, activation=None):
     dev, code, C, W, w, b = _conv_args(x, weight, bias, state, activation, 1)
     B = x.shape[0]
     _state_in_place(state, (B, W - 1, C), x.dtype, dev, "causal_conv_step")
-    y = torch.empty((B, C), device=dev, dtype=x.dtype)
+    y = x.new_empty((B, C))
     if B == 0:
         return y
-    xr, ldx = _rows(x, 1, x.element_size())
+    xr, ldx = _rows(x, 1, x.element_size(), C)
     with on_device(dev):
         st = _lib.load().ttt_causal_conv_step(xr.data_ptr(), ldx, state.data_ptr(), w.data_ptr(), _opt(b), B, C, W,
                                               _lib.ACTIVATIONS[activation], code, y.data_ptr(), _stream(dev))
@@ -246,13 +242,13 @@ def causal_conv_step(x, state, weight, bias=None, activation=None):
 
 def _scan_args(x, dt, A, Bm, Cm, D, dt_bias, state, lead):
     """(device, (B, L, H, P, G, N), code of x, code of dt, A, D, dt_bias)"""
-    if x.dim() != lead + 2:
-        raise ValueError(f"x must be [{'B,L,H,P' if lead == 2 else 'B,H,P'}], got {list(x.shape)}")
-    rows = x.shape[:lead]
-    H, P = x.shape[lead:]
-    if Bm.dim() != lead + 2 or Bm.shape[:lead] != rows or Bm.shape != Cm.shape:
-        raise ValueError(f"Bm and Cm must be {[*rows, 'G', 'N']}, got {list(Bm.shape)} and {list(Cm.shape)}")
-    G, N = Bm.shape[lead:]
+    shape, of_b, act = x.shape, Bm.shape, x.dtype
+    if len(shape) != lead + 2:
+        raise ValueError(f"x must be [{'B,L,H,P' if lead == 2 else 'B,H,P'}], got {list(shape)}")
+    *rows, H, P = shape
+    if len(of_b) != lead + 2 or list(of_b[:lead]) != rows or of_b != Cm.shape:
+        raise ValueError(f"Bm and Cm must be {[*rows, 'G', 'N']}, got {list(of_b)} and {list(Cm.shape)}")
+    G, N = of_b[lead:]
     if P not in HEAD_DIMS:
         raise ValueError(f"the head dim P must be one of {HEAD_DIMS}, got {P}")
     if N % 16 or not 16 <= N <= MAX_STATE:
@@ -261,18 +257,18 @@ def _scan_args(x, dt, A, Bm, Cm, D, dt_bias, state, lead):
         raise ValueError(f"the {G} groups of Bm and Cm must divide the {H} heads")
     if dt.shape != (*rows, H):
         raise ValueError(f"dt must be {[*rows, H]}, got {list(dt.shape)}")
-    for name, t in (("Bm", Bm), ("Cm", Cm)):
-        if t.dtype != x.dtype:
-            raise ValueError(f"{name} must have x's dtype {x.dtype}, got {t.dtype}")
-    if dt.dtype not in (x.dtype, torch.float32):
-        raise ValueError(f"dt must be in {x.dtype} or float32, got {dt.dtype}")
+    if Bm.dtype != act or Cm.dtype != act:
+        raise ValueError(f"Bm and Cm must have x's dtype {act}, got {Bm.dtype} and {Cm.dtype}")
+    of_dt = dt.dtype
+    if of_dt != act and of_dt != torch.float32:
+        raise ValueError(f"dt must be in {act} or float32, got {of_dt}")
     if A is None:
         raise ValueError("A is needed")
-    dev = check_device(x, dt, A, Bm, Cm, *(t for t in (D, dt_bias, state) if t is not None))
-    _sizes(*x.shape)
-    a = _param(A, (H,), "A")
-    return (dev, (rows[0], rows[1] if lead == 2 else 1, H, P, G, N), dtype_code(x.dtype), dtype_code(dt.dtype), a,
-            _param(D, (H,), "D"), _param(dt_bias, (H,), "dt_bias"))
+    dev = check_device(x, dt, A, Bm, Cm, *[t for t in (D, dt_bias, state) if t is not None])
+    _sizes(*rows, H)
+    code = dtype_code(act)
+    return (dev, (rows[0], rows[1] if lead == 2 else 1, H, P, G, N), code, code if of_dt == act else dtype_code(of_dt),
+            _param(A, (H,), "A"), _param(D, (H,), "D"), _param(dt_bias, (H,), "dt_bias"))
 
 
 def _scan_state(h0, shape):
@@ -283,27 +279,34 @@ def _scan_state(h0, shape):
     return f32c(h0)
 
 
-def _scan_rows(x, dt, Bm, Cm, lead, align):
-    """The four inputs and their row strides as the kernels take them."""
-    out = []
-    for t, al in ((x, align), (dt, dt.element_size()), (Bm, align), (Cm, align)):
-        out += _rows(t, lead, al) if t is dt or lead == 1 else _near_rows(t, al)
-    return out
+def _scan_rows(x, dt, Bm, Cm, rows, align, sizes):
+    """The four inputs and their row strides as the kernels take them: x, Bm and Cm by
+    rows(t, align, width)"""
+    _, _, H, P, G, N = sizes
+    return (*rows(x, align, H * P), *_rows(dt, dt.dim() - 1, dt.element_size(), H), *rows(Bm, align, G * N),
+            *rows(Cm, align, G * N))
 
 
-def _near_rows(t, align):
+def _token_rows(t, align, width):
+    return _rows(t, 1, align, width)
+
+
+def _near_rows(t, align, width):
     """_rows of [B,L,..], copied too where the rows of a chunk are out of a 32-bit offset's reach"""
-    r, ld = _rows(t, 2, align)
-    return _rows(t.detach().contiguous(), 2, align) if ld * t.element_size() >= 1 << 26 and t.shape[1] > 1 else (r, ld)
+    r, ld = _rows(t, 2, align, width)
+    if ld * t.element_size() >= 1 << 26 and t.shape[1] > 1:
+        return _rows(t.detach().contiguous(), 2, align, width)
+    return r, ld
 
 
 def _scan_forward(x, dt, A, Bm, Cm, D, dt_bias, h0, softplus, want_last, train):
     """(y, last state or None, what the backward reads)"""
-    dev, (B, L, H, P, G, N), code, dcode, a, d, bias = _scan_args(x, dt, A, Bm, Cm, D, dt_bias, h0, 2)
+    dev, sizes, code, dcode, a, d, bias = _scan_args(x, dt, A, Bm, Cm, D, dt_bias, h0, 2)
+    B, L, H, P, G, N = sizes
     h0 = _scan_state(h0, (B, H, P, N))
-    rows = _scan_rows(x, dt, Bm, Cm, 2, 16)
+    rows = _scan_rows(x, dt, Bm, Cm, _near_rows, 16, sizes)
     xr, ldx, dr, ldd, br, ldb, cr, ldc = rows
-    y = torch.empty((B, L, H, P), device=dev, dtype=x.dtype)
+    y = x.new_empty((B, L, H, P))
     last = torch.empty((B, H, P, N), device=dev, dtype=torch.float32) if want_last else None
     lib = _lib.load()
     nst = _bytes("ttt_scan_states_bytes", B, L, H, P, N, code) if train else 0
@@ -343,17 +346,16 @@ class SelectiveScanFunction(torch.autograd.Function):
         dev, act = x.device, x.dtype
         code = dtype_code(act)
         dy = torch.zeros((B, L, H, P), device=dev, dtype=act) if dy is None else dy
-        dyr, ldy = _near_rows(dy.to(act), 16)
+        dyr, ldy = _near_rows(dy.to(act), 16, H * P)
         dlast = None if dlast is None else f32c(dlast)
-        f32 = dict(device=dev, dtype=torch.float32)
-        dx = torch.empty((B, L, H, P), device=dev, dtype=act)
-        ddt = torch.empty((B, L, H), device=dev, dtype=dt.dtype)
-        dB, dC = (torch.empty((B, L, G, N), device=dev, dtype=act) for _ in range(2))
-        dA, dD, dbias = torch.empty((3, H), **f32).unbind()
-        dh0 = torch.empty((B, H, P, N), **f32) if ctx.needs_input_grad[7] else None
+        dx = x.new_empty((B, L, H, P))
+        ddt = dt.new_empty((B, L, H))
+        dB, dC = x.new_empty((B, L, G, N)), x.new_empty((B, L, G, N))
+        dA, dD, dbias = a.new_empty((3, H)).unbind()
+        dh0 = a.new_empty((B, H, P, N)) if ctx.needs_input_grad[7] else None
         lib = _lib.load()
         nws = _bytes("ttt_scan_bwd_workspace_bytes", B, L, H, P, G, N, code)
-        ws = torch.empty(nws, device=dev, dtype=torch.uint8)
+        ws = states.new_empty(nws)
         with on_device(dev):
             st = lib.ttt_scan_bwd(x.data_ptr(), ldx, dt.data_ptr(), ldd, a.data_ptr(), Bm.data_ptr(), ldb, Cm.data_ptr(), ldc, _opt(d), _opt(bias),
                                   dyr.data_ptr(), ldy, _opt(dlast), states.data_ptr(), states.numel(), B, L, H, P, G, N, code,
@@ -393,12 +395,13 @@ def selective_scan_step(x, dt, A, Bm, Cm, state, D=None, dt_bias=None, dt_softpl
     """One token of every sequence: x [B,H,P], dt [B,H], Bm and Cm [B,G,N].  Updates
     state [B,H,P,N] (fp32, contiguous) in place and returns y [B,H,P].  No gradient."""
     _no_grad_through("selective_scan_step", x, dt, A, Bm, Cm, state, D, dt_bias)
-    dev, (B, _, H, P, G, N), code, dcode, a, d, bias = _scan_args(x, dt, A, Bm, Cm, D, dt_bias, state, 1)
+    dev, sizes, code, dcode, a, d, bias = _scan_args(x, dt, A, Bm, Cm, D, dt_bias, state, 1)
+    B, _, H, P, G, N = sizes
     _state_in_place(state, (B, H, P, N), torch.float32, dev, "selective_scan_step")
-    y = torch.empty((B, H, P), device=dev, dtype=x.dtype)
+    y = x.new_empty((B, H, P))
     if B == 0:
         return y
-    xr, ldx, dr, ldd, br, ldb, cr, ldc = _scan_rows(x, dt, Bm, Cm, 1, 4 * x.element_size())
+    xr, ldx, dr, ldd, br, ldb, cr, ldc = _scan_rows(x, dt, Bm, Cm, _token_rows, 4 * x.element_size(), sizes)
     with on_device(dev):
         st = _lib.load().ttt_scan_step(xr.data_ptr(), ldx, dr.data_ptr(), ldd, a.data_ptr(), br.data_ptr(), ldb, cr.data_ptr(), ldc, _opt(d),
                                        _opt(bias), state.data_ptr(), B, H, P, G, N, code, dcode, int(dt_softplus), y.data_ptr(),
