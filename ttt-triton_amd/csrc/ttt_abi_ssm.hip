@@ -65,11 +65,13 @@ int walk_resident(int P, int NP, int dtype) {
 // How a scan is cut up.  Segments: a workgroup walks a sequence and head; where that
 // makes too few of them, the tokens are shared out as well, whole chunks each, to at
 // most the full rounds of the card nearest above three workgroups of 64 features or
-// five of 32 a compute unit.  (Forward and backward of 32,768 tokens: 768 at once, 12 heads of
+// five of 32 a compute unit, 8 segments though, which a workgroup joins by itself.  (Forward and backward of 32,768 tokens: 768 at once, 12 heads of
 // 64 x 64 in bf16: 322, 296 and 318 us with 3, 4 and 6 segments; 512 at once, in fp16: 480,
 // 449, 422, 435 with 3, 4, 5, 6; 1,024 at once, 24 heads of 32 x 64: 484, 463, 430, 447 with
-// 3, 4, 5, 8.)  More segments than a workgroup joins by itself cost two launches: not where 8
-// fill three quarters of the card (128 chains of 32 x 64: 166 us with 8 and 189 with 11).
+// 3, 4, 5, 8.)  More segments cost two launches and a pass over them all: one round of the card,
+// where 8 do not fill three quarters of it.  (128 chains of 32 x 64: 166 us with 8, 189 with 11.
+// Forward of 40,000 tokens of 5 heads of 64 x 128 in fp16, 512 at once: 138, 128 and 155 us with 128, 86 and 52
+// segments; 2 x 5,000 of 9 in bf16: 53, 47 and 54 with 40, 27 and 20.)
 // Splits: the backward's workgroups have a chunk and go over a group's heads; below
 // 512 of them the heads are shared out.
 ScanPlan plan(int B, int L, int H, int P, int G, int N, int dtype) {
@@ -80,8 +82,12 @@ ScanPlan plan(int B, int L, int H, int P, int G, int N, int dtype) {
   const long long chains = (long long)B * H;
   const int at_once = 256 * walk_resident(P, s.NP, dtype), least = P == 64 ? 768 : 1280;
   const int most = (least + at_once - 1) / at_once * at_once;
-  long long want = std::max(1LL, std::min<long long>(s.NC, most / chains));
-  if (want > kSelfJoined && 4 * kSelfJoined * chains >= 3 * at_once) want = kSelfJoined;
+  long long want = at_once / chains;
+  if (want <= kSelfJoined)
+    want = std::min<long long>(kSelfJoined, most / chains);
+  else if (4 * kSelfJoined * chains >= 3 * at_once)
+    want = kSelfJoined;
+  want = std::max(1LL, std::min<long long>(s.NC, want));
   s.per = (int)((s.NC + want - 1) / want);
   s.S = (s.NC + s.per - 1) / s.per;
   const long long groups = (long long)B * s.NC * G;
