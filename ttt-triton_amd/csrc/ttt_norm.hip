@@ -280,11 +280,14 @@ template <typename T, int NW> hipError_t lanes_t(const NormParams& p, bool bwd, 
   }
   return four == 3 ? gate_t<T, NW, 4, 3>(p, bwd, s) : gate_t<T, NW, 8, 2>(p, bwd, s);
 }
+// (Gated bf16 rows, forward and backward: 32,768 of 768 with one wave 85 us, with four 126;
+// 8,192 of 2,304 with four 71, with eight 133; of 4,096 131 and 156; 4,096 of 5,120 with eight
+// 91, with sixteen 265.)
+constexpr int waves_of(int D) { return D <= 1024 ? 1 : D <= 4096 ? 4 : D <= 8192 ? 8 : 16; }
 template <typename T> hipError_t waves_t(const NormParams& p, bool bwd, hipStream_t s) {
-  return p.D <= 1024   ? lanes_t<T, 1>(p, bwd, s)
-         : p.D <= 4096 ? lanes_t<T, 4>(p, bwd, s)
-         : p.D <= 8192 ? lanes_t<T, 8>(p, bwd, s)
-                       : lanes_t<T, 16>(p, bwd, s);
+  const int w = waves_of(p.D);
+  return w == 1 ? lanes_t<T, 1>(p, bwd, s) : w == 4 ? lanes_t<T, 4>(p, bwd, s) : w == 8 ? lanes_t<T, 8>(p, bwd, s)
+                                                                               : lanes_t<T, 16>(p, bwd, s);
 }
 hipError_t launch(const NormParams& p, int dtype, bool bwd, hipStream_t s) {
   if (p.D < 1 || p.D > kNormMaxD) return hipErrorInvalidValue;
@@ -294,9 +297,14 @@ hipError_t launch(const NormParams& p, int dtype, bool bwd, hipStream_t s) {
 
 }  // namespace
 
-// workgroups of the backward: as many as are there at once, 12 waves to a compute unit (16 of longer rows)
+// Workgroups of the backward: as many as are there at once, 12 waves to a compute unit (16 of
+// longer rows), or 8 where a lane has 16 values.  (With 12 values 12 and 8 waves: 768 gated
+// 57 and 62 us, 5,001 without a gate 44 and 52; with 16 values: 1,024 gated 48 and 38, 4,096
+// 92 and 78, 8,192 91 and 84.)
 int norm_bwd_parts(long long R, int D) {
-  const long long rows = D <= 1024 ? (R + 3) / 4 : R, most = D <= 4096 ? 768 : D <= 8192 ? 512 : 256;
+  const int w = waves_of(D);
+  const bool full = (D + 256 * w - 1) / (256 * w) > 3;  // 16 values to a lane
+  const long long rows = w == 1 ? (R + 3) / 4 : R, most = w == 16 ? 256 : w == 8 ? (full ? 256 : 512) : full ? 512 : 768;
   return (int)std::max(1LL, std::min(rows, most));
 }
 hipError_t launch_norm_fwd(const NormParams& p, int dtype, hipStream_t s) { return launch(p, dtype, false, s); }
