@@ -102,15 +102,18 @@ __device__ __forceinline__ float sigmoid_f(float z) {
 __device__ __forceinline__ float sum_parts(const float* __restrict__ part, long long n, long long i, int parts) {
   __shared__ float red[16][17];
   const int g = threadIdx.x >> 4, c = threadIdx.x & 15;
-  float s[4] = {0.f, 0.f, 0.f, 0.f};
+  constexpr int AT_ONCE = 8;
+  float s[AT_ONCE] = {};
   if (i < n) {
     int q = g;
-    for (; q + 48 < parts; q += 64)
+    for (; q + 16 * (AT_ONCE - 1) < parts; q += 16 * AT_ONCE)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) s[k] += part[(long long)(q + 16 * k) * n + i];
-    for (; q < parts; q += 16) s[0] += part[(long long)q * n + i];
+      for (int k = 0; k < AT_ONCE; ++k) s[k] += part[(long long)(q + 16 * k) * n + i];
+#pragma unroll
+    for (int k = 0; k < AT_ONCE - 1; ++k)
+      if (q + 16 * k < parts) s[k] += part[(long long)(q + 16 * k) * n + i];
   }
-  red[g][c] = (s[0] + s[1]) + (s[2] + s[3]);
+  red[g][c] = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
   __syncthreads();
   float v = 0.f;
   if (threadIdx.x < 16)
