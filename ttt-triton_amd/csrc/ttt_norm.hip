@@ -14,8 +14,8 @@
 // waves, which have 128 registers), with the sums of dw and db in registers, and write one
 // partial sum each, added up by a second launch in a fixed order.
 // 32,768 gated rows of 768 in bf16: forward 28 us (151 MB, 5.4 TB/s), backward 53 (252 MB,
-// 4.8 TB/s) and 6 for the partial sums; 4,099 rows of 5,001 in fp16, whose rows begin on odd
-// addresses: 26, 38 and 9 (82 and 123 MB, 3.2 TB/s).  A device copy runs at 5.2 TB/s.
+// 4.8 TB/s) and 4 for the partial sums; 4,099 rows of 5,001 in fp16, whose rows begin on odd
+// addresses: 24, 35 and 9 (82 and 123 MB, 3.5 TB/s).  A device copy runs at 5.2 TB/s.
 #include <math.h>
 
 #include <algorithm>
