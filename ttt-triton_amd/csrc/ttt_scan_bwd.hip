@@ -483,8 +483,9 @@ template <typename T, int P, int NP> hipError_t bwd_t(const ScanParams& p, hipSt
                                              hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL((scan_bwd_kernel<T, P, NP, kRoles<T, P, NP>>), dim3((unsigned)((long long)p.B * NC * p.G * p.splits)), dim3(4 * P * kRoles<T, P, NP>), lds,
-                     stream, p);
+  const long long blocks = (long long)p.B * NC * p.G * p.splits;
+  hipLaunchKernelGGL((scan_bwd_kernel<T, P, NP, kRoles<T, P, NP>>), dim3((unsigned)blocks), dim3(4 * P * kRoles<T, P, NP>),
+                     lds, stream, p);
   if (p.dBp != nullptr) {
     const long long quads = (long long)p.B * p.L * p.G * p.N / 4;
     hipLaunchKernelGGL(scan_groups_kernel<T>, dim3((unsigned)((2 * quads + 255) / 256)), dim3(256), 0, stream, p, quads);
@@ -540,7 +541,10 @@ template <typename T, int LANES> hipError_t step_t(const ScanStepParams& p, hipS
   return hipGetLastError();
 }
 template <typename T> hipError_t step_lanes(const ScanStepParams& p, hipStream_t s) {
-  return p.N <= 16 ? step_t<T, 4>(p, s) : p.N <= 32 ? step_t<T, 8>(p, s) : p.N <= 64 ? step_t<T, 16>(p, s) : step_t<T, 32>(p, s);
+  return p.N <= 16   ? step_t<T, 4>(p, s)
+         : p.N <= 32 ? step_t<T, 8>(p, s)
+         : p.N <= 64 ? step_t<T, 16>(p, s)
+                     : step_t<T, 32>(p, s);
 }
 
 }  // namespace

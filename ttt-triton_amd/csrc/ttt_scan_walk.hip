@@ -363,7 +363,9 @@ template <typename T, int P, int NP, Walk WALK> hipError_t walk_t(const ScanPara
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL((scan_walk_kernel<T, P, NP, WALK, false>), dim3((unsigned)(chains * (p.S - 1))), dim3(4 * P), lds1,
                        stream, p);
-    if (p.joined) hipLaunchKernelGGL((scan_join_kernel<P, NP, WALK>), dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, stream, p, quads);
+    if (p.joined)
+      hipLaunchKernelGGL((scan_join_kernel<P, NP, WALK>), dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, stream, p,
+                         quads);
   }
   hipLaunchKernelGGL((scan_walk_kernel<T, P, NP, WALK, true>), dim3((unsigned)(chains * p.S)), dim3(4 * P), lds, stream, p);
   return hipGetLastError();
@@ -381,7 +383,9 @@ template <Walk WALK> hipError_t launch(const ScanParams& p, int P, int dtype, hi
 
 }  // namespace
 
-hipError_t launch_scan_fwd(const ScanParams& p, int P, int dtype, hipStream_t s) { return launch<Walk::Forward>(p, P, dtype, s); }
+hipError_t launch_scan_fwd(const ScanParams& p, int P, int dtype, hipStream_t s) {
+  return launch<Walk::Forward>(p, P, dtype, s);
+}
 hipError_t launch_scan_walk_back(const ScanParams& p, int P, int dtype, hipStream_t s) {
   return launch<Walk::Back>(p, P, dtype, s);
 }

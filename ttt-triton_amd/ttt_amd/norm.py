@@ -82,9 +82,9 @@ class LayerNormFunction(torch.autograd.Function):
             n = _bytes("ttt_layer_norm_partial_bytes", R, D)
             part = torch.empty(n // 4, device=dev, dtype=torch.float32)
         with on_device(dev):
-            st = lib.ttt_layer_norm_bwd(x.data_ptr(), ctx.lds[0], _opt(gate), ctx.lds[1], _opt(w), stats.data_ptr(), dy.data_ptr(), R, D,
-                                        dtype_code(dt), dx.data_ptr(), _opt(dg), _opt(dw), _opt(db), _opt(part), n,
-                                        _stream(dev))
+            st = lib.ttt_layer_norm_bwd(x.data_ptr(), ctx.lds[0], _opt(gate), ctx.lds[1], _opt(w), stats.data_ptr(),
+                                        dy.data_ptr(), R, D, dtype_code(dt), dx.data_ptr(), _opt(dg), _opt(dw),
+                                        _opt(db), _opt(part), n, _stream(dev))
         _lib.check(st, "ttt_layer_norm_bwd")
         if dw is not None:
             dw, db = _as(dw, ctx.dtypes[0]), _as(db, ctx.dtypes[1])

@@ -189,9 +189,10 @@ class CausalConvFunction(torch.autograd.Function):
         lib = _lib.load()
         part = w.new_empty(_bytes("ttt_causal_conv_partial_bytes", B, L, C, W) // 4)
         with on_device(dev):
-            st = lib.ttt_causal_conv_bwd(x.data_ptr(), ctx.ldx, _opt(s0), w.data_ptr(), _opt(b), _opt(dy), _opt(dlast), B, L, C, W,
-                                         _lib.ACTIVATIONS[ctx.activation], dtype_code(dt), dx.data_ptr(), _opt(ds), dw.data_ptr(),
-                                         _opt(db), part.data_ptr(), part.numel() * 4, _stream(dev))
+            st = lib.ttt_causal_conv_bwd(x.data_ptr(), ctx.ldx, _opt(s0), w.data_ptr(), _opt(b), _opt(dy), _opt(dlast),
+                                         B, L, C, W, _lib.ACTIVATIONS[ctx.activation], dtype_code(dt), dx.data_ptr(),
+                                         _opt(ds), dw.data_ptr(), _opt(db), part.data_ptr(), part.numel() * 4,
+                                         _stream(dev))
         _lib.check(st, "ttt_causal_conv_bwd")
         wt, bt, sd = ctx.dtypes
         return dx, _as(dw, wt), _as(db, bt), _as(ds, sd), None, None
@@ -314,9 +315,9 @@ def _scan_forward(x, dt, A, Bm, Cm, D, dt_bias, h0, softplus, want_last, train):
     states = torch.empty(nst, device=dev, dtype=torch.uint8) if train else None
     ws = torch.empty(nws, device=dev, dtype=torch.uint8) if nws else None
     with on_device(dev):
-        st = lib.ttt_scan_fwd(xr.data_ptr(), ldx, dr.data_ptr(), ldd, a.data_ptr(), br.data_ptr(), ldb, cr.data_ptr(), ldc, _opt(d), _opt(bias),
-                              _opt(h0), B, L, H, P, G, N, code, dcode, int(softplus), y.data_ptr(), _opt(last), _opt(states),
-                              nst, _opt(ws), nws, _stream(dev))
+        st = lib.ttt_scan_fwd(xr.data_ptr(), ldx, dr.data_ptr(), ldd, a.data_ptr(), br.data_ptr(), ldb, cr.data_ptr(),
+                              ldc, _opt(d), _opt(bias), _opt(h0), B, L, H, P, G, N, code, dcode, int(softplus),
+                              y.data_ptr(), _opt(last), _opt(states), nst, _opt(ws), nws, _stream(dev))
     _lib.check(st, "ttt_scan_fwd")
     return y, last, (rows, a, d, bias, states)
 
@@ -357,10 +358,12 @@ class SelectiveScanFunction(torch.autograd.Function):
         nws = _bytes("ttt_scan_bwd_workspace_bytes", B, L, H, P, G, N, code)
         ws = states.new_empty(nws)
         with on_device(dev):
-            st = lib.ttt_scan_bwd(x.data_ptr(), ldx, dt.data_ptr(), ldd, a.data_ptr(), Bm.data_ptr(), ldb, Cm.data_ptr(), ldc, _opt(d), _opt(bias),
-                                  dyr.data_ptr(), ldy, _opt(dlast), states.data_ptr(), states.numel(), B, L, H, P, G, N, code,
-                                  dtype_code(dt.dtype), int(ctx.softplus), dx.data_ptr(), ddt.data_ptr(), dA.data_ptr(), dB.data_ptr(), dC.data_ptr(),
-                                  _opt(None if d is None else dD), _opt(None if bias is None else dbias), _opt(dh0), ws.data_ptr(), nws, _stream(dev))
+            st = lib.ttt_scan_bwd(x.data_ptr(), ldx, dt.data_ptr(), ldd, a.data_ptr(), Bm.data_ptr(), ldb, Cm.data_ptr(),
+                                  ldc, _opt(d), _opt(bias), dyr.data_ptr(), ldy, _opt(dlast), states.data_ptr(),
+                                  states.numel(), B, L, H, P, G, N, code, dtype_code(dt.dtype), int(ctx.softplus),
+                                  dx.data_ptr(), ddt.data_ptr(), dA.data_ptr(), dB.data_ptr(), dC.data_ptr(),
+                                  _opt(None if d is None else dD), _opt(None if bias is None else dbias), _opt(dh0),
+                                  ws.data_ptr(), nws, _stream(dev))
         _lib.check(st, "ttt_scan_bwd")
         dts = ctx.dtypes
         return (dx, ddt, _as(dA, dts[0]), dB, dC, None if d is None else _as(dD, dts[1]),
@@ -403,9 +406,9 @@ def selective_scan_step(x, dt, A, Bm, Cm, state, D=None, dt_bias=None, dt_softpl
         return y
     xr, ldx, dr, ldd, br, ldb, cr, ldc = _scan_rows(x, dt, Bm, Cm, _token_rows, 4 * x.element_size(), sizes)
     with on_device(dev):
-        st = _lib.load().ttt_scan_step(xr.data_ptr(), ldx, dr.data_ptr(), ldd, a.data_ptr(), br.data_ptr(), ldb, cr.data_ptr(), ldc, _opt(d),
-                                       _opt(bias), state.data_ptr(), B, H, P, G, N, code, dcode, int(dt_softplus), y.data_ptr(),
-                                       _stream(dev))
+        st = _lib.load().ttt_scan_step(xr.data_ptr(), ldx, dr.data_ptr(), ldd, a.data_ptr(), br.data_ptr(), ldb,
+                                       cr.data_ptr(), ldc, _opt(d), _opt(bias), state.data_ptr(), B, H, P, G, N, code,
+                                       dcode, int(dt_softplus), y.data_ptr(), _stream(dev))
     _lib.check(st, "ttt_scan_step")
     torch.autograd.graph.increment_version(state)
     return y
