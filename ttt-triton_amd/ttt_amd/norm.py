@@ -11,7 +11,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._common import check_device, dtype_code, on_device
-from .ssm import _as, _bytes, _empty, _opt, _param, _rows, _stream, _wants_grad
+from .ssm import _as, _bytes, _empty, _layout, _opt, _param, _rows, _rows_again, _stream, _wants_grad, _whole
 
 LAYER_NORM_EPS = 1e-6
 MAX_WIDTH = 16384
@@ -59,7 +59,7 @@ class LayerNormFunction(torch.autograd.Function):
     def forward(ctx, x, weight, bias, gate, eps):
         y, (xr, ldx, gr, ldg, w, stats) = _norm_forward(x, weight, bias, gate, eps, True)
         ctx.save_for_backward(xr, gr, w, stats)
-        ctx.lds = ldx, ldg
+        ctx.layouts = _layout(xr, ldx), None if gr is None else _layout(gr, ldg)
         ctx.dtypes = None if weight is None else (weight.dtype, bias.dtype)
         ctx.shape = x.shape
         return y
@@ -71,6 +71,11 @@ class LayerNormFunction(torch.autograd.Function):
         dev, dt = x.device, x.dtype
         D = ctx.shape[-1]
         R = stats.shape[0]
+        es, lead = x.element_size(), len(ctx.shape) - 1
+        rows = lambda t, align, width: _rows(t, lead, align, width)  # noqa: E731
+        x, ldx = _rows_again(x, ctx.layouts[0], es, D, rows)
+        gate, ldg = (None, 0) if gate is None else _rows_again(gate, ctx.layouts[1], es, D, rows)
+        w, stats = _whole(w), _whole(stats)
         dy = dy.to(dt).contiguous()
         dx = x.new_empty(ctx.shape)
         dg = x.new_empty(ctx.shape) if gate is not None else None
@@ -82,7 +87,7 @@ class LayerNormFunction(torch.autograd.Function):
             n = _bytes("ttt_layer_norm_partial_bytes", R, D)
             part = torch.empty(n // 4, device=dev, dtype=torch.float32)
         with on_device(dev):
-            st = lib.ttt_layer_norm_bwd(x.data_ptr(), ctx.lds[0], _opt(gate), ctx.lds[1], _opt(w), stats.data_ptr(),
+            st = lib.ttt_layer_norm_bwd(x.data_ptr(), ldx, _opt(gate), ldg, _opt(w), stats.data_ptr(),
                                         dy.data_ptr(), R, D, dtype_code(dt), dx.data_ptr(), _opt(dg), _opt(dw),
                                         _opt(db), _opt(part), n, _stream(dev))
         _lib.check(st, "ttt_layer_norm_bwd")

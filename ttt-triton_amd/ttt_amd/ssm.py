@@ -63,6 +63,44 @@ def _rows(t: torch.Tensor, lead: int, align: int, width: int):
     return t.detach().contiguous(), width
 
 
+def _token_rows(t, align, width):
+    return _rows(t, 1, align, width)
+
+
+def _sequence_rows(t, align, width):
+    return _rows(t, 2, align, width)
+
+
+def _near_rows(t, align, width):
+    """_rows of [B,L,..], copied too where the rows of a chunk are out of a 32-bit offset's reach"""
+    r, ld = _rows(t, 2, align, width)
+    if ld * t.element_size() >= 1 << 26 and t.shape[1] > 1:
+        return _rows(t.detach().contiguous(), 2, align, width)
+    return r, ld
+
+
+# Hooks on saved tensors may bring one back in another layout than it was saved in (a
+# contiguous one most often, after a stay on the CPU): the backwards take addresses and
+# strides from the tensors that they unpack.
+
+def _layout(t, ld):
+    """What _rows_again compares a saved tensor with."""
+    return t.stride(), ld
+
+
+def _rows_again(t, was, align, width, rows):
+    """rows(t, align, width) of a saved tensor; its stride is known where t lies as it was saved"""
+    strides, ld = was
+    return (t, ld) if t.stride() == strides and t.data_ptr() % align == 0 else rows(t, align, width)
+
+
+def _whole(t, align: int = 1):
+    """A saved tensor as one contiguous block on `align` bytes"""
+    if t is None or t.is_contiguous() and (align == 1 or t.data_ptr() % align == 0):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
 def _stream(dev: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(dev.index)
 
@@ -166,8 +204,9 @@ class CausalConvFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, state, activation, want_last):
-        y, last, (xr, ctx.ldx, s0, w, b) = _conv_forward(x, weight, bias, state, activation, want_last)
+        y, last, (xr, ldx, s0, w, b) = _conv_forward(x, weight, bias, state, activation, want_last)
         ctx.save_for_backward(xr, s0, w, b)
+        ctx.layout = _layout(xr, ldx)
         ctx.activation = activation
         ctx.dtypes = weight.dtype, None if bias is None else bias.dtype, None if state is None else state.dtype
         ctx.shape = (*x.shape, weight.shape[1])
@@ -181,6 +220,8 @@ class CausalConvFunction(torch.autograd.Function):
         B, L, C, W = ctx.shape
         dev = x.device
         dt = x.dtype
+        x, ldx = _rows_again(x, ctx.layout, x.element_size(), C, _sequence_rows)
+        s0, w, b = _whole(s0), _whole(w), _whole(b)
         dy, dlast = (None if g is None else g.to(dt).contiguous() for g in (dy, dlast))
         dx = x.new_empty((B, L, C))
         ds = x.new_empty((B, W - 1, C)) if ctx.needs_input_grad[3] else None
@@ -189,7 +230,7 @@ class CausalConvFunction(torch.autograd.Function):
         lib = _lib.load()
         part = w.new_empty(_bytes("ttt_causal_conv_partial_bytes", B, L, C, W) // 4)
         with on_device(dev):
-            st = lib.ttt_causal_conv_bwd(x.data_ptr(), ctx.ldx, _opt(s0), w.data_ptr(), _opt(b), _opt(dy), _opt(dlast),
+            st = lib.ttt_causal_conv_bwd(x.data_ptr(), ldx, _opt(s0), w.data_ptr(), _opt(b), _opt(dy), _opt(dlast),
                                          B, L, C, W, _lib.ACTIVATIONS[ctx.activation], dtype_code(dt), dx.data_ptr(),
                                          _opt(ds), dw.data_ptr(), _opt(db), part.data_ptr(), part.numel() * 4,
                                          _stream(dev))
@@ -288,18 +329,6 @@ def _scan_rows(x, dt, Bm, Cm, rows, align, sizes):
             *rows(Cm, align, G * N))
 
 
-def _token_rows(t, align, width):
-    return _rows(t, 1, align, width)
-
-
-def _near_rows(t, align, width):
-    """_rows of [B,L,..], copied too where the rows of a chunk are out of a 32-bit offset's reach"""
-    r, ld = _rows(t, 2, align, width)
-    if ld * t.element_size() >= 1 << 26 and t.shape[1] > 1:
-        return _rows(t.detach().contiguous(), 2, align, width)
-    return r, ld
-
-
 def _scan_forward(x, dt, A, Bm, Cm, D, dt_bias, h0, softplus, want_last, train):
     """(y, last state or None, what the backward reads)"""
     dev, sizes, code, dcode, a, d, bias = _scan_args(x, dt, A, Bm, Cm, D, dt_bias, h0, 2)
@@ -330,9 +359,8 @@ class SelectiveScanFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, dt, A, Bm, Cm, D, dt_bias, h0, softplus, want_last):
         y, last, (rows, a, d, bias, states) = _scan_forward(x, dt, A, Bm, Cm, D, dt_bias, h0, softplus, want_last, True)
-        xr, ldx, dr, ldd, br, ldb, cr, ldc = rows
-        ctx.save_for_backward(xr, dr, br, cr, a, d, bias, states)
-        ctx.lds, ctx.softplus = (ldx, ldd, ldb, ldc), softplus
+        ctx.save_for_backward(*rows[::2], a, d, bias, states)
+        ctx.layouts, ctx.softplus = [_layout(t, ld) for t, ld in zip(rows[::2], rows[1::2])], softplus
         ctx.shape = (*x.shape, *Bm.shape[2:])
         ctx.dtypes = tuple(None if t is None else t.dtype for t in (A, D, dt_bias, h0))
         ctx.set_materialize_grads(False)
@@ -343,7 +371,12 @@ class SelectiveScanFunction(torch.autograd.Function):
     def backward(ctx, dy, dlast):
         x, dt, Bm, Cm, a, d, bias, states = ctx.saved_tensors
         B, L, H, P, G, N = ctx.shape
-        ldx, ldd, ldb, ldc = ctx.lds
+        of_x, of_dt, of_b, of_c = ctx.layouts
+        x, ldx = _rows_again(x, of_x, 16, H * P, _near_rows)
+        dt, ldd = _rows_again(dt, of_dt, dt.element_size(), H, _sequence_rows)
+        Bm, ldb = _rows_again(Bm, of_b, 16, G * N, _near_rows)
+        Cm, ldc = _rows_again(Cm, of_c, 16, G * N, _near_rows)
+        a, d, bias, states = _whole(a), _whole(d), _whole(bias), _whole(states, 16)
         dev, act = x.device, x.dtype
         code = dtype_code(act)
         dy = torch.zeros((B, L, H, P), device=dev, dtype=act) if dy is None else dy
