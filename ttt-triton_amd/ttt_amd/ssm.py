@@ -24,6 +24,7 @@ from __future__ import annotations
 import functools
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -137,11 +138,21 @@ def _empty(x, *params):
     return y
 
 
+def _has_tangent(*ts) -> bool:
+    """Whether forward-mode derivatives are on their way through one of these."""
+    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
+                                                  for t in ts)
+
+
 def _wants_grad(*ts) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+    """Whether the call goes through its autograd function: for gradients, and for tangents,
+    which the function refuses (without it they would be dropped, under no_grad too)."""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts) or _has_tangent(*ts)
 
 
 def _no_grad_through(what, *ts):
+    if _has_tangent(*ts):
+        raise NotImplementedError(f"{what} has no forward-mode derivative")
     if _wants_grad(*ts):
         raise ValueError(f"{what} updates its state in place and has no gradient: call it under torch.no_grad()")
 
