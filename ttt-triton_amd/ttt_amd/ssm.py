@@ -96,10 +96,10 @@ def _rows_again(t, was, align, width, rows):
 
 
 def _whole(t, align: int = 1):
-    """A saved tensor as one contiguous block on `align` bytes"""
+    """t as one contiguous block on `align` bytes"""
     if t is None or t.is_contiguous() and (align == 1 or t.data_ptr() % align == 0):
         return t
-    return t.clone(memory_format=torch.contiguous_format)
+    return t.detach().clone(memory_format=torch.contiguous_format)
 
 
 def _stream(dev: torch.device) -> int:
@@ -329,7 +329,7 @@ def _scan_state(h0, shape):
         return None
     if tuple(h0.shape) != shape:
         raise ValueError(f"initial_state must be [B,H,P,N]={list(shape)}, got {list(h0.shape)}")
-    return f32c(h0)
+    return _whole(f32c(h0), 16)
 
 
 def _scan_rows(x, dt, Bm, Cm, rows, align, sizes):
@@ -392,7 +392,7 @@ class SelectiveScanFunction(torch.autograd.Function):
         code = dtype_code(act)
         dy = torch.zeros((B, L, H, P), device=dev, dtype=act) if dy is None else dy
         dyr, ldy = _near_rows(dy.to(act), 16, H * P)
-        dlast = None if dlast is None else f32c(dlast)
+        dlast = None if dlast is None else _whole(f32c(dlast), 16)
         dx = x.new_empty((B, L, H, P))
         ddt = dt.new_empty((B, L, H))
         dB, dC = x.new_empty((B, L, G, N)), x.new_empty((B, L, G, N))
