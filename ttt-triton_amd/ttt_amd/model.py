@@ -28,9 +28,9 @@ learnable_ttt_lr_weight [H,1,D], learnable_ttt_lr_bias [H,1],
 ttt_norm_weight/bias [H,F], post_norm, W1/b1/W2/b2), so a reference state
 dict loads unchanged.  Shapes the layer takes (ModelConfig raises ValueError
 for others): head dim F = model_dim / num_heads in {32, 64} (the producer,
-post-norm and memory-cache kernels), model_dim <= 1024, and a mini-batch
-size K that is a multiple of 16 up to 64.  The layer's hidden width is F, as
-TTTMLP builds it: K = 16 runs on the specialised kernels (F = 32 MLP: the
+post-norm and memory-cache kernels), model_dim <= 1024, and, of the TTT layers, a
+mini-batch size K that is a multiple of 16 up to 64 and divides the length.  The
+layer's hidden width is F, as TTTMLP builds it: K = 16 runs on the specialised kernels (F = 32 MLP: the
 register-resident ones), K of 32 to 64 on the mini-batch-in-LDS kernels at F = 64
 and the register-resident ones at F = 32."""
 
@@ -136,7 +136,8 @@ class ModelConfig:
             self.compressed_num_frames = self.seq_len
         if self.model_dim % self.num_heads:
             raise ValueError("model_dim must be a multiple of num_heads")
-        if self.seq_len % self.mini_batch_size:
+        mini_batches = self.ssm_layer != "selective_scan"  # which takes any length and has none
+        if mini_batches and self.seq_len % self.mini_batch_size:
             raise ValueError("seq_len must be a multiple of mini_batch_size")
         if (self.model_dim // self.num_heads) % 2:
             raise ValueError("RoPE needs an even head dim")
@@ -148,7 +149,7 @@ class ModelConfig:
             raise ValueError(f"head dim model_dim/num_heads = {F}: this build's layer kernels take 32 or 64")
         if self.model_dim > MAX_MODEL_DIM:
             raise ValueError(f"model_dim {self.model_dim} > {MAX_MODEL_DIM}, the widest the layer kernels take")
-        if self.mini_batch_size % 16 or not 16 <= self.mini_batch_size <= 64:
+        if mini_batches and (self.mini_batch_size % 16 or not 16 <= self.mini_batch_size <= 64):
             raise ValueError(f"mini_batch_size {self.mini_batch_size}: a multiple of 16 from 16 to 64 is needed")
         if self.ssm_layer == "selective_scan":
             if self.state_dim % 16 or not 16 <= self.state_dim <= MAX_STATE:
