@@ -301,7 +301,7 @@ __device__ __forceinline__ double lane_value(double v, int l) {
 
 // d_t, the running sum c_t of log2(e) d_t A over the chunk in two floats, and its
 // factors from the chunk's start, 2^c_t, and to its end, 2^(c_Q - c_t)
-template <int Q, bool WALK = false> struct Decays {
+template <int Q, bool WALK = false> struct alignas(16) Decays {  // (read four values at a time)
   float hi[Q], lo[Q], d[Q];
   float head[Q], tail[Q];
   float in[WALK ? Q : 4];  // d_t 2^(c_Q - c_t): what token t adds to the state

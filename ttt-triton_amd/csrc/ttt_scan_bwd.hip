@@ -24,6 +24,7 @@
 // sums, then the products into dB and dC, with three barriers between them and eight waves a
 // compute unit (237 registers).
 #include <math.h>
+#include <stddef.h>
 
 #include "ttt_scan.h"
 
@@ -55,7 +56,7 @@ template <typename T, int P, int NP> struct BwdShared {
   // What is left of a head for the gradient of its steps: of W (C . B) by tiles the sums of
   // the columns, before d_j, and of the rows (of a block that meets itself what crosses its
   // tokens), and shares of u_i and of v_j / d_j by 16 columns
-  struct Head {
+  struct alignas(16) Head {
     float row[TILES][16], col[TILES][16];
     float u[NB][Q], v[NB][Q];
     float dD[W * kRoles<T, P, NP>], gh[W];
@@ -179,6 +180,10 @@ __device__ __forceinline__ void steps_grad(const ScanParams& p, const BwdShared<
 template <typename T, int P, int NP, int ROLES>
 __global__ __launch_bounds__(4 * P * ROLES) void scan_bwd_kernel(ScanParams p) {
   using Sh = BwdShared<T, P, NP>;
+  static_assert(offsetof(Sh, dec) % 16 == 0 && sizeof(Sh::dec[0]) % 16 == 0 && offsetof(Sh, head) % 16 == 0 &&
+                    sizeof(Sh::head[0]) % 16 == 0 && offsetof(Sh, dy) % 16 == 0 && offsetof(Sh, b) % 16 == 0 &&
+                    offsetof(Sh, c) % 16 == 0 && offsetof(Sh, wv) % 16 == 0,
+                "read and written 16 bytes at a time");
   constexpr int IN = Sh::IN, MID = Sh::MID, Q = Sh::Q, TB = Sh::TB, W = Sh::W, NB = Sh::NB, NC2 = NP / 32;
   constexpr int WAVES = W * ROLES, NT = 64 * WAVES, BOTH = 3 - ROLES;
   constexpr int TILES = Sh::TILES, OWN = (TILES + WAVES - 1) / WAVES;

@@ -27,6 +27,7 @@
 // another.  27 us more for the end states of three segments: 8 chunks one after the other,
 // latency.  Walking back the same.
 #include <math.h>
+#include <stddef.h>
 
 #include <type_traits>
 
@@ -73,6 +74,9 @@ constexpr int kWaves = NP == 128 || ScanType<T>::IN > 1 || (P == 32 && NP == 64)
 template <typename T, int P, int NP, Walk WALK, bool OUT>
 __global__ __launch_bounds__(4 * P, (kWaves<T, P, NP>)) void scan_walk_kernel(ScanParams p) {
   using Sh = WalkShared<T, P, NP, OUT>;
+  static_assert(offsetof(Sh, dec) % 16 == 0 && sizeof(Sh::dec[0]) % 16 == 0 && offsetof(Sh, key) % 16 == 0 &&
+                    offsetof(Sh, query) % 16 == 0 && offsetof(Sh, m) % 16 == 0,
+                "read 16 bytes at a time");
   constexpr bool BACK = WALK == Walk::Back;
   constexpr int IN = Sh::IN, MID = Sh::MID, Q = Sh::Q, TB = Sh::TB, W = P / 16, NT = 4 * P, NC2 = NP / 32;
   constexpr int NB = StateTiles<NP>::NB;
