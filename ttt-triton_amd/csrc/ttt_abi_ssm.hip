@@ -57,9 +57,13 @@ struct ScanPlan {
   int Q, NC, NP, S, per, splits;
   size_t states, seg, decay, partial, split;
 };
-// Workgroups of the walk that a compute unit holds, by its registers and LDS
-int walk_resident(int P, int NP, int dtype) {
-  constexpr signed char t[2][3][3] = {{{5, 3, 5}, {4, 2, 3}, {2, 3, 2}}, {{3, 3, 4}, {3, 2, 3}, {2, 2, 2}}};
+// Workgroups of the walk that a compute unit holds, by its registers and LDS.  Heads of 64
+// with states up to 32 need fewer registers walking back: fp16 171 forwards and 155 back,
+// fp32 132 and 116.  (With the numbers of the walk back for both, us of 32 x 1,024 tokens of 8
+// heads forwards: fp16 70 and now 61, fp32 76 and 72; of 4 x 4,096 of 12: 58 and 65, 71 and 64.)
+int walk_resident(int P, int NP, int dtype, bool back) {
+  constexpr signed char t[2][3][3] = {{{5, 3, 5}, {4, 2, 3}, {2, 3, 2}}, {{3, 2, 3}, {3, 2, 3}, {2, 2, 2}}};
+  if (back && P == 64 && NP == 32 && dtype != TTT_DTYPE_BF16) return dtype == TTT_DTYPE_F16 ? 3 : 4;
   return t[P == 64][NP == 32 ? 0 : NP == 64 ? 1 : 2][dtype == TTT_DTYPE_BF16 ? 0 : dtype == TTT_DTYPE_F16 ? 1 : 2];
 }
 // How a scan is cut up.  Segments: a workgroup walks a sequence and head; where that
@@ -75,13 +79,13 @@ int walk_resident(int P, int NP, int dtype) {
 // Splits: the backward's workgroups have a chunk and go over a group's heads; below
 // 512 of them, two a compute unit, the heads are shared out.  (16,384 tokens of 12 heads of
 // 64 x 64 in bf16: 175 us forward and backward, 200 with half and 186 with twice as many.)
-ScanPlan plan(int B, int L, int H, int P, int G, int N, int dtype) {
+ScanPlan plan(int B, int L, int H, int P, int G, int N, int dtype, bool back) {
   ScanPlan s;
   s.NP = ttt::scan_padded(N);
   s.Q = ttt::scan_chunk(dtype, s.NP);
   s.NC = (L + s.Q - 1) / s.Q;
   const long long chains = (long long)B * H;
-  const int at_once = 256 * walk_resident(P, s.NP, dtype), least = P == 64 ? 768 : 1280;
+  const int at_once = 256 * walk_resident(P, s.NP, dtype, back), least = P == 64 ? 768 : 1280;
   const int most = (least + at_once - 1) / at_once * at_once;
   long long want = at_once / chains;
   if (want <= kSelfJoined)
@@ -105,9 +109,9 @@ bool grid_ok(const ScanPlan& s, int B, int H, int P, int G) {
   return (long long)B * H * s.S <= kMaxThreads / (4 * P) && (long long)B * s.NC <= kMaxGrid &&
          (long long)B * s.NC * G <= kMaxThreads / (8 * P) / s.splits;
 }
-bool plan_ok(int B, int L, int H, int P, int G, int N, int dtype, ScanPlan& s) {
+bool plan_ok(int B, int L, int H, int P, int G, int N, int dtype, bool back, ScanPlan& s) {
   if (check_scan(B, L, H, P, G, N, dtype, dtype) != TTT_OK) return false;
-  s = plan(B, L, H, P, G, N, dtype);
+  s = plan(B, L, H, P, G, N, dtype, back);
   return grid_ok(s, B, H, P, G);
 }
 
@@ -226,15 +230,15 @@ int ttt_causal_conv_step(const void* x, long long ldx, void* state, const float*
 
 size_t ttt_scan_states_bytes(int B, int L, int H, int P, int N, int dtype) {
   ScanPlan s;
-  return plan_ok(B, L, H, P, 1, N, dtype, s) ? s.states : 0;
+  return plan_ok(B, L, H, P, 1, N, dtype, false, s) ? s.states : 0;
 }
 size_t ttt_scan_workspace_bytes(int B, int L, int H, int P, int N, int dtype) {
   ScanPlan s;
-  return plan_ok(B, L, H, P, 1, N, dtype, s) ? s.seg + s.decay : 0;
+  return plan_ok(B, L, H, P, 1, N, dtype, false, s) ? s.seg + s.decay : 0;
 }
 size_t ttt_scan_bwd_workspace_bytes(int B, int L, int H, int P, int G, int N, int dtype) {
   ScanPlan s;
-  return plan_ok(B, L, H, P, G, N, dtype, s) ? up256(s.states) + s.seg + s.decay + s.partial + 2 * s.split : 0;
+  return plan_ok(B, L, H, P, G, N, dtype, true, s) ? up256(s.states) + s.seg + s.decay + s.partial + 2 * s.split : 0;
 }
 
 int ttt_scan_fwd(const void* x, long long ldx, const void* dt, long long lddt, const float* A, const void* Bm,
@@ -244,7 +248,7 @@ int ttt_scan_fwd(const void* x, long long ldx, const void* dt, long long lddt, c
                  void* stream) {
   int st = check_scan(B, L, H, P, G, N, dtype, dt_dtype);
   if (st != TTT_OK) return st;
-  const ScanPlan s = plan(B, L, H, P, G, N, dtype);
+  const ScanPlan s = plan(B, L, H, P, G, N, dtype, false);
   if (!grid_ok(s, B, H, P, G)) return TTT_ERR_SHAPE;
   if (lddt < H) return TTT_ERR_SHAPE;
   if ((st = check_row(ldx, (long long)H * P, L, dtype)) != TTT_OK) return st;
@@ -305,7 +309,7 @@ int ttt_scan_bwd(const void* x, long long ldx, const void* dt, long long lddt, c
                  void* stream) {
   int st = check_scan(B, L, H, P, G, N, dtype, dt_dtype);
   if (st != TTT_OK) return st;
-  const ScanPlan s = plan(B, L, H, P, G, N, dtype);
+  const ScanPlan s = plan(B, L, H, P, G, N, dtype, true);
   if (!grid_ok(s, B, H, P, G)) return TTT_ERR_SHAPE;
   if (lddt < H) return TTT_ERR_SHAPE;
   if ((st = check_row(ldx, (long long)H * P, L, dtype)) != TTT_OK) return st;
