@@ -176,12 +176,12 @@ template <int PL, int ROWS, int COLS> struct Planes {
     return o;
   }
   // free index r: column c0 + r, or with NAT8 c0 + 8 (r >> 2) + (r & 3);
-  // contraction: rows k0 + 4g + e and k0 + 16 + 4g + e (e < 4), or with KROW8 k0 + 8g + e.
+  // contraction: rows k0 + 4g + e and k0 + 16 + 4g + e (e < 4).
   // (the transposing read: lane 4k + q of a group names row k's columns 4q..4q+3
   // and lane i receives column i of the group's 16 for its four rows)
-  template <bool NAT8 = false, bool KROW8 = false> __device__ __forceinline__ Op<PL> cols(int k0, int c0) const {
+  template <bool NAT8 = false> __device__ __forceinline__ Op<PL> cols(int k0, int c0) const {
     const int l = lane_id(), g = l >> 4, k = (l & 15) >> 2, c = (l & 3) * (NAT8 ? 8 : 4);
-    const int ra = k0 + (KROW8 ? 8 : 4) * g + k, rb = ra + (KROW8 ? 4 : 16);
+    const int ra = k0 + 4 * g + k, rb = ra + 16;
     Op<PL> o;
 #pragma unroll
     for (int q = 0; q < PL; ++q) o.v[q] = cat(read_tr(&d[q][ra][c0 + c]), read_tr(&d[q][rb][c0 + c]));
