@@ -5,7 +5,7 @@ import pytest
 
 from tests.test_kernel_resources import kernels  # noqa: F401
 
-TYPES = {0: ("f", 3, 3), 1: ("DF16b", 1, 2), 2: ("DF16_", 2, 2)}  # mangled name, planes of an input, of a formed value
+TYPES = {0: ("f", 3, 3), 1: ("DF16b", 1, 2), 2: ("DF16_", 2, 3)}  # mangled name, planes of an input, of a formed value
 F32, BF16, F16 = 0, 1, 2
 
 

@@ -58,12 +58,12 @@ struct ScanPlan {
   size_t states, seg, decay, partial, split;
 };
 // Workgroups of the walk that a compute unit holds, by its registers and LDS.  Heads of 64
-// with states up to 32 need fewer registers walking back: fp16 171 forwards and 155 back,
-// fp32 132 and 116.  (With the numbers of the walk back for both, us of 32 x 1,024 tokens of 8
-// heads forwards: fp16 70 and now 61, fp32 76 and 72; of 4 x 4,096 of 12: 58 and 65, 71 and 64.)
+// with states up to 32 in fp32 need fewer registers walking back: 132 forwards and 116 back.
+// (With one workgroup more than is held, us forwards of 32 x 1,024 tokens of 8 heads of 64 x 32:
+// fp16 70 and now 61, fp32 76 and 72; of 4 x 4,096 of 12: 58 and 65, 71 and 64.)
 int walk_resident(int P, int NP, int dtype, bool back) {
   constexpr signed char t[2][3][3] = {{{5, 3, 5}, {4, 2, 3}, {2, 3, 2}}, {{3, 2, 3}, {3, 2, 3}, {2, 2, 2}}};
-  if (back && P == 64 && NP == 32 && dtype != TTT_DTYPE_BF16) return dtype == TTT_DTYPE_F16 ? 3 : 4;
+  if (back && P == 64 && NP == 32 && dtype == TTT_DTYPE_F32) return 4;
   return t[P == 64][NP == 32 ? 0 : NP == 64 ? 1 : 2][dtype == TTT_DTYPE_BF16 ? 0 : dtype == TTT_DTYPE_F16 ? 1 : 2];
 }
 // How a scan is cut up.  Segments: a workgroup walks a sequence and head; where that

@@ -15,11 +15,16 @@
 // bf16, two in fp16 and three in fp32, exact in each (8 bits a plane), so a single
 // matrix instruction (v_mfma_f32_16x16x32_bf16) and one range serve all types.
 // Values formed on the way are fp32 and split into planes where they are
-// multiplied.  What leads to fp32 results (states, the gradients of states and
-// parameters) takes three planes and all products p q with p + q < 3, 2^-24 of the
-// value: such results of 16-bit calls are as exact as those of fp32 ones.  What
-// leads to 16-bit results alone takes two, 2^-17, which leaves the rounding at the
-// store as the error.
+// multiplied: three planes and all products p q with p + q < 3, 2^-24 of the value.
+// Fp32 results (states, the gradients of states and parameters) of 16-bit calls are
+// as exact as those of fp32 ones.  Where a value leads to bf16 results alone (the masked
+// products, the state as the outputs read it, the weights W of the backward) it has
+// two, 2^-17 of it: over 1,000 tokens that moves a result by 1.2e-5 of their root mean square
+// at most, 1/300 of the largest rounding at the store, and 1 value in 1,000 to its other
+// neighbour.  Three there would cost 281 and 295 us, forward and backward of 32,768 tokens of 12
+// heads of 64 x 64, and 78 and 96, a prompt of 16,384 of 12 of 64 x 128.  In fp16, whose store
+// rounds 8 times finer, two were 1.3e-4 off, a quarter of the store's rounding, and one value in
+// 100 went to its other neighbour: it has three (12 heads of 64 x 64: 395 and 415 us).
 #pragma once
 
 #include "ttt_ssm.h"
@@ -71,7 +76,7 @@ constexpr int scan_padded(int N) { return N <= 32 ? 32 : N <= 64 ? 64 : 128; }
 template <typename T> struct ScanType;
 // planes of an input, and of a formed value that leads to results of this type alone
 template <> struct ScanType<__bf16> { static constexpr int IN = 1, MID = 2; };
-template <> struct ScanType<_Float16> { static constexpr int IN = 2, MID = 2; };
+template <> struct ScanType<_Float16> { static constexpr int IN = 2, MID = 3; };
 template <> struct ScanType<float> { static constexpr int IN = 3, MID = 3; };
 constexpr int kFull = 3;  // planes of a formed value that leads to fp32 results
 // tokens of a chunk: 64, or 32 where the backward's planes would not fit in LDS

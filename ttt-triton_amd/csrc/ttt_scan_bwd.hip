@@ -33,18 +33,25 @@ namespace ttt {
 namespace {
 
 // Waves for 16 features, one or two: two where a workgroup has two waves for its features
-// and the state of each is small, and where one would hold two planes of everything.
+// and the state of each is small, and where one would hold two planes of everything (but not
+// where a compute unit then has one workgroup in place of two: fp16, 32 x 64).
 // us with one and with two, 32,768 tokens (fp32 16,384), 12 heads of 64 or 24 of 32:
 //              N 32        64        128
-//   P 32 bf16  165 125   192 234   150 181 (16,384 tokens)
-//        fp16  185 134   221 266
-//        fp32  128 108   170 139   217 280
-//   P 64 bf16   85 117   106 127   204 536
-//        fp16  101 138   206 169   244 322
-//        fp32   75 102    95 130   184 188
+//   P 32 bf16  163 124   177 157   249 308
+//        fp16  192 136   210 270   320 426
+//        fp32  120 102   154 135   185 278
+//   P 64 bf16   84 114   101 142   193 303
+//        fp16   94 128   197 164   242 327
+//        fp32   74 103    91 129   172 230
 template <typename T, int P, int NP>
-constexpr int kRoles = P == 32 ? (NP == 32 || (NP == 64 && ScanType<T>::IN == 3) ? 2 : 1)
+constexpr int kRoles = P == 32 ? (NP == 32 || (NP == 64 && ScanType<T>::IN != 2) ? 2 : 1)
                                : (NP == 64 && ScanType<T>::IN == 2 ? 2 : 1);
+
+// Whether a wave adds up its columns' shares of u and v before they go to LDS.  32,768 tokens, us
+// without and with: 24 heads of 32 x 64 in fp16 417 and 209 (two workgroups a compute unit in place of
+// one, by 1.4 KB of LDS), in bf16 186 and 177, of 32 x 128 273 and 249; but 12 of 64 x 128 in fp16 242
+// and 304 (four registers more than two workgroups have).
+template <typename T, int P, int NP> constexpr bool kByWave = !(ScanType<T>::IN == 2 && P == 64 && NP == 128);
 
 template <typename T, int P, int NP> struct BwdShared {
   static constexpr int IN = ScanType<T>::IN, MID = ScanType<T>::MID, Q = chunk_of<T, NP>(), TB = Q / 16;
@@ -55,10 +62,11 @@ template <typename T, int P, int NP> struct BwdShared {
   Decays<Q> dec[3];        // of the head before, this one and the next
   // What is left of a head for the gradient of its steps: of W (C . B) by tiles the sums of
   // the columns, before d_j, and of the rows (of a block that meets itself what crosses its
-  // tokens), and shares of u_i and of v_j / d_j by 16 columns
+  // tokens), and shares of u_i and of v_j / d_j by a wave's columns or by 16 columns
+  static constexpr int PARTS = kByWave<T, P, NP> && W < NB ? W : NB;
   struct alignas(16) Head {
     float row[TILES][16], col[TILES][16];
-    float u[NB][Q], v[NB][Q];
+    float u[PARTS][Q], v[PARTS][Q];
     float dD[W * kRoles<T, P, NP>], gh[W];
   } head[2];
 };
@@ -129,7 +137,7 @@ __device__ __forceinline__ void steps_grad(const ScanParams& p, const BwdShared<
   if (in) {
     for (int k = tb + 1; k < TB; ++k) before += s.col[tri(k, tb)][tr];
 #pragma unroll
-    for (int k = 0; k < NB; ++k) {
+    for (int k = 0; k < Sh::PARTS; ++k) {
       u += s.u[k][t];
       v += s.v[k][t];
     }
@@ -191,6 +199,7 @@ __global__ __launch_bounds__(4 * P * ROLES) void scan_bwd_kernel(ScanParams p) {
   // all tokens of its blocks; else one block and every SHARE-th 16 tokens
   constexpr int COLS = NB >= W ? NB / W : 1, SHARE = NB >= W ? 1 : W / NB, TOK = TB / SHARE;
   static_assert(COLS * W * TOK == NB * TB, "whole shares");
+  constexpr bool BY_WAVE = kByWave<T, P, NP>;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   Sh& sh = *reinterpret_cast<Sh*>(smem);
   const int w = wave_id(), l = lane_id(), g = l >> 4, r = l & 15;
@@ -353,6 +362,7 @@ __global__ __launch_bounds__(4 * P * ROLES) void scan_bwd_kernel(ScanParams p) {
 #pragma unroll
         for (int k = 0; k < P / 32; ++k) s[q][k] = st[0][q].op(k);
       if (h + 1 < h1) states(h + 1, 0);
+      float part[TOK] = {};
 #pragma unroll
       for (int q = 0; q < COLS; ++q) {
         const int n0 = 16 * (nb0 + W * q);
@@ -367,8 +377,11 @@ __global__ __launch_bounds__(4 * P * ROLES) void scan_bwd_kernel(ScanParams p) {
           for (int k = 0; k < P / 32; ++k) mma<kFull>(acc, s[q][k], sh.x.rows(16 * jb, 32 * k));
           acc *= dec.tail[j];
           const f4 vv = acc * sh.b.quad(j, n0 + 4 * g);
-          const float sv = sum_col4((vv[0] + vv[1]) + (vv[2] + vv[3]));
-          if (g == 0) hd.v[nb0 + W * q][j] = sv;
+          part[o] = (BY_WAVE ? part[o] : 0.f) + ((vv[0] + vv[1]) + (vv[2] + vv[3]));
+          if (!BY_WAVE || q + 1 == COLS) {
+            const float sv = sum_col4(part[o]);
+            if (g == 0) hd.v[BY_WAVE ? nb0 : nb0 + W * q][j] = sv;
+          }
           sum[0][q][o] += acc * dec.d[j];
 #pragma unroll
           for (int k = 0; k < Q / 32; ++k) {
@@ -391,6 +404,7 @@ __global__ __launch_bounds__(4 * P * ROLES) void scan_bwd_kernel(ScanParams p) {
 #pragma unroll
         for (int k = 0; k < P / 32; ++k) s[q][k] = st[Z][q].op(k);
       if (h + 1 < h1) states(h + 1, 1);
+      float part[TOK] = {};
 #pragma unroll
       for (int q = 0; q < COLS; ++q) {
         const int n0 = 16 * (nb0 + W * q);
@@ -405,8 +419,11 @@ __global__ __launch_bounds__(4 * P * ROLES) void scan_bwd_kernel(ScanParams p) {
           for (int k = 0; k < P / 32; ++k) mma<kFull>(acc, s[q][k], sh.dy.rows(16 * ib, 32 * k));
           acc *= dec.head[i];
           const f4 uu = acc * sh.c.quad(i, n0 + 4 * g);
-          const float su = sum_col4((uu[0] + uu[1]) + (uu[2] + uu[3]));
-          if (g == 0) hd.u[nb0 + W * q][i] = su;
+          part[o] = (BY_WAVE ? part[o] : 0.f) + ((uu[0] + uu[1]) + (uu[2] + uu[3]));
+          if (!BY_WAVE || q + 1 == COLS) {
+            const float su = sum_col4(part[o]);
+            if (g == 0) hd.u[BY_WAVE ? nb0 : nb0 + W * q][i] = su;
+          }
           sum[Z][q][o] += acc;
           // W as an operand with free i and contraction j: the transposing read of its tiles,
           // whose lane 16 a + j holds rows 4a..4a+3 of column j
