@@ -10,8 +10,8 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._common import check_device, dtype_code, on_device
-from .ssm import _as, _bytes, _empty, _layout, _opt, _param, _rows, _rows_again, _stream, _wants_grad, _whole
+from ._common import as_act, check_device, dtype_code, on_device
+from .ssm import _as, _bytes, _empty, _opt, _param, _rows, _stream, _wants_grad, _whole
 
 LAYER_NORM_EPS = 1e-6
 MAX_WIDTH = 16384
@@ -59,7 +59,7 @@ class LayerNormFunction(torch.autograd.Function):
     def forward(ctx, x, weight, bias, gate, eps):
         y, (xr, ldx, gr, ldg, w, stats) = _norm_forward(x, weight, bias, gate, eps, True)
         ctx.save_for_backward(xr, gr, w, stats)
-        ctx.layouts = _layout(xr, ldx), None if gr is None else _layout(gr, ldg)
+        ctx.lds, ctx.strides = (ldx, ldg), (xr.stride(), None if gr is None else gr.stride())
         ctx.dtypes = None if weight is None else (weight.dtype, bias.dtype)
         ctx.shape = x.shape
         return y
@@ -71,12 +71,13 @@ class LayerNormFunction(torch.autograd.Function):
         dev, dt = x.device, x.dtype
         D = ctx.shape[-1]
         R = stats.shape[0]
-        es, lead = x.element_size(), len(ctx.shape) - 1
-        rows = lambda t, align, width: _rows(t, lead, align, width)  # noqa: E731
-        x, ldx = _rows_again(x, ctx.layouts[0], es, D, rows)
-        gate, ldg = (None, 0) if gate is None else _rows_again(gate, ctx.layouts[1], es, D, rows)
+        ldx, ldg = ctx.lds
+        if (x.stride(), None if gate is None else gate.stride()) != ctx.strides:  # (as in ssm.py)
+            x, ldx = _rows(x, len(ctx.shape) - 1, x.element_size(), D)
+            if gate is not None:
+                gate, ldg = _rows(gate, len(ctx.shape) - 1, x.element_size(), D)
         w, stats = _whole(w), _whole(stats)
-        dy = dy.to(dt).contiguous()
+        dy = as_act(dy, dt)
         dx = x.new_empty(ctx.shape)
         dg = x.new_empty(ctx.shape) if gate is not None else None
         lib = _lib.load()

@@ -28,7 +28,7 @@ from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._common import check_device, dtype_code, f32c, on_device
+from ._common import as_act, check_device, dtype_code, f32c, on_device
 
 HEAD_DIMS = (32, 64)
 MAX_STATE = 128
@@ -81,23 +81,12 @@ def _near_rows(t, align, width):
 
 
 # Hooks on saved tensors may bring one back in another layout than it was saved in (a
-# contiguous one most often, after a stay on the CPU): the backwards take addresses and
-# strides from the tensors that they unpack.
-
-def _layout(t, ld):
-    """What _rows_again compares a saved tensor with."""
-    return t.stride(), ld
-
-
-def _rows_again(t, was, align, width, rows):
-    """rows(t, align, width) of a saved tensor; its stride is known where t lies as it was saved"""
-    strides, ld = was
-    return (t, ld) if t.stride() == strides and t.data_ptr() % align == 0 else rows(t, align, width)
-
+# contiguous one most often, after a stay on the CPU): the backwards compare the layouts of
+# what they unpack with those that they kept, and find rows and strides again where one differs.
 
 def _whole(t, align: int = 1):
     """t as one contiguous block on `align` bytes"""
-    if t is None or t.is_contiguous() and (align == 1 or t.data_ptr() % align == 0):
+    if t is None or t.is_contiguous() and t.data_ptr() % align == 0:
         return t
     return t.detach().clone(memory_format=torch.contiguous_format)
 
@@ -217,7 +206,7 @@ class CausalConvFunction(torch.autograd.Function):
     def forward(ctx, x, weight, bias, state, activation, want_last):
         y, last, (xr, ldx, s0, w, b) = _conv_forward(x, weight, bias, state, activation, want_last)
         ctx.save_for_backward(xr, s0, w, b)
-        ctx.layout = _layout(xr, ldx)
+        ctx.ldx, ctx.strides = ldx, xr.stride()
         ctx.activation = activation
         ctx.dtypes = weight.dtype, None if bias is None else bias.dtype, None if state is None else state.dtype
         ctx.shape = (*x.shape, weight.shape[1])
@@ -231,9 +220,11 @@ class CausalConvFunction(torch.autograd.Function):
         B, L, C, W = ctx.shape
         dev = x.device
         dt = x.dtype
-        x, ldx = _rows_again(x, ctx.layout, x.element_size(), C, _sequence_rows)
+        ldx = ctx.ldx
+        if x.stride() != ctx.strides:
+            x, ldx = _sequence_rows(x, x.element_size(), C)
         s0, w, b = _whole(s0), _whole(w), _whole(b)
-        dy, dlast = (None if g is None else g.to(dt).contiguous() for g in (dy, dlast))
+        dy, dlast = None if dy is None else as_act(dy, dt), None if dlast is None else as_act(dlast, dt)
         dx = x.new_empty((B, L, C))
         ds = x.new_empty((B, W - 1, C)) if ctx.needs_input_grad[3] else None
         dw = w.new_empty((C, W))
@@ -370,8 +361,10 @@ class SelectiveScanFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, dt, A, Bm, Cm, D, dt_bias, h0, softplus, want_last):
         y, last, (rows, a, d, bias, states) = _scan_forward(x, dt, A, Bm, Cm, D, dt_bias, h0, softplus, want_last, True)
-        ctx.save_for_backward(*rows[::2], a, d, bias, states)
-        ctx.layouts, ctx.softplus = [_layout(t, ld) for t, ld in zip(rows[::2], rows[1::2])], softplus
+        ctx.save_for_backward(rows[0], rows[2], rows[4], rows[6], a, d, bias, states)
+        xr, ldx, dr, ldd, br, ldb, cr, ldc = rows
+        ctx.lds, ctx.strides = (ldx, ldd, ldb, ldc), (xr.stride(), dr.stride(), br.stride(), cr.stride())
+        ctx.softplus = softplus
         ctx.shape = (*x.shape, *Bm.shape[2:])
         ctx.dtypes = tuple(None if t is None else t.dtype for t in (A, D, dt_bias, h0))
         ctx.set_materialize_grads(False)
@@ -382,16 +375,15 @@ class SelectiveScanFunction(torch.autograd.Function):
     def backward(ctx, dy, dlast):
         x, dt, Bm, Cm, a, d, bias, states = ctx.saved_tensors
         B, L, H, P, G, N = ctx.shape
-        of_x, of_dt, of_b, of_c = ctx.layouts
-        x, ldx = _rows_again(x, of_x, 16, H * P, _near_rows)
-        dt, ldd = _rows_again(dt, of_dt, dt.element_size(), H, _sequence_rows)
-        Bm, ldb = _rows_again(Bm, of_b, 16, G * N, _near_rows)
-        Cm, ldc = _rows_again(Cm, of_c, 16, G * N, _near_rows)
+        ldx, ldd, ldb, ldc = ctx.lds
+        if ((x.stride(), dt.stride(), Bm.stride(), Cm.stride()) != ctx.strides
+                or (x.data_ptr() | Bm.data_ptr() | Cm.data_ptr()) % 16):
+            x, ldx, dt, ldd, Bm, ldb, Cm, ldc = _scan_rows(x, dt, Bm, Cm, _near_rows, 16, ctx.shape)
         a, d, bias, states = _whole(a), _whole(d), _whole(bias), _whole(states, 16)
         dev, act = x.device, x.dtype
         code = dtype_code(act)
         dy = torch.zeros((B, L, H, P), device=dev, dtype=act) if dy is None else dy
-        dyr, ldy = _near_rows(dy.to(act), 16, H * P)
+        dyr, ldy = _near_rows(dy if dy.dtype == act else dy.to(act), 16, H * P)
         dlast = None if dlast is None else _whole(f32c(dlast), 16)
         dx = x.new_empty((B, L, H, P))
         ddt = dt.new_empty((B, L, H))
