@@ -15,9 +15,17 @@ on 16 bytes in every row, and from a copy elsewhere.  Results do not depend on
 which; nothing of a call depends on another sequence of its batch, but its
 rounding may: the length is cut up by the number of sequences and heads.
 
+Sums, states and their products are fp32; in bf16 calls the masked products, the state
+that an output reads and the weights of the gradients of B and C are rounded to 2^-17
+of themselves where they are multiplied (the outputs to 2^-8).
+
 A token that is not finite reaches the outputs and states of its own sequence from
 that token on, and no earlier output.  In the backward it may reach every gradient
-of its sequence."""
+of its sequence.  (An fp32 value above 3.39e38, which bf16 would round to infinity,
+counts as not finite in the scan.)
+
+Gradients are of the first order and in reverse mode; forward-mode derivatives raise
+NotImplementedError."""
 
 from __future__ import annotations
 
