@@ -439,6 +439,8 @@ int ttt_causal_conv_step(const void* x, long long ldx, void* state, const float*
  *   y       [B][L][H][P]                   h_last [B][H][P][N], or NULL
  *   states  NULL, or ttt_scan_states_bytes: what ttt_scan_bwd needs of the forward
  *   workspace  ttt_scan_workspace_bytes (NULL where that is 0)
+ * With dtype BF16, values formed on the way to bf16 results alone are rounded to 2^-17 of
+ * themselves where they are multiplied; everywhere else products are fp32's.
  * x, Bm and Cm and their rows start on 16 bytes; where there are more tokens than
  * one, rows of x, Bm, Cm (and dy) are less than 64 MiB apart. */
 size_t ttt_scan_states_bytes(int B, int L, int H, int P, int N, int dtype);

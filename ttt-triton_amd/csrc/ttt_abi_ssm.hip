@@ -59,8 +59,9 @@ struct ScanPlan {
 };
 // Workgroups of the walk that a compute unit holds, by its registers and LDS.  Heads of 64
 // with states up to 32 in fp32 need fewer registers walking back: 132 forwards and 116 back.
-// (With one workgroup more than is held, us forwards of 32 x 1,024 tokens of 8 heads of 64 x 32:
-// fp16 70 and now 61, fp32 76 and 72; of 4 x 4,096 of 12: 58 and 65, 71 and 64.)
+// (With one workgroup more than is held, and with those that are, us forwards of 32 x 1,024
+// tokens of 8 heads of 64 x 32: fp16 69 and 64, fp32 75 and 72; of 16 x 2,048 of 12: 100 and 96, 108
+// and 102; of 4 x 4,096 of 12: 61 and 68, 72 and 64.)
 int walk_resident(int P, int NP, int dtype, bool back) {
   constexpr signed char t[2][3][3] = {{{5, 3, 5}, {4, 2, 3}, {2, 3, 2}}, {{3, 2, 3}, {3, 2, 3}, {2, 2, 2}}};
   if (back && P == 64 && NP == 32 && dtype == TTT_DTYPE_F32) return 4;
@@ -69,16 +70,17 @@ int walk_resident(int P, int NP, int dtype, bool back) {
 // How a scan is cut up.  Segments: a workgroup walks a sequence and head; where that
 // makes too few of them, the tokens are shared out as well, whole chunks each, to at
 // most the full rounds of the card nearest above three workgroups of 64 features or
-// five of 32 a compute unit, 8 segments though, which a workgroup joins by itself.  (Forward and backward of 32,768 tokens: 768 at once, 12 heads of
-// 64 x 64 in bf16: 322, 296 and 318 us with 3, 4 and 6 segments; 512 at once, in fp16: 480,
-// 449, 422, 435 with 3, 4, 5, 6; 1,024 at once, 24 heads of 32 x 64: 484, 463, 430, 447 with
-// 3, 4, 5, 8.)  More segments cost two launches and a pass over them all: one round of the card,
-// where 8 do not fill three quarters of it.  (128 chains of 32 x 64: 166 us with 8, 189 with 11.
-// Forward of 40,000 tokens of 5 heads of 64 x 128 in fp16, 512 at once: 138, 128 and 155 us with 128, 86 and 52
-// segments; 2 x 5,000 of 9 in bf16: 53, 47 and 54 with 40, 27 and 20.)
+// five of 32 a compute unit, 8 segments though, which a workgroup joins by itself.  (Forward
+// and backward of 32,768 tokens: 768 at once, 12 heads of 64 x 64 in bf16: 306, 279 and 299 us
+// with 3, 4 and 6 segments; 512 at once, in fp16: 469, 439, 413, 423 with 3, 4, 5, 6; 1,024 at
+// once, 24 heads of 32 x 64: 406, 383, 362, 383 with 3, 4, 5, 8.)  More segments cost two launches
+// and a pass over them all: one round of the card, where 8 do not fill three quarters of it.
+// (128 chains of 32 x 64: 139 us with 8, 159 with 11.  Forward of 40,000 tokens of 5 heads of
+// 64 x 128 in fp16, 512 at once: 141, 122, 134 and 164 us with 128, 102, 86 and 52 segments; 2 x
+// 5,000 of 9 in bf16: 53, 47 and 52 with 40, 27 and 20.)
 // Splits: the backward's workgroups have a chunk and go over a group's heads; below
 // 512 of them, two a compute unit, the heads are shared out.  (16,384 tokens of 12 heads of
-// 64 x 64 in bf16: 175 us forward and backward, 200 with half and 186 with twice as many.)
+// 64 x 64 in bf16: 157 us forward and backward, 174 with half and 168 with twice as many.)
 ScanPlan plan(int B, int L, int H, int P, int G, int N, int dtype, bool back) {
   ScanPlan s;
   s.NP = ttt::scan_padded(N);

@@ -12,8 +12,12 @@
 // read once and W-1 rows again per run; z is formed again in the backward, which
 // costs W multiply-adds instead of a stored row.  Eight channels a thread need twice the
 // registers for the rows on their way: 176 us for forward and backward of 32,768 tokens of
-// 896 bf16 channels, 94 with four (31 forward, 117 MB: 3.8 TB/s; 59 backward, 176 MB: 3.0;
-// a device copy runs at 5.2).  One token of 64 sequences: 4 us, a launch.
+// 896 bf16 channels, 94 with four.  Of that 36 are the forward's in a graph of its own (117 MB,
+// 3.3 TB/s); in a trace of whole passes it has 40 us and the backward 62 (176 MB, 2.8 TB/s),
+// where a device copy runs at 5.2.  What is missing: every row's load stands behind branches of its
+// own (is the row there, are all four channels), and waits with them, so that a thread has one
+// row on its way; and the backward's 139 registers leave three waves to a SIMD.  One token of 64
+// sequences: 4 us, a launch.
 #include <math.h>
 
 #include <algorithm>
@@ -126,7 +130,7 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvParams p, int groups,
     const long long b = job / runs;
     const int u0 = run * kRunBwd;
     // Step m handles token t = u0 - (W-1) + m, in groups of W steps whose rows are
-    // loaded a group ahead.  Row s[t + W-1] has place m % W, dz[t] too, so that
+    // asked for a group ahead (each behind its own branches).  Row s[t + W-1] has place m % W, dz[t] too, so that
     // s[t + k] is at (m + 1 + k) % W and dz[t - k] at (m - k) % W.
     Raw<T, kV> win[W], nx[W], ng[W];
     float dz[W][kV];

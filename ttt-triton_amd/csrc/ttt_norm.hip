@@ -13,9 +13,13 @@
 // brings.  The backward's workgroups walk rows, the next one on its way (not with 16
 // waves, which have 128 registers), with the sums of dw and db in registers, and write one
 // partial sum each, added up by a second launch in a fixed order.
-// 32,768 gated rows of 768 in bf16: forward 28 us (151 MB, 5.4 TB/s), backward 53 (252 MB,
-// 4.8 TB/s) and 4 for the partial sums; 4,099 rows of 5,001 in fp16, whose rows begin on odd
-// addresses: 24, 35 and 9 (82 and 123 MB, 3.5 TB/s).  A device copy runs at 5.2 TB/s.
+// In a trace of whole passes, 32,768 gated rows of 768 in bf16: forward 34 us (151 MB, 4.5 TB/s),
+// backward 51 (252 MB, 4.9) and 4 for the partial sums; 4,099 rows of 5,001 in fp16, whose rows
+// begin on odd addresses: 24, 38 and 9 (82 and 123 MB, 3.4 and 3.3 TB/s).  A device copy runs at
+// 5.2 TB/s.  Above 8,192 values the backward does not fit its 128 registers, but for
+// 12 values a lane without a gate: up to 32 bytes a lane go to scratch without one, 56 to 204 with
+// one.  4,096 rows of 12,288 in bf16, forward and backward: 136 us without a gate (3.0 TB/s), 404
+// with one (1.5), where 8,192 values take 87 and 123 (3.1 and 3.3).
 #include <math.h>
 
 #include <algorithm>
@@ -270,8 +274,7 @@ hipError_t run_t(const NormParams& p, bool bwd, hipStream_t stream) {
 template <typename T, int NW, int V, int NCH> hipError_t gate_t(const NormParams& p, bool bwd, hipStream_t s) {
   return p.gate != nullptr ? run_t<T, NW, V, NCH, true>(p, bwd, s) : run_t<T, NW, V, NCH, false>(p, bwd, s);
 }
-// Waves to a row and values to a lane, so that few lanes' places are empty and no more than
-// 128 registers are needed with 16 waves
+// Waves to a row and values to a lane, so that few lanes' places are empty
 template <typename T, int NW> hipError_t lanes_t(const NormParams& p, bool bwd, hipStream_t s) {
   const int four = (p.D + 256 * NW - 1) / (256 * NW);  // values to a lane, in fours
   if constexpr (NW <= 4) {
@@ -280,9 +283,9 @@ template <typename T, int NW> hipError_t lanes_t(const NormParams& p, bool bwd, 
   }
   return four == 3 ? gate_t<T, NW, 4, 3>(p, bwd, s) : gate_t<T, NW, 8, 2>(p, bwd, s);
 }
-// (Gated bf16 rows, forward and backward: 32,768 of 768 with one wave 85 us, with four 126;
-// 8,192 of 2,304 with four 71, with eight 133; of 4,096 131 and 156; 4,096 of 5,120 with eight
-// 91, with sixteen 265.)
+// (Gated bf16 rows, forward and backward: 32,768 of 768 with one wave 90 us, with four 124;
+// 8,192 of 2,304 with four 73, with eight 134; of 4,096 119 and 159; 4,096 of 5,120 with eight
+// 94, with sixteen 266.)
 constexpr int waves_of(int D) { return D <= 1024 ? 1 : D <= 4096 ? 4 : D <= 8192 ? 8 : 16; }
 template <typename T> hipError_t waves_t(const NormParams& p, bool bwd, hipStream_t s) {
   const int w = waves_of(p.D);
@@ -297,10 +300,12 @@ hipError_t launch(const NormParams& p, int dtype, bool bwd, hipStream_t s) {
 
 }  // namespace
 
-// Workgroups of the backward: as many as are there at once, 12 waves to a compute unit (16 of
-// longer rows), or 8 where a lane has 16 values.  (With 12 values 12 and 8 waves: 768 gated
-// 57 and 62 us, 5,001 without a gate 44 and 52; with 16 values: 1,024 gated 48 and 38, 4,096
-// 92 and 78, 8,192 91 and 84.)
+// Workgroups of the backward, in waves to a compute unit: 12 of rows of one and of four waves, 16
+// of rows of eight; 8 of all three where a lane has 16 values; 16, one workgroup, of rows of sixteen
+// waves.  Forward and backward in us with fewer, these and more: 32,768 gated rows of 768, 95 (8), 89
+// (12), 100 (16); 4,099 of 5,001 without a gate 81 (8), 75 (12), 70 (16), 4,096 gated of 5,000 85, 100, 91;
+// with 16 values 16,384 gated of 1,024, 60 (8) and 69 (12), 8,192 of 4,096, 119 and 133, 4,096 of 8,192,
+// 125 (8) and 132 (16); 2,048 of 16,384, 277 (16) and 300 (two workgroups for one place).
 int norm_bwd_parts(long long R, int D) {
   const int w = waves_of(D);
   const bool full = (D + 256 * w - 1) / (256 * w) > 3;  // 16 values to a lane

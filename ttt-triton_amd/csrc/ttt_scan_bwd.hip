@@ -19,8 +19,8 @@
 //   dd_t = sum_{i>=t} F_it (x_t . dy_i) (C_i . B_t) + w_t B_t . (Gam^T x_t) + A da_t
 //
 // At 32,768 tokens of 12 heads of 64 x 64 in bf16: 106 us, 308 MB (two states of 16 KB to
-// a chunk and head are 201 of them; 2.9 TB/s).  Loads and stores alone take 75, the arithmetic
-// alone 92: per head ten 16 x 16 tiles of x . dy with their exponentials, row and column
+// a chunk and head are 201 of them; 2.9 TB/s).  Loads and stores alone take 76, the arithmetic
+// alone 82: per head ten 16 x 16 tiles of x . dy with their exponentials, row and column
 // sums, then the products into dB and dC, with three barriers between them and eight waves a
 // compute unit (237 registers).
 #include <math.h>
@@ -525,7 +525,7 @@ template <typename T> hipError_t head_t(const ScanParams& p, int P, hipStream_t 
 // One token of every sequence: h = e^{dA} h + d x (x) B in place, y = h C + D x.  The
 // state is read and written once, which bounds it; LANES lanes have a feature's row of
 // the state, four values each, and add up their share of h C.  64 sequences, 12 heads of 64 x 64:
-// 10.7 us for 25 MB from HBM (2.4 TB/s; one round of loads, latency), one sequence 4 us, a launch.
+// 10.3 us for 25 MB from HBM (2.4 TB/s; one round of loads, latency), one sequence 4 us, a launch.
 template <typename T, int LANES> __global__ __launch_bounds__(256) void scan_step_kernel(ScanStepParams p, long long rows) {
   const long long row = (long long)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;  // (b, h, feature)
   if (row >= rows) return;  // (whole groups of LANES)

@@ -20,12 +20,12 @@
 // joined beforehand (scan_join_kernel).
 //
 // What bounds it, at 32,768 tokens of 12 heads of 64 features and 64 states in bf16 (4
-// segments of 192 chains, three workgroups a compute unit): 69 us for the outputs with the
-// states kept for the backward, 210 MB of which 101 are those states, 3.0 TB/s; the loads
-// and stores alone take 60, the arithmetic alone 49 to 56 (exponentials, masks and planes
+// segments of 192 chains, three workgroups a compute unit): 68 us for the outputs with the
+// states kept for the backward, 210 MB of which 101 are those states, 3.1 TB/s; the loads
+// and stores alone take 57, the arithmetic alone 48 (exponentials, masks and planes
 // of the products more than the matrix instructions), with three workgroups to cover one
 // another.  27 us more for the end states of three segments: 8 chunks one after the other,
-// latency.  Walking back the same.
+// latency.  Walking back the same (67, 59 and 45).
 #include <math.h>
 #include <stddef.h>
 
