@@ -49,7 +49,7 @@
 extern "C" {
 #endif
 
-#define TTT_AMD_ABI_VERSION 12
+#define TTT_AMD_ABI_VERSION 13
 
 enum ttt_dtype { TTT_DTYPE_F32 = 0, TTT_DTYPE_BF16 = 1, TTT_DTYPE_F16 = 2 };
 
@@ -483,6 +483,48 @@ size_t ttt_layer_norm_partial_bytes(long long R, int D);
 int ttt_layer_norm_bwd(const void* x, long long ldx, const void* gate, long long ldg, const float* weight,
                        const float* stats, const void* dy, long long R, int D, int dtype, void* dx, void* dgate,
                        float* dweight, float* dbias, float* partial, size_t partial_bytes, void* stream);
+
+/* ---- a gated delta-rule block: delta rule, norms around it, gated feed-forward ----
+ * Activations, rows and overlaps as with the state-space layer's; no counterpart in the
+ * reference either. */
+
+/* S_t = e^{g_t} S_{t-1} + u_t (x) k_t,  u_t = beta_t (v_t - e^{g_t} S_{t-1} k_t),
+ * o_t = scale S_t q_t  per sequence and head, S [P][N]; with `unit` q and k are taken at unit
+ * length, x / sqrt(|x|^2 + 1e-6).
+ *   q, k     [B*L][ldq], [B*L][ldk]: G groups of N values (a multiple of 16 up to 128);
+ *            head h uses group h / (H/G)
+ *   v        [B*L][ldv]: H heads of P values (a multiple of 32 up to 256)
+ *   g, beta  [B*L][ldg], [B*L][ldbeta]: H values each, in `g_dtype` and `beta_dtype` (dtype or
+ *            TTT_DTYPE_F32); g <= 0, -inf for a state that is forgotten
+ *   h0       [B][H][P][N], or NULL for zeros
+ *   o        [B][L][H][P]                   h_last [B][H][P][N], or NULL
+ *   saved    NULL, or ttt_delta_saved_bytes: what ttt_delta_bwd needs of the forward
+ *   workspace  ttt_delta_workspace_bytes
+ * Precision, alignment and rows as with ttt_scan_fwd. */
+size_t ttt_delta_saved_bytes(int B, int L, int H, int P, int N, int dtype);
+size_t ttt_delta_workspace_bytes(int B, int L, int H, int P, int N, int dtype);
+int ttt_delta_fwd(const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv,
+                  const void* g, long long ldg, const void* beta, long long ldbeta, const float* h0, int B, int L,
+                  int H, int P, int G, int N, float scale, int unit, int dtype, int g_dtype, int beta_dtype, void* o,
+                  float* h_last, void* saved, size_t saved_bytes, void* workspace, size_t workspace_bytes,
+                  void* stream);
+
+/* Its gradients from dO [B*L][lddo] and dh_last (NULL: zeros), given what ttt_delta_fwd
+ * saved for the same inputs: dq, dk [B][L][G][N], dv [B][L][H][P], dg, dbeta [B][L][H] in the
+ * types of g and beta, dh0 [B][H][P][N] (or NULL). */
+size_t ttt_delta_bwd_workspace_bytes(int B, int L, int H, int P, int G, int N, int dtype);
+int ttt_delta_bwd(const void* q, long long ldq, const void* k, long long ldk, const void* g, long long ldg,
+                  const void* beta, long long ldbeta, const void* dO, long long lddo, const float* dh_last,
+                  const void* saved, size_t saved_bytes, int B, int L, int H, int P, int G, int N, float scale,
+                  int unit, int dtype, int g_dtype, int beta_dtype, void* dq, void* dk, void* dv, void* dg,
+                  void* dbeta, float* dh0, void* workspace, size_t workspace_bytes, void* stream);
+
+/* One token of every sequence: rows as above with one a sequence, h [B][H][P][N] updated
+ * in place, o [B][H][P]. */
+int ttt_delta_step(const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv,
+                   const void* g, long long ldg, const void* beta, long long ldbeta, float* h, int B, int H, int P,
+                   int G, int N, float scale, int unit, int dtype, int g_dtype, int beta_dtype, void* o,
+                   void* stream);
 
 /* Bytes of the static device scratch of ttt_mlp_bwd_noalloc (per GPU). */
 #define TTT_MLP_BWD_NOALLOC_SCRATCH_BYTES (64u << 20)

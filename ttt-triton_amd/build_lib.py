@@ -56,6 +56,7 @@ PER_FILE = {
     "ttt_linear_bwd.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"],
     "ttt_scan_walk.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"],
     "ttt_scan_bwd.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"],
+    "ttt_delta_walk.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"],
 }
 
 

@@ -1,0 +1,267 @@
+// extern "C" entry points of a gated delta-rule block's operators: host-side validation
+// and workspace layout, then launches on the caller's stream.  Declarations and argument
+// contracts are in include/ttt_amd.h.
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "ttt_abi_check.h"
+#include "ttt_delta.h"
+
+namespace {
+
+// ---- gated delta rule
+int check_delta(int B, int L, int H, int P, int G, int N, int dtype, int g_dtype, int beta_dtype) {
+  if (!dtype_ok(dtype)) return TTT_ERR_DTYPE;
+  for (int d : {g_dtype, beta_dtype})
+    if (d != dtype && d != TTT_DTYPE_F32) return TTT_ERR_DTYPE;
+  if (B <= 0 || L <= 0 || H <= 0 || G <= 0 || H % G != 0) return TTT_ERR_SHAPE;
+  if (P < 32 || P > ttt::kDeltaMaxP || P % 32 != 0 || N < 16 || N > 128 || N % 16 != 0) return TTT_ERR_SHAPE;
+  if (L > 0x7fffff00 || (long long)B * H > kMaxGrid || H > (1 << 23) / P || G > (1 << 23) / N) return TTT_ERR_SHAPE;
+  return TTT_OK;
+}
+struct DeltaPlan {
+  int Q, NC, PB, parts, share;
+  size_t tok, z, m, mb, states, rows, qk, gb;
+};
+DeltaPlan delta_plan(int B, int L, int H, int P, int G, int N, int dtype) {
+  DeltaPlan s;
+  s.Q = ttt::delta_chunk(dtype);
+  s.NC = (L + s.Q - 1) / s.Q;
+  s.PB = ttt::delta_part(P);
+  s.parts = P / s.PB;
+  s.share = H / G * s.parts;
+  const size_t chunks = (size_t)B * H * s.NC;
+  s.tok = up256(chunks * ttt::delta_tok_floats(s.Q) * 4);
+  s.z = chunks * ttt::delta_operands(s.Q, 3);
+  s.m = chunks * ttt::delta_operands(s.Q, ttt::delta_mid(dtype));
+  s.mb = chunks * ttt::delta_operands(s.Q, 3);
+  s.states = chunks * P * ttt::scan_padded(N) * 4;
+  s.rows = chunks * P * s.Q * 4;
+  s.qk = s.share > 1 ? (size_t)s.share * B * L * G * N * 4 : 0;
+  s.gb = s.parts > 1 ? up256((size_t)s.parts * B * L * H * 4) : 0;
+  return s;
+}
+bool delta_grid_ok(const DeltaPlan& s, int B, int H, int P) {
+  // (prep: 256 threads a chunk and head; walk: four for a feature and sequence; gradients: 512 a chunk and part)
+  return (long long)B * H * P <= kMaxThreads / 4 && (long long)B * H <= kMaxThreads / 512 / s.NC / s.parts;
+}
+bool delta_plan_ok(int B, int L, int H, int P, int G, int N, int dtype, DeltaPlan& s) {
+  if (check_delta(B, L, H, P, G, N, dtype, dtype, dtype) != TTT_OK) return false;
+  s = delta_plan(B, L, H, P, G, N, dtype);
+  return delta_grid_ok(s, B, H, P);
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t ttt_delta_saved_bytes(int B, int L, int H, int P, int N, int dtype) {
+  DeltaPlan s;
+  return delta_plan_ok(B, L, H, P, 1, N, dtype, s) ? s.states + s.rows : 0;
+}
+size_t ttt_delta_workspace_bytes(int B, int L, int H, int P, int N, int dtype) {
+  DeltaPlan s;
+  return delta_plan_ok(B, L, H, P, 1, N, dtype, s) ? s.tok + s.z + s.m : 0;
+}
+size_t ttt_delta_bwd_workspace_bytes(int B, int L, int H, int P, int G, int N, int dtype) {
+  DeltaPlan s;
+  return delta_plan_ok(B, L, H, P, G, N, dtype, s) ? s.tok + s.z + s.mb + s.states + s.rows + 2 * s.gb + 2 * s.qk : 0;
+}
+
+int ttt_delta_fwd(const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv,
+                  const void* g, long long ldg, const void* beta, long long ldbeta, const float* h0, int B, int L,
+                  int H, int P, int G, int N, float scale, int unit, int dtype, int g_dtype, int beta_dtype, void* o,
+                  float* h_last, void* saved, size_t saved_bytes, void* workspace, size_t workspace_bytes,
+                  void* stream) {
+  int st = check_delta(B, L, H, P, G, N, dtype, g_dtype, beta_dtype);
+  if (st != TTT_OK) return st;
+  const DeltaPlan s = delta_plan(B, L, H, P, G, N, dtype);
+  if (!delta_grid_ok(s, B, H, P)) return TTT_ERR_SHAPE;
+  if (ldg < H || ldbeta < H) return TTT_ERR_SHAPE;
+  if ((st = check_row(ldq, (long long)G * N, L, dtype)) != TTT_OK) return st;
+  if ((st = check_row(ldk, (long long)G * N, L, dtype)) != TTT_OK) return st;
+  if ((st = check_row(ldv, (long long)H * P, L, dtype)) != TTT_OK) return st;
+  REQUIRE(q, 16);
+  REQUIRE(k, 16);
+  REQUIRE(v, 16);
+  REQUIRE(g, size_of(g_dtype));
+  REQUIRE(beta, size_of(beta_dtype));
+  REQUIRE(o, 16);
+  OPTIONAL(h0, 16);
+  OPTIONAL(h_last, 16);
+  OPTIONAL(saved, 16);
+  if (saved != nullptr && saved_bytes < s.states + s.rows) return TTT_ERR_WORKSPACE;
+  if (workspace == nullptr || workspace_bytes < s.tok + s.z + s.m) return TTT_ERR_WORKSPACE;
+  OPTIONAL(workspace, 16);
+  ttt::DeltaParams p{};
+  p.q = q;
+  p.k = k;
+  p.v = v;
+  p.g = g;
+  p.beta = beta;
+  p.ldq = ldq;
+  p.ldk = ldk;
+  p.ldv = ldv;
+  p.ldg = ldg;
+  p.ldbeta = ldbeta;
+  p.h0 = h0;
+  p.o = o;
+  p.h_last = h_last;
+  p.B = B;
+  p.L = L;
+  p.H = H;
+  p.G = G;
+  p.N = N;
+  p.P = P;
+  p.scale = scale;
+  p.l2 = unit != 0;
+  p.g_f32 = g_dtype == TTT_DTYPE_F32;
+  p.beta_f32 = beta_dtype == TTT_DTYPE_F32;
+  char* ws = static_cast<char*>(workspace);
+  p.tok = reinterpret_cast<float*>(ws);
+  p.z = ws + s.tok;
+  p.m = ws + s.tok + s.z;
+  if (saved != nullptr) {
+    p.states = static_cast<float*>(saved);
+    p.rows = reinterpret_cast<float*>(static_cast<char*>(saved) + s.states);
+  }
+  const hipError_t e = ttt::launch_delta_prep(p, dtype, false, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_status(e);
+  return hip_status(ttt::launch_delta_fwd(p, dtype, static_cast<hipStream_t>(stream)));
+}
+
+int ttt_delta_bwd(const void* q, long long ldq, const void* k, long long ldk, const void* g, long long ldg,
+                  const void* beta, long long ldbeta, const void* dO, long long lddo, const float* dh_last,
+                  const void* saved, size_t saved_bytes, int B, int L, int H, int P, int G, int N, float scale,
+                  int unit, int dtype, int g_dtype, int beta_dtype, void* dq, void* dk, void* dv, void* dg,
+                  void* dbeta, float* dh0, void* workspace, size_t workspace_bytes, void* stream) {
+  int st = check_delta(B, L, H, P, G, N, dtype, g_dtype, beta_dtype);
+  if (st != TTT_OK) return st;
+  const DeltaPlan s = delta_plan(B, L, H, P, G, N, dtype);
+  if (!delta_grid_ok(s, B, H, P)) return TTT_ERR_SHAPE;
+  if (ldg < H || ldbeta < H) return TTT_ERR_SHAPE;
+  if ((st = check_row(ldq, (long long)G * N, L, dtype)) != TTT_OK) return st;
+  if ((st = check_row(ldk, (long long)G * N, L, dtype)) != TTT_OK) return st;
+  if ((st = check_row(lddo, (long long)H * P, L, dtype)) != TTT_OK) return st;
+  REQUIRE(q, 16);
+  REQUIRE(k, 16);
+  REQUIRE(g, size_of(g_dtype));
+  REQUIRE(beta, size_of(beta_dtype));
+  REQUIRE(dO, 16);
+  REQUIRE(saved, 16);
+  REQUIRE(dq, 16);
+  REQUIRE(dk, 16);
+  REQUIRE(dv, 16);
+  REQUIRE(dg, size_of(g_dtype));
+  REQUIRE(dbeta, size_of(beta_dtype));
+  OPTIONAL(dh_last, 16);
+  OPTIONAL(dh0, 16);
+  if (saved_bytes < s.states + s.rows) return TTT_ERR_WORKSPACE;
+  if (workspace == nullptr ||
+      workspace_bytes < s.tok + s.z + s.mb + s.states + s.rows + 2 * s.gb + 2 * s.qk)
+    return TTT_ERR_WORKSPACE;
+  OPTIONAL(workspace, 16);
+  ttt::DeltaParams p{};
+  p.q = q;
+  p.k = k;
+  p.g = g;
+  p.beta = beta;
+  p.ldq = ldq;
+  p.ldk = ldk;
+  p.ldg = ldg;
+  p.ldbeta = ldbeta;
+  p.dO = dO;
+  p.lddo = lddo;
+  p.h0 = dh_last;
+  p.o = dv;
+  p.h_last = dh0;
+  p.B = B;
+  p.L = L;
+  p.H = H;
+  p.G = G;
+  p.N = N;
+  p.P = P;
+  p.scale = scale;
+  p.l2 = unit != 0;
+  p.g_f32 = g_dtype == TTT_DTYPE_F32;
+  p.beta_f32 = beta_dtype == TTT_DTYPE_F32;
+  char* ws = static_cast<char*>(workspace);
+  const auto take = [&ws](size_t n) {
+    char* at = ws;
+    ws += n;
+    return at;
+  };
+  p.tok = reinterpret_cast<float*>(take(s.tok));
+  p.z = take(s.z);
+  p.m = take(s.mb);
+  p.states = reinterpret_cast<float*>(take(s.states));
+  p.rows = reinterpret_cast<float*>(take(s.rows));
+  if (s.parts > 1) {
+    p.dgp = reinterpret_cast<float*>(take(s.gb));
+    p.dbp = reinterpret_cast<float*>(take(s.gb));
+  }
+  if (s.share > 1) {
+    p.dqp = reinterpret_cast<float*>(take(s.qk));
+    p.dkp = reinterpret_cast<float*>(take(s.qk));
+  }
+  const hipStream_t on = static_cast<hipStream_t>(stream);
+  hipError_t e = ttt::launch_delta_prep(p, dtype, true, on);
+  if (e != hipSuccess) return hip_status(e);
+  e = ttt::launch_delta_walk_back(p, dtype, on);
+  if (e != hipSuccess) return hip_status(e);
+  p.gstates = p.states;
+  p.states = const_cast<float*>(static_cast<const float*>(saved));
+  p.x = reinterpret_cast<const float*>(static_cast<const char*>(saved) + s.states);
+  p.dq = dq;
+  p.dk = dk;
+  p.dg = dg;
+  p.dbeta = dbeta;
+  return hip_status(ttt::launch_delta_bwd(p, dtype, on));
+}
+
+int ttt_delta_step(const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv,
+                   const void* g, long long ldg, const void* beta, long long ldbeta, float* h, int B, int H, int P,
+                   int G, int N, float scale, int unit, int dtype, int g_dtype, int beta_dtype, void* o,
+                   void* stream) {
+  const int st = check_delta(B, 1, H, P, G, N, dtype, g_dtype, beta_dtype);
+  if (st != TTT_OK) return st;
+  // (up to 32 threads to a feature, and the last workgroup's idle ones)
+  if ((long long)B * H > kMaxThreads / 32 / P - 1) return TTT_ERR_SHAPE;
+  if (ldg < H || ldbeta < H || ldv < (long long)H * P || ldq < (long long)G * N || ldk < (long long)G * N || ldq % 4 != 0 ||
+      ldk % 4 != 0)
+    return TTT_ERR_SHAPE;
+  const size_t n = size_of(dtype);
+  REQUIRE(q, 4 * n);
+  REQUIRE(k, 4 * n);
+  REQUIRE(v, n);
+  REQUIRE(g, size_of(g_dtype));
+  REQUIRE(beta, size_of(beta_dtype));
+  REQUIRE(h, 16);
+  REQUIRE(o, n);
+  ttt::DeltaStepParams p{};
+  p.q = q;
+  p.k = k;
+  p.v = v;
+  p.g = g;
+  p.beta = beta;
+  p.ldq = ldq;
+  p.ldk = ldk;
+  p.ldv = ldv;
+  p.ldg = ldg;
+  p.ldbeta = ldbeta;
+  p.h = h;
+  p.o = o;
+  p.B = B;
+  p.H = H;
+  p.P = P;
+  p.G = G;
+  p.N = N;
+  p.scale = scale;
+  p.l2 = unit != 0;
+  p.g_f32 = g_dtype == TTT_DTYPE_F32;
+  p.beta_f32 = beta_dtype == TTT_DTYPE_F32;
+  return hip_status(ttt::launch_delta_step(p, dtype, static_cast<hipStream_t>(stream)));
+}
+
+}  // extern "C"

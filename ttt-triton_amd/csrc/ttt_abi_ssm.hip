@@ -5,28 +5,10 @@
 
 #include <algorithm>
 
+#include "ttt_abi_check.h"
 #include "ttt_scan.h"
 
 namespace {
-
-bool dtype_ok(int d) { return d == TTT_DTYPE_F32 || d == TTT_DTYPE_BF16 || d == TTT_DTYPE_F16; }
-int size_of(int d) { return d == TTT_DTYPE_F32 ? 4 : 2; }
-bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
-int hip_status(hipError_t e) { return e == hipSuccess ? TTT_OK : TTT_ERR_HIP; }
-size_t up256(size_t n) { return (n + 255) / 256 * 256; }
-
-#define REQUIRE(p, n)                           \
-  do {                                          \
-    if ((p) == nullptr) return TTT_ERR_NULL;    \
-    if (!aligned(p, n)) return TTT_ERR_ALIGN;   \
-  } while (0)
-#define OPTIONAL(p, n)                                                \
-  do {                                                                \
-    if ((p) != nullptr && !aligned(p, n)) return TTT_ERR_ALIGN;       \
-  } while (0)
-
-constexpr long long kMaxGrid = 0x7fffffffLL;
-constexpr long long kMaxThreads = 0xffffffffLL;  // of a launch
 
 // ---- convolution
 int check_conv(int B, int L, int C, int W, int act, int dtype) {
@@ -46,11 +28,6 @@ int check_scan(int B, int L, int H, int P, int G, int N, int dtype, int dt_dtype
   if ((P != 32 && P != 64) || N < 16 || N > 128 || N % 16 != 0) return TTT_ERR_SHAPE;
   if (L > 0x7fffff00 || (long long)B * H > kMaxGrid || H > (1 << 23) / P || G > (1 << 23) / N) return TTT_ERR_SHAPE;
   return TTT_OK;
-}
-// a chunk's rows, up to 64, are reached by 32-bit offsets
-int check_row(long long ld, long long least, int L, int dtype) {
-  if (ld < least || ld * size_of(dtype) % 16 != 0) return TTT_ERR_SHAPE;
-  return L > 1 && ld >= (1LL << 26) / size_of(dtype) ? TTT_ERR_SHAPE : TTT_OK;
 }
 constexpr int kSelfJoined = 8;  // segments whose states the walk's workgroups join themselves
 struct ScanPlan {

@@ -16,7 +16,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 # TTT_AMD_LIB names another build of the same library (e.g. the host-ASan
 # checking build of build_lib.py --asan)
 LIB_PATH = os.environ.get("TTT_AMD_LIB") or os.path.join(_HERE, "libttt_amd.so")
-ABI_VERSION = 12
+ABI_VERSION = 13
 
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
@@ -92,6 +92,12 @@ SIGNATURES = {
     "ttt_scan_bwd": (_I, [_P, _L] * 2 + [_P] + [_P, _L] * 2 + [_P] * 2 + [_P, _L, _P, _P, _S] + [_I] * 9 + [_P] * 8
                      + [_P, _S, _P]),
     "ttt_scan_step": (_I, [_P, _L] * 2 + [_P] + [_P, _L] * 2 + [_P] * 3 + [_I] * 8 + [_P, _P]),
+    "ttt_delta_saved_bytes": (_S, [_I] * 6),
+    "ttt_delta_workspace_bytes": (_S, [_I] * 6),
+    "ttt_delta_fwd": (_I, [_P, _L] * 5 + [_P] + [_I] * 6 + [_F] + [_I] * 4 + [_P, _P] + [_P, _S] * 2 + [_P]),
+    "ttt_delta_bwd_workspace_bytes": (_S, [_I] * 7),
+    "ttt_delta_bwd": (_I, [_P, _L] * 5 + [_P, _P, _S] + [_I] * 6 + [_F] + [_I] * 4 + [_P] * 6 + [_P, _S, _P]),
+    "ttt_delta_step": (_I, [_P, _L] * 5 + [_P] + [_I] * 5 + [_F] + [_I] * 4 + [_P, _P]),
     "ttt_layer_norm_fwd": (_I, [_P, _L] * 2 + [_P] * 2 + [_L, _I, _F, _I] + [_P] * 3),
     "ttt_layer_norm_partial_bytes": (_S, [_L, _I]),
     "ttt_layer_norm_bwd": (_I, [_P, _L] * 2 + [_P] * 3 + [_L, _I, _I] + [_P] * 5 + [_S, _P]),
