@@ -526,6 +526,28 @@ int ttt_delta_step(const void* q, long long ldq, const void* k, long long ldk, c
                    int G, int N, float scale, int unit, int dtype, int g_dtype, int beta_dtype, void* o,
                    void* stream);
 
+/* r = residual + s * gate sigmoid(gate) * x / sqrt(mean x^2 + eps) * w over rows of D values
+ * (up to 8192), each part where it is given (without w, x is not normed), and with w2 and a
+ * residual y = r / sqrt(mean r^2 + eps) * w2.
+ *   x [R/heads][ldx], gate [..][ldg], residual [..][ldr] (or NULL), `heads` rows of D side by
+ *   side in each, any alignment; the residual in `res_dtype`, dtype or TTT_DTYPE_F32, or -1
+ *   without one; w, s, w2 [D] fp32, or NULL
+ *   r [R][D] in the residual's type (dtype without one), y [R][D], or NULL without w2
+ *   stats [R][2] fp32 for the backward, or NULL */
+int ttt_block_norm_fwd(const void* x, long long ldx, const void* gate, long long ldg, const void* residual,
+                       long long ldr, const float* w, const float* s, const float* w2, long long R, int D, int heads,
+                       float eps, int dtype, int res_dtype, void* r, void* y, float* stats, void* stream);
+
+/* Its gradients from dr and dy [R][D] (each may be NULL: zeros): dx, dgate (where there is
+ * a gate), dresidual (or NULL) [R][D], dw, ds, dw2 [D] (each may be NULL; `partial` of
+ * ttt_block_norm_partial_bytes for any of them, else NULL).  `residual` is read with w2 only. */
+size_t ttt_block_norm_partial_bytes(long long R, int D);
+int ttt_block_norm_bwd(const void* x, long long ldx, const void* gate, long long ldg, const void* residual,
+                       long long ldr, const float* w, const float* s, const float* w2, const float* stats,
+                       const void* dr, const void* dy, long long R, int D, int heads, int dtype, int res_dtype,
+                       void* dx, void* dgate, void* dresidual, float* dw, float* ds, float* dw2, float* partial,
+                       size_t partial_bytes, void* stream);
+
 /* Bytes of the static device scratch of ttt_mlp_bwd_noalloc (per GPU). */
 #define TTT_MLP_BWD_NOALLOC_SCRATCH_BYTES (64u << 20)
 

@@ -6,6 +6,7 @@
 #include <algorithm>
 
 #include "ttt_abi_check.h"
+#include "ttt_block_norm.h"
 #include "ttt_delta.h"
 
 namespace {
@@ -52,9 +53,123 @@ bool delta_plan_ok(int B, int L, int H, int P, int G, int N, int dtype, DeltaPla
   return delta_grid_ok(s, B, H, P);
 }
 
+// ---- norms around a block
+int check_block(long long R, int D, int heads, long long ldx, long long ldg, long long ldr, bool gate, bool res,
+                const float* w2, int dtype, int res_dtype) {
+  if (!dtype_ok(dtype) || (res_dtype != -1 && res_dtype != dtype && res_dtype != TTT_DTYPE_F32)) return TTT_ERR_DTYPE;
+  if (R <= 0 || R > kMaxGrid || D <= 0 || D > ttt::kBlockNormMaxD || heads <= 0 || R % heads != 0) return TTT_ERR_SHAPE;
+  const long long least = (long long)heads * D;
+  if (ldx < least || (gate && ldg < least) || (res && ldr < least)) return TTT_ERR_SHAPE;
+  // (a launch has whole wider rows: 2^31 threads are enough for one)
+  if ((long long)heads * ttt::block_lanes(D) > 0x7fffffffLL) return TTT_ERR_SHAPE;
+  if (w2 != nullptr && res_dtype == -1) return TTT_ERR_ARG;
+  return TTT_OK;
+}
+
 }  // namespace
 
 extern "C" {
+
+int ttt_block_norm_fwd(const void* x, long long ldx, const void* gate, long long ldg, const void* residual,
+                       long long ldr, const float* w, const float* s, const float* w2, long long R, int D, int heads,
+                       float eps, int dtype, int res_dtype, void* r, void* y, float* stats, void* stream) {
+  const int st = check_block(R, D, heads, ldx, ldg, ldr, gate != nullptr, residual != nullptr, w2, dtype, res_dtype);
+  if (st != TTT_OK) return st;
+  if (!(eps > 0.0f) || eps > 1.0f) return TTT_ERR_ARG;
+  const size_t n = size_of(dtype), nr = res_dtype == -1 ? n : size_of(res_dtype);
+  REQUIRE(x, n);
+  OPTIONAL(gate, n);
+  if (res_dtype != -1)
+    REQUIRE(residual, nr);
+  else if (residual != nullptr)
+    return TTT_ERR_ARG;
+  OPTIONAL(w, 4);
+  OPTIONAL(s, 4);
+  OPTIONAL(w2, 4);
+  REQUIRE(r, nr);
+  if (w2 != nullptr) REQUIRE(y, n);
+  OPTIONAL(stats, 4);
+  ttt::BlockNormParams p{};
+  p.x = x;
+  p.ldx = ldx;
+  p.gate = gate;
+  p.ldg = ldg;
+  p.res = residual;
+  p.ldr = ldr;
+  p.w = w;
+  p.s = s;
+  p.w2 = w2;
+  p.R = R;
+  p.D = D;
+  p.heads = heads;
+  p.eps = eps;
+  p.r = r;
+  p.y = y;
+  p.stats = stats;
+  return hip_status(ttt::launch_block_norm_fwd(p, dtype, res_dtype, static_cast<hipStream_t>(stream)));
+}
+
+size_t ttt_block_norm_partial_bytes(long long R, int D) {
+  if (R <= 0 || R > kMaxGrid || D <= 0 || D > ttt::kBlockNormMaxD) return 0;
+  return (size_t)ttt::block_norm_parts(R, D) * 3 * D * sizeof(float);
+}
+
+int ttt_block_norm_bwd(const void* x, long long ldx, const void* gate, long long ldg, const void* residual,
+                       long long ldr, const float* w, const float* s, const float* w2, const float* stats,
+                       const void* dr, const void* dy, long long R, int D, int heads, int dtype, int res_dtype,
+                       void* dx, void* dgate, void* dresidual, float* dw, float* ds, float* dw2, float* partial,
+                       size_t partial_bytes, void* stream) {
+  const bool reads = w2 != nullptr;
+  const int st = check_block(R, D, heads, ldx, ldg, ldr, gate != nullptr, reads, w2, dtype, res_dtype);
+  if (st != TTT_OK) return st;
+  const size_t n = size_of(dtype), nr = res_dtype == -1 ? n : size_of(res_dtype);
+  REQUIRE(x, n);
+  OPTIONAL(gate, n);
+  if (reads) REQUIRE(residual, nr);
+  OPTIONAL(w, 4);
+  OPTIONAL(s, 4);
+  OPTIONAL(w2, 4);
+  REQUIRE(stats, 4);
+  OPTIONAL(dr, nr);
+  OPTIONAL(dy, n);
+  REQUIRE(dx, n);
+  if (gate != nullptr) REQUIRE(dgate, n);
+  OPTIONAL(dresidual, nr);
+  OPTIONAL(dw, 4);
+  OPTIONAL(ds, 4);
+  OPTIONAL(dw2, 4);
+  if ((dw != nullptr && w == nullptr) || (ds != nullptr && s == nullptr) || (dw2 != nullptr && w2 == nullptr) ||
+      (dresidual != nullptr && res_dtype == -1))
+    return TTT_ERR_ARG;
+  if (dw != nullptr || ds != nullptr || dw2 != nullptr) {
+    if (partial == nullptr || partial_bytes < ttt_block_norm_partial_bytes(R, D)) return TTT_ERR_WORKSPACE;
+    if (!aligned(partial, 4)) return TTT_ERR_ALIGN;
+  }
+  ttt::BlockNormParams p{};
+  p.x = x;
+  p.ldx = ldx;
+  p.gate = gate;
+  p.ldg = ldg;
+  p.res = residual;
+  p.ldr = ldr;
+  p.w = w;
+  p.s = s;
+  p.w2 = w2;
+  p.stats = const_cast<float*>(stats);
+  p.dr = dr;
+  p.dy = dy;
+  p.R = R;
+  p.D = D;
+  p.heads = heads;
+  p.dx = dx;
+  p.dgate = dgate;
+  p.dres = dresidual;
+  p.dw = dw;
+  p.ds = ds;
+  p.dw2 = dw2;
+  if (dw != nullptr || ds != nullptr || dw2 != nullptr) p.partial = partial;
+  return hip_status(ttt::launch_block_norm_bwd(p, dtype, res_dtype, static_cast<hipStream_t>(stream)));
+}
 
 size_t ttt_delta_saved_bytes(int B, int L, int H, int P, int N, int dtype) {
   DeltaPlan s;

@@ -43,32 +43,39 @@ MAX_STATE = 128
 CONV_WIDTHS = (2, 3, 4)
 
 
-def _rows(t: torch.Tensor, lead: int, align: int, width: int):
-    """(t, row stride) with t's first `lead` axes as rows a fixed stride apart and
-    the rest, `width` values, contiguous inside a row, `align` bytes of alignment; a
-    contiguous copy where t is not laid out so."""
+def _row_stride(t: torch.Tensor, lead: int, width: int):
+    """The stride of t's first `lead` axes as rows a fixed stride apart with the rest,
+    `width` values, contiguous inside a row; None where t is not laid out so."""
     if t.is_contiguous():
-        if (t.data_ptr() | width * t.element_size()) % align == 0:
-            return t, width
-        return t.clone(), width  # (fresh memory starts on more than any of them)
+        return width
     shape, strides = t.shape, t.stride()
     inner, ld, step = 1, None, 0
     for i in range(t.dim() - 1, -1, -1):
         n, st = shape[i], strides[i]
         if i >= lead:
             if n != 1 and st != inner:
-                break
+                return None
             inner *= n
         elif n != 1:
             if ld is None:  # the innermost leading axis of more than one row gives the stride
                 ld = step = st
             elif st != step:
-                break
+                return None
             step *= n
-    else:
-        ld = width if ld is None else ld
-        if ld >= width and (t.data_ptr() | ld * t.element_size()) % align == 0:
-            return t, ld
+    ld = width if ld is None else ld
+    return ld if ld >= width else None
+
+
+def _rows(t: torch.Tensor, lead: int, align: int, width: int):
+    """(t, row stride) with t's first `lead` axes as rows (_row_stride), `align` bytes of
+    alignment; a contiguous copy where t is not laid out so."""
+    if t.is_contiguous():
+        if (t.data_ptr() | width * t.element_size()) % align == 0:
+            return t, width
+        return t.clone(), width  # (fresh memory starts on more than any of them)
+    ld = _row_stride(t, lead, width)
+    if ld is not None and (t.data_ptr() | ld * t.element_size()) % align == 0:
+        return t, ld
     return t.detach().contiguous(), width
 
 
