@@ -402,7 +402,7 @@ int ttt_post_norm_bwd(const void* XQW, const float* gamma, const float* stats, c
  * No counterpart in the reference, whose layer types are TTT-Linear and TTT-MLP;
  * these are a third one's. */
 
-enum ttt_activation { TTT_ACT_NONE = 0, TTT_ACT_SILU = 1 };
+enum ttt_activation { TTT_ACT_NONE = 0, TTT_ACT_SILU = 1, TTT_ACT_GELU = 2 };
 
 /* y[t][c] = act(bias[c] + sum_k weight[c][k] s[t+k][c]) with s the W-1 inputs
  * before the first token followed by x; W in {2, 3, 4}.
@@ -547,6 +547,24 @@ int ttt_block_norm_bwd(const void* x, long long ldx, const void* gate, long long
                        const void* dr, const void* dy, long long R, int D, int heads, int dtype, int res_dtype,
                        void* dx, void* dgate, void* dresidual, float* dw, float* ds, float* dw2, float* partial,
                        size_t partial_bytes, void* stream);
+
+/* y = act(x Wg^T + bg) * (x Wu^T + bu), act TTT_ACT_SILU or TTT_ACT_GELU (a times the normal
+ * distribution's integral up to a), every tensor in `dtype`.
+ *   x [R][ldx], wg, wu [F][D], bg, bu [F] (each may be NULL), y [R][F]
+ *   workspace  ttt_ffn_workspace_bytes (NULL where that is 0)
+ * D and F up to 2^20.  In 16 bits with D a multiple of 8 and R above 64, x, its rows, wg and wu
+ * start on 16 bytes and x's rows are up to 4 MiB apart; elsewhere any alignment will do. */
+size_t ttt_ffn_workspace_bytes(int R, int D, int F, int dtype);
+int ttt_ffn_fwd(const void* x, long long ldx, const void* wg, const void* wu, const void* bg, const void* bu, int R,
+                int D, int F, int activation, int dtype, void* y, void* workspace, size_t workspace_bytes,
+                void* stream);
+
+/* Its gradients from dy [R][lddy], any alignment: dx [R][D] (or NULL), dwg and dwu [F][D] (both
+ * or neither), dbg and dbu [F] (each may be NULL).  Alignment as above, whatever R is. */
+size_t ttt_ffn_bwd_workspace_bytes(int R, int D, int F, int dtype);
+int ttt_ffn_bwd(const void* x, long long ldx, const void* wg, const void* wu, const void* bg, const void* bu,
+                const void* dy, long long lddy, int R, int D, int F, int activation, int dtype, void* dx, void* dwg,
+                void* dwu, void* dbg, void* dbu, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Bytes of the static device scratch of ttt_mlp_bwd_noalloc (per GPU). */
 #define TTT_MLP_BWD_NOALLOC_SCRATCH_BYTES (64u << 20)

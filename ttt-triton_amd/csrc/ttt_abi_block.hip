@@ -8,6 +8,7 @@
 #include "ttt_abi_check.h"
 #include "ttt_block_norm.h"
 #include "ttt_delta.h"
+#include "ttt_ffn.h"
 
 namespace {
 
@@ -66,9 +67,174 @@ int check_block(long long R, int D, int heads, long long ldx, long long ldg, lon
   return TTT_OK;
 }
 
+// ---- gated feed-forward projections
+constexpr int kFfnMaxWidth = 1 << 20;  // rows of a tile are reached by 31-bit offsets
+int check_ffn(int R, int D, int F, int act, int dtype) {
+  if (!dtype_ok(dtype)) return TTT_ERR_DTYPE;
+  if (R <= 0 || D <= 0 || F <= 0 || D > kFfnMaxWidth || F > kFfnMaxWidth || R > 0x7fffff00) return TTT_ERR_SHAPE;
+  if (act != TTT_ACT_SILU && act != TTT_ACT_GELU) return TTT_ERR_ARG;
+  // (tiles of 128 x 128 with 256 threads; planes 8 values a thread)
+  const long long n = std::max(2LL * F, (long long)D), m = std::max<long long>(R, 2LL * F + 16);
+  if (((m + 127) / 128) * ((n + 127) / 128) > kMaxThreads / 256) return TTT_ERR_SHAPE;
+  if (std::max<long long>(R, F) * (ttt::ffn_pad(D) / 8) > kMaxThreads) return TTT_ERR_SHAPE;
+  return TTT_OK;
+}
+struct FfnPlan {
+  bool in_place;
+  size_t x, w, grad, part, bias;
+};
+FfnPlan ffn_plan(int R, int D, int F, int dtype) {
+  FfnPlan s;
+  const size_t Dp = ttt::ffn_pad(D), Fp = ttt::ffn_pad(F), planes = ttt::ffn_planes(dtype);
+  s.in_place = planes == 1 && D % 8 == 0;
+  s.x = s.in_place ? 0 : up256(planes * R * Dp * 2);
+  s.w = s.in_place ? 0 : up256(planes * F * Dp * 2);
+  s.grad = up256(planes * R * 2 * Fp * 2);
+  const int splits = ttt::ffn_splits(R, D, F, dtype);
+  s.part = splits > 1 ? up256((size_t)splits * 2 * Fp * Dp * 4) : 0;
+  s.bias = up256((size_t)ttt::ffn_bias_parts(R, F) * 2 * Fp * 4);
+  return s;
+}
+// x, wg and wu as the products read them: in place, or as planes in the workspace
+hipError_t ffn_operands(ttt::FfnParams& p, const FfnPlan& s, const void* x, long long ldx, const void* wg, const void* wu,
+                        int dtype, char*& ws, hipStream_t stream) {
+  const long long es = size_of(dtype);
+  if (s.in_place) {
+    p.x = {x, ldx * es, 0};
+    p.wg = {wg, p.D * es, 0};
+    p.wu = {wu, p.D * es, 0};
+    return hipSuccess;
+  }
+  const auto make = [&](ttt::FfnMatrix& m, const void* from, long long ld, int rows, size_t bytes) {
+    m = {ws, p.Dp * 2LL, (long long)rows * p.Dp * 2};
+    ws += bytes;
+    return ttt::launch_ffn_planes(from, ld, rows, p.D, const_cast<void*>(m.p), dtype, stream);
+  };
+  hipError_t e = make(p.x, x, ldx, p.R, s.x);
+  if (e == hipSuccess) e = make(p.wg, wg, p.D, p.F, s.w);
+  if (e == hipSuccess) e = make(p.wu, wu, p.D, p.F, s.w);
+  return e;
+}
+int check_ffn_rows(bool in_place, const void* x, long long ldx, const void* wg, const void* wu, int D, int dtype) {
+  if (ldx < D) return TTT_ERR_SHAPE;
+  const size_t n = in_place ? 16 : size_of(dtype);
+  if (in_place && (ldx % 8 != 0 || ldx > (4 << 20) / 2)) return TTT_ERR_SHAPE;
+  REQUIRE(x, n);
+  REQUIRE(wg, n);
+  REQUIRE(wu, n);
+  return TTT_OK;
+}
+
 }  // namespace
 
 extern "C" {
+
+size_t ttt_ffn_workspace_bytes(int R, int D, int F, int dtype) {
+  if (check_ffn(R, D, F, TTT_ACT_SILU, dtype) != TTT_OK || R <= ttt::kFfnFew) return 0;
+  const FfnPlan s = ffn_plan(R, D, F, dtype);
+  return s.x + 2 * s.w;
+}
+size_t ttt_ffn_bwd_workspace_bytes(int R, int D, int F, int dtype) {
+  if (check_ffn(R, D, F, TTT_ACT_SILU, dtype) != TTT_OK) return 0;
+  const FfnPlan s = ffn_plan(R, D, F, dtype);
+  return s.x + 2 * s.w + s.grad + s.part + s.bias;
+}
+
+int ttt_ffn_fwd(const void* x, long long ldx, const void* wg, const void* wu, const void* bg, const void* bu, int R,
+                int D, int F, int activation, int dtype, void* y, void* workspace, size_t workspace_bytes,
+                void* stream) {
+  int st = check_ffn(R, D, F, activation, dtype);
+  if (st != TTT_OK) return st;
+  const bool few = R <= ttt::kFfnFew;
+  const FfnPlan s = ffn_plan(R, D, F, dtype);
+  if ((st = check_ffn_rows(!few && s.in_place, x, ldx, wg, wu, D, dtype)) != TTT_OK) return st;
+  const size_t n = size_of(dtype);
+  OPTIONAL(bg, n);
+  OPTIONAL(bu, n);
+  REQUIRE(y, n);
+  ttt::FfnParams p{};
+  p.bg = bg;
+  p.bu = bu;
+  p.y = y;
+  p.R = R;
+  p.D = D;
+  p.F = F;
+  p.Dp = ttt::ffn_pad(D);
+  p.Fp = ttt::ffn_pad(F);
+  p.planes = ttt::ffn_planes(dtype);
+  p.act = activation;
+  const hipStream_t on = static_cast<hipStream_t>(stream);
+  if (few) {
+    const long long es = size_of(dtype);
+    p.x = {x, ldx * es, 0};
+    p.wg = {wg, D * es, 0};
+    p.wu = {wu, D * es, 0};
+    return hip_status(ttt::launch_ffn_few(p, dtype, on));
+  }
+  const size_t need = s.x + 2 * s.w;
+  if (need > 0) {
+    if (workspace == nullptr || workspace_bytes < need) return TTT_ERR_WORKSPACE;
+    if (!aligned(workspace, 16)) return TTT_ERR_ALIGN;
+  }
+  char* ws = static_cast<char*>(workspace);
+  const hipError_t e = ffn_operands(p, s, x, ldx, wg, wu, dtype, ws, on);
+  if (e != hipSuccess) return hip_status(e);
+  return hip_status(ttt::launch_ffn_fwd(p, dtype, on));
+}
+
+int ttt_ffn_bwd(const void* x, long long ldx, const void* wg, const void* wu, const void* bg, const void* bu,
+                const void* dy, long long lddy, int R, int D, int F, int activation, int dtype, void* dx, void* dwg,
+                void* dwu, void* dbg, void* dbu, void* workspace, size_t workspace_bytes, void* stream) {
+  int st = check_ffn(R, D, F, activation, dtype);
+  if (st != TTT_OK) return st;
+  const FfnPlan s = ffn_plan(R, D, F, dtype);
+  if ((st = check_ffn_rows(s.in_place, x, ldx, wg, wu, D, dtype)) != TTT_OK) return st;
+  if (lddy < F) return TTT_ERR_SHAPE;
+  const size_t n = size_of(dtype);
+  OPTIONAL(bg, n);
+  OPTIONAL(bu, n);
+  REQUIRE(dy, n);
+  OPTIONAL(dx, n);
+  OPTIONAL(dwg, n);
+  OPTIONAL(dwu, n);
+  OPTIONAL(dbg, n);
+  OPTIONAL(dbu, n);
+  if ((dwg == nullptr) != (dwu == nullptr)) return TTT_ERR_ARG;
+  if (workspace == nullptr || workspace_bytes < s.x + 2 * s.w + s.grad + s.part + s.bias) return TTT_ERR_WORKSPACE;
+  if (!aligned(workspace, 16)) return TTT_ERR_ALIGN;
+  ttt::FfnParams p{};
+  p.bg = bg;
+  p.bu = bu;
+  p.dy = dy;
+  p.lddy = lddy;
+  p.R = R;
+  p.D = D;
+  p.F = F;
+  p.Dp = ttt::ffn_pad(D);
+  p.Fp = ttt::ffn_pad(F);
+  p.planes = ttt::ffn_planes(dtype);
+  p.act = activation;
+  p.dx = dx;
+  p.dwg = dwg;
+  p.dwu = dwu;
+  p.dbg = dbg;
+  p.dbu = dbu;
+  p.splits = ttt::ffn_splits(R, D, F, dtype);
+  p.bias_parts = ttt::ffn_bias_parts(R, F);
+  const hipStream_t on = static_cast<hipStream_t>(stream);
+  char* ws = static_cast<char*>(workspace);
+  hipError_t e = ffn_operands(p, s, x, ldx, wg, wu, dtype, ws, on);
+  if (e != hipSuccess) return hip_status(e);
+  p.grad = {ws, 4LL * p.Fp, (long long)R * 4 * p.Fp};
+  ws += s.grad;
+  if (s.part > 0) p.part = reinterpret_cast<float*>(ws);
+  ws += s.part;
+  if (dbg != nullptr || dbu != nullptr) p.bias_part = reinterpret_cast<float*>(ws);
+  e = ttt::launch_ffn_grad(p, dtype, on);
+  if (e == hipSuccess && dx != nullptr) e = ttt::launch_ffn_dx(p, dtype, on);
+  if (e == hipSuccess && dwg != nullptr) e = ttt::launch_ffn_dw(p, dtype, on);
+  return hip_status(e);
+}
 
 int ttt_block_norm_fwd(const void* x, long long ldx, const void* gate, long long ldg, const void* residual,
                        long long ldr, const float* w, const float* s, const float* w2, long long R, int D, int heads,

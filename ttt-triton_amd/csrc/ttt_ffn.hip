@@ -1,0 +1,486 @@
+// The gated feed-forward projections on gfx950: y = act(x Wg^T + bg) * (x Wu^T + bu), forward
+// and backward.
+//
+//   a = x Wg^T + bg,  b = x Wu^T + bu,  y = f(a) b
+//   da = dy b f'(a),  db = dy f(a)                        (a and b formed again, not kept)
+//   dx = da Wg + db Wu,   dWg = da^T x,   dWu = db^T x,   dbg = sum da,   dbu = sum db
+//
+// All four products are one kernel: tiles of 256 x 256 (eight waves) or 128 x 128 (four) from
+// steps of 64 contracted values, which go from memory straight to LDS, two steps' places in
+// turn.  An operand whose contracted values are neighbours in memory is read 16 bytes a lane;
+// one whose free values are (the weights for dx, both operands of dW) by the transposing
+// read, so that nothing is transposed in memory.  The 16-byte pieces of a row lie in LDS
+// permuted by the row's number, for reads without bank conflicts; pieces outside a matrix read 0.
+// The gate's and the other projection's columns of a tile meet in one wave, which forms y, or
+// da and db, from its accumulators.
+//
+// fp32 operands are three bf16 planes, exact in each, and a product is the six of the planes
+// a, b with a + b < 3, one after the other, smallest first: 2^-24 of the value, at a sixth of
+// the rate of bf16 (the fp32 matrix instructions have a sixteenth).  da and db of 16-bit calls
+// are rounded to the activations' type where dx and dW read them, as a layer that formed them
+// one after the other would hand them on: their rounding adds to that at the store, each
+// half a step (1.4 times the store's alone); two planes would double the two products.
+//
+// Few rows (up to 64, a token of each sequence): the weights are read once, by as many
+// workgroups as have 16 columns, the contraction shared out over eight waves; nothing goes
+// through LDS but the waves' sums.
+#include <math.h>
+
+#include <algorithm>
+
+#include "ttt_ffn.h"
+#include "ttt_scan.h"
+
+namespace ttt {
+
+namespace {
+
+typedef __attribute__((address_space(3))) void lds_void;
+
+template <typename T> struct Elem { typedef T type; };
+template <> struct Elem<float> { typedef __bf16 type; };
+
+template <typename E> __device__ __forceinline__ f4 product(bf8 p, bf8 q, f4 acc) {
+  if constexpr (sizeof(E) == 2 && __is_same(E, _Float16))
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, p), __builtin_bit_cast(h8, q), acc, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(p, q, acc, 0, 0, 0);
+}
+
+// f(a) and f'(a)
+template <bool GRAD> __device__ __forceinline__ float act_value(int act, float a, float& d) {
+  if (act == TTT_ACT_SILU) {
+    const float s = sigmoid_f(a);
+    if (GRAD) d = s * __builtin_fmaf(a, 1.0f - s, 1.0f);
+    return a * s;
+  }
+  const float c = 0.5f * erfcf(-0.7071067811865476f * a);  // the normal distribution's integral
+  if (GRAD) d = __builtin_fmaf(a * 0.3989422804014327f, expf(-0.5f * a * a), c);
+  return a * c;
+}
+
+enum class Job { Fwd, Grad, Dx, Dw };
+// how an operand lies: its contracted values side by side, or its free ones
+enum class Lies { Contracted, Free };
+
+// A step's part of an operand in LDS: FREE rows of 64 contracted values, or 64 rows of FREE
+template <Lies L, int FREE> struct Panel {
+  static constexpr int PIECES = L == Lies::Contracted ? 8 : FREE / 8;  // of 16 bytes, to a row
+  static constexpr int ROWS = L == Lies::Contracted ? FREE : kFfnStep;
+  static constexpr int BYTES = FREE * kFfnStep * 2;
+  __device__ __forceinline__ static int place(int row, int piece) {
+    return L == Lies::Contracted ? piece ^ (row & 7) : piece ^ ((row & 7) << 1);
+  }
+};
+
+// Sends the step's rows of a matrix on their way to LDS.  `base`: the panel's first value;
+// `rows` and `pieces` of it are in the matrix (whole rows `ld` bytes apart).
+template <Lies L, int FREE, int NW>
+__device__ __forceinline__ void send(const char* base, long long ld, int rows, int pieces, unsigned char* lds, int w) {
+  using P = Panel<L, FREE>;
+  constexpr int CNT = P::BYTES / 1024 / NW;
+  static_assert(CNT * NW * 1024 == P::BYTES, "whole kilobytes to a wave");
+  const int l = lane_id();
+  rows = rows < P::ROWS ? rows : P::ROWS;
+  const unsigned bytes = rows > 0 && pieces > 0 ? (unsigned)(rows - 1) * (unsigned)ld + (unsigned)min(pieces, P::PIECES) * 16u : 0u;
+  const auto rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), (short)0, (int)bytes, 0x00020000);
+#pragma unroll
+  for (int i = 0; i < CNT; ++i) {
+    const int at = (i * NW + w) * 64 + l, row = at / P::PIECES, piece = P::place(row, at % P::PIECES);
+    unsigned off = (unsigned)row * (unsigned)ld + (unsigned)piece * 16u;
+    if (piece >= pieces) off = 0x80000000u;  // (past every panel: they stay below 2^31 bytes)
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(lds + (i * NW + w) * 1024), 16, (int)off, 0, 0, 0);
+  }
+}
+// A panel's operands of the free values 16 t.. and contracted values 32 k.. + 8g + (0..7)
+template <Lies L, int FREE> __device__ __forceinline__ bf8 take(const unsigned char* lds, int t, int k) {
+  const int l = lane_id(), g = l >> 4, r = l & 15;
+  if constexpr (L == Lies::Contracted) {
+    const int row = 16 * t + r;
+    return *reinterpret_cast<const bf8*>(lds + row * 128 + (((4 * k + g) ^ (r & 7)) << 4));
+  } else {
+    const int row = 32 * k + 8 * g + (r >> 2), piece = 2 * t + ((l & 3) >> 1);
+    const auto at = [&](int rw) {
+      return reinterpret_cast<const __bf16*>(lds + rw * FREE * 2 + ((piece ^ ((rw & 7) << 1)) << 4) + (l & 1) * 8);
+    };
+    return cat(read_tr(at(row)), read_tr(at(row + 4)));
+  }
+}
+
+// 4 values of T behind each other from p, of n there are
+template <typename T> __device__ __forceinline__ f4 load_up_to4(const T* p, int n) {
+  Raw<T, 4> v;
+  v.load(p, n);
+  return f4{v.f(0), v.f(1), v.f(2), v.f(3)};
+}
+template <typename T> __device__ __forceinline__ void store_up_to4(T* p, int n, f4 v) {
+  const float o[4] = {v[0], v[1], v[2], v[3]};
+  store_row<T, 4>(p, n, o);
+}
+// da or db, in planes where T is fp32
+template <typename T> __device__ __forceinline__ void store_grad(const FfnMatrix& m, long long row, int col, f4 v) {
+  char* to = static_cast<char*>(const_cast<void*>(m.p)) + row * m.ld + col * 2;
+  if constexpr (sizeof(T) == 4) {
+    bf4 o[3];
+    split4<3>(v, o);
+#pragma unroll
+    for (int a = 0; a < 3; ++a) *reinterpret_cast<bf4*>(to + a * m.plane) = o[a];
+  } else {
+    store4(reinterpret_cast<T*>(to), v);
+  }
+}
+
+// Tiles of WN TN 16 columns (the first operand's free values, four to a lane's registers) by
+// WM TM 16 rows (the second's, a lane each)
+template <typename T, Job JOB, int WN, int WM, int TN, int TM>
+__global__ __launch_bounds__(64 * WN * WM) void ffn_kernel(FfnParams p) {
+  typedef typename Elem<T>::type E;
+  constexpr bool UP = JOB == Job::Fwd || JOB == Job::Grad;  // both projections' columns in a tile
+  constexpr Lies LN = UP ? Lies::Contracted : Lies::Free, LM = JOB == Job::Dw ? Lies::Free : Lies::Contracted;
+  constexpr int BN = 16 * WN * TN, BM = 16 * WM * TM, NW = WN * WM, HALF = BN / 2;
+  constexpr int STEP = Panel<LN, BN>::BYTES + Panel<LM, BM>::BYTES;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  const int w = wave_id(), l = lane_id(), g = l >> 4, r = l & 15, wn = w % WN, wm = w / WN;
+  // rows and columns of all tiles, and contracted values
+  const int M = JOB == Job::Dw ? 2 * p.Fp : p.R, N = UP ? p.F : p.D, K = JOB == Job::Dw ? p.R : JOB == Job::Dx ? p.Fp : p.Dp;
+  const int tm = (M + BM - 1) / BM, tn = (N + (UP ? HALF : BN) - 1) / (UP ? HALF : BN);
+  const int splits = JOB == Job::Dw ? p.splits : 1;
+  // Neighbours on a die have eight rows of tiles by all columns, one column after the other
+  unsigned id = on_xcd(blockIdx.x, gridDim.x);
+  const int split = (int)(id / (unsigned)(tm * tn));
+  id -= split * (tm * tn);
+  const int band = (int)(id / (8u * tn)), high = min(8, tm - 8 * band);
+  id -= band * 8 * tn;
+  const int m0 = (8 * band + (int)(id % high)) * BM, n0 = (int)(id / high) * (UP ? HALF : BN);
+
+  const int ksteps = (K + kFfnStep - 1) / kFfnStep, per = (ksteps + splits - 1) / splits;
+  const int k0 = split * per, kn = min(ksteps, k0 + per) - k0;
+  const int pairs = p.planes == 3 ? 6 : 1;
+  const int segs = JOB == Job::Dx ? 2 : 1;
+  const int steps = kn > 0 ? kn * pairs * segs : 0;
+
+  // the step that is sent next
+  int sk = 0, sp = 0, ss = 0;
+  const auto next = [&](int buf) {
+    // planes a of the first operand and b of the second: (2,0) (1,1) (0,2) (1,0) (0,1) (0,0)
+    const int pa = pairs == 1 ? 0 : (0x001012 >> (4 * sp)) & 15, pb = pairs == 1 ? 0 : (0x010210 >> (4 * sp)) & 15;
+    const int k = (k0 + sk) * kFfnStep, left = K - k;
+    unsigned char* to = smem + buf * STEP;
+    if constexpr (UP) {
+      const int pieces = left / 8;
+      const long long a = pa * p.wg.plane + (long long)n0 * p.wg.ld + k * 2;
+      send<LN, HALF, NW>(static_cast<const char*>(p.wg.p) + a, p.wg.ld, N - n0, pieces, to, w);
+      send<LN, HALF, NW>(static_cast<const char*>(p.wu.p) + a, p.wu.ld, N - n0, pieces, to + HALF * kFfnStep * 2, w);
+      send<LM, BM, NW>(static_cast<const char*>(p.x.p) + pb * p.x.plane + (long long)m0 * p.x.ld + k * 2, p.x.ld, M - m0,
+                       pieces, to + Panel<LN, BN>::BYTES, w);
+    } else if constexpr (JOB == Job::Dx) {
+      const FfnMatrix& wt = ss == 0 ? p.wg : p.wu;
+      send<LN, BN, NW>(static_cast<const char*>(wt.p) + pa * wt.plane + (long long)k * wt.ld + n0 * 2, wt.ld, p.F - k,
+                       (p.Dp - n0) / 8, to, w);
+      send<LM, BM, NW>(static_cast<const char*>(p.grad.p) + pb * p.grad.plane + (long long)m0 * p.grad.ld +
+                           ((long long)ss * p.Fp + k) * 2,
+                       p.grad.ld, M - m0, left / 8, to + Panel<LN, BN>::BYTES, w);
+    } else {
+      send<LN, BN, NW>(static_cast<const char*>(p.x.p) + pa * p.x.plane + (long long)k * p.x.ld + n0 * 2, p.x.ld, left,
+                       (p.Dp - n0) / 8, to, w);
+      send<LM, BM, NW>(static_cast<const char*>(p.grad.p) + pb * p.grad.plane + (long long)k * p.grad.ld + m0 * 2, p.grad.ld,
+                       left, (M - m0) / 8, to + Panel<LN, BN>::BYTES, w);
+    }
+    if (++sk == kn) {
+      sk = 0;
+      if (++ss == segs) {
+        ss = 0;
+        ++sp;
+      }
+    }
+  };
+
+  f4 acc[TN][TM];
+#pragma unroll
+  for (int i = 0; i < TN; ++i)
+#pragma unroll
+    for (int j = 0; j < TM; ++j) acc[i][j] = f4{0.f, 0.f, 0.f, 0.f};
+  // a wave's tiles of columns: of both halves where a tile has both projections
+  const auto tile_n = [&](int i) { return UP ? (i < TN / 2 ? wn * (TN / 2) + i : HALF / 16 + wn * (TN / 2) + i - TN / 2) : wn * TN + i; };
+  if (steps > 0) next(0);
+#pragma unroll 1
+  for (int s = 0; s < steps; ++s) {
+    // the step is here, in all waves, and the one before it has been read
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // (vmcnt(0))
+    __syncthreads();
+    if (s + 1 < steps) next((s + 1) & 1);
+    const unsigned char* at = smem + (s & 1) * STEP;
+#pragma unroll
+    for (int k = 0; k < kFfnStep / 32; ++k) {
+      bf8 pn[TN], pm[TM];
+#pragma unroll
+      for (int i = 0; i < TN; ++i) pn[i] = take<LN, BN>(at, tile_n(i), k);
+#pragma unroll
+      for (int j = 0; j < TM; ++j) pm[j] = take<LM, BM>(at + Panel<LN, BN>::BYTES, wm * TM + j, k);
+#pragma unroll
+      for (int j = 0; j < TM; ++j)
+#pragma unroll
+        for (int i = 0; i < TN; ++i) acc[i][j] = product<E>(pn[i], pm[j], acc[i][j]);
+    }
+  }
+
+  if constexpr (UP) {
+#pragma unroll
+    for (int i = 0; i < TN / 2; ++i) {
+      const int f = n0 + 16 * (wn * (TN / 2) + i) + 4 * g, left = N - f;
+      f4 bg = f4{0.f, 0.f, 0.f, 0.f}, bu = bg, sg = bg, su = bg;
+      if (p.bg != nullptr && left > 0) bg = load_up_to4(static_cast<const T*>(p.bg) + f, left);
+      if (p.bu != nullptr && left > 0) bu = load_up_to4(static_cast<const T*>(p.bu) + f, left);
+#pragma unroll
+      for (int j = 0; j < TM; ++j) {
+        const int m = m0 + 16 * (wm * TM + j) + r;
+        const f4 a = acc[i][j] + bg, b = acc[TN / 2 + i][j] + bu;
+        if constexpr (JOB == Job::Fwd) {
+          f4 y;
+          float d;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[e] = act_value<false>(p.act, a[e], d) * b[e];
+          if (m < M && left > 0) store_up_to4(static_cast<T*>(p.y) + (long long)m * p.F + f, left, y);
+        } else {
+          if (m < M && f < p.Fp) {
+            f4 dy = f4{0.f, 0.f, 0.f, 0.f}, da, db;
+            if (left > 0) dy = load_up_to4(static_cast<const T*>(p.dy) + (long long)m * p.lddy + f, left);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float d;
+              db[e] = dy[e] * act_value<true>(p.act, a[e], d);
+              da[e] = dy[e] * b[e] * d;
+              if (e >= left) da[e] = db[e] = 0.f;
+            }
+            store_grad<T>(p.grad, m, f, da);
+            store_grad<T>(p.grad, m, p.Fp + f, db);
+            sg += da;
+            su += db;
+          }
+        }
+      }
+      if (JOB == Job::Grad && p.bias_part != nullptr) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          sg[e] = sum_row16(sg[e]);
+          su[e] = sum_row16(su[e]);
+        }
+        if (r == 0 && f < p.Fp) {
+          float* to = p.bias_part + (long long)(m0 / BM * WM + wm) * 2 * p.Fp + f;
+          *reinterpret_cast<f4*>(to) = sg;
+          *reinterpret_cast<f4*>(to + p.Fp) = su;
+        }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < TN; ++i) {
+      const int n = n0 + 16 * (wn * TN + i) + 4 * g, left = N - n;
+      if (left <= 0) continue;
+#pragma unroll
+      for (int j = 0; j < TM; ++j) {
+        const int m = m0 + 16 * (wm * TM + j) + r;
+        if (m >= M) continue;
+        if constexpr (JOB == Job::Dx) {
+          store_up_to4(static_cast<T*>(p.dx) + (long long)m * p.D + n, left, acc[i][j]);
+        } else if (p.part != nullptr) {
+          *reinterpret_cast<f4*>(p.part + ((long long)split * M + m) * p.Dp + n) = acc[i][j];
+        } else {
+          const int f = m < p.Fp ? m : m - p.Fp;
+          if (f < p.F) store_up_to4(static_cast<T*>(m < p.Fp ? p.dwg : p.dwu) + (long long)f * p.D + n, left, acc[i][j]);
+        }
+      }
+    }
+  }
+}
+
+// dWg and dWu from the sums over shares of the rows
+template <typename T> __global__ __launch_bounds__(256) void ffn_join_kernel(FfnParams p, long long quads) {
+  const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (id >= quads) return;
+  const int per = p.Dp / 4, m = (int)(id / per), n = 4 * (int)(id - (long long)m * per);
+  const int f = m < p.Fp ? m : m - p.Fp;
+  if (f >= p.F) return;
+  const float* s = p.part + 4 * id;
+  f4 v = *reinterpret_cast<const f4*>(s);
+  for (int k = 1; k < p.splits; ++k) v += *reinterpret_cast<const f4*>(s + 4 * k * quads);
+  store_up_to4(static_cast<T*>(m < p.Fp ? p.dwg : p.dwu) + (long long)f * p.D + n, p.D - n, v);
+}
+template <typename T> __global__ __launch_bounds__(256) void ffn_bias_kernel(FfnParams p) {
+  const int n = 2 * p.Fp, c = blockIdx.x * 16 + (threadIdx.x & 15);
+  const float s = sum_parts(p.bias_part, n, c, p.bias_parts);
+  if (threadIdx.x >= 16 || c >= n) return;
+  const int f = c < p.Fp ? c : c - p.Fp;
+  T* to = static_cast<T*>(c < p.Fp ? p.dbg : p.dbu);
+  if (f < p.F && to != nullptr) to[f] = (T)s;
+}
+
+// 8 values to a thread
+template <typename T> __global__ __launch_bounds__(256) void ffn_planes_kernel(const T* from, long long ld, int width, int pieces,
+                                                                              long long all, char* to, long long plane) {
+  const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (id >= all) return;
+  const long long row = id / pieces;
+  const int c = 8 * (int)(id - row * pieces);
+  Raw<T, 8> v;
+  v.load(from + row * ld + c, width - c);
+  if constexpr (sizeof(T) == 4) {
+    const Op<3> o = split8<3>(f4{v.f(0), v.f(1), v.f(2), v.f(3)}, f4{v.f(4), v.f(5), v.f(6), v.f(7)});
+#pragma unroll
+    for (int a = 0; a < 3; ++a) *reinterpret_cast<bf8*>(to + a * plane + id * 16) = o.v[a];
+  } else {
+    Raw<T, 8> o = v;
+    *reinterpret_cast<u4v*>(to + id * 16) = __builtin_bit_cast(u4v, o.v);
+  }
+}
+
+// Few rows: a workgroup has 16 columns of both projections and up to 64 rows, a wave every
+// eighth 32 contracted values
+constexpr int kFewWaves = 8;
+template <typename T> struct FewOp { typedef Op<3> type; };
+template <> struct FewOp<__bf16> { typedef bf8 type; };
+template <> struct FewOp<_Float16> { typedef bf8 type; };
+template <typename T> __device__ __forceinline__ typename FewOp<T>::type few_op(const T* p, int n) {
+  Raw<T, 8> v;
+  v.load(p, n);
+  if constexpr (sizeof(T) == 4)
+    return split8<3>(f4{v.f(0), v.f(1), v.f(2), v.f(3)}, f4{v.f(4), v.f(5), v.f(6), v.f(7)});
+  else
+    return __builtin_bit_cast(bf8, v.v);
+}
+__device__ __forceinline__ void few_mma(f4& acc, const Op<3>& a, const Op<3>& b, float) { mma<3>(acc, a, b); }
+__device__ __forceinline__ void few_mma(f4& acc, bf8 a, bf8 b, __bf16) { acc = product<__bf16>(a, b, acc); }
+__device__ __forceinline__ void few_mma(f4& acc, bf8 a, bf8 b, _Float16) { acc = product<_Float16>(a, b, acc); }
+
+template <typename T, int TM> __global__ __launch_bounds__(64 * kFewWaves) void ffn_few_kernel(FfnParams p) {
+  const int w = wave_id(), l = lane_id(), g = l >> 4, r = l & 15;
+  const int f0 = 16 * blockIdx.x, m0 = 16 * TM * blockIdx.y, fr = min(f0 + r, p.F - 1);
+  const long long ldw = p.wg.ld / (long long)sizeof(T), ldx = p.x.ld / (long long)sizeof(T);
+  const T *wg = static_cast<const T*>(p.wg.p) + fr * ldw, *wu = static_cast<const T*>(p.wu.p) + fr * ldw;
+  const T* x = static_cast<const T*>(p.x.p);
+  f4 acc[2][TM];
+#pragma unroll
+  for (int j = 0; j < TM; ++j) acc[0][j] = acc[1][j] = f4{0.f, 0.f, 0.f, 0.f};
+  for (int k = 32 * w; k < p.D; k += 32 * kFewWaves) {
+    const int c = k + 8 * g, n = p.D - c, cc = n > 0 ? c : 0;
+    // (a lane without values reads none: Raw's loads take n <= 0 as zeros)
+    const auto a = few_op<T>(wg + cc, n), b = few_op<T>(wu + cc, n);
+#pragma unroll
+    for (int j = 0; j < TM; ++j) {
+      const int m = min(m0 + 16 * j + r, p.R - 1);
+      const auto q = few_op<T>(x + m * ldx + cc, n);
+      few_mma(acc[0][j], a, q, T());
+      few_mma(acc[1][j], b, q, T());
+    }
+  }
+  __shared__ f4 red[kFewWaves][2][TM][64];
+#pragma unroll
+  for (int j = 0; j < TM; ++j) {
+    red[w][0][j][l] = acc[0][j];
+    red[w][1][j][l] = acc[1][j];
+  }
+  __syncthreads();
+  if (w >= TM) return;
+  f4 a = red[0][0][w][l], b = red[0][1][w][l];
+#pragma unroll
+  for (int k = 1; k < kFewWaves; ++k) {
+    a += red[k][0][w][l];
+    b += red[k][1][w][l];
+  }
+  const int f = f0 + 4 * g, left = p.F - f, m = m0 + 16 * w + r;
+  if (left <= 0 || m >= p.R) return;
+  if (p.bg != nullptr) a += load_up_to4(static_cast<const T*>(p.bg) + f, left);
+  if (p.bu != nullptr) b += load_up_to4(static_cast<const T*>(p.bu) + f, left);
+  f4 y;
+  float d;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) y[e] = act_value<false>(p.act, a[e], d) * b[e];
+  store_up_to4(static_cast<T*>(p.y) + (long long)m * p.F + f, left, y);
+}
+
+template <typename K> hipError_t allow_lds(K k, size_t bytes) {
+  return bytes <= 65536 ? hipSuccess
+                        : hipFuncSetAttribute(reinterpret_cast<const void*>(k),
+                                              hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+}
+template <typename T, Job JOB, int WN, int WM, int TN, int TM> hipError_t tile_t(const FfnParams& p, hipStream_t s) {
+  constexpr int BN = 16 * WN * TN, BM = 16 * WM * TM, lds = 2 * (BN + BM) * kFfnStep * 2;
+  const auto kernel = ffn_kernel<T, JOB, WN, WM, TN, TM>;
+  const hipError_t e = allow_lds(kernel, lds);
+  if (e != hipSuccess) return e;
+  constexpr bool up = JOB == Job::Fwd || JOB == Job::Grad;
+  const long long M = JOB == Job::Dw ? 2LL * p.Fp : p.R, N = up ? 2LL * p.F : p.D;
+  const long long blocks = ((M + BM - 1) / BM) * ((N + BN - 1) / BN) * (JOB == Job::Dw ? p.splits : 1);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(64 * WN * WM), lds, s, p);
+  return hipGetLastError();
+}
+template <typename T, Job JOB> hipError_t job_t(const FfnParams& p, hipStream_t s) {
+  constexpr bool up = JOB == Job::Fwd || JOB == Job::Grad;
+  const long long M = JOB == Job::Dw ? 2LL * p.Fp : p.R, N = up ? 2LL * p.F : p.D;
+  return ffn_large(M, N) ? tile_t<T, JOB, 4, 2, 4, 8>(p, s) : tile_t<T, JOB, 2, 2, 4, 4>(p, s);
+}
+template <Job JOB> hipError_t type_t(const FfnParams& p, int dtype, hipStream_t s) {
+  return dtype == TTT_DTYPE_BF16 ? job_t<__bf16, JOB>(p, s)
+         : dtype == TTT_DTYPE_F16 ? job_t<_Float16, JOB>(p, s) : job_t<float, JOB>(p, s);
+}
+
+template <typename T> hipError_t few_t(const FfnParams& p, hipStream_t s) {
+  const unsigned cols = (unsigned)((p.F + 15) / 16);
+  if (p.R <= 16)
+    hipLaunchKernelGGL((ffn_few_kernel<T, 1>), dim3(cols), dim3(64 * kFewWaves), 0, s, p);
+  else
+    hipLaunchKernelGGL((ffn_few_kernel<T, 2>), dim3(cols, (unsigned)((p.R + 31) / 32)), dim3(64 * kFewWaves), 0, s, p);
+  return hipGetLastError();
+}
+template <typename T> hipError_t join_t(const FfnParams& p, hipStream_t s) {
+  const long long quads = 2LL * p.Fp * p.Dp / 4;
+  hipLaunchKernelGGL(ffn_join_kernel<T>, dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, s, p, quads);
+  return hipGetLastError();
+}
+template <typename T> hipError_t bias_t(const FfnParams& p, hipStream_t s) {
+  hipLaunchKernelGGL(ffn_bias_kernel<T>, dim3((unsigned)((2 * p.Fp + 15) / 16)), dim3(256), 0, s, p);
+  return hipGetLastError();
+}
+template <typename T>
+hipError_t planes_t(const void* from, long long ld, int rows, int width, void* to, hipStream_t s) {
+  const int pieces = ffn_pad(width) / 8;
+  const long long all = (long long)rows * pieces;
+  hipLaunchKernelGGL(ffn_planes_kernel<T>, dim3((unsigned)((all + 255) / 256)), dim3(256), 0, s, static_cast<const T*>(from), ld,
+                     width, pieces, all, static_cast<char*>(to), all * 16);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+// Shares of the rows that dW contracts over: its tiles times these make whole rounds of the
+// card, each share 512 rows or more
+int ffn_splits(int R, int D, int F, int dtype) {
+  const long long M = 2LL * ffn_pad(F), N = D;
+  const bool large = ffn_large(M, N);
+  const long long b = large ? 256 : 128, tiles = ((M + b - 1) / b) * ((N + b - 1) / b), places = large ? 256 : 512;
+  const long long most = std::max<long long>(1, (R + 511) / 512);
+  return (int)std::max<long long>(1, std::min(most, places / tiles));
+}
+
+hipError_t launch_ffn_few(const FfnParams& p, int dtype, hipStream_t s) {
+  return dtype == TTT_DTYPE_BF16 ? few_t<__bf16>(p, s) : dtype == TTT_DTYPE_F16 ? few_t<_Float16>(p, s) : few_t<float>(p, s);
+}
+hipError_t launch_ffn_fwd(const FfnParams& p, int dtype, hipStream_t s) { return type_t<Job::Fwd>(p, dtype, s); }
+hipError_t launch_ffn_grad(const FfnParams& p, int dtype, hipStream_t s) {
+  const hipError_t e = type_t<Job::Grad>(p, dtype, s);
+  if (e != hipSuccess || p.bias_part == nullptr) return e;
+  return dtype == TTT_DTYPE_BF16 ? bias_t<__bf16>(p, s) : dtype == TTT_DTYPE_F16 ? bias_t<_Float16>(p, s) : bias_t<float>(p, s);
+}
+hipError_t launch_ffn_dx(const FfnParams& p, int dtype, hipStream_t s) { return type_t<Job::Dx>(p, dtype, s); }
+hipError_t launch_ffn_dw(const FfnParams& p, int dtype, hipStream_t s) {
+  const hipError_t e = type_t<Job::Dw>(p, dtype, s);
+  if (e != hipSuccess || p.part == nullptr) return e;
+  return dtype == TTT_DTYPE_BF16 ? join_t<__bf16>(p, s) : dtype == TTT_DTYPE_F16 ? join_t<_Float16>(p, s) : join_t<float>(p, s);
+}
+hipError_t launch_ffn_planes(const void* from, long long ld, int rows, int width, void* to, int dtype, hipStream_t s) {
+  return dtype == TTT_DTYPE_BF16 ? planes_t<__bf16>(from, ld, rows, width, to, s)
+         : dtype == TTT_DTYPE_F16 ? planes_t<_Float16>(from, ld, rows, width, to, s)
+                                  : planes_t<float>(from, ld, rows, width, to, s);
+}
+
+}  // namespace ttt

@@ -33,7 +33,8 @@ STATE_SHARED = 0x200  # (forward): initial states [H,...], one for every sequenc
 SAVED_SLOTS = 0x400  # `saved` without the place of the backward's handoff (slot_saved below)
 ETA_RULES = {"dense": ETA_DENSE, "layer": ETA_LAYER, "causal": ETA_CAUSAL}
 
-ACTIVATIONS = {None: 0, "silu": 1}  # enum ttt_activation
+ACTIVATIONS = {None: 0, "silu": 1}  # enum ttt_activation, the convolution's
+GATE_ACTIVATIONS = {"silu": 1, "gelu": 2}  # the gated feed-forward projections'
 
 # process-wide options (enum ttt_option)
 OPT_MLP_BWD_POLL_LIMIT = 1
@@ -101,6 +102,10 @@ SIGNATURES = {
     "ttt_block_norm_fwd": (_I, [_P, _L] * 3 + [_P] * 3 + [_L, _I, _I, _F, _I, _I] + [_P] * 4),
     "ttt_block_norm_partial_bytes": (_S, [_L, _I]),
     "ttt_block_norm_bwd": (_I, [_P, _L] * 3 + [_P] * 6 + [_L] + [_I] * 4 + [_P] * 7 + [_S, _P]),
+    "ttt_ffn_workspace_bytes": (_S, [_I] * 4),
+    "ttt_ffn_fwd": (_I, [_P, _L] + [_P] * 4 + [_I] * 5 + [_P, _P, _S, _P]),
+    "ttt_ffn_bwd_workspace_bytes": (_S, [_I] * 4),
+    "ttt_ffn_bwd": (_I, [_P, _L] + [_P] * 5 + [_L] + [_I] * 5 + [_P] * 6 + [_S, _P]),
     "ttt_layer_norm_fwd": (_I, [_P, _L] * 2 + [_P] * 2 + [_L, _I, _F, _I] + [_P] * 3),
     "ttt_layer_norm_partial_bytes": (_S, [_L, _I]),
     "ttt_layer_norm_bwd": (_I, [_P, _L] * 2 + [_P] * 3 + [_L, _I, _I] + [_P] * 5 + [_S, _P]),
