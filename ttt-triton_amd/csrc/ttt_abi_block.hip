@@ -24,7 +24,7 @@ int check_delta(int B, int L, int H, int P, int G, int N, int dtype, int g_dtype
 }
 struct DeltaPlan {
   int Q, NC, PB, parts, share;
-  size_t tok, z, m, mb, states, rows, qk, gb;
+  size_t tok, zm, states, rows, qk, gb;
 };
 DeltaPlan delta_plan(int B, int L, int H, int P, int G, int N, int dtype) {
   DeltaPlan s;
@@ -35,9 +35,7 @@ DeltaPlan delta_plan(int B, int L, int H, int P, int G, int N, int dtype) {
   s.share = H / G * s.parts;
   const size_t chunks = (size_t)B * H * s.NC;
   s.tok = up256(chunks * ttt::delta_tok_floats(s.Q) * 4);
-  s.z = chunks * ttt::delta_operands(s.Q, 3);
-  s.m = chunks * ttt::delta_operands(s.Q, ttt::delta_mid(dtype));
-  s.mb = chunks * ttt::delta_operands(s.Q, 3);
+  s.zm = chunks * ttt::delta_tiles(s.Q) * 1024;
   s.states = chunks * P * ttt::scan_padded(N) * 4;
   s.rows = chunks * P * s.Q * 4;
   s.qk = s.share > 1 ? (size_t)s.share * B * L * G * N * 4 : 0;
@@ -75,7 +73,7 @@ int check_ffn(int R, int D, int F, int act, int dtype) {
   if (act != TTT_ACT_SILU && act != TTT_ACT_GELU) return TTT_ERR_ARG;
   // (tiles of 128 x 128 with 256 threads; planes 8 values a thread)
   const long long n = std::max(2LL * F, (long long)D), m = std::max<long long>(R, 2LL * F + 16);
-  if (((m + 127) / 128) * ((n + 127) / 128) > kMaxThreads / 256) return TTT_ERR_SHAPE;
+  if (((m + 127) / 128) * ((n + 127) / 128) > kMaxThreads / 256 / ttt::kFfnMostSplits) return TTT_ERR_SHAPE;
   if (std::max<long long>(R, F) * (ttt::ffn_pad(D) / 8) > kMaxThreads) return TTT_ERR_SHAPE;
   return TTT_OK;
 }
@@ -90,9 +88,10 @@ FfnPlan ffn_plan(int R, int D, int F, int dtype) {
   s.x = s.in_place ? 0 : up256(planes * R * Dp * 2);
   s.w = s.in_place ? 0 : up256(planes * F * Dp * 2);
   s.grad = up256(planes * R * 2 * Fp * 2);
-  const int splits = ttt::ffn_splits(R, D, F, dtype);
-  s.part = splits > 1 ? up256((size_t)splits * 2 * Fp * Dp * 4) : 0;
-  s.bias = up256((size_t)ttt::ffn_bias_parts(R, F) * 2 * Fp * 4);
+  const int of_dx = ttt::ffn_cut_dx(R, D, F, dtype).splits, of_dw = ttt::ffn_cut_dw(R, D, F, dtype).splits;
+  const size_t dx = of_dx > 1 ? (size_t)of_dx * R * Dp * 4 : 0, dw = of_dw > 1 ? (size_t)of_dw * 2 * Fp * Dp * 4 : 0;
+  s.part = up256(std::max(dx, dw));  // (one after the other)
+  s.bias = up256((size_t)ttt::ffn_bias_parts(R, D, F, dtype) * 2 * Fp * 4);
   return s;
 }
 // x, wg and wu as the products read them: in place, or as planes in the workspace
@@ -219,8 +218,7 @@ int ttt_ffn_bwd(const void* x, long long ldx, const void* wg, const void* wu, co
   p.dwu = dwu;
   p.dbg = dbg;
   p.dbu = dbu;
-  p.splits = ttt::ffn_splits(R, D, F, dtype);
-  p.bias_parts = ttt::ffn_bias_parts(R, F);
+  p.bias_parts = ttt::ffn_bias_parts(R, D, F, dtype);
   const hipStream_t on = static_cast<hipStream_t>(stream);
   char* ws = static_cast<char*>(workspace);
   hipError_t e = ffn_operands(p, s, x, ldx, wg, wu, dtype, ws, on);
@@ -343,11 +341,11 @@ size_t ttt_delta_saved_bytes(int B, int L, int H, int P, int N, int dtype) {
 }
 size_t ttt_delta_workspace_bytes(int B, int L, int H, int P, int N, int dtype) {
   DeltaPlan s;
-  return delta_plan_ok(B, L, H, P, 1, N, dtype, s) ? s.tok + s.z + s.m : 0;
+  return delta_plan_ok(B, L, H, P, 1, N, dtype, s) ? s.tok + 2 * s.zm : 0;
 }
 size_t ttt_delta_bwd_workspace_bytes(int B, int L, int H, int P, int G, int N, int dtype) {
   DeltaPlan s;
-  return delta_plan_ok(B, L, H, P, G, N, dtype, s) ? s.tok + s.z + s.mb + s.states + s.rows + 2 * s.gb + 2 * s.qk : 0;
+  return delta_plan_ok(B, L, H, P, G, N, dtype, s) ? s.tok + 2 * s.zm + s.states + s.rows + 2 * s.gb + 2 * s.qk : 0;
 }
 
 int ttt_delta_fwd(const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv,
@@ -373,7 +371,7 @@ int ttt_delta_fwd(const void* q, long long ldq, const void* k, long long ldk, co
   OPTIONAL(h_last, 16);
   OPTIONAL(saved, 16);
   if (saved != nullptr && saved_bytes < s.states + s.rows) return TTT_ERR_WORKSPACE;
-  if (workspace == nullptr || workspace_bytes < s.tok + s.z + s.m) return TTT_ERR_WORKSPACE;
+  if (workspace == nullptr || workspace_bytes < s.tok + 2 * s.zm) return TTT_ERR_WORKSPACE;
   OPTIONAL(workspace, 16);
   ttt::DeltaParams p{};
   p.q = q;
@@ -401,8 +399,8 @@ int ttt_delta_fwd(const void* q, long long ldq, const void* k, long long ldk, co
   p.beta_f32 = beta_dtype == TTT_DTYPE_F32;
   char* ws = static_cast<char*>(workspace);
   p.tok = reinterpret_cast<float*>(ws);
-  p.z = ws + s.tok;
-  p.m = ws + s.tok + s.z;
+  p.z = reinterpret_cast<float*>(ws + s.tok);
+  p.m = reinterpret_cast<float*>(ws + s.tok + s.zm);
   if (saved != nullptr) {
     p.states = static_cast<float*>(saved);
     p.rows = reinterpret_cast<float*>(static_cast<char*>(saved) + s.states);
@@ -440,7 +438,7 @@ int ttt_delta_bwd(const void* q, long long ldq, const void* k, long long ldk, co
   OPTIONAL(dh0, 16);
   if (saved_bytes < s.states + s.rows) return TTT_ERR_WORKSPACE;
   if (workspace == nullptr ||
-      workspace_bytes < s.tok + s.z + s.mb + s.states + s.rows + 2 * s.gb + 2 * s.qk)
+      workspace_bytes < s.tok + 2 * s.zm + s.states + s.rows + 2 * s.gb + 2 * s.qk)
     return TTT_ERR_WORKSPACE;
   OPTIONAL(workspace, 16);
   ttt::DeltaParams p{};
@@ -474,8 +472,8 @@ int ttt_delta_bwd(const void* q, long long ldq, const void* k, long long ldk, co
     return at;
   };
   p.tok = reinterpret_cast<float*>(take(s.tok));
-  p.z = take(s.z);
-  p.m = take(s.mb);
+  p.z = reinterpret_cast<float*>(take(s.zm));
+  p.m = reinterpret_cast<float*>(take(s.zm));
   p.states = reinterpret_cast<float*>(take(s.states));
   p.rows = reinterpret_cast<float*>(take(s.rows));
   if (s.parts > 1) {

@@ -39,7 +39,7 @@ struct DeltaParams {
   void* o;                // [B][L][H][P]; backwards dv
   float* h_last;          // [B][H][P][N] (may be null); backwards the gradient of the initial state
   float* tok;             // [B*H][NC] DeltaTok
-  void *z, *m;            // [B*H][NC] operands of Z and M in planes
+  float *z, *m;           // [B*H][NC][tiles][64][4]: Z and M by blocks and lanes
   float* states;          // [B*H*parts][NC][NP][PB]: the states entering the chunks, or walking back the
                           // gradients of those leaving them (may be null)
   float* rows;            // [B*H*parts][NC*Q][PB]: x, or walking back y (may be null)
@@ -76,10 +76,9 @@ constexpr int kDeltaMaxP = 256;
 constexpr int delta_part(int P) { return P % 64 == 0 ? 64 : 32; }
 // tokens of a chunk: 64, or 32 where the backward's planes would not fit in LDS
 constexpr int delta_chunk(int dtype) { return dtype == TTT_DTYPE_BF16 ? 64 : 32; }
-// operands of 32 contracted tokens to a chunk's triangle of blocks
+// blocks of 16 x 16 in a chunk's triangle, and operands of 32 contracted tokens
+constexpr int delta_tiles(int Q) { return Q == 64 ? 10 : 3; }
 constexpr int delta_pairs(int Q) { return Q == 64 ? 6 : 2; }
-constexpr int delta_mid(int dtype) { return dtype == TTT_DTYPE_BF16 ? 2 : 3; }
-constexpr size_t delta_operands(int Q, int planes) { return (size_t)planes * delta_pairs(Q) * 1024; }  // bytes
 constexpr int delta_tok_floats(int Q) { return 8 * Q + 4; }
 
 template <typename T> constexpr int kDeltaQ = sizeof(T) == 2 && ScanType<T>::IN == 1 ? 64 : 32;
@@ -94,8 +93,10 @@ template <int Q> struct alignas(16) DeltaTok {
   __device__ __forceinline__ static f4 four(const float* a, int t) { return *reinterpret_cast<const f4*>(a + t); }
 };
 
-// The operands of a triangle of 16 x 16 blocks with 32 contracted tokens each: forwards of
-// row block b, columns 32q.. (q <= b / 2), backwards of column block b, rows 32q.. (q >= b / 2)
+// A block of Z or M has its free token to a lane (forwards the row, backwards the column) and four
+// contracted ones to a lane's registers.  Two of them are an operand of 32 contracted tokens:
+// forwards of row block b, columns 32q.. (q <= b / 2), backwards of column block b, rows 32q..
+// (q >= b / 2); the place of an operand among the triangle's:
 __device__ __forceinline__ constexpr int pair_at(bool back, int Q, int b, int q) {
   if (Q == 32) return b;
   if (!back) return b < 2 ? b : 2 * b - 2 + q;

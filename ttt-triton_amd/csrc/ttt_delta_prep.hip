@@ -7,8 +7,7 @@
 //     Z_IJ = Y - Z_II b Y,  Y = A_IJ - sum_{J<=K<I} A_IK b Z_KJ
 //                                       a wave to a column of blocks, in fp32 products
 //   M_ij = s F_ij (q_i . k_j), j <= i
-// Z and M are written as operands in planes, of 32 contracted tokens: their columns for the
-// walk forwards, their rows for the walk back.
+// Z and M are written in fp32 by blocks, as the walks' operands take them.
 #include <math.h>
 
 #include "ttt_delta.h"
@@ -45,8 +44,7 @@ __device__ __forceinline__ void row_squares(const Stage<T, ROWS, COLS, NT>& s, f
 
 template <typename T, int NP, bool BACK> __global__ __launch_bounds__(256) void delta_prep_kernel(DeltaParams p) {
   using Sh = PrepShared<T, NP>;
-  constexpr int IN = Sh::IN, Q = Sh::Q, TB = Q / 16, NC2 = NP / 32, PAIRS = delta_pairs(Q);
-  constexpr int MP = BACK || IN > 1 ? kFull : 2;  // planes of M: backwards fp32 results come of it
+  constexpr int IN = Sh::IN, Q = Sh::Q, TB = Q / 16, NC2 = NP / 32;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   Sh& sh = *reinterpret_cast<Sh*>(smem);
   const int w = wave_id(), l = lane_id(), g = l >> 4, r = l & 15;
@@ -122,37 +120,26 @@ template <typename T, int NP, bool BACK> __global__ __launch_bounds__(256) void 
 #pragma unroll
     for (int e = 0; e < 4; ++e) sh.a[i + e][j] = only_if(j < i + e, acc[e]);
   }
-  // M, by operands: forwards the free token i and contracted j, backwards the other way
-  char* mp = static_cast<char*>(p.m) + chunk * (long long)delta_operands(Q, MP);
+  // M: forwards the free token i and contracted j, backwards the other way
+  float* mp = p.m + chunk * (TILES * 256);
 #pragma unroll
-  for (int u = w; u < PAIRS; u += 4) {
-    const int blk = Q == 32 ? u : BACK ? (u < 4 ? u / 2 : u - 2) : (u < 2 ? u : u / 2 + 1);
-    const int q32 = Q == 32 ? 0 : BACK ? (u < 4 ? u % 2 : 1) : (u < 2 ? 0 : u % 2);
-    f4 v[2];
+  for (int t = w; t < TILES; t += 4) {
+    const int ib = tri_row(t), jb = t - tri(ib, 0);  // blocks of q and of k
+    f4 acc = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int o = 0; o < 2; ++o) {
-      const int in = 2 * q32 + o;
-      v[o] = f4{0.f, 0.f, 0.f, 0.f};
-      if (!meets(BACK, blk, in)) continue;
-      const int ib = BACK ? in : blk, jb = BACK ? blk : in;  // blocks of q and of k
-      f4 acc = f4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int q = 0; q < NC2; ++q) {
-        const Op<IN> oq = sh.q.rows(16 * ib, 32 * q), ok = sh.k.rows(16 * jb, 32 * q);
-        if constexpr (BACK)
-          mma<kFull>(acc, oq, ok);
-        else
-          mma<kFull>(acc, ok, oq);
-      }
-      const int tr = 16 * in + 4 * g, tc = 16 * blk + r;
-      const float fc = BACK ? tok.rk[tc] : tok.rq[tc];
-      acc *= decays(tr, tc, BACK) * tok.four(BACK ? tok.rq : tok.rk, tr) * (fc * p.scale);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[o][e] = only_if(BACK ? tc <= tr + e : tr + e <= tc, acc[e]);
+    for (int q = 0; q < NC2; ++q) {
+      const Op<IN> oq = sh.q.rows(16 * ib, 32 * q), ok = sh.k.rows(16 * jb, 32 * q);
+      if constexpr (BACK)
+        mma<kFull>(acc, oq, ok);
+      else
+        mma<kFull>(acc, ok, oq);
     }
-    const Op<MP> op = split8<MP>(v[0], v[1]);
+    const int tr = 16 * (BACK ? ib : jb) + 4 * g, tc = 16 * (BACK ? jb : ib) + r;
+    const float fc = BACK ? tok.rk[tc] : tok.rq[tc];
+    acc *= decays(tr, tc, BACK) * tok.four(BACK ? tok.rq : tok.rk, tr) * (fc * p.scale);
 #pragma unroll
-    for (int a = 0; a < MP; ++a) *reinterpret_cast<bf8*>(mp + ((a * PAIRS + u) * 64 + l) * 16) = op.v[a];
+    for (int e = 0; e < 4; ++e) acc[e] = only_if(BACK ? tc <= tr + e : tr + e <= tc, acc[e]);
+    *reinterpret_cast<f4*>(mp + (t * 64 + l) * 4) = acc;
   }
   __syncthreads();
   // the blocks of Z on the diagonal: lane (g, r) has column r of block g
@@ -215,27 +202,18 @@ template <typename T, int NP, bool BACK> __global__ __launch_bounds__(256) void 
         for (int e = 0; e < 4; ++e) sh.a[16 * I + 4 * g + e][16 * w + r] = zt[I][e];
   }
   __syncthreads();
-  char* zp = static_cast<char*>(p.z) + chunk * (long long)delta_operands(Q, kFull);
+  float* zp = p.z + chunk * (TILES * 256);
 #pragma unroll
-  for (int u = w; u < PAIRS; u += 4) {
-    const int blk = Q == 32 ? u : BACK ? (u < 4 ? u / 2 : u - 2) : (u < 2 ? u : u / 2 + 1);
-    const int q32 = Q == 32 ? 0 : BACK ? (u < 4 ? u % 2 : 1) : (u < 2 ? 0 : u % 2);
-    f4 v[2];
+  for (int t = w; t < TILES; t += 4) {
+    const int ib = tri_row(t), jb = t - tri(ib, 0);
+    f4 v;
+    if constexpr (BACK) {
 #pragma unroll
-    for (int o = 0; o < 2; ++o) {
-      const int in = 2 * q32 + o;
-      v[o] = f4{0.f, 0.f, 0.f, 0.f};
-      if (!meets(BACK, blk, in)) continue;
-      if constexpr (BACK) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[o][e] = sh.a[16 * in + 4 * g + e][16 * blk + r];
-      } else {
-        v[o] = *reinterpret_cast<const f4*>(&sh.a[16 * blk + r][16 * in + 4 * g]);
-      }
+      for (int e = 0; e < 4; ++e) v[e] = sh.a[16 * ib + 4 * g + e][16 * jb + r];
+    } else {
+      v = *reinterpret_cast<const f4*>(&sh.a[16 * ib + r][16 * jb + 4 * g]);
     }
-    const Op<kFull> op = split8<kFull>(v[0], v[1]);
-#pragma unroll
-    for (int a = 0; a < kFull; ++a) *reinterpret_cast<bf8*>(zp + ((a * PAIRS + u) * 64 + l) * 16) = op.v[a];
+    *reinterpret_cast<f4*>(zp + (t * 64 + l) * 4) = v;
   }
 }
 

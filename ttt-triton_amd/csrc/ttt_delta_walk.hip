@@ -26,22 +26,45 @@ template <typename T, int W, int NP, bool BACK> struct WalkShared {
   DeltaTok<Q> tok;
 };
 
-// bytes on their way to LDS as they lie in memory
-template <int BYTES, int NT> struct Copy {
-  static constexpr int ALL = BYTES / 16, CNT = (ALL + NT - 1) / NT;
-  u4v v[CNT];
-  __device__ __forceinline__ void load(const void* p) {
+// a chunk's blocks of Z or M on their way from memory to operands in planes
+template <int Q, int W, bool BACK> struct Blocks {
+  static constexpr int ALL = delta_tiles(Q), CNT = (ALL + W - 1) / W;
+  f4 v[CNT];
+  __device__ __forceinline__ void load(const float* p, int w) {
+#pragma unroll
+    for (int i = 0; i < CNT; ++i)
+      if (i * W + w < ALL) v[i] = *reinterpret_cast<const f4*>(p + ((i * W + w) * 64 + lane_id()) * 4);
+  }
+  template <int PL> __device__ __forceinline__ void store(bf8 (*to)[delta_pairs(Q)][64], int w) const {
 #pragma unroll
     for (int i = 0; i < CNT; ++i) {
-      const int o = i * NT + (int)threadIdx.x;
-      if (ALL % NT == 0 || o < ALL) v[i] = static_cast<const u4v*>(p)[o];
+      const int t = i * W + w;
+      if (t >= ALL) continue;
+      const int hb = tri_row(t), lb = t - tri(hb, 0), blk = BACK ? lb : hb, in = BACK ? hb : lb;
+      bf4 o[PL];
+      split4<PL>(v[i], o);
+#pragma unroll
+      for (int a = 0; a < PL; ++a)
+        reinterpret_cast<bf4*>(&to[a][pair_at(BACK, Q, blk, in / 2)][lane_id()])[in & 1] = o[a];
     }
   }
-  __device__ __forceinline__ void store(void* p) const {
+};
+// floats on their way to LDS as they lie in memory
+template <int FLOATS, int NT> struct Copy {
+  static constexpr int ALL = FLOATS / 4, CNT = (ALL + NT - 1) / NT;
+  f4 v[CNT];
+  __device__ __forceinline__ void load(const float* p) {
 #pragma unroll
     for (int i = 0; i < CNT; ++i) {
       const int o = i * NT + (int)threadIdx.x;
-      if (ALL % NT == 0 || o < ALL) static_cast<u4v*>(p)[o] = v[i];
+      if (o < ALL) v[i] = reinterpret_cast<const f4*>(p)[o];
+    }
+  }
+  __device__ __forceinline__ void store(float* p) const {
+#pragma unroll
+    for (int i = 0; i < CNT; ++i) {
+      const int o = i * NT + (int)threadIdx.x;
+      if (o < ALL) reinterpret_cast<f4*>(p)[o] = v[i];
     }
   }
 };
@@ -75,9 +98,8 @@ template <typename T, int W, int NP, bool BACK> __global__ __launch_bounds__(64 
 
   Stage<T, Q, NP, NT> sk, sq;
   Stage<T, Q, 16 * W, NT> sv;
-  Copy<sizeof(Sh::z), NT> cz;
-  Copy<sizeof(Sh::m), NT> cm;
-  Copy<sizeof(DeltaTok<Q>), NT> ct;
+  Blocks<Q, W, BACK> bz, bm;
+  Copy<delta_tok_floats(Q), NT> ct;
   sk.place(p.ldk, p.N);
   sq.place(p.ldq, p.N);
   sv.place(ldv, 16 * W);
@@ -87,8 +109,8 @@ template <typename T, int W, int NP, bool BACK> __global__ __launch_bounds__(64 
     sk.load(K + row * p.ldk, left);
     sq.load(Qr + row * p.ldq, left);
     sv.load(V + row * ldv, left);
-    cz.load(static_cast<const char*>(p.z) + chunk * (long long)sizeof(Sh::z));
-    cm.load(static_cast<const char*>(p.m) + chunk * (long long)sizeof(Sh::m));
+    bz.load(p.z + chunk * (delta_tiles(Q) * 256), w);
+    bm.load(p.m + chunk * (delta_tiles(Q) * 256), w);
     ct.load(p.tok + chunk * delta_tok_floats(Q));
   };
   const auto z_op = [&](int u) {
@@ -104,6 +126,10 @@ template <typename T, int W, int NP, bool BACK> __global__ __launch_bounds__(64 
     return o;
   };
   fetch(BACK ? NC - 1 : 0);
+  // (an operand's half beside the triangle stays 0)
+  for (int i = threadIdx.x; i < (int)(offsetof(Sh, tok) - offsetof(Sh, z)) / 16; i += NT)
+    reinterpret_cast<f4*>(&sh.z)[i] = f4{0.f, 0.f, 0.f, 0.f};
+  __syncthreads();
 #pragma unroll 1
   for (int k = 0; k < NC; ++k) {
     const int c = BACK ? NC - 1 - k : k;
@@ -111,9 +137,9 @@ template <typename T, int W, int NP, bool BACK> __global__ __launch_bounds__(64 
     sk.store(sh.k);
     sq.store(sh.q);
     sv.store(sh.v);
-    cz.store(sh.z);
-    cm.store(sh.m);
-    ct.store(&sh.tok);
+    bz.template store<kFull>(sh.z, w);
+    bm.template store<MP>(sh.m, w);
+    ct.store(sh.tok.hi);
     __syncthreads();
     if (k + 1 < NC) fetch(BACK ? c - 1 : c + 1);
     if (p.states != nullptr) st.keep(p.states + (chain * NC + c) * (long long)(NP * PB) + f0, PB, w);

@@ -22,12 +22,12 @@ struct FfnParams {
   void* y;                    // [R][F]
   void *dx, *dwg, *dwu;       // [R][D], [F][D], [F][D]
   void *dbg, *dbu;            // [F], or null
-  float* part;                // [splits][2 Fp][Dp] of dwg and dwu where the rows are split, else null
+  float* part;                // [splits][R or 2 Fp][Dp] of dx, or dwg and dwu, where their steps are split
   float* bias_part;           // [bias_parts][2 Fp], or null
   long long lddy;
   int R, D, F, Dp, Fp;        // widths as the user's and padded to 8
   int planes, act;
-  int splits, bias_parts;
+  int splits, bias_parts;     // (splits: of the product that is launched)
 };
 // few rows: the operands as the user's, rows of x ldx elements apart
 hipError_t launch_ffn_few(const FfnParams& p, int dtype, hipStream_t stream);
@@ -40,12 +40,51 @@ hipError_t launch_ffn_planes(const void* from, long long ld, int rows, int width
 
 constexpr int ffn_pad(int n) { return (n + 7) / 8 * 8; }
 constexpr int ffn_planes(int dtype) { return dtype == TTT_DTYPE_F32 ? 3 : 1; }
-// Tiles of 256 x 256 where they make three quarters of a workgroup to each compute unit, else of 128 x 128
-constexpr bool ffn_large(long long m, long long n) { return ((m + 255) / 256) * ((n + 255) / 256) >= 192; }
-// rows of partial sums of the bias gradients: one to a wave's rows
-constexpr int ffn_bias_parts(long long R, int F) {
-  return ffn_large(R, 2LL * F) ? (int)((R + 255) / 256) * 2 : (int)((R + 127) / 128) * 2;
+
+// How a product is cut up: tiles of 256 x 256, a workgroup to a compute unit, or of 128 x 128,
+// two; and the steps of 64 contracted values of a tile into shares, whose sums are joined by
+// another launch.
+struct FfnCut {
+  bool large;
+  int splits;
+};
+// M x N results (the width of both projections together), `steps` of 64 contracted values, joined
+// over `most` shares or fewer.  In units of a step of a large tile (1,024 clocks at the matrix
+// instructions' rate, about 1,500 measured), a small tile's takes 0.6 with another on the compute
+// unit; a tile's start and end take about 5; a join reads and writes its sums at the card's bandwidth.
+inline FfnCut ffn_cut(long long M, long long N, long long steps, int most) {
+  FfnCut best{false, 1};
+  double least = 0.0;
+  for (int large = 0; large < 2; ++large) {
+    const long long side = large ? 256 : 128, places = large ? 256 : 512;
+    const long long tiles = ((M + side - 1) / side) * ((N + side - 1) / side);
+    for (int k = 1; k <= most && (k == 1 || k * 8 <= steps); ++k) {
+      const double rounds = (double)((tiles * k + places - 1) / places);
+      const double join = k > 1 ? 8.0 + 1e-6 * (double)(M * N) * (k + 1) : 0.0;
+      const double time = rounds * ((double)((steps + k - 1) / k) * (large ? 1.0 : 0.6) + 5.0) + join;
+      if ((large == 0 && k == 1) || time < least) {
+        least = time;
+        best = {large != 0, k};
+      }
+    }
+  }
+  return best;
 }
-int ffn_splits(int R, int D, int F, int dtype);
+constexpr int kFfnMostSplits = 16;
+inline long long ffn_steps(long long contracted, int dtype) {
+  return (contracted + kFfnStep - 1) / kFfnStep * (dtype == TTT_DTYPE_F32 ? 6 : 1);
+}
+inline FfnCut ffn_cut_up(long long R, int D, int F, int dtype) { return ffn_cut(R, 2LL * F, ffn_steps(ffn_pad(D), dtype), 1); }
+inline FfnCut ffn_cut_dx(long long R, int D, int F, int dtype) {
+  return ffn_cut(R, D, 2 * ffn_steps(ffn_pad(F), dtype), kFfnMostSplits);
+}
+inline FfnCut ffn_cut_dw(long long R, int D, int F, int dtype) {
+  return ffn_cut(2LL * ffn_pad(F), D, ffn_steps(R, dtype), kFfnMostSplits);
+}
+// rows of partial sums of the bias gradients: one to a wave's rows
+inline int ffn_bias_parts(long long R, int D, int F, int dtype) {
+  const long long side = ffn_cut_up(R, D, F, dtype).large ? 256 : 128;
+  return (int)((R + side - 1) / side) * 2;
+}
 
 }  // namespace ttt

@@ -144,7 +144,6 @@ __global__ __launch_bounds__(64 * WN * WM) void ffn_kernel(FfnParams p) {
   // rows and columns of all tiles, and contracted values
   const int M = JOB == Job::Dw ? 2 * p.Fp : p.R, N = UP ? p.F : p.D, K = JOB == Job::Dw ? p.R : JOB == Job::Dx ? p.Fp : p.Dp;
   const int tm = (M + BM - 1) / BM, tn = (N + (UP ? HALF : BN) - 1) / (UP ? HALF : BN);
-  const int splits = JOB == Job::Dw ? p.splits : 1;
   // Neighbours on a die have eight rows of tiles by all columns, one column after the other
   unsigned id = on_xcd(blockIdx.x, gridDim.x);
   const int split = (int)(id / (unsigned)(tm * tn));
@@ -153,18 +152,16 @@ __global__ __launch_bounds__(64 * WN * WM) void ffn_kernel(FfnParams p) {
   id -= band * 8 * tn;
   const int m0 = (8 * band + (int)(id % high)) * BM, n0 = (int)(id / high) * (UP ? HALF : BN);
 
-  const int ksteps = (K + kFfnStep - 1) / kFfnStep, per = (ksteps + splits - 1) / splits;
-  const int k0 = split * per, kn = min(ksteps, k0 + per) - k0;
-  const int pairs = p.planes == 3 ? 6 : 1;
-  const int segs = JOB == Job::Dx ? 2 : 1;
-  const int steps = kn > 0 ? kn * pairs * segs : 0;
+  const int ksteps = (K + kFfnStep - 1) / kFfnStep, pairs = p.planes == 3 ? 6 : 1, segs = JOB == Job::Dx ? 2 : 1;
+  const int all = ksteps * pairs * segs, per = UP ? all : (all + p.splits - 1) / p.splits;
+  const int first = split * per, steps = min(all, first + per) - first;
 
-  // the step that is sent next
-  int sk = 0, sp = 0, ss = 0;
+  // the step that is sent next: its contracted values, of which weights, and the planes
+  int sk = first % ksteps, ss = first / ksteps % segs, sp = first / (ksteps * segs);
   const auto next = [&](int buf) {
     // planes a of the first operand and b of the second: (2,0) (1,1) (0,2) (1,0) (0,1) (0,0)
     const int pa = pairs == 1 ? 0 : (0x001012 >> (4 * sp)) & 15, pb = pairs == 1 ? 0 : (0x010210 >> (4 * sp)) & 15;
-    const int k = (k0 + sk) * kFfnStep, left = K - k;
+    const int k = sk * kFfnStep, left = K - k;
     unsigned char* to = smem + buf * STEP;
     if constexpr (UP) {
       const int pieces = left / 8;
@@ -186,7 +183,7 @@ __global__ __launch_bounds__(64 * WN * WM) void ffn_kernel(FfnParams p) {
       send<LM, BM, NW>(static_cast<const char*>(p.grad.p) + pb * p.grad.plane + (long long)k * p.grad.ld + m0 * 2, p.grad.ld,
                        left, (M - m0) / 8, to + Panel<LN, BN>::BYTES, w);
     }
-    if (++sk == kn) {
+    if (++sk == ksteps) {
       sk = 0;
       if (++ss == segs) {
         ss = 0;
@@ -281,10 +278,10 @@ __global__ __launch_bounds__(64 * WN * WM) void ffn_kernel(FfnParams p) {
       for (int j = 0; j < TM; ++j) {
         const int m = m0 + 16 * (wm * TM + j) + r;
         if (m >= M) continue;
-        if constexpr (JOB == Job::Dx) {
-          store_up_to4(static_cast<T*>(p.dx) + (long long)m * p.D + n, left, acc[i][j]);
-        } else if (p.part != nullptr) {
+        if (p.splits > 1) {
           *reinterpret_cast<f4*>(p.part + ((long long)split * M + m) * p.Dp + n) = acc[i][j];
+        } else if constexpr (JOB == Job::Dx) {
+          store_up_to4(static_cast<T*>(p.dx) + (long long)m * p.D + n, left, acc[i][j]);
         } else {
           const int f = m < p.Fp ? m : m - p.Fp;
           if (f < p.F) store_up_to4(static_cast<T*>(m < p.Fp ? p.dwg : p.dwu) + (long long)f * p.D + n, left, acc[i][j]);
@@ -294,17 +291,18 @@ __global__ __launch_bounds__(64 * WN * WM) void ffn_kernel(FfnParams p) {
   }
 }
 
-// dWg and dWu from the sums over shares of the rows
-template <typename T> __global__ __launch_bounds__(256) void ffn_join_kernel(FfnParams p, long long quads) {
+// dx, or dWg and dWu, from the sums of the shares
+template <typename T, Job JOB> __global__ __launch_bounds__(256) void ffn_join_kernel(FfnParams p, long long quads) {
   const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
   if (id >= quads) return;
   const int per = p.Dp / 4, m = (int)(id / per), n = 4 * (int)(id - (long long)m * per);
-  const int f = m < p.Fp ? m : m - p.Fp;
-  if (f >= p.F) return;
+  const int f = JOB == Job::Dx ? m : m < p.Fp ? m : m - p.Fp;
+  if (JOB == Job::Dw && f >= p.F) return;
   const float* s = p.part + 4 * id;
   f4 v = *reinterpret_cast<const f4*>(s);
   for (int k = 1; k < p.splits; ++k) v += *reinterpret_cast<const f4*>(s + 4 * k * quads);
-  store_up_to4(static_cast<T*>(m < p.Fp ? p.dwg : p.dwu) + (long long)f * p.D + n, p.D - n, v);
+  T* to = static_cast<T*>(JOB == Job::Dx ? p.dx : m < p.Fp ? p.dwg : p.dwu);
+  store_up_to4(to + (long long)f * p.D + n, p.D - n, v);
 }
 template <typename T> __global__ __launch_bounds__(256) void ffn_bias_kernel(FfnParams p) {
   const int n = 2 * p.Fp, c = blockIdx.x * 16 + (threadIdx.x & 15);
@@ -410,18 +408,21 @@ template <typename T, Job JOB, int WN, int WM, int TN, int TM> hipError_t tile_t
   if (e != hipSuccess) return e;
   constexpr bool up = JOB == Job::Fwd || JOB == Job::Grad;
   const long long M = JOB == Job::Dw ? 2LL * p.Fp : p.R, N = up ? 2LL * p.F : p.D;
-  const long long blocks = ((M + BM - 1) / BM) * ((N + BN - 1) / BN) * (JOB == Job::Dw ? p.splits : 1);
+  const long long blocks = ((M + BM - 1) / BM) * ((N + BN - 1) / BN) * p.splits;
   hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(64 * WN * WM), lds, s, p);
+  if (p.splits > 1) {
+    const long long quads = M * p.Dp / 4;
+    hipLaunchKernelGGL((ffn_join_kernel<T, JOB>), dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, s, p, quads);
+  }
   return hipGetLastError();
 }
-template <typename T, Job JOB> hipError_t job_t(const FfnParams& p, hipStream_t s) {
-  constexpr bool up = JOB == Job::Fwd || JOB == Job::Grad;
-  const long long M = JOB == Job::Dw ? 2LL * p.Fp : p.R, N = up ? 2LL * p.F : p.D;
-  return ffn_large(M, N) ? tile_t<T, JOB, 4, 2, 4, 8>(p, s) : tile_t<T, JOB, 2, 2, 4, 4>(p, s);
+template <typename T, Job JOB> hipError_t job_t(const FfnParams& p, bool large, hipStream_t s) {
+  return large ? tile_t<T, JOB, 4, 2, 4, 8>(p, s) : tile_t<T, JOB, 2, 2, 4, 4>(p, s);
 }
-template <Job JOB> hipError_t type_t(const FfnParams& p, int dtype, hipStream_t s) {
-  return dtype == TTT_DTYPE_BF16 ? job_t<__bf16, JOB>(p, s)
-         : dtype == TTT_DTYPE_F16 ? job_t<_Float16, JOB>(p, s) : job_t<float, JOB>(p, s);
+template <Job JOB> hipError_t type_t(FfnParams p, FfnCut cut, int dtype, hipStream_t s) {
+  p.splits = cut.splits;
+  return dtype == TTT_DTYPE_BF16 ? job_t<__bf16, JOB>(p, cut.large, s)
+         : dtype == TTT_DTYPE_F16 ? job_t<_Float16, JOB>(p, cut.large, s) : job_t<float, JOB>(p, cut.large, s);
 }
 
 template <typename T> hipError_t few_t(const FfnParams& p, hipStream_t s) {
@@ -430,11 +431,6 @@ template <typename T> hipError_t few_t(const FfnParams& p, hipStream_t s) {
     hipLaunchKernelGGL((ffn_few_kernel<T, 1>), dim3(cols), dim3(64 * kFewWaves), 0, s, p);
   else
     hipLaunchKernelGGL((ffn_few_kernel<T, 2>), dim3(cols, (unsigned)((p.R + 31) / 32)), dim3(64 * kFewWaves), 0, s, p);
-  return hipGetLastError();
-}
-template <typename T> hipError_t join_t(const FfnParams& p, hipStream_t s) {
-  const long long quads = 2LL * p.Fp * p.Dp / 4;
-  hipLaunchKernelGGL(ffn_join_kernel<T>, dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, s, p, quads);
   return hipGetLastError();
 }
 template <typename T> hipError_t bias_t(const FfnParams& p, hipStream_t s) {
@@ -452,30 +448,20 @@ hipError_t planes_t(const void* from, long long ld, int rows, int width, void* t
 
 }  // namespace
 
-// Shares of the rows that dW contracts over: its tiles times these make whole rounds of the
-// card, each share 512 rows or more
-int ffn_splits(int R, int D, int F, int dtype) {
-  const long long M = 2LL * ffn_pad(F), N = D;
-  const bool large = ffn_large(M, N);
-  const long long b = large ? 256 : 128, tiles = ((M + b - 1) / b) * ((N + b - 1) / b), places = large ? 256 : 512;
-  const long long most = std::max<long long>(1, (R + 511) / 512);
-  return (int)std::max<long long>(1, std::min(most, places / tiles));
-}
-
 hipError_t launch_ffn_few(const FfnParams& p, int dtype, hipStream_t s) {
   return dtype == TTT_DTYPE_BF16 ? few_t<__bf16>(p, s) : dtype == TTT_DTYPE_F16 ? few_t<_Float16>(p, s) : few_t<float>(p, s);
 }
-hipError_t launch_ffn_fwd(const FfnParams& p, int dtype, hipStream_t s) { return type_t<Job::Fwd>(p, dtype, s); }
+hipError_t launch_ffn_fwd(const FfnParams& p, int dtype, hipStream_t s) { return type_t<Job::Fwd>(p, ffn_cut_up(p.R, p.D, p.F, dtype), dtype, s); }
 hipError_t launch_ffn_grad(const FfnParams& p, int dtype, hipStream_t s) {
-  const hipError_t e = type_t<Job::Grad>(p, dtype, s);
+  const hipError_t e = type_t<Job::Grad>(p, ffn_cut_up(p.R, p.D, p.F, dtype), dtype, s);
   if (e != hipSuccess || p.bias_part == nullptr) return e;
   return dtype == TTT_DTYPE_BF16 ? bias_t<__bf16>(p, s) : dtype == TTT_DTYPE_F16 ? bias_t<_Float16>(p, s) : bias_t<float>(p, s);
 }
-hipError_t launch_ffn_dx(const FfnParams& p, int dtype, hipStream_t s) { return type_t<Job::Dx>(p, dtype, s); }
+hipError_t launch_ffn_dx(const FfnParams& p, int dtype, hipStream_t s) {
+  return type_t<Job::Dx>(p, ffn_cut_dx(p.R, p.D, p.F, dtype), dtype, s);
+}
 hipError_t launch_ffn_dw(const FfnParams& p, int dtype, hipStream_t s) {
-  const hipError_t e = type_t<Job::Dw>(p, dtype, s);
-  if (e != hipSuccess || p.part == nullptr) return e;
-  return dtype == TTT_DTYPE_BF16 ? join_t<__bf16>(p, s) : dtype == TTT_DTYPE_F16 ? join_t<_Float16>(p, s) : join_t<float>(p, s);
+  return type_t<Job::Dw>(p, ffn_cut_dw(p.R, p.D, p.F, dtype), dtype, s);
 }
 hipError_t launch_ffn_planes(const void* from, long long ld, int rows, int width, void* to, int dtype, hipStream_t s) {
   return dtype == TTT_DTYPE_BF16 ? planes_t<__bf16>(from, ld, rows, width, to, s)
