@@ -64,20 +64,28 @@ enum class Job { Fwd, Grad, Dx, Dw };
 enum class Lies { Contracted, Free };
 
 // A step's part of an operand in LDS: FREE rows of 64 contracted values, or 64 rows of FREE
-template <Lies L, int FREE> struct Panel {
-  static constexpr int PIECES = L == Lies::Contracted ? 8 : FREE / 8;  // of 16 bytes, to a row
+// (SIDE of an operand: the first's free values go to a lane's registers, eight neighbours of
+// a pair of tiles, so that results are read and written 16 bytes a lane; the second's to lanes)
+enum class Side { First, Second };
+template <Lies L, Side S, int FREE> struct Panel {
+  static constexpr int PIECES = (L == Lies::Contracted ? kFfnStep : FREE) / 8;  // of 16 bytes, to a row
   static constexpr int ROWS = L == Lies::Contracted ? FREE : kFfnStep;
   static constexpr int BYTES = FREE * kFfnStep * 2;
+  // the rows that are read at once: 0..7 of eight, or of the first operand 0..3 and 8..11 of
+  // sixteen; of free values the four of a transposing read, whose lanes have 32 or 64 bytes of each
   __device__ __forceinline__ static int place(int row, int piece) {
-    return L == Lies::Contracted ? piece ^ (row & 7) : piece ^ ((row & 7) << 1);
+    if constexpr (L == Lies::Contracted)
+      return piece ^ (S == Side::First ? (row & 3) | ((row >> 1) & 4) : row & 7);
+    else
+      return piece ^ (S == Side::First ? (row & 3) << 2 : (row & 7) << 1);
   }
 };
 
 // Sends the step's rows of a matrix on their way to LDS.  `base`: the panel's first value;
 // `rows` and `pieces` of it are in the matrix (whole rows `ld` bytes apart).
-template <Lies L, int FREE, int NW>
+template <Lies L, Side S, int FREE, int NW>
 __device__ __forceinline__ void send(const char* base, long long ld, int rows, int pieces, unsigned char* lds, int w) {
-  using P = Panel<L, FREE>;
+  using P = Panel<L, S, FREE>;
   constexpr int CNT = P::BYTES / 1024 / NW;
   static_assert(CNT * NW * 1024 == P::BYTES, "whole kilobytes to a wave");
   const int l = lane_id();
@@ -92,16 +100,21 @@ __device__ __forceinline__ void send(const char* base, long long ld, int rows, i
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(lds + (i * NW + w) * 1024), 16, (int)off, 0, 0, 0);
   }
 }
-// A panel's operands of the free values 16 t.. and contracted values 32 k.. + 8g + (0..7)
-template <Lies L, int FREE> __device__ __forceinline__ bf8 take(const unsigned char* lds, int t, int k) {
+// A panel's operands of a tile's 16 free values and contracted values 32 k.. + 8g + (0..7).
+// Tile t of the second operand has the free values 16 t + r; of the first, two tiles have 32, the
+// even one 8 (r >> 2) + (r & 3) of them and the odd one those 4 behind.
+template <Lies L, Side S, int FREE> __device__ __forceinline__ bf8 take(const unsigned char* lds, int t, int k) {
+  using P = Panel<L, S, FREE>;
   const int l = lane_id(), g = l >> 4, r = l & 15;
   if constexpr (L == Lies::Contracted) {
-    const int row = 16 * t + r;
-    return *reinterpret_cast<const bf8*>(lds + row * 128 + (((4 * k + g) ^ (r & 7)) << 4));
+    const int row = S == Side::First ? 32 * (t >> 1) + 8 * (r >> 2) + 4 * (t & 1) + (r & 3) : 16 * t + r;
+    return *reinterpret_cast<const bf8*>(lds + row * kFfnStep * 2 + (P::place(row, 4 * k + g) << 4));
   } else {
-    const int row = 32 * k + 8 * g + (r >> 2), piece = 2 * t + ((l & 3) >> 1);
+    const int row = 32 * k + 8 * g + (r >> 2);
+    const int piece = S == Side::First ? 4 * (t >> 1) + (l & 3) : 2 * t + ((l & 3) >> 1);
+    const int half = S == Side::First ? t & 1 : l & 1;
     const auto at = [&](int rw) {
-      return reinterpret_cast<const __bf16*>(lds + rw * FREE * 2 + ((piece ^ ((rw & 7) << 1)) << 4) + (l & 1) * 8);
+      return reinterpret_cast<const __bf16*>(lds + rw * FREE * 2 + (P::place(rw, piece) << 4) + half * 8);
     };
     return cat(read_tr(at(row)), read_tr(at(row + 4)));
   }
@@ -117,16 +130,15 @@ template <typename T> __device__ __forceinline__ void store_up_to4(T* p, int n, 
   const float o[4] = {v[0], v[1], v[2], v[3]};
   store_row<T, 4>(p, n, o);
 }
-// da or db, in planes where T is fp32
-template <typename T> __device__ __forceinline__ void store_grad(const FfnMatrix& m, long long row, int col, f4 v) {
+// eight values of da or db, in planes where T is fp32
+template <typename T> __device__ __forceinline__ void store_grad(const FfnMatrix& m, long long row, int col, const float (&v)[8]) {
   char* to = static_cast<char*>(const_cast<void*>(m.p)) + row * m.ld + col * 2;
   if constexpr (sizeof(T) == 4) {
-    bf4 o[3];
-    split4<3>(v, o);
+    const Op<3> o = split8<3>(f4{v[0], v[1], v[2], v[3]}, f4{v[4], v[5], v[6], v[7]});
 #pragma unroll
-    for (int a = 0; a < 3; ++a) *reinterpret_cast<bf4*>(to + a * m.plane) = o[a];
+    for (int a = 0; a < 3; ++a) *reinterpret_cast<bf8*>(to + a * m.plane) = o.v[a];
   } else {
-    store4(reinterpret_cast<T*>(to), v);
+    store_row<T, 8>(reinterpret_cast<T*>(to), 8, v);
   }
 }
 
@@ -138,7 +150,7 @@ __global__ __launch_bounds__(64 * WN * WM) void ffn_kernel(FfnParams p) {
   constexpr bool UP = JOB == Job::Fwd || JOB == Job::Grad;  // both projections' columns in a tile
   constexpr Lies LN = UP ? Lies::Contracted : Lies::Free, LM = JOB == Job::Dw ? Lies::Free : Lies::Contracted;
   constexpr int BN = 16 * WN * TN, BM = 16 * WM * TM, NW = WN * WM, HALF = BN / 2;
-  constexpr int STEP = Panel<LN, BN>::BYTES + Panel<LM, BM>::BYTES;
+  constexpr int STEP = Panel<LN, Side::First, BN>::BYTES + Panel<LM, Side::Second, BM>::BYTES;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int w = wave_id(), l = lane_id(), g = l >> 4, r = l & 15, wn = w % WN, wm = w / WN;
   // rows and columns of all tiles, and contracted values
@@ -166,22 +178,22 @@ __global__ __launch_bounds__(64 * WN * WM) void ffn_kernel(FfnParams p) {
     if constexpr (UP) {
       const int pieces = left / 8;
       const long long a = pa * p.wg.plane + (long long)n0 * p.wg.ld + k * 2;
-      send<LN, HALF, NW>(static_cast<const char*>(p.wg.p) + a, p.wg.ld, N - n0, pieces, to, w);
-      send<LN, HALF, NW>(static_cast<const char*>(p.wu.p) + a, p.wu.ld, N - n0, pieces, to + HALF * kFfnStep * 2, w);
-      send<LM, BM, NW>(static_cast<const char*>(p.x.p) + pb * p.x.plane + (long long)m0 * p.x.ld + k * 2, p.x.ld, M - m0,
-                       pieces, to + Panel<LN, BN>::BYTES, w);
+      send<LN, Side::First, HALF, NW>(static_cast<const char*>(p.wg.p) + a, p.wg.ld, N - n0, pieces, to, w);
+      send<LN, Side::First, HALF, NW>(static_cast<const char*>(p.wu.p) + a, p.wu.ld, N - n0, pieces, to + HALF * kFfnStep * 2, w);
+      send<LM, Side::Second, BM, NW>(static_cast<const char*>(p.x.p) + pb * p.x.plane + (long long)m0 * p.x.ld + k * 2, p.x.ld, M - m0,
+                       pieces, to + Panel<LN, Side::First, BN>::BYTES, w);
     } else if constexpr (JOB == Job::Dx) {
       const FfnMatrix& wt = ss == 0 ? p.wg : p.wu;
-      send<LN, BN, NW>(static_cast<const char*>(wt.p) + pa * wt.plane + (long long)k * wt.ld + n0 * 2, wt.ld, p.F - k,
+      send<LN, Side::First, BN, NW>(static_cast<const char*>(wt.p) + pa * wt.plane + (long long)k * wt.ld + n0 * 2, wt.ld, p.F - k,
                        (p.Dp - n0) / 8, to, w);
-      send<LM, BM, NW>(static_cast<const char*>(p.grad.p) + pb * p.grad.plane + (long long)m0 * p.grad.ld +
+      send<LM, Side::Second, BM, NW>(static_cast<const char*>(p.grad.p) + pb * p.grad.plane + (long long)m0 * p.grad.ld +
                            ((long long)ss * p.Fp + k) * 2,
-                       p.grad.ld, M - m0, left / 8, to + Panel<LN, BN>::BYTES, w);
+                       p.grad.ld, M - m0, left / 8, to + Panel<LN, Side::First, BN>::BYTES, w);
     } else {
-      send<LN, BN, NW>(static_cast<const char*>(p.x.p) + pa * p.x.plane + (long long)k * p.x.ld + n0 * 2, p.x.ld, left,
+      send<LN, Side::First, BN, NW>(static_cast<const char*>(p.x.p) + pa * p.x.plane + (long long)k * p.x.ld + n0 * 2, p.x.ld, left,
                        (p.Dp - n0) / 8, to, w);
-      send<LM, BM, NW>(static_cast<const char*>(p.grad.p) + pb * p.grad.plane + (long long)k * p.grad.ld + m0 * 2, p.grad.ld,
-                       left, (M - m0) / 8, to + Panel<LN, BN>::BYTES, w);
+      send<LM, Side::Second, BM, NW>(static_cast<const char*>(p.grad.p) + pb * p.grad.plane + (long long)k * p.grad.ld + m0 * 2, p.grad.ld,
+                       left, (M - m0) / 8, to + Panel<LN, Side::First, BN>::BYTES, w);
     }
     if (++sk == ksteps) {
       sk = 0;
@@ -211,9 +223,9 @@ __global__ __launch_bounds__(64 * WN * WM) void ffn_kernel(FfnParams p) {
     for (int k = 0; k < kFfnStep / 32; ++k) {
       bf8 pn[TN], pm[TM];
 #pragma unroll
-      for (int i = 0; i < TN; ++i) pn[i] = take<LN, BN>(at, tile_n(i), k);
+      for (int i = 0; i < TN; ++i) pn[i] = take<LN, Side::First, BN>(at, tile_n(i), k);
 #pragma unroll
-      for (int j = 0; j < TM; ++j) pm[j] = take<LM, BM>(at + Panel<LN, BN>::BYTES, wm * TM + j, k);
+      for (int j = 0; j < TM; ++j) pm[j] = take<LM, Side::Second, BM>(at + Panel<LN, Side::First, BN>::BYTES, wm * TM + j, k);
 #pragma unroll
       for (int j = 0; j < TM; ++j)
 #pragma unroll
@@ -221,70 +233,88 @@ __global__ __launch_bounds__(64 * WN * WM) void ffn_kernel(FfnParams p) {
     }
   }
 
+  // A pair of tiles' columns are eight neighbours in a lane: 8g + 4i + e of 32
   if constexpr (UP) {
 #pragma unroll
-    for (int i = 0; i < TN / 2; ++i) {
-      const int f = n0 + 16 * (wn * (TN / 2) + i) + 4 * g, left = N - f;
-      f4 bg = f4{0.f, 0.f, 0.f, 0.f}, bu = bg, sg = bg, su = bg;
-      if (p.bg != nullptr && left > 0) bg = load_up_to4(static_cast<const T*>(p.bg) + f, left);
-      if (p.bu != nullptr && left > 0) bu = load_up_to4(static_cast<const T*>(p.bu) + f, left);
+    for (int i = 0; i < TN / 2; i += 2) {
+      const int f = n0 + 16 * (wn * (TN / 2) + i) + 8 * g, left = N - f;
+      Raw<T, 8> bg, bu;
+      bg.zero();
+      bu.zero();
+      if (p.bg != nullptr && left > 0) bg.load(static_cast<const T*>(p.bg) + f, left);
+      if (p.bu != nullptr && left > 0) bu.load(static_cast<const T*>(p.bu) + f, left);
+      float sg[8], su[8];
+      Raw<T, 8> dy[JOB == Job::Grad ? TM : 1];
+      if constexpr (JOB == Job::Grad) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sg[e] = su[e] = 0.f;
+#pragma unroll
+        for (int j = 0; j < TM; ++j) {
+          const int m = m0 + 16 * (wm * TM + j) + r;
+          dy[j].zero();
+          if (m < M && left > 0) dy[j].load(static_cast<const T*>(p.dy) + (long long)m * p.lddy + f, left);
+        }
+      }
 #pragma unroll
       for (int j = 0; j < TM; ++j) {
         const int m = m0 + 16 * (wm * TM + j) + r;
-        const f4 a = acc[i][j] + bg, b = acc[TN / 2 + i][j] + bu;
-        if constexpr (JOB == Job::Fwd) {
-          f4 y;
-          float d;
+        float u[8], v[8];  // y; or da and db
 #pragma unroll
-          for (int e = 0; e < 4; ++e) y[e] = act_value<false>(p.act, a[e], d) * b[e];
-          if (m < M && left > 0) store_up_to4(static_cast<T*>(p.y) + (long long)m * p.F + f, left, y);
-        } else {
-          if (m < M && f < p.Fp) {
-            f4 dy = f4{0.f, 0.f, 0.f, 0.f}, da, db;
-            if (left > 0) dy = load_up_to4(static_cast<const T*>(p.dy) + (long long)m * p.lddy + f, left);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              float d;
-              db[e] = dy[e] * act_value<true>(p.act, a[e], d);
-              da[e] = dy[e] * b[e] * d;
-              if (e >= left) da[e] = db[e] = 0.f;
-            }
-            store_grad<T>(p.grad, m, f, da);
-            store_grad<T>(p.grad, m, p.Fp + f, db);
-            sg += da;
-            su += db;
+        for (int e = 0; e < 8; ++e) {
+          const float a = acc[i + e / 4][j][e & 3] + bg.f(e), b = acc[TN / 2 + i + e / 4][j][e & 3] + bu.f(e);
+          if constexpr (JOB == Job::Fwd) {
+            float d;
+            u[e] = act_value<false>(p.act, a, d) * b;
+          } else {
+            // (0 past the last row and column: nothing from there reaches the sums)
+            float d;
+            const float y = dy[j].f(e), f = act_value<true>(p.act, a, d);
+            const bool in = m < M && e < left;
+            v[e] = in ? y * f : 0.f;
+            u[e] = in ? y * b * d : 0.f;
+            sg[e] += u[e];
+            su[e] += v[e];
           }
+        }
+        if constexpr (JOB == Job::Fwd) {
+          if (m < M && left > 0) store_row<T, 8>(static_cast<T*>(p.y) + (long long)m * p.F + f, left, u);
+        } else if (m < M && f < p.Fp) {
+          store_grad<T>(p.grad, m, f, u);
+          store_grad<T>(p.grad, m, p.Fp + f, v);
         }
       }
       if (JOB == Job::Grad && p.bias_part != nullptr) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < 8; ++e) {
           sg[e] = sum_row16(sg[e]);
           su[e] = sum_row16(su[e]);
         }
         if (r == 0 && f < p.Fp) {
           float* to = p.bias_part + (long long)(m0 / BM * WM + wm) * 2 * p.Fp + f;
-          *reinterpret_cast<f4*>(to) = sg;
-          *reinterpret_cast<f4*>(to + p.Fp) = su;
+          store_row<float, 8>(to, 8, sg);
+          store_row<float, 8>(to + p.Fp, 8, su);
         }
       }
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < TN; ++i) {
-      const int n = n0 + 16 * (wn * TN + i) + 4 * g, left = N - n;
+    for (int i = 0; i < TN; i += 2) {
+      const int n = n0 + 16 * (wn * TN + i) + 8 * g, left = N - n;
       if (left <= 0) continue;
 #pragma unroll
       for (int j = 0; j < TM; ++j) {
         const int m = m0 + 16 * (wm * TM + j) + r;
         if (m >= M) continue;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = acc[i + e / 4][j][e & 3];
         if (p.splits > 1) {
-          *reinterpret_cast<f4*>(p.part + ((long long)split * M + m) * p.Dp + n) = acc[i][j];
+          store_row<float, 8>(p.part + ((long long)split * M + m) * p.Dp + n, 8, v);
         } else if constexpr (JOB == Job::Dx) {
-          store_up_to4(static_cast<T*>(p.dx) + (long long)m * p.D + n, left, acc[i][j]);
+          store_row<T, 8>(static_cast<T*>(p.dx) + (long long)m * p.D + n, left, v);
         } else {
           const int f = m < p.Fp ? m : m - p.Fp;
-          if (f < p.F) store_up_to4(static_cast<T*>(m < p.Fp ? p.dwg : p.dwu) + (long long)f * p.D + n, left, acc[i][j]);
+          if (f < p.F) store_row<T, 8>(static_cast<T*>(m < p.Fp ? p.dwg : p.dwu) + (long long)f * p.D + n, left, v);
         }
       }
     }
