@@ -2,6 +2,7 @@
 // and workspace layout, then launches on the caller's stream.  Declarations and argument
 // contracts are in include/ttt_amd.h.
 #include <stdint.h>
+#include <stdlib.h>
 
 #include <algorithm>
 
@@ -23,28 +24,35 @@ int check_delta(int B, int L, int H, int P, int G, int N, int dtype, int g_dtype
   return TTT_OK;
 }
 struct DeltaPlan {
-  int Q, NC, PB, parts, share;
-  size_t tok, zm, states, rows, qk, gb;
+  int Q, NC, share, S, per;
+  size_t tok, zm, states, rows, qk, seg, trans;
 };
+// Segments that the tokens are cut into: as many as make the walk quickest.
+int delta_segments(long long heads, int P, int NP, int NC) {
+  if (const char* e = getenv("DSEG")) return std::max(1, std::min(NC, atoi(e)));
+  return 1;
+}
 DeltaPlan delta_plan(int B, int L, int H, int P, int G, int N, int dtype) {
   DeltaPlan s;
   s.Q = ttt::delta_chunk(dtype);
   s.NC = (L + s.Q - 1) / s.Q;
-  s.PB = ttt::delta_part(P);
-  s.parts = P / s.PB;
-  s.share = H / G * s.parts;
+  s.share = H / G;
   const size_t chunks = (size_t)B * H * s.NC;
   s.tok = up256(chunks * ttt::delta_tok_floats(s.Q) * 4);
   s.zm = chunks * ttt::delta_tiles(s.Q) * 1024;
   s.states = chunks * P * ttt::scan_padded(N) * 4;
   s.rows = chunks * P * s.Q * 4;
   s.qk = s.share > 1 ? (size_t)s.share * B * L * G * N * 4 : 0;
-  s.gb = s.parts > 1 ? up256((size_t)s.parts * B * L * H * 4) : 0;
+  const int NP = ttt::scan_padded(N), want = delta_segments((long long)B * H, P, NP, s.NC);
+  s.per = (s.NC + want - 1) / want;
+  s.S = (s.NC + s.per - 1) / s.per;
+  s.seg = s.S > 1 ? (size_t)B * H * s.S * NP * P * 4 : 0;
+  s.trans = s.S > 1 ? (size_t)B * H * s.S * NP * NP * 4 : 0;
   return s;
 }
 bool delta_grid_ok(const DeltaPlan& s, int B, int H, int P) {
-  // (prep: 256 threads a chunk and head; walk: four for a feature and sequence; gradients: 512 a chunk and part)
-  return (long long)B * H * P <= kMaxThreads / 4 && (long long)B * H <= kMaxThreads / 512 / s.NC / s.parts;
+  // (prep: 256 threads a chunk and head; walk: four for a feature and sequence; gradients: 512 a chunk and head)
+  return (long long)B * H * (P + 128) <= kMaxThreads / 4 / s.S && (long long)B * H <= kMaxThreads / 512 / s.NC;
 }
 bool delta_plan_ok(int B, int L, int H, int P, int G, int N, int dtype, DeltaPlan& s) {
   if (check_delta(B, L, H, P, G, N, dtype, dtype, dtype) != TTT_OK) return false;
@@ -341,11 +349,11 @@ size_t ttt_delta_saved_bytes(int B, int L, int H, int P, int N, int dtype) {
 }
 size_t ttt_delta_workspace_bytes(int B, int L, int H, int P, int N, int dtype) {
   DeltaPlan s;
-  return delta_plan_ok(B, L, H, P, 1, N, dtype, s) ? s.tok + 2 * s.zm : 0;
+  return delta_plan_ok(B, L, H, P, 1, N, dtype, s) ? s.tok + 2 * s.zm + s.seg + s.trans : 0;
 }
 size_t ttt_delta_bwd_workspace_bytes(int B, int L, int H, int P, int G, int N, int dtype) {
   DeltaPlan s;
-  return delta_plan_ok(B, L, H, P, G, N, dtype, s) ? s.tok + 2 * s.zm + s.states + s.rows + 2 * s.gb + 2 * s.qk : 0;
+  return delta_plan_ok(B, L, H, P, G, N, dtype, s) ? s.tok + 2 * s.zm + s.states + s.rows + 2 * s.qk + s.seg + s.trans : 0;
 }
 
 int ttt_delta_fwd(const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv,
@@ -371,7 +379,7 @@ int ttt_delta_fwd(const void* q, long long ldq, const void* k, long long ldk, co
   OPTIONAL(h_last, 16);
   OPTIONAL(saved, 16);
   if (saved != nullptr && saved_bytes < s.states + s.rows) return TTT_ERR_WORKSPACE;
-  if (workspace == nullptr || workspace_bytes < s.tok + 2 * s.zm) return TTT_ERR_WORKSPACE;
+  if (workspace == nullptr || workspace_bytes < s.tok + 2 * s.zm + s.seg + s.trans) return TTT_ERR_WORKSPACE;
   OPTIONAL(workspace, 16);
   ttt::DeltaParams p{};
   p.q = q;
@@ -401,6 +409,12 @@ int ttt_delta_fwd(const void* q, long long ldq, const void* k, long long ldk, co
   p.tok = reinterpret_cast<float*>(ws);
   p.z = reinterpret_cast<float*>(ws + s.tok);
   p.m = reinterpret_cast<float*>(ws + s.tok + s.zm);
+  p.S = s.S;
+  p.per = s.per;
+  if (s.S > 1) {
+    p.seg = reinterpret_cast<float*>(ws + s.tok + 2 * s.zm);
+    p.trans = reinterpret_cast<float*>(ws + s.tok + 2 * s.zm + s.seg);
+  }
   if (saved != nullptr) {
     p.states = static_cast<float*>(saved);
     p.rows = reinterpret_cast<float*>(static_cast<char*>(saved) + s.states);
@@ -438,7 +452,7 @@ int ttt_delta_bwd(const void* q, long long ldq, const void* k, long long ldk, co
   OPTIONAL(dh0, 16);
   if (saved_bytes < s.states + s.rows) return TTT_ERR_WORKSPACE;
   if (workspace == nullptr ||
-      workspace_bytes < s.tok + 2 * s.zm + s.states + s.rows + 2 * s.gb + 2 * s.qk)
+      workspace_bytes < s.tok + 2 * s.zm + s.states + s.rows + 2 * s.qk + s.seg + s.trans)
     return TTT_ERR_WORKSPACE;
   OPTIONAL(workspace, 16);
   ttt::DeltaParams p{};
@@ -476,9 +490,11 @@ int ttt_delta_bwd(const void* q, long long ldq, const void* k, long long ldk, co
   p.m = reinterpret_cast<float*>(take(s.zm));
   p.states = reinterpret_cast<float*>(take(s.states));
   p.rows = reinterpret_cast<float*>(take(s.rows));
-  if (s.parts > 1) {
-    p.dgp = reinterpret_cast<float*>(take(s.gb));
-    p.dbp = reinterpret_cast<float*>(take(s.gb));
+  p.S = s.S;
+  p.per = s.per;
+  if (s.S > 1) {
+    p.seg = reinterpret_cast<float*>(take(s.seg));
+    p.trans = reinterpret_cast<float*>(take(s.trans));
   }
   if (s.share > 1) {
     p.dqp = reinterpret_cast<float*>(take(s.qk));

@@ -43,8 +43,10 @@ struct DeltaParams {
   float* states;          // [B*H*parts][NC][NP][PB]: the states entering the chunks, or walking back the
                           // gradients of those leaving them (may be null)
   float* rows;            // [B*H*parts][NC*Q][PB]: x, or walking back y (may be null)
+  float *seg, *trans;     // [B*H*parts][S][NP][PB] and [B*H][S][NP][NP]: per segment of the sequence
   long long ldq, ldk, ldv, ldg, ldbeta;
   int B, L, H, G, N, P;
+  int S, per;             // segments, and chunks in one
   float scale;
   bool l2, g_f32, beta_f32;
   // backward
@@ -52,8 +54,7 @@ struct DeltaParams {
   long long lddo;
   const float *gstates, *x;    // what the walk back and the forward's walk kept
   void *dq, *dk, *dg, *dbeta;  // [B][L][G][N] and [B][L][H]
-  float *dqp, *dkp;            // [H/G*parts][B*L][G][N] where heads or parts share q and k, else null
-  float *dgp, *dbp;            // [parts][B*L][H] where there is more than one, else null
+  float *dqp, *dkp;            // [H/G][B*L][G][N] where heads share q and k, else null
 };
 hipError_t launch_delta_fwd(const DeltaParams& p, int dtype, hipStream_t stream);
 hipError_t launch_delta_walk_back(const DeltaParams& p, int dtype, hipStream_t stream);

@@ -2,7 +2,7 @@
 // gradients of q, k, the decays and b (mathematics: ttt_delta.h).
 //
 // Given the states S entering the chunks and x (kept by the forward), and the gradients dS'
-// of those leaving them, y and dv = b y (kept by the walk back), every chunk of a part stands
+// of those leaving them, y and dv = b y (kept by the walk back), every chunk of a head stands
 // alone.  With u = b x, h_i = e^{c_i}, w_j = e^{c_Q - c_j}, and q, k at unit length or as they are:
 //   X_ij = s F_ij (do_i . u_j), j <= i;   Y_ij = -F_ij (dv_i . u_j), j < i
 //   dq_i = s h_i S^T do_i + sum_j X_ij k_j
@@ -18,6 +18,9 @@
 // that the products take the raw rows; what comes out is dq rq and dk rk, and
 //   dq <- dq - rq^2 (q . dq) q
 // is the gradient of the raw rows.
+//
+// A workgroup has a chunk of one head.  32 features of do, u and dv are in LDS at once, the next
+// 32 on their way, with the sums over the features in registers: two workgroups to a compute unit.
 #include <math.h>
 #include <stddef.h>
 
@@ -27,38 +30,41 @@ namespace ttt {
 
 namespace {
 
-template <typename T, int PB, int NP> struct GradShared {
+constexpr int kSlice = 32;  // features that are in LDS at once
+
+template <typename T, int NP> struct GradShared {
   static constexpr int IN = ScanType<T>::IN, MID = ScanType<T>::MID, Q = kDeltaQ<T>, TB = Q / 16;
-  static constexpr int TILES = TB * (TB + 1) / 2, NB = NP / 16;
+  static constexpr int TILES = delta_tiles(Q), NB = NP / 16;
   static constexpr int WAVES = NB * TB < 8 ? NB * TB : 8;
   Planes<IN, Q, NP> q, k;
-  Planes<IN, Q, PB> dO;
-  Planes<kFull, Q, PB> u, dv;
-  bf4 x[MID][TILES][64], y[MID][TILES][64];
+  union {
+    struct {
+      Planes<IN, Q, kSlice> dO;
+      Planes<kFull, Q, kSlice> u, dv;
+    };
+    struct {  // behind the slices
+      bf4 x[MID][TILES][64], y[MID][TILES][64];
+      float a[NB][Q], d[NB][Q];    // by blocks of columns
+      float qd[NB][Q], kd[NB][Q];  // q . dq and k . dk
+    };
+  };
   DeltaTok<Q> tok;
   float row[TILES][16], col[TILES][16];  // of X (q . k) + Y (k . k)
-  float a[NB][Q], d[NB][Q];              // by blocks of columns
-  float qd[NB][Q], kd[NB][Q];            // q . dq and k . dk
   float db[Q], gh[WAVES];
 };
 
-// Columns n = 16 nb + r of a state [NP][P] in memory, all P values of them: lane (g, r) has
-// values 32k + 8g + e of column r
-template <int P> struct Columns {
-  static constexpr int K = P / 32;
-  f4 v[K][2];
-  __device__ __forceinline__ void load(const float* __restrict__ s, int nb) {
+// 32 features of columns n = 16 nb + r of a state [NP][PB] in memory: lane (g, r) has values
+// 8g + e of column r
+struct Columns {
+  f4 v[2];
+  __device__ __forceinline__ void load(const float* __restrict__ s, int ld, int nb) {
     const int l = lane_id(), g = l >> 4, r = l & 15;
 #pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-      for (int o = 0; o < 2; ++o) v[k][o] = *reinterpret_cast<const f4*>(s + (16 * nb + r) * P + 32 * k + 8 * g + 4 * o);
+    for (int o = 0; o < 2; ++o) v[o] = *reinterpret_cast<const f4*>(s + (16 * nb + r) * ld + 8 * g + 4 * o);
   }
-  __device__ __forceinline__ Op<kFull> op(int k) const { return split8<kFull>(v[k][0], v[k][1]); }
+  __device__ __forceinline__ Op<kFull> op() const { return split8<kFull>(v[0], v[1]); }
   __device__ __forceinline__ float dot(const Columns& o) const {
-    f4 s = f4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int k = 0; k < K; ++k) s += v[k][0] * o.v[k][0] + v[k][1] * o.v[k][1];
+    const f4 s = v[0] * o.v[0] + v[1] * o.v[1];
     return (s[0] + s[1]) + (s[2] + s[3]);
   }
 };
@@ -71,96 +77,131 @@ template <typename T> __device__ __forceinline__ void put(void* to, bool f32, lo
     static_cast<T*>(to)[o] = (T)v;
 }
 
-template <typename T, int PB, int NP>
-__global__ __launch_bounds__((64 * GradShared<T, PB, NP>::WAVES)) void delta_bwd_kernel(DeltaParams p) {
-  using Sh = GradShared<T, PB, NP>;
+template <typename T, int NP>
+__global__ __launch_bounds__((64 * GradShared<T, NP>::WAVES), (NP == 128 && ScanType<T>::IN != 2 ? 2 : 4)) void delta_bwd_kernel(DeltaParams p) {
+  using Sh = GradShared<T, NP>;
   static_assert(offsetof(Sh, tok) % 16 == 0 && offsetof(Sh, x) % 16 == 0 && offsetof(Sh, y) % 16 == 0 &&
                     offsetof(Sh, k) % 16 == 0 && offsetof(Sh, dO) % 16 == 0 && offsetof(Sh, u) % 16 == 0 &&
                     offsetof(Sh, dv) % 16 == 0 && offsetof(Sh, row) % 16 == 0,
                 "read 16 bytes at a time");
   constexpr int IN = Sh::IN, MID = Sh::MID, Q = Sh::Q, TB = Sh::TB, QB = Q / 32, TILES = Sh::TILES, NB = Sh::NB;
-  constexpr int WAVES = Sh::WAVES, NT = 64 * WAVES, NC2 = NP / 32, PC = PB / 32;
+  constexpr int WAVES = Sh::WAVES, NT = 64 * WAVES, NC2 = NP / 32, OWN = (TILES + WAVES - 1) / WAVES;
   // a wave has a block of 16 columns and every SHARE-th block of 16 tokens
   constexpr int SHARE = WAVES / NB, TOK = TB / SHARE;
   static_assert(SHARE * NB == WAVES && TOK * SHARE == TB, "whole shares");
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   Sh& sh = *reinterpret_cast<Sh*>(smem);
   const int w = wave_id(), l = lane_id(), g = l >> 4, r = l & 15, nb = w % NB, tb0 = w / NB, n0 = 16 * nb;
-  const int parts = p.P / PB, NC = (p.L + Q - 1) / Q;
+  const int PB = delta_part(p.P), parts = p.P / PB, NC = (p.L + Q - 1) / Q;
   const unsigned at = on_xcd(blockIdx.x, gridDim.x);
-  const int hp = (int)(at % (p.H * parts)), c = (int)(at / (p.H * parts) % NC), b = (int)(at / (p.H * parts) / NC);
-  const int h = hp / parts, HG = p.H / p.G, grp = h / HG;
+  const int h = (int)(at % p.H), c = (int)(at / p.H % NC), b = (int)(at / p.H / NC);
+  const int HG = p.H / p.G, grp = h / HG;
   const int t0 = c * Q, left = min(Q, p.L - t0);
-  const long long row0 = (long long)b * p.L + t0, chain = (long long)b * p.H * parts + hp;
-  const long long chunk = chain * NC + c;
+  const long long row0 = (long long)b * p.L + t0, head = (long long)b * p.H + h;
 
-  Columns<PB> st, gs;  // S and dS'
-  st.load(p.states + chunk * (NP * PB), nb);
-  gs.load(p.gstates + chunk * (NP * PB), nb);
+  // a slice's rows and columns on their way
+  using Sf = Stage<float, Q, kSlice, NT>;
+  Stage<T, Q, kSlice, NT> so;
+  Sf sx, sy;
+  Columns st, gs;  // S and dS'
+  so.place(p.lddo, kSlice);
+  sx.place(PB, kSlice);
+  sy.place(PB, kSlice);
+  const auto fetch = [&](int f) {
+    const int part = f / PB, off = f - part * PB;
+    const long long chunk = (head * parts + part) * NC + c;
+    so.load(static_cast<const T*>(p.dO) + row0 * p.lddo + (long long)h * p.P + f, left);
+    sx.load(p.x + chunk * (Q * PB) + off, Q);
+    sy.load(p.rows + chunk * (Q * PB) + off, Q);
+    st.load(p.states + chunk * (NP * PB) + off, PB, nb);
+    gs.load(p.gstates + chunk * (NP * PB) + off, PB, nb);
+  };
   {
     Stage<T, Q, NP, NT> sk, sq;
-    Stage<T, Q, PB, NT> so;
-    Stage<float, Q, PB, NT> sx, sy;
     sk.place(p.ldk, p.N);
     sq.place(p.ldq, p.N);
-    so.place(p.lddo, PB);
-    sx.place(PB, PB);
-    sy.place(PB, PB);
     sk.load(static_cast<const T*>(p.k) + row0 * p.ldk + (long long)grp * p.N, left);
     sq.load(static_cast<const T*>(p.q) + row0 * p.ldq + (long long)grp * p.N, left);
-    so.load(static_cast<const T*>(p.dO) + row0 * p.lddo + (long long)hp * PB, left);
-    sx.load(p.x + chunk * (Q * PB), Q);
-    sy.load(p.rows + chunk * (Q * PB), Q);
-    const float* tok = p.tok + (((long long)b * p.H + h) * NC + c) * delta_tok_floats(Q);
+    fetch(0);
+    const float* tok = p.tok + (head * NC + c) * delta_tok_floats(Q);
     for (int i = threadIdx.x; i < delta_tok_floats(Q) / 4; i += NT)
       reinterpret_cast<f4*>(&sh.tok)[i] = reinterpret_cast<const f4*>(tok)[i];
     sk.store(sh.k);
     sq.store(sh.q);
-    so.store(sh.dO);
-    __syncthreads();
-    using Sf = Stage<float, Q, PB, NT>;
-#pragma unroll
-    for (int i = 0; i < Sf::CNT; ++i) {
-      const f4 x = __builtin_bit_cast(f4, sx.v[i]), y = __builtin_bit_cast(f4, sy.v[i]);
-      const int row = Sf::row(i) < Q ? Sf::row(i) : 0;
-      const float beta = sh.tok.beta[row];
-      const f4 xy = x * y;
-      float s = (xy[0] + xy[1]) + (xy[2] + xy[3]);
-#pragma unroll
-      for (int m = 1; m < Sf::PER; m *= 2) s += __shfl_xor(s, m);
-      if (Sf::has() && Sf::col(i) == 0) sh.db[row] = s;
-      sx.v[i] = __builtin_bit_cast(u4v, x * beta);
-      sy.v[i] = __builtin_bit_cast(u4v, y * beta);
-    }
-    sx.store(sh.u);
-    sy.store(sh.dv);
   }
   __syncthreads();
   const DeltaTok<Q>& tok = sh.tok;
+  f4 tx[OWN], ty[OWN];  // do . u and dv . u, tiles of rows i and columns j
 #pragma unroll
-  for (int t = w; t < TILES; t += WAVES) {
-    const int ib = tri_row(t), jb = t - tri(ib, 0);
-    f4 x = f4{0.f, 0.f, 0.f, 0.f}, y = x, qk = x, kk = x;  // rows i, columns j
+  for (int k = 0; k < OWN; ++k) tx[k] = ty[k] = f4{0.f, 0.f, 0.f, 0.f};
+  f4 ia[TOK], iv[TOK], id[TOK];  // S^T do, S^T dv, dS'^T u, rows n and columns tokens
 #pragma unroll
-    for (int q = 0; q < PC; ++q) {
-      const Op<kFull> u = sh.u.rows(16 * jb, 32 * q);
-      mma<kFull>(x, sh.dO.rows(16 * ib, 32 * q), u);
-      mma<kFull>(y, sh.dv.rows(16 * ib, 32 * q), u);
+  for (int o = 0; o < TOK; ++o) ia[o] = iv[o] = id[o] = f4{0.f, 0.f, 0.f, 0.f};
+  float db[Sf::CNT] = {}, gh = 0.f;
+#pragma unroll 1
+  for (int f = 0; f < p.P; f += kSlice) {
+    if (f > 0) __syncthreads();  // the last slice's readers are done
+#pragma unroll
+    for (int i = 0; i < Sf::CNT; ++i) {
+      const f4 x = __builtin_bit_cast(f4, sx.v[i]), y = __builtin_bit_cast(f4, sy.v[i]);
+      const float beta = tok.beta[Sf::row(i) < Q ? Sf::row(i) : 0];
+      const f4 xy = x * y;
+      db[i] += (xy[0] + xy[1]) + (xy[2] + xy[3]);
+      sx.v[i] = __builtin_bit_cast(u4v, x * beta);
+      sy.v[i] = __builtin_bit_cast(u4v, y * beta);
+    }
+    so.store(sh.dO);
+    sx.store(sh.u);
+    sy.store(sh.dv);
+    const Op<kFull> so_ = st.op(), go_ = gs.op();
+    if (tb0 == 0) gh += gs.dot(st);
+    __syncthreads();
+    if (f + kSlice < p.P) fetch(f + kSlice);
+#pragma unroll
+    for (int k = 0; k < OWN; ++k) {
+      const int t = w + WAVES * k;
+      if (t >= TILES) break;
+      const int ib = tri_row(t), jb = t - tri(ib, 0);
+      const Op<kFull> u = sh.u.rows(16 * jb, 0);
+      mma<kFull>(tx[k], sh.dO.rows(16 * ib, 0), u);
+      mma<kFull>(ty[k], sh.dv.rows(16 * ib, 0), u);
     }
 #pragma unroll
+    for (int o = 0; o < TOK; ++o) {
+      const int tb = SHARE * o + tb0;
+      mma<kFull>(ia[o], so_, sh.dO.rows(16 * tb, 0));
+      mma<kFull>(iv[o], so_, sh.dv.rows(16 * tb, 0));
+      mma<kFull>(id[o], go_, sh.u.rows(16 * tb, 0));
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < Sf::CNT; ++i) {
+#pragma unroll
+    for (int m = 1; m < Sf::PER; m *= 2) db[i] += __shfl_xor(db[i], m);
+    if (Sf::has() && Sf::col(i) == 0) sh.db[Sf::row(i)] = db[i];
+  }
+  gh = sum_wave(gh);
+  if (l == 0) sh.gh[w] = gh;
+  __syncthreads();  // X and Y go where the slices were
+#pragma unroll
+  for (int k = 0; k < OWN; ++k) {
+    const int t = w + WAVES * k;
+    if (t >= TILES) break;
+    const int ib = tri_row(t), jb = t - tri(ib, 0);
+    f4 qk = f4{0.f, 0.f, 0.f, 0.f}, kk = qk;
+#pragma unroll
     for (int q = 0; q < NC2; ++q) {
-      const Op<IN> k = sh.k.rows(16 * jb, 32 * q);
-      mma<kFull>(qk, sh.q.rows(16 * ib, 32 * q), k);
-      mma<kFull>(kk, sh.k.rows(16 * ib, 32 * q), k);
+      const Op<IN> kj = sh.k.rows(16 * jb, 32 * q);
+      mma<kFull>(qk, sh.q.rows(16 * ib, 32 * q), kj);
+      mma<kFull>(kk, sh.k.rows(16 * ib, 32 * q), kj);
     }
     const int i0 = 16 * ib + 4 * g, j = 16 * jb + r;
     const f4 ih = tok.four(tok.hi, i0), il = tok.four(tok.lo, i0);
     const float jh = tok.hi[j], jl = tok.lo[j], rj = tok.rk[j];
-    f4 f;
+    f4 fr;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) f[e] = __builtin_amdgcn_exp2f((ih[e] - jh) + (il[e] - jl)) * rj;
-    x *= f * tok.four(tok.rq, i0) * p.scale;
-    y *= f * tok.four(tok.rk, i0) * -1.f;
+    for (int e = 0; e < 4; ++e) fr[e] = __builtin_amdgcn_exp2f((ih[e] - jh) + (il[e] - jl)) * rj;
+    f4 x = tx[k] * fr * tok.four(tok.rq, i0) * p.scale, y = ty[k] * fr * tok.four(tok.rk, i0) * -1.f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       x[e] = only_if(j <= i0 + e, x[e]);
@@ -183,11 +224,6 @@ __global__ __launch_bounds__((64 * GradShared<T, PB, NP>::WAVES)) void delta_bwd
 #pragma unroll
     for (int e = 0; e < 4; ++e) pass[e] = sum_row16(pass[e]);
     if (r == 0) *reinterpret_cast<f4*>(&sh.row[t][4 * g]) = pass;
-  }
-  {
-    float s = tb0 == 0 ? gs.dot(st) : 0.f;
-    s = sum_wave(s);
-    if (l == 0) sh.gh[w] = s;
   }
   __syncthreads();
 
@@ -214,12 +250,6 @@ __global__ __launch_bounds__((64 * GradShared<T, PB, NP>::WAVES)) void delta_bwd
     }
     return o;
   };
-  Op<kFull> so[PC], go[PC];
-#pragma unroll
-  for (int q = 0; q < PC; ++q) {
-    so[q] = st.op(q);
-    go[q] = gs.op(q);
-  }
   Op<IN> qt[QB], kt[QB];  // columns of q and k: free n, contracted tokens
 #pragma unroll
   for (int q = 0; q < QB; ++q) {
@@ -230,16 +260,7 @@ __global__ __launch_bounds__((64 * GradShared<T, PB, NP>::WAVES)) void delta_bwd
 #pragma unroll
   for (int o = 0; o < TOK; ++o) {
     const int tb = SHARE * o + tb0, i = 16 * tb + r;
-    f4 a = f4{0.f, 0.f, 0.f, 0.f}, d = a, v = a;
-#pragma unroll
-    for (int q = 0; q < PC; ++q) {
-      mma<kFull>(a, so[q], sh.dO.rows(16 * tb, 32 * q));
-      mma<kFull>(v, so[q], sh.dv.rows(16 * tb, 32 * q));
-      mma<kFull>(d, go[q], sh.u.rows(16 * tb, 32 * q));
-    }
-    a *= tok.eq[i];
-    v *= tok.er[i];
-    d *= tok.wr[i];
+    f4 a = ia[o] * tok.eq[i], v = iv[o] * tok.er[i], d = id[o] * tok.wr[i];
     const f4 qi = sh.q.quad(i, n0 + 4 * g), ki = sh.k.quad(i, n0 + 4 * g);
     const f4 pa = a * qi - v * ki, pd = d * ki;
     const float sa = sum_col4((pa[0] + pa[1]) + (pa[2] + pa[3])), sd = sum_col4((pd[0] + pd[1]) + (pd[2] + pd[3]));
@@ -267,7 +288,6 @@ __global__ __launch_bounds__((64 * GradShared<T, PB, NP>::WAVES)) void delta_bwd
     }
   }
   __syncthreads();
-  const int share = (h - grp * HG) * parts + hp - h * parts;  // among those of q and k's group
 #pragma unroll
   for (int o = 0; o < TOK; ++o) {
     const int tb = SHARE * o + tb0, i = 16 * tb + r;
@@ -286,8 +306,8 @@ __global__ __launch_bounds__((64 * GradShared<T, PB, NP>::WAVES)) void delta_bwd
       const long long at = ((row0 + i) * p.G + grp) * p.N + n;
       if (p.dqp != nullptr) {
         const long long all = (long long)p.B * p.L * p.G * p.N;
-        *reinterpret_cast<f4*>(p.dqp + share * all + at) = dq[o];
-        *reinterpret_cast<f4*>(p.dkp + share * all + at) = dk[o];
+        *reinterpret_cast<f4*>(p.dqp + (h - grp * HG) * all + at) = dq[o];
+        *reinterpret_cast<f4*>(p.dkp + (h - grp * HG) * all + at) = dk[o];
       } else {
         store4(static_cast<T*>(p.dq) + at, dq[o]);
         store4(static_cast<T*>(p.dk) + at, dk[o]);
@@ -308,25 +328,19 @@ __global__ __launch_bounds__((64 * GradShared<T, PB, NP>::WAVES)) void delta_bwd
       reach += (double)sh.d[k][t];
     }
   }
-  float gh = 0.f;
+  gh = 0.f;
 #pragma unroll
   for (int k = 0; k < NB; ++k) gh += sh.gh[k];
   const double upto = lane_sums(passes), all = lane_value(upto, 63), before = lane_sums(reach) - reach;
   if (in && t < left) {
     const float dg = (float)((all - upto + passes) + before + (double)(tok.end * gh));
     const long long at = (row0 + t) * p.H + h;
-    if (p.dgp != nullptr) {
-      const long long n = (long long)p.B * p.L * p.H, part = hp - h * parts;
-      p.dgp[part * n + at] = dg;
-      p.dbp[part * n + at] = sh.db[t];
-    } else {
-      put<T>(p.dg, p.g_f32, at, dg);
-      put<T>(p.dbeta, p.beta_f32, at, sh.db[t]);
-    }
+    put<T>(p.dg, p.g_f32, at, dg);
+    put<T>(p.dbeta, p.beta_f32, at, sh.db[t]);
   }
 }
 
-// q's and k's gradients of the heads and parts that share them
+// q's and k's gradients of the heads that share them
 template <typename T> __global__ __launch_bounds__(256) void delta_shared_kernel(DeltaParams p, long long quads, int n) {
   const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
   if (id >= 2 * quads) return;
@@ -337,50 +351,30 @@ template <typename T> __global__ __launch_bounds__(256) void delta_shared_kernel
   for (int k = 1; k < n; ++k) v += *reinterpret_cast<const f4*>(s + 4 * k * quads);
   store4(static_cast<T*>(second ? p.dk : p.dq) + 4 * q, v);
 }
-// the decays' and b's gradients of a head's parts
-template <typename T> __global__ __launch_bounds__(256) void delta_parts_kernel(DeltaParams p, long long n, int parts) {
-  const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (id >= 2 * n) return;
-  const bool second = id >= n;
-  const long long o = second ? id - n : id;
-  const float* s = (second ? p.dbp : p.dgp) + o;
-  float v = s[0];
-  for (int k = 1; k < parts; ++k) v += s[k * n];
-  put<T>(second ? p.dbeta : p.dg, second ? p.beta_f32 : p.g_f32, o, v);
-}
-
-template <typename T, int PB, int NP> hipError_t bwd_t(const DeltaParams& p, hipStream_t stream) {
-  using Sh = GradShared<T, PB, NP>;
+template <typename T, int NP> hipError_t bwd_t(const DeltaParams& p, hipStream_t stream) {
+  using Sh = GradShared<T, NP>;
   constexpr size_t lds = sizeof(Sh);
-  static_assert(lds <= 160 * 1024, "LDS of a compute unit");
-  const hipError_t e = allow_lds(delta_bwd_kernel<T, PB, NP>, lds);
+  static_assert(2 * lds <= 160 * 1024, "two workgroups to a compute unit");
+  const hipError_t e = allow_lds(delta_bwd_kernel<T, NP>, lds);
   if (e != hipSuccess) return e;
-  const int parts = p.P / PB;
-  const long long blocks = (long long)p.B * ((p.L + Sh::Q - 1) / Sh::Q) * p.H * parts;
-  hipLaunchKernelGGL((delta_bwd_kernel<T, PB, NP>), dim3((unsigned)blocks), dim3(64 * Sh::WAVES), lds, stream, p);
+  const long long blocks = (long long)p.B * ((p.L + Sh::Q - 1) / Sh::Q) * p.H;
+  hipLaunchKernelGGL((delta_bwd_kernel<T, NP>), dim3((unsigned)blocks), dim3(64 * Sh::WAVES), lds, stream, p);
   if (p.dqp != nullptr) {
     const long long quads = (long long)p.B * p.L * p.G * p.N / 4;
     hipLaunchKernelGGL(delta_shared_kernel<T>, dim3((unsigned)((2 * quads + 255) / 256)), dim3(256), 0, stream, p, quads,
-                       p.H / p.G * parts);
-  }
-  if (p.dgp != nullptr) {
-    const long long n = (long long)p.B * p.L * p.H;
-    hipLaunchKernelGGL(delta_parts_kernel<T>, dim3((unsigned)((2 * n + 255) / 256)), dim3(256), 0, stream, p, n, parts);
+                       p.H / p.G);
   }
   return hipGetLastError();
 }
-template <typename T, int PB> hipError_t width_t(const DeltaParams& p, hipStream_t s) {
-  return p.N <= 32 ? bwd_t<T, PB, 32>(p, s) : p.N <= 64 ? bwd_t<T, PB, 64>(p, s) : bwd_t<T, PB, 128>(p, s);
-}
-template <typename T> hipError_t part_t(const DeltaParams& p, hipStream_t s) {
-  return delta_part(p.P) == 64 ? width_t<T, 64>(p, s) : width_t<T, 32>(p, s);
+template <typename T> hipError_t width_t(const DeltaParams& p, hipStream_t s) {
+  return p.N <= 32 ? bwd_t<T, 32>(p, s) : p.N <= 64 ? bwd_t<T, 64>(p, s) : bwd_t<T, 128>(p, s);
 }
 
 }  // namespace
 
 hipError_t launch_delta_bwd(const DeltaParams& p, int dtype, hipStream_t s) {
-  return dtype == TTT_DTYPE_BF16 ? part_t<__bf16>(p, s)
-         : dtype == TTT_DTYPE_F16 ? part_t<_Float16>(p, s) : part_t<float>(p, s);
+  return dtype == TTT_DTYPE_BF16 ? width_t<__bf16>(p, s)
+         : dtype == TTT_DTYPE_F16 ? width_t<_Float16>(p, s) : width_t<float>(p, s);
 }
 
 }  // namespace ttt

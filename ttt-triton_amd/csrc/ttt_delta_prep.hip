@@ -18,8 +18,12 @@ namespace {
 
 template <typename T, int NP> struct PrepShared {
   static constexpr int IN = ScanType<T>::IN, Q = kDeltaQ<T>;
-  Planes<IN, Q, NP> k, q;
-  float a[Q][Q + 4];
+  union {  // A, then Z, in the place of the rows that it comes of: more workgroups to a compute unit
+    struct {
+      Planes<IN, Q, NP> k, q;
+    };
+    float a[Q][Q + 4];
+  };
   DeltaTok<Q> tok;
   Decays<Q> dec;
   float nq[Q], nk[Q];
@@ -49,8 +53,8 @@ template <typename T, int NP, bool BACK> __global__ __launch_bounds__(256) void 
   Sh& sh = *reinterpret_cast<Sh*>(smem);
   const int w = wave_id(), l = lane_id(), g = l >> 4, r = l & 15;
   const int NC = (p.L + Q - 1) / Q;
-  const unsigned at = on_xcd(blockIdx.x, gridDim.x);
-  const int h = (int)(at % p.H), c = (int)(at / p.H % NC), b = (int)(at / p.H / NC), grp = h / (p.H / p.G);
+  const unsigned id = on_xcd(blockIdx.x, gridDim.x);
+  const int h = (int)(id % p.H), c = (int)(id / p.H % NC), b = (int)(id / p.H / NC), grp = h / (p.H / p.G);
   const int t0 = c * Q, left = min(Q, p.L - t0);
   const long long row0 = (long long)b * p.L + t0, chunk = ((long long)b * p.H + h) * NC + c;
 
@@ -108,9 +112,12 @@ template <typename T, int NP, bool BACK> __global__ __launch_bounds__(256) void 
     return f;
   };
   // A, tiles of rows i and columns j
-  constexpr int TILES = TB * (TB + 1) / 2;
+  constexpr int TILES = TB * (TB + 1) / 2, OWN = (TILES + 3) / 4;
+  f4 at[OWN];
 #pragma unroll
-  for (int t = w; t < TILES; t += 4) {
+  for (int u = 0; u < OWN; ++u) {
+    const int t = w + 4 * u;
+    if (t >= TILES) break;
     const int ib = tri_row(t), jb = t - tri(ib, 0);
     f4 acc = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -118,7 +125,7 @@ template <typename T, int NP, bool BACK> __global__ __launch_bounds__(256) void 
     const int i = 16 * ib + 4 * g, j = 16 * jb + r;
     acc *= decays(i, j, true) * tok.four(tok.rk, i) * tok.rk[j];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) sh.a[i + e][j] = only_if(j < i + e, acc[e]);
+    for (int e = 0; e < 4; ++e) at[u][e] = only_if(j < i + e, acc[e]);
   }
   // M: forwards the free token i and contracted j, backwards the other way
   float* mp = p.m + chunk * (TILES * 256);
@@ -140,6 +147,15 @@ template <typename T, int NP, bool BACK> __global__ __launch_bounds__(256) void 
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[e] = only_if(BACK ? tc <= tr + e : tr + e <= tc, acc[e]);
     *reinterpret_cast<f4*>(mp + (t * 64 + l) * 4) = acc;
+  }
+  __syncthreads();  // the rows have been read
+#pragma unroll
+  for (int u = 0; u < OWN; ++u) {
+    const int t = w + 4 * u;
+    if (t >= TILES) break;
+    const int ib = tri_row(t), jb = t - tri(ib, 0);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sh.a[16 * ib + 4 * g + e][16 * jb + r] = at[u][e];
   }
   __syncthreads();
   // the blocks of Z on the diagonal: lane (g, r) has column r of block g

@@ -8,6 +8,12 @@
 // by itself, and each product's result is, where it lies, an operand of the next:
 //   S (rows n) -> K S (rows tokens) -> r -> Z b r -> x -> u -> S' = e^{c_Q} S + K^T u
 // and the outputs, transposed (rows features), from S, Q and u, M.
+//
+// Where there are few sequences and heads, the tokens are cut into segments.  A segment takes
+// the state S that enters it to T S + E, with T = prod e^{g_t} (1 - b_t k_t (x) k_t): a first walk
+// without outputs, of all segments at once, gives E from the state 0 and T from the columns of
+// the identity, as features without values; one launch goes over the segments with their
+// products (delta_join_kernel), and then all segments are walked at once.
 #include <math.h>
 #include <stddef.h>
 
@@ -69,32 +75,62 @@ template <int FLOATS, int NT> struct Copy {
   }
 };
 
-template <typename T, int W, int NP, bool BACK> __global__ __launch_bounds__(64 * W) void delta_walk_kernel(DeltaParams p) {
+// what StateTiles::keep wrote
+template <int NP> __device__ __forceinline__ void take_kept(StateTiles<NP>& st, const float* __restrict__ s, int ld, int w) {
+  const int l = lane_id();
+#pragma unroll
+  for (int i = 0; i < NP / 16; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) st.t[i][e] = s[(StateTiles<NP>::col(i >> 1) + 4 * (i & 1) + e) * ld + 16 * w + (l & 15)];
+}
+
+// OUT: outputs too; else the segments' ends alone
+template <typename T, int W, int NP, bool BACK, bool OUT>
+__global__ __launch_bounds__(64 * W) void delta_walk_kernel(DeltaParams p) {
   using Sh = WalkShared<T, W, NP, BACK>;
   static_assert(offsetof(Sh, q) % 16 == 0 && offsetof(Sh, v) % 16 == 0 && offsetof(Sh, z) % 16 == 0 &&
                     offsetof(Sh, m) % 16 == 0 && offsetof(Sh, tok) % 16 == 0,
                 "read 16 bytes at a time");
   constexpr int IN = Sh::IN, MP = Sh::MP, Q = Sh::Q, TB = Q / 16, QB = Q / 32, NT = 64 * W, NC2 = NP / 32, NB = NP / 16;
   constexpr int MID = IN > 1 ? kFull : 2;
+  constexpr bool READS = OUT || BACK;  // q and M
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   Sh& sh = *reinterpret_cast<Sh*>(smem);
   const int w = wave_id(), l = lane_id(), g = l >> 4, r = l & 15;
   const int PB = delta_part(p.P), parts = p.P / PB, cols = PB / (16 * W), NC = (p.L + Q - 1) / Q;
   const unsigned at = on_xcd(blockIdx.x, gridDim.x);
-  const int f0 = 16 * W * (int)(at % cols);  // the first feature in its part
-  const long long chain = at / cols;         // sequence, head, part
-  const int hp = (int)(chain % (p.H * parts)), b = (int)(chain / (p.H * parts)), h = hp / parts;
-  const int grp = h / (p.H / p.G);
-  const long long head = (long long)b * p.H + h;
+  // groups of columns to a head: of its features, and without outputs of the identity behind them
+  const int own = parts * cols, groups = own + (OUT ? 0 : NP / (16 * W)), segs = OUT ? p.S : p.S - 1;
+  const int grp_c = (int)(at % groups);
+  const int s = (int)(at / groups % segs) + (!OUT && BACK ? 1 : 0);
+  const long long head = at / groups / segs;  // sequence and head
+  const bool features = OUT || grp_c < own;
+  const int b = (int)(head / p.H), h = (int)(head - (long long)b * p.H), grp = h / (p.H / p.G);
+  const int part = features ? grp_c / cols : 0, f0 = features ? 16 * W * (grp_c % cols) : 16 * W * (grp_c - own);
+  const int hp = h * parts + part;
+  const long long chain = head * parts + part;  // f0: the first feature in the part, or column of the identity
   const T* K = static_cast<const T*>(p.k) + (long long)grp * p.N;
   const T* Qr = static_cast<const T*>(p.q) + (long long)grp * p.N;
   const long long ldv = BACK ? p.lddo : p.ldv;
-  const T* V = static_cast<const T*>(BACK ? p.dO : p.v) + (long long)hp * PB + f0;
+  const T* V = static_cast<const T*>(BACK ? p.dO : p.v) + (features ? (long long)hp * PB + f0 : 0);
   T* O = static_cast<T*>(p.o) + (long long)hp * PB + f0;
   const long long ldo = (long long)p.H * p.P;
+  const int c0 = s * p.per, n = min(NC, c0 + p.per) - c0;
 
   StateTiles<NP> st;
-  st.load(p.h0 != nullptr ? p.h0 + (chain * PB + f0) * p.N : nullptr, p.N, p.N, w);
+  if (!OUT) {
+    st.load(nullptr, 0, 0, w);
+    if (!features) {
+#pragma unroll
+      for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) st.t[i][e] = StateTiles<NP>::col(i >> 1) + 4 * (i & 1) + e == f0 + 16 * w + r ? 1.f : 0.f;
+    }
+  } else if (p.S > 1) {
+    take_kept(st, p.seg + (chain * p.S + s) * (NP * PB) + f0, PB, w);
+  } else {
+    st.load(p.h0 != nullptr ? p.h0 + (chain * PB + f0) * p.N : nullptr, p.N, p.N, w);
+  }
 
   Stage<T, Q, NP, NT> sk, sq;
   Stage<T, Q, 16 * W, NT> sv;
@@ -107,10 +143,12 @@ template <typename T, int W, int NP, bool BACK> __global__ __launch_bounds__(64 
     const int left = min(Q, p.L - c * Q);
     const long long row = (long long)b * p.L + (long long)c * Q, chunk = head * NC + c;
     sk.load(K + row * p.ldk, left);
-    sq.load(Qr + row * p.ldq, left);
-    sv.load(V + row * ldv, left);
+    sv.load(V + row * ldv, features ? left : 0);
     bz.load(p.z + chunk * (delta_tiles(Q) * 256), w);
-    bm.load(p.m + chunk * (delta_tiles(Q) * 256), w);
+    if constexpr (READS) {
+      sq.load(Qr + row * p.ldq, left);
+      bm.load(p.m + chunk * (delta_tiles(Q) * 256), w);
+    }
     ct.load(p.tok + chunk * delta_tok_floats(Q));
   };
   const auto z_op = [&](int u) {
@@ -125,24 +163,27 @@ template <typename T, int W, int NP, bool BACK> __global__ __launch_bounds__(64 
     for (int a = 0; a < MP; ++a) o.v[a] = sh.m[a][u][l];
     return o;
   };
-  fetch(BACK ? NC - 1 : 0);
+  const auto chunk_of_step = [&](int k) { return BACK ? c0 + n - 1 - k : c0 + k; };
+  fetch(chunk_of_step(0));
   // (an operand's half beside the triangle stays 0)
   for (int i = threadIdx.x; i < (int)(offsetof(Sh, tok) - offsetof(Sh, z)) / 16; i += NT)
     reinterpret_cast<f4*>(&sh.z)[i] = f4{0.f, 0.f, 0.f, 0.f};
   __syncthreads();
 #pragma unroll 1
-  for (int k = 0; k < NC; ++k) {
-    const int c = BACK ? NC - 1 - k : k;
+  for (int k = 0; k < n; ++k) {
+    const int c = chunk_of_step(k);
     if (k > 0) __syncthreads();  // the last chunk's readers are done
     sk.store(sh.k);
-    sq.store(sh.q);
     sv.store(sh.v);
     bz.template store<kFull>(sh.z, w);
-    bm.template store<MP>(sh.m, w);
+    if constexpr (READS) {
+      sq.store(sh.q);
+      bm.template store<MP>(sh.m, w);
+    }
     ct.store(sh.tok.hi);
     __syncthreads();
-    if (k + 1 < NC) fetch(BACK ? c - 1 : c + 1);
-    if (p.states != nullptr) st.keep(p.states + (chain * NC + c) * (long long)(NP * PB) + f0, PB, w);
+    if (k + 1 < n) fetch(chunk_of_step(k + 1));
+    if (OUT && p.states != nullptr) st.keep(p.states + (chain * NC + c) * (long long)(NP * PB) + f0, PB, w);
     const DeltaTok<Q>& tok = sh.tok;
     const int left = p.L - c * Q;
     const long long row = (long long)b * p.L + (long long)c * Q;
@@ -214,14 +255,15 @@ template <typename T, int W, int NP, bool BACK> __global__ __launch_bounds__(64 
           }
       }
     }
-    if (p.rows != nullptr) {
+    if (OUT && p.rows != nullptr) {
       float* to = p.rows + ((chain * NC + c) * Q) * PB + f0 + 16 * w + r;
 #pragma unroll
       for (int ob = 0; ob < TB; ++ob)
 #pragma unroll
         for (int e = 0; e < 4; ++e) to[(16 * ob + 4 * g + e) * PB] = t[ob][e];
     }
-    if constexpr (BACK) {
+    if constexpr (!OUT) {
+    } else if constexpr (BACK) {
       T* to = O + row * ldo + 16 * w + r;
 #pragma unroll
       for (int ob = 0; ob < TB; ++ob) {
@@ -300,16 +342,74 @@ template <typename T, int W, int NP, bool BACK> __global__ __launch_bounds__(64 
       }
     }
   }
-  if (p.h_last != nullptr) st.store(p.h_last + (chain * PB + f0) * p.N, p.N, p.N, w);
+  if (!OUT) {
+    if (features)
+      st.keep(p.seg + (chain * p.S + s) * (NP * PB) + f0, PB, w);
+    else
+      st.keep(p.trans + (head * p.S + s) * (NP * NP) + f0, NP, w);
+  } else if (p.h_last != nullptr && s == (BACK ? 0 : p.S - 1)) {
+    st.store(p.h_last + (chain * PB + f0) * p.N, p.N, p.N, w);
+  }
+}
+
+// The segments' ends -> the states they start from, in place: a wave has 16 features of a part and
+// goes over the segments, the next one's product on its way.
+template <int NP, bool BACK> __global__ __launch_bounds__(64) void delta_join_kernel(DeltaParams p) {
+  constexpr int NB = NP / 16, NC2 = NP / 32;
+  const int l = lane_id(), g = l >> 4, r = l & 15;
+  const int PB = delta_part(p.P), cols = PB / 16, parts = p.P / PB;
+  const int w = (int)(blockIdx.x % cols);
+  const long long chain = blockIdx.x / cols, head = chain / parts;
+  StateTiles<NP> st, end;
+  st.load(p.h0 != nullptr ? p.h0 + chain * PB * p.N : nullptr, p.N, p.N, w);
+  const auto seg = [&](int k) { return BACK ? p.S - 1 - k : k; };
+  const auto at = [&](int k) { return p.seg + (chain * p.S + seg(k)) * (NP * PB); };
+  f4 a[NB][NC2][2];  // rows n as a state's tiles have them, columns 32q + 8g..
+  const auto fetch = [&](int k) {
+    const float* t = p.trans + (head * p.S + seg(k)) * (NP * NP);
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+      for (int q = 0; q < NC2; ++q)
+#pragma unroll
+        for (int o = 0; o < 2; ++o)
+          a[i][q][o] = *reinterpret_cast<const f4*>(
+              t + (32 * (i >> 1) + 8 * (r >> 2) + 4 * (i & 1) + (r & 3)) * NP + 32 * q + 8 * g + 4 * o);
+    take_kept(end, at(k), PB, w);
+  };
+  fetch(0);
+#pragma unroll 1
+  for (int k = 0; k + 1 < p.S; ++k) {
+    st.keep(at(k), PB, w);
+    Op<kFull> s[NC2];
+#pragma unroll
+    for (int q = 0; q < NC2; ++q) s[q] = st.template op<kFull>(q);
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      st.t[i] = end.t[i];
+#pragma unroll
+      for (int q = 0; q < NC2; ++q) mma<kFull>(st.t[i], split8<kFull>(a[i][q][0], a[i][q][1]), s[q]);
+    }
+    if (k + 2 < p.S) fetch(k + 1);
+  }
+  st.keep(at(p.S - 1), PB, w);
 }
 
 template <typename T, int W, int NP, bool BACK> hipError_t walk_t(const DeltaParams& p, hipStream_t stream) {
   constexpr size_t lds = sizeof(WalkShared<T, W, NP, BACK>);
   static_assert(lds <= 160 * 1024, "LDS of a compute unit");
-  const hipError_t e = allow_lds(delta_walk_kernel<T, W, NP, BACK>, lds);
+  hipError_t e = allow_lds(delta_walk_kernel<T, W, NP, BACK, true>, lds);
   if (e != hipSuccess) return e;
-  const long long blocks = (long long)p.B * p.H * p.P / (16 * W);
-  hipLaunchKernelGGL((delta_walk_kernel<T, W, NP, BACK>), dim3((unsigned)blocks), dim3(64 * W), lds, stream, p);
+  const long long heads = (long long)p.B * p.H;
+  if (p.S > 1) {
+    e = allow_lds(delta_walk_kernel<T, W, NP, BACK, false>, lds);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((delta_walk_kernel<T, W, NP, BACK, false>), dim3((unsigned)(heads * (p.S - 1) * (p.P + NP) / (16 * W))),
+                       dim3(64 * W), lds, stream, p);
+    hipLaunchKernelGGL((delta_join_kernel<NP, BACK>), dim3((unsigned)(heads * p.P / 16)), dim3(64), 0, stream, p);
+  }
+  hipLaunchKernelGGL((delta_walk_kernel<T, W, NP, BACK, true>), dim3((unsigned)(heads * p.S * p.P / (16 * W))), dim3(64 * W),
+                     lds, stream, p);
   return hipGetLastError();
 }
 template <typename T, int W, bool BACK> hipError_t width_t(const DeltaParams& p, hipStream_t s) {
