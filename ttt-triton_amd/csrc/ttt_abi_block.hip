@@ -2,7 +2,6 @@
 // and workspace layout, then launches on the caller's stream.  Declarations and argument
 // contracts are in include/ttt_amd.h.
 #include <stdint.h>
-#include <stdlib.h>
 
 #include <algorithm>
 
@@ -27,10 +26,25 @@ struct DeltaPlan {
   int Q, NC, share, S, per;
   size_t tok, zm, states, rows, qk, seg, trans;
 };
-// Segments that the tokens are cut into: as many as make the walk quickest.
+// Segments that the tokens are cut into: as many as make the walk quickest.  In units of a chunk's
+// walk with outputs (3.6 to 4.6 us with 64 tokens, 2.2 to 3.8 with 32), one without takes 0.7, a
+// segment's join 0.3 and two more launches 2; a compute unit holds one workgroup of 64 features or
+// of states over 64 wide, else two.  (Kernels of 16,384 tokens of 12 heads of 64 x 64 in bf16: 930 us
+// with one, 190 with 20.)
 int delta_segments(long long heads, int P, int NP, int NC) {
-  if (const char* e = getenv("DSEG")) return std::max(1, std::min(NC, atoi(e)));
-  return 1;
+  const int wide = P % 64 == 0 && NP < 128 ? 64 : 32, places = wide == 64 || NP == 128 ? 256 : 512;
+  const auto rounds = [&](long long columns) { return (double)((heads * columns / wide + places - 1) / places); };
+  int best = 1;
+  double least = rounds(P) * NC;
+  for (int want = 2; want <= std::min(NC, 128); ++want) {
+    const int per = (NC + want - 1) / want, S = (NC + per - 1) / per;
+    const double time = rounds((long long)P * S) * per + rounds((long long)(P + NP) * (S - 1)) * per * 0.7 + 0.3 * S + 2.0;
+    if (time < least) {
+      least = time;
+      best = S;
+    }
+  }
+  return best;
 }
 DeltaPlan delta_plan(int B, int L, int H, int P, int G, int N, int dtype) {
   DeltaPlan s;

@@ -2,12 +2,16 @@
 // ttt_delta.h): forwards the outputs and the states, backwards dv and the gradients of the
 // states.
 //
-// A workgroup walks 16 W features of one sequence and head, chunk by chunk; wave w has 16 of
-// them, with their part of the state in registers.  The features do not meet: behind the one
-// barrier at which a chunk's rows and operands are in LDS, a wave goes through its products
-// by itself, and each product's result is, where it lies, an operand of the next:
+// A workgroup walks 16 W features of one sequence and head, chunk by chunk.  W waves have 16 of
+// them each, with their part of the state in registers, and go through what a chunk's state needs
+// of the one before it alone.  The features do not meet, and each product's result is, where it
+// lies, an operand of the next, without LDS or barriers in between:
 //   S (rows n) -> K S (rows tokens) -> r -> Z b r -> x -> u -> S' = e^{c_Q} S + K^T u
-// and the outputs, transposed (rows features), from S, Q and u, M.
+// W more waves do the rest beside them: they bring the next chunk's rows to LDS, and forwards
+// form the outputs of the chunk before (transposed, rows features, from S, Q and u, M) from the
+// state's planes and x, backwards the next chunk's M^T do and Q^T do; both are handed over through
+// LDS.  A barrier ends a chunk; another one, in its course, lets what was handed over be written
+// again.
 //
 // Where there are few sequences and heads, the tokens are cut into segments.  A segment takes
 // the state S that enters it to T S + E, with T = prod e^{g_t} (1 - b_t k_t (x) k_t): a first walk
@@ -17,6 +21,7 @@
 #include <math.h>
 #include <stddef.h>
 
+#include "ttt_buf.h"
 #include "ttt_delta.h"
 
 namespace ttt {
@@ -24,15 +29,24 @@ namespace ttt {
 namespace {
 
 template <typename T, int W, int NP, bool BACK> struct WalkShared {
-  static constexpr int IN = ScanType<T>::IN, Q = kDeltaQ<T>, PAIRS = delta_pairs(Q);
-  static constexpr int MP = BACK || IN > 1 ? kFull : 2;
-  Planes<IN, Q, NP> k, q;
-  Planes<IN, Q, 16 * W> v;
-  bf8 z[kFull][PAIRS][64], m[MP][PAIRS][64];
-  DeltaTok<Q> tok;
+  static constexpr int IN = ScanType<T>::IN, MID = ScanType<T>::MID, Q = kDeltaQ<T>, PAIRS = delta_pairs(Q);
+  static constexpr int TB = Q / 16, NB = NP / 16, NC2 = NP / 32;
+  struct alignas(16) Side {  // a chunk's, in turn
+    Planes<IN, Q, NP> k;
+    bf8 z[kFull][PAIRS][64];
+    DeltaTok<Q> tok;
+    Planes<IN, BACK ? 1 : Q, 16 * W> v;
+  } side[2];
+  // backwards the chunk's that the helpers form M^T do and Q^T do of
+  Planes<IN, BACK ? Q : 1, NP> q;
+  Planes<IN, BACK ? Q : 1, 16 * W> dO;
+  // what is handed over
+  bf8 s[BACK ? 1 : W][BACK ? 1 : MID][BACK ? 1 : NC2][64];
+  f4 x[BACK ? 1 : W][BACK ? 1 : TB][64];
+  f4 md[BACK ? W : 1][BACK ? TB : 1][64], qd[BACK ? W : 1][BACK ? NB : 1][64];
 };
 
-// a chunk's blocks of Z or M on their way from memory to operands in planes
+// a chunk's blocks of Z on their way from memory to operands in planes
 template <int Q, int W, bool BACK> struct Blocks {
   static constexpr int ALL = delta_tiles(Q), CNT = (ALL + W - 1) / W;
   f4 v[CNT];
@@ -41,35 +55,52 @@ template <int Q, int W, bool BACK> struct Blocks {
     for (int i = 0; i < CNT; ++i)
       if (i * W + w < ALL) v[i] = *reinterpret_cast<const f4*>(p + ((i * W + w) * 64 + lane_id()) * 4);
   }
-  template <int PL> __device__ __forceinline__ void store(bf8 (*to)[delta_pairs(Q)][64], int w) const {
+  __device__ __forceinline__ void store(bf8 (*to)[delta_pairs(Q)][64], int w) const {
 #pragma unroll
     for (int i = 0; i < CNT; ++i) {
       const int t = i * W + w;
       if (t >= ALL) continue;
       const int hb = tri_row(t), lb = t - tri(hb, 0), blk = BACK ? lb : hb, in = BACK ? hb : lb;
-      bf4 o[PL];
-      split4<PL>(v[i], o);
+      bf4 o[kFull];
+      split4<kFull>(v[i], o);
 #pragma unroll
-      for (int a = 0; a < PL; ++a)
+      for (int a = 0; a < kFull; ++a)
         reinterpret_cast<bf4*>(&to[a][pair_at(BACK, Q, blk, in / 2)][lane_id()])[in & 1] = o[a];
     }
+  }
+};
+// a chunk's blocks of M in a wave's registers, as operands
+template <int Q, bool BACK> struct Masked {
+  f4 v[delta_tiles(Q)];
+  __device__ __forceinline__ void load(const float* p) {
+#pragma unroll
+    for (int t = 0; t < delta_tiles(Q); ++t) v[t] = *reinterpret_cast<const f4*>(p + (t * 64 + lane_id()) * 4);
+  }
+  // of the free block b, contracted blocks 2q and 2q + 1
+  template <int PL> __device__ __forceinline__ Op<PL> op(int b, int q) const {
+    const auto tile = [&](int in) {
+      const bool has = meets(BACK, b, in);
+      return has ? v[has ? (BACK ? tri(in, b) : tri(b, in)) : 0] : f4{0.f, 0.f, 0.f, 0.f};
+    };
+    return split8<PL>(tile(2 * q), tile(2 * q + 1));
   }
 };
 // floats on their way to LDS as they lie in memory
 template <int FLOATS, int NT> struct Copy {
   static constexpr int ALL = FLOATS / 4, CNT = (ALL + NT - 1) / NT;
   f4 v[CNT];
+  __device__ __forceinline__ static int at(int i) { return i * NT + (int)threadIdx.x; }
   __device__ __forceinline__ void load(const float* p) {
 #pragma unroll
     for (int i = 0; i < CNT; ++i) {
-      const int o = i * NT + (int)threadIdx.x;
+      const int o = at(i);
       if (o < ALL) v[i] = reinterpret_cast<const f4*>(p)[o];
     }
   }
   __device__ __forceinline__ void store(float* p) const {
 #pragma unroll
     for (int i = 0; i < CNT; ++i) {
-      const int o = i * NT + (int)threadIdx.x;
+      const int o = at(i);
       if (o < ALL) reinterpret_cast<f4*>(p)[o] = v[i];
     }
   }
@@ -84,19 +115,31 @@ template <int NP> __device__ __forceinline__ void take_kept(StateTiles<NP>& st, 
     for (int e = 0; e < 4; ++e) st.t[i][e] = s[(StateTiles<NP>::col(i >> 1) + 4 * (i & 1) + e) * ld + 16 * w + (l & 15)];
 }
 
+// a row's eight values as an operand in planes
+template <typename T> __device__ __forceinline__ Op<ScanType<T>::IN> row_op(const T* p) {
+  constexpr int IN = ScanType<T>::IN;
+  if constexpr (IN == 1) {
+    Op<1> o;
+    o.v[0] = *reinterpret_cast<const bf8*>(p);
+    return o;
+  } else {
+    return split8<IN>(load4(p), load4(p + 4));
+  }
+}
+
 // OUT: outputs too; else the segments' ends alone
 template <typename T, int W, int NP, bool BACK, bool OUT>
-__global__ __launch_bounds__(64 * W) void delta_walk_kernel(DeltaParams p) {
+__global__ __launch_bounds__(128 * W) void delta_walk_kernel(DeltaParams p) {
   using Sh = WalkShared<T, W, NP, BACK>;
-  static_assert(offsetof(Sh, q) % 16 == 0 && offsetof(Sh, v) % 16 == 0 && offsetof(Sh, z) % 16 == 0 &&
-                    offsetof(Sh, m) % 16 == 0 && offsetof(Sh, tok) % 16 == 0,
+  static_assert(offsetof(Sh, q) % 16 == 0 && offsetof(Sh, dO) % 16 == 0 && offsetof(Sh, s) % 16 == 0 &&
+                    offsetof(Sh, x) % 16 == 0 && offsetof(typename Sh::Side, z) % 16 == 0 &&
+                    offsetof(typename Sh::Side, tok) % 16 == 0 && offsetof(typename Sh::Side, v) % 16 == 0,
                 "read 16 bytes at a time");
-  constexpr int IN = Sh::IN, MP = Sh::MP, Q = Sh::Q, TB = Q / 16, QB = Q / 32, NT = 64 * W, NC2 = NP / 32, NB = NP / 16;
-  constexpr int MID = IN > 1 ? kFull : 2;
-  constexpr bool READS = OUT || BACK;  // q and M
+  constexpr int IN = Sh::IN, MID = Sh::MID, Q = Sh::Q, TB = Sh::TB, QB = Q / 32, NT = 64 * W, NC2 = Sh::NC2, NB = Sh::NB;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   Sh& sh = *reinterpret_cast<Sh*>(smem);
-  const int w = wave_id(), l = lane_id(), g = l >> 4, r = l & 15;
+  const bool helps = wave_id() < W;  // (a stage's threads are a workgroup's first)
+  const int w = helps ? wave_id() : wave_id() - W, l = lane_id(), g = l >> 4, r = l & 15;
   const int PB = delta_part(p.P), parts = p.P / PB, cols = PB / (16 * W), NC = (p.L + Q - 1) / Q;
   const unsigned at = on_xcd(blockIdx.x, gridDim.x);
   // groups of columns to a head: of its features, and without outputs of the identity behind them
@@ -109,13 +152,228 @@ __global__ __launch_bounds__(64 * W) void delta_walk_kernel(DeltaParams p) {
   const int part = features ? grp_c / cols : 0, f0 = features ? 16 * W * (grp_c % cols) : 16 * W * (grp_c - own);
   const int hp = h * parts + part;
   const long long chain = head * parts + part;  // f0: the first feature in the part, or column of the identity
-  const T* K = static_cast<const T*>(p.k) + (long long)grp * p.N;
-  const T* Qr = static_cast<const T*>(p.q) + (long long)grp * p.N;
-  const long long ldv = BACK ? p.lddo : p.ldv;
-  const T* V = static_cast<const T*>(BACK ? p.dO : p.v) + (features ? (long long)hp * PB + f0 : 0);
-  T* O = static_cast<T*>(p.o) + (long long)hp * PB + f0;
   const long long ldo = (long long)p.H * p.P;
   const int c0 = s * p.per, n = min(NC, c0 + p.per) - c0;
+  const auto chunk_of = [&](int k) { return BACK ? c0 + n - 1 - k : c0 + k; };
+  const auto first_row = [&](int c) { return (long long)b * p.L + (long long)c * Q; };
+  // (an operand's half beside the triangle stays 0)
+  for (int i = threadIdx.x; i < 2 * (int)sizeof(Sh::Side::z) / 16; i += 2 * NT) {
+    const int side = i >= (int)sizeof(Sh::Side::z) / 16, o = i - side * (int)sizeof(Sh::Side::z) / 16;
+    reinterpret_cast<f4*>(&sh.side[side].z)[o] = f4{0.f, 0.f, 0.f, 0.f};
+  }
+  __syncthreads();
+
+  if (helps) {
+    const T* K = static_cast<const T*>(p.k) + (long long)grp * p.N;
+    const T* Qr = static_cast<const T*>(p.q) + (long long)grp * p.N;
+    const long long ldv = BACK ? p.lddo : p.ldv;
+    const T* V = static_cast<const T*>(BACK ? p.dO : p.v) + (features ? (long long)hp * PB + f0 : 0);
+    Stage<T, Q, NP, NT> sk, sq;
+    Stage<T, Q, 16 * W, NT> sv;
+    Blocks<Q, W, BACK> bz;
+    Copy<delta_tok_floats(Q), NT> ct;
+    Masked<Q, BACK> m;
+    sk.place(p.ldk, p.N);
+    sq.place(p.ldq, p.N);
+    sv.place(ldv, 16 * W);
+    // what the other waves take of a chunk
+    const auto fetch = [&](int c) {
+      const int left = min(Q, p.L - c * Q);
+      sk.load(K + first_row(c) * p.ldk, left);
+      if constexpr (!BACK) sv.load(V + first_row(c) * ldv, features ? left : 0);
+      bz.load(p.z + (head * NC + c) * (delta_tiles(Q) * 256), w);
+      ct.load(p.tok + (head * NC + c) * delta_tok_floats(Q));
+    };
+    const auto put = [&](typename Sh::Side& to) {
+      sk.store(to.k);
+      if constexpr (!BACK) sv.store(to.v);
+      bz.store(to.z, w);
+      ct.store(to.tok.hi);
+    };
+    if constexpr (!BACK) {
+      Op<IN> qr[TB][NC2];  // rows of q
+      // (rows and columns past the last ones are those again: nothing that is written comes of them)
+      const auto fetch_out = [&](int c) {
+        m.load(p.m + (head * NC + c) * (delta_tiles(Q) * 256));
+        const int last = min(Q, p.L - c * Q) - 1;
+#pragma unroll
+        for (int ob = 0; ob < TB; ++ob)
+#pragma unroll
+          for (int q = 0; q < NC2; ++q)
+            qr[ob][q] = row_op<T>(Qr + (first_row(c) + min(16 * ob + r, last)) * p.ldq + min(32 * q + 8 * g, p.N - 8));
+      };
+      // What is asked for past the last chunk is the last one again, and outputs past the last
+      // token are dropped by the buffers' ranges: no branches, so that a wait for loads waits for
+      // nothing that was sent after them
+      const auto stage = [&](int k) {
+        put(sh.side[(k + 1) & 1]);
+        fetch(chunk_of(min(k + 2, n - 1)));
+      };
+      fetch(chunk_of(0));
+      put(sh.side[0]);
+      fetch(chunk_of(min(1, n - 1)));
+      if (OUT) fetch_out(chunk_of(0));
+      __syncthreads();
+      __syncthreads();
+      stage(0);
+      __syncthreads();
+#pragma unroll 1
+      for (int k = 1; k <= n; ++k) {
+        if constexpr (!OUT) {
+          __syncthreads();
+          stage(k);
+          __syncthreads();
+          continue;
+        }
+        // the outputs of the chunk before
+        const DeltaTok<Q>& tok = sh.side[(k - 1) & 1].tok;
+        Op<MID> so[NC2];
+        f4 x[TB], u[TB];
+        float eq[TB];
+#pragma unroll
+        for (int q = 0; q < NC2; ++q)
+#pragma unroll
+          for (int a = 0; a < MID; ++a) so[q].v[a] = sh.s[w][a][q][l];
+#pragma unroll
+        for (int ob = 0; ob < TB; ++ob) {
+          x[ob] = sh.x[w][ob][l];
+          u[ob] = x[ob] * tok.four(tok.beta, 16 * ob + 4 * g);
+          eq[ob] = tok.eq[16 * ob + r];
+        }
+        __syncthreads();  // what was handed over has been read
+        const int c = chunk_of(k - 1), left = min(Q, p.L - c * Q);
+        // (x is no number from the first token on whose row is not finite: ttt_delta.h)
+        const int bad = first_not_finite(x);
+        if (__ballot(bad < Q) != 0) {
+#pragma unroll
+          for (int ob = 0; ob < TB; ++ob)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) u[ob][e] = 16 * ob + 4 * g + e < bad ? u[ob][e] : 0.f;
+        }
+        f4 y[TB];
+#pragma unroll
+        for (int ob = 0; ob < TB; ++ob) {
+          y[ob] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int q = 0; q < NC2; ++q) mma<MID>(y[ob], so[q], qr[ob][q]);
+          y[ob] *= eq[ob];
+        }
+        Op<MID> uo[QB];
+#pragma unroll
+        for (int q = 0; q < QB; ++q) uo[q] = split8<MID>(u[2 * q], u[2 * q + 1]);
+#pragma unroll
+        for (int ob = 0; ob < TB; ++ob)
+#pragma unroll
+          for (int q = 0; q < QB; ++q)
+            if (meets(false, ob, 2 * q)) mma<MID>(y[ob], uo[q], m.template op<MID>(ob, q));
+        if (__ballot(bad < Q) != 0) {  // (a lane has the features 4g + e of a token here)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int first = __shfl(bad, 4 * g + e);
+#pragma unroll
+            for (int ob = 0; ob < TB; ++ob) y[ob][e] = 16 * ob + r < first ? y[ob][e] : __builtin_nanf("");
+          }
+        }
+        fetch_out(chunk_of(min(k, n - 1)));
+        const rsrc_t rows = make_rsrc(p.rows + ((chain * NC + c) * Q) * PB + f0 + 16 * w,
+                                      p.rows != nullptr ? (unsigned)(Q * PB * 4) : 0u);
+        const int at_row = (4 * g * PB + r) * 4, at_o = (r * (int)ldo + 4 * g) * (int)sizeof(T);
+#pragma unroll
+        for (int ob = 0; ob < TB; ++ob)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) bstore_f32(rows, at_row + (16 * ob + e) * PB * 4, 0, x[ob][e]);
+        const rsrc_t out = make_rsrc(static_cast<T*>(p.o) + first_row(c) * ldo + (long long)hp * PB + f0 + 16 * w,
+                                     (unsigned)left * (unsigned)ldo * (unsigned)sizeof(T));
+#pragma unroll
+        for (int ob = 0; ob < TB; ++ob)
+          bstore_frag<T>(out, at_o + 16 * ob * (int)ldo * (int)sizeof(T), 0, to_frag<T>(y[ob]));
+        stage(k);
+        __syncthreads();
+      }
+    } else {
+      const auto fetch_do = [&](int c) {
+        const int left = min(Q, p.L - c * Q);
+        sq.load(Qr + first_row(c) * p.ldq, left);
+        sv.load(V + first_row(c) * ldv, features ? left : 0);
+      };
+      f4 eq[QB][2];
+      const auto fetch_m = [&](int c) {
+        m.load(p.m + (head * NC + c) * (delta_tiles(Q) * 256));
+        const float* of = p.tok + (head * NC + c) * delta_tok_floats(Q) + 7 * Q + 4 * g;
+#pragma unroll
+        for (int q = 0; q < QB; ++q)
+#pragma unroll
+          for (int o = 0; o < 2; ++o) eq[q][o] = *reinterpret_cast<const f4*>(of + 32 * q + 16 * o);
+      };
+      const auto put_do = [&] {
+        sq.store(sh.q);
+        sv.store(sh.dO);
+      };
+      // M^T do and Q^T do, the latter with its factors
+      f4 md[TB], qd[NB];
+      const auto form = [&] {
+        Op<IN> dt[QB];  // do: free feature, contracted token
+#pragma unroll
+        for (int q = 0; q < QB; ++q) dt[q] = sh.dO.template cols<>(32 * q, 16 * w);
+#pragma unroll
+        for (int ob = 0; ob < TB; ++ob) {
+          md[ob] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int q = 0; q < QB; ++q)
+            if (meets(true, ob, 2 * q + 1)) mma<kFull>(md[ob], m.template op<kFull>(ob, q), dt[q]);
+        }
+#pragma unroll
+        for (int i = 0; i < NB; ++i) qd[i] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int q = 0; q < QB; ++q) {
+          const Op<kFull> d = split8<kFull>(join4(dt[q], 0) * eq[q][0], join4(dt[q], 1) * eq[q][1]);
+#pragma unroll
+          for (int i = 0; i < NB; ++i) mma<kFull>(qd[i], sh.q.template cols<true>(32 * q, 32 * (i >> 1) + 4 * (i & 1)), d);
+        }
+      };
+      const auto hand = [&] {
+#pragma unroll
+        for (int ob = 0; ob < TB; ++ob) sh.md[w][ob][l] = md[ob];
+#pragma unroll
+        for (int i = 0; i < NB; ++i) sh.qd[w][i][l] = qd[i];
+      };
+      fetch(chunk_of(0));
+      fetch_do(chunk_of(0));
+      fetch_m(chunk_of(0));
+      put(sh.side[0]);
+      put_do();
+      __syncthreads();
+      form();
+      hand();
+      if (n > 1) {
+        fetch(chunk_of(1));
+        fetch_do(chunk_of(1));
+        fetch_m(chunk_of(1));
+      }
+      __syncthreads();
+      if (n > 1) put_do();
+      __syncthreads();
+#pragma unroll 1
+      for (int k = 0; k < n; ++k) {
+        if (k + 2 < n) fetch_do(chunk_of(k + 2));
+        if (k + 1 < n) {
+          form();
+          if (k + 2 < n) fetch_m(chunk_of(k + 2));
+        }
+        __syncthreads();  // what was handed over has been read, and so have q and do
+        if (k + 1 < n) {
+          hand();
+          put(sh.side[(k + 1) & 1]);
+          if (k + 2 < n) {
+            fetch(chunk_of(k + 2));
+            put_do();
+          }
+        }
+        __syncthreads();
+      }
+    }
+    return;
+  }
 
   StateTiles<NP> st;
   if (!OUT) {
@@ -131,86 +389,48 @@ __global__ __launch_bounds__(64 * W) void delta_walk_kernel(DeltaParams p) {
   } else {
     st.load(p.h0 != nullptr ? p.h0 + (chain * PB + f0) * p.N : nullptr, p.N, p.N, w);
   }
-
-  Stage<T, Q, NP, NT> sk, sq;
-  Stage<T, Q, 16 * W, NT> sv;
-  Blocks<Q, W, BACK> bz, bm;
-  Copy<delta_tok_floats(Q), NT> ct;
-  sk.place(p.ldk, p.N);
-  sq.place(p.ldq, p.N);
-  sv.place(ldv, 16 * W);
-  const auto fetch = [&](int c) {
-    const int left = min(Q, p.L - c * Q);
-    const long long row = (long long)b * p.L + (long long)c * Q, chunk = head * NC + c;
-    sk.load(K + row * p.ldk, left);
-    sv.load(V + row * ldv, features ? left : 0);
-    bz.load(p.z + chunk * (delta_tiles(Q) * 256), w);
-    if constexpr (READS) {
-      sq.load(Qr + row * p.ldq, left);
-      bm.load(p.m + chunk * (delta_tiles(Q) * 256), w);
-    }
-    ct.load(p.tok + chunk * delta_tok_floats(Q));
-  };
-  const auto z_op = [&](int u) {
-    Op<kFull> o;
-#pragma unroll
-    for (int a = 0; a < kFull; ++a) o.v[a] = sh.z[a][u][l];
-    return o;
-  };
-  const auto m_op = [&](int u) {
-    Op<MP> o;
-#pragma unroll
-    for (int a = 0; a < MP; ++a) o.v[a] = sh.m[a][u][l];
-    return o;
-  };
-  const auto chunk_of_step = [&](int k) { return BACK ? c0 + n - 1 - k : c0 + k; };
-  fetch(chunk_of_step(0));
-  // (an operand's half beside the triangle stays 0)
-  for (int i = threadIdx.x; i < (int)(offsetof(Sh, tok) - offsetof(Sh, z)) / 16; i += NT)
-    reinterpret_cast<f4*>(&sh.z)[i] = f4{0.f, 0.f, 0.f, 0.f};
   __syncthreads();
+  if constexpr (BACK) {
+    __syncthreads();
+    __syncthreads();
+  }
 #pragma unroll 1
   for (int k = 0; k < n; ++k) {
-    const int c = chunk_of_step(k);
-    if (k > 0) __syncthreads();  // the last chunk's readers are done
-    sk.store(sh.k);
-    sv.store(sh.v);
-    bz.template store<kFull>(sh.z, w);
-    if constexpr (READS) {
-      sq.store(sh.q);
-      bm.template store<MP>(sh.m, w);
-    }
-    ct.store(sh.tok.hi);
-    __syncthreads();
-    if (k + 1 < n) fetch(chunk_of_step(k + 1));
+    const int c = chunk_of(k);
+    const typename Sh::Side& in = sh.side[k & 1];
+    const DeltaTok<Q>& tok = in.tok;
     if (OUT && p.states != nullptr) st.keep(p.states + (chain * NC + c) * (long long)(NP * PB) + f0, PB, w);
-    const DeltaTok<Q>& tok = sh.tok;
-    const int left = p.L - c * Q;
-    const long long row = (long long)b * p.L + (long long)c * Q;
-
     f4 t[TB];  // K S, rows tokens
 #pragma unroll
     for (int ob = 0; ob < TB; ++ob) t[ob] = f4{0.f, 0.f, 0.f, 0.f};
+    Op<kFull> so[NC2];
 #pragma unroll
     for (int q = 0; q < NC2; ++q) {
-      const Op<kFull> s = st.template op<kFull>(q);
+      so[q] = st.template op<kFull>(q);
 #pragma unroll
-      for (int ob = 0; ob < TB; ++ob) mma<kFull>(t[ob], sh.k.rows(16 * ob, 32 * q), s);
+      for (int ob = 0; ob < TB; ++ob) mma<kFull>(t[ob], in.k.rows(16 * ob, 32 * q), so[q]);
     }
-    Op<IN> vt[QB];  // v or do: free feature, contracted token
+    f4 qd[BACK ? NB : 1];
+    if constexpr (BACK) {  // du
 #pragma unroll
-    for (int q = 0; q < QB; ++q) vt[q] = sh.v.template cols<>(32 * q, 16 * w);
-    // r, or du
+      for (int ob = 0; ob < TB; ++ob) t[ob] = t[ob] * tok.four(tok.wr, 16 * ob + 4 * g) + sh.md[w][ob][l];
 #pragma unroll
-    for (int ob = 0; ob < TB; ++ob) {
-      const int i = 16 * ob + 4 * g;
-      if constexpr (BACK) {
-        t[ob] *= tok.four(tok.wr, i);
+      for (int i = 0; i < NB; ++i) qd[i] = sh.qd[w][i][l];
+    } else {  // r
 #pragma unroll
-        for (int q = 0; q < QB; ++q)
-          if (meets(true, ob, 2 * q + 1)) mma<kFull>(t[ob], m_op(pair_at(true, Q, ob, q)), vt[q]);
-      } else {
-        t[ob] = join4(vt[ob / 2], ob & 1) - t[ob] * tok.four(tok.er, i);
+      for (int q = 0; q < QB; ++q) {
+        const Op<IN> v = in.v.template cols<>(32 * q, 16 * w);
+#pragma unroll
+        for (int o = 0; o < 2; ++o) t[2 * q + o] = join4(v, o) - t[2 * q + o] * tok.four(tok.er, 32 * q + 16 * o + 4 * g);
+      }
+    }
+    if constexpr (!BACK) {
+      __syncthreads();
+      if constexpr (OUT) {
+#pragma unroll
+        for (int q = 0; q < NC2; ++q)
+#pragma unroll
+          for (int a = 0; a < MID; ++a) sh.s[w][a][q][l] = so[q].v[a];
       }
     }
     // x = r - Z b r, or y = du - Z^T b du
@@ -233,105 +453,69 @@ __global__ __launch_bounds__(64 * W) void delta_walk_kernel(DeltaParams p) {
 #pragma unroll
       for (int q = 0; q < QB; ++q) br[q] = split8<kFull>(by[2 * q], by[2 * q + 1]);
     }
-    f4 u[TB];  // b x, or dv
 #pragma unroll
     for (int ob = 0; ob < TB; ++ob) {
       f4 s = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int q = 0; q < QB; ++q)
-        if (BACK ? meets(true, ob, 2 * q + 1) : meets(false, ob, 2 * q)) mma<kFull>(s, z_op(pair_at(BACK, Q, ob, q)), br[q]);
+        if (BACK ? meets(true, ob, 2 * q + 1) : meets(false, ob, 2 * q)) {
+          Op<kFull> z;
+#pragma unroll
+          for (int a = 0; a < kFull; ++a) z.v[a] = in.z[a][pair_at(BACK, Q, ob, q)][l];
+          mma<kFull>(s, z, br[q]);
+        }
       t[ob] -= s;
-      u[ob] = t[ob] * tok.four(tok.beta, 16 * ob + 4 * g);
     }
     if constexpr (!BACK) {
       if (__ballot(bad < Q) != 0) {
 #pragma unroll
         for (int ob = 0; ob < TB; ++ob)
 #pragma unroll
+          for (int e = 0; e < 4; ++e) t[ob][e] = 16 * ob + 4 * g + e < bad ? t[ob][e] : __builtin_nanf("");
+      }
+      if constexpr (OUT) {
+#pragma unroll
+        for (int ob = 0; ob < TB; ++ob) sh.x[w][ob][l] = t[ob];
+      }
+    }
+    f4 u[TB];  // b x, or dv
+#pragma unroll
+    for (int ob = 0; ob < TB; ++ob) u[ob] = t[ob] * tok.four(tok.beta, 16 * ob + 4 * g);
+    if constexpr (BACK) {
+      __syncthreads();
+      if constexpr (OUT) {
+        float* rows = p.rows + ((chain * NC + c) * Q) * PB + f0 + 16 * w + r;
+        const int left = p.L - c * Q;
+        T* to = static_cast<T*>(p.o) + first_row(c) * ldo + (long long)hp * PB + f0 + 16 * w + r;
+#pragma unroll
+        for (int ob = 0; ob < TB; ++ob) {
+          const auto d = to_frag<T>(u[ob]).v;
+#pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const bool keep = 16 * ob + 4 * g + e < bad;
-            u[ob][e] = keep ? u[ob][e] : 0.f;
-            t[ob][e] = keep ? t[ob][e] : __builtin_nanf("");
+            const int i = 16 * ob + 4 * g + e;
+            rows[i * PB] = t[ob][e];
+            if (i < left) to[i * ldo] = d[e];
           }
-      }
-    }
-    if (OUT && p.rows != nullptr) {
-      float* to = p.rows + ((chain * NC + c) * Q) * PB + f0 + 16 * w + r;
-#pragma unroll
-      for (int ob = 0; ob < TB; ++ob)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) to[(16 * ob + 4 * g + e) * PB] = t[ob][e];
-    }
-    if constexpr (!OUT) {
-    } else if constexpr (BACK) {
-      T* to = O + row * ldo + 16 * w + r;
-#pragma unroll
-      for (int ob = 0; ob < TB; ++ob) {
-        const auto d = to_frag<T>(u[ob]).v;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int i = 16 * ob + 4 * g + e;
-          if (i < left) to[i * ldo] = d[e];
         }
       }
-    } else {
-      f4 y[TB];
-#pragma unroll
-      for (int ob = 0; ob < TB; ++ob) y[ob] = f4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int q = 0; q < NC2; ++q) {
-        const Op<MID> s = st.template op<MID>(q);
-#pragma unroll
-        for (int ob = 0; ob < TB; ++ob) mma<MID>(y[ob], s, sh.q.rows(16 * ob, 32 * q));
-      }
-      Op<MID> uo[QB];
-#pragma unroll
-      for (int q = 0; q < QB; ++q) uo[q] = split8<MID>(u[2 * q], u[2 * q + 1]);
-#pragma unroll
-      for (int ob = 0; ob < TB; ++ob) {
-        const int i = 16 * ob + r;
-        y[ob] *= tok.eq[i];
-#pragma unroll
-        for (int q = 0; q < QB; ++q)
-          if (meets(false, ob, 2 * q)) mma<MID>(y[ob], uo[q], m_op(pair_at(false, Q, ob, q)));
-      }
-      if (__ballot(bad < Q) != 0) {  // (a lane has the features 4g + e of a token here)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int first = __shfl(bad, 4 * g + e);
-#pragma unroll
-          for (int ob = 0; ob < TB; ++ob) y[ob][e] = 16 * ob + r < first ? y[ob][e] : __builtin_nanf("");
-        }
-      }
-#pragma unroll
-      for (int ob = 0; ob < TB; ++ob)
-        if (16 * ob + r < left) store4(O + (row + 16 * ob + r) * ldo + 16 * w + 4 * g, y[ob]);
     }
     // the state behind the chunk, or the gradient of the one before it
     const float end = tok.end;
 #pragma unroll
-    for (int i = 0; i < NB; ++i) st.t[i] *= end;
+    for (int i = 0; i < NB; ++i) {
+      st.t[i] *= end;
+      if constexpr (BACK) st.t[i] += qd[i];
+    }
 #pragma unroll
     for (int q = 0; q < QB; ++q) {
-      f4 a[2], d[2];
+      f4 d[2];
 #pragma unroll
-      for (int o = 0; o < 2; ++o) {
-        const int i = 32 * q + 16 * o + 4 * g;
-        if constexpr (BACK) {
-          a[o] = join4(vt[q], o) * tok.four(tok.eq, i);
-          d[o] = u[2 * q + o] * tok.four(tok.er, i) * -1.f;
-        } else {
-          d[o] = u[2 * q + o] * tok.four(tok.wr, i);
-        }
-      }
+      for (int o = 0; o < 2; ++o)
+        d[o] = BACK ? u[2 * q + o] * tok.four(tok.er, 32 * q + 16 * o + 4 * g) * -1.f
+                    : u[2 * q + o] * tok.four(tok.wr, 32 * q + 16 * o + 4 * g);
       const Op<kFull> dk = split8<kFull>(d[0], d[1]);
 #pragma unroll
-      for (int i = 0; i < NB; ++i) mma<kFull>(st.t[i], sh.k.template cols<true>(32 * q, 32 * (i >> 1) + 4 * (i & 1)), dk);
-      if constexpr (BACK) {
-        const Op<kFull> dq = split8<kFull>(a[0], a[1]);
-#pragma unroll
-        for (int i = 0; i < NB; ++i) mma<kFull>(st.t[i], sh.q.template cols<true>(32 * q, 32 * (i >> 1) + 4 * (i & 1)), dq);
-      }
+      for (int i = 0; i < NB; ++i) mma<kFull>(st.t[i], in.k.template cols<true>(32 * q, 32 * (i >> 1) + 4 * (i & 1)), dk);
     }
     if constexpr (!BACK) {
       if (__ballot(bad < Q) != 0) {
@@ -341,6 +525,11 @@ __global__ __launch_bounds__(64 * W) void delta_walk_kernel(DeltaParams p) {
           for (int e = 0; e < 4; ++e) st.t[i][e] = bad < Q ? __builtin_nanf("") : st.t[i][e];
       }
     }
+    __syncthreads();
+  }
+  if constexpr (!BACK) {  // the helpers' last outputs
+    __syncthreads();
+    __syncthreads();
   }
   if (!OUT) {
     if (features)
@@ -352,47 +541,55 @@ __global__ __launch_bounds__(64 * W) void delta_walk_kernel(DeltaParams p) {
   }
 }
 
-// The segments' ends -> the states they start from, in place: a wave has 16 features of a part and
-// goes over the segments, the next one's product on its way.
-template <int NP, bool BACK> __global__ __launch_bounds__(64) void delta_join_kernel(DeltaParams p) {
+// The segments' ends -> the states they start from, in place: a workgroup has 16 features of a
+// part and goes over the segments, a wave to 16 rows of the state, which go from one to the next
+// through LDS; the next segment's product is on its way.
+template <int NP, bool BACK> __global__ __launch_bounds__(4 * NP) void delta_join_kernel(DeltaParams p) {
   constexpr int NB = NP / 16, NC2 = NP / 32;
-  const int l = lane_id(), g = l >> 4, r = l & 15;
-  const int PB = delta_part(p.P), cols = PB / 16, parts = p.P / PB;
-  const int w = (int)(blockIdx.x % cols);
+  __shared__ Planes<kFull, 16, NP> sh[2];  // features by n
+  const int w = wave_id(), l = lane_id(), g = l >> 4, r = l & 15;
+  const int PB = delta_part(p.P), cols = PB / 16, parts = p.P / PB, f = 16 * (int)(blockIdx.x % cols) + r;
   const long long chain = blockIdx.x / cols, head = chain / parts;
-  StateTiles<NP> st, end;
-  st.load(p.h0 != nullptr ? p.h0 + chain * PB * p.N : nullptr, p.N, p.N, w);
+  const int n = 16 * w + 4 * g;  // a lane's rows
+  f4 st = f4{0.f, 0.f, 0.f, 0.f}, end;
+  if (p.h0 != nullptr && n < p.N) st = *reinterpret_cast<const f4*>(p.h0 + (chain * PB + f) * p.N + n);
   const auto seg = [&](int k) { return BACK ? p.S - 1 - k : k; };
-  const auto at = [&](int k) { return p.seg + (chain * p.S + seg(k)) * (NP * PB); };
-  f4 a[NB][NC2][2];  // rows n as a state's tiles have them, columns 32q + 8g..
+  const auto at = [&](int k) { return p.seg + (chain * p.S + seg(k)) * (NP * PB) + n * PB + f; };
+  f4 a[NC2][2];  // row 16 w + r, columns 32q + 8g..
   const auto fetch = [&](int k) {
-    const float* t = p.trans + (head * p.S + seg(k)) * (NP * NP);
+    const float* t = p.trans + (head * p.S + seg(k)) * (NP * NP) + (16 * w + r) * NP + 8 * g;
 #pragma unroll
-    for (int i = 0; i < NB; ++i)
+    for (int q = 0; q < NC2; ++q)
 #pragma unroll
-      for (int q = 0; q < NC2; ++q)
+      for (int o = 0; o < 2; ++o) a[q][o] = *reinterpret_cast<const f4*>(t + 32 * q + 4 * o);
 #pragma unroll
-        for (int o = 0; o < 2; ++o)
-          a[i][q][o] = *reinterpret_cast<const f4*>(
-              t + (32 * (i >> 1) + 8 * (r >> 2) + 4 * (i & 1) + (r & 3)) * NP + 32 * q + 8 * g + 4 * o);
-    take_kept(end, at(k), PB, w);
+    for (int e = 0; e < 4; ++e) end[e] = at(k)[e * PB];
+  };
+  const auto keep = [&](int k, f4 v) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) at(k)[e * PB] = v[e];
   };
   fetch(0);
 #pragma unroll 1
   for (int k = 0; k + 1 < p.S; ++k) {
-    st.keep(at(k), PB, w);
-    Op<kFull> s[NC2];
+    Planes<kFull, 16, NP>& of = sh[k & 1];
+    bf4 o[kFull];
+    split4<kFull>(st, o);
 #pragma unroll
-    for (int q = 0; q < NC2; ++q) s[q] = st.template op<kFull>(q);
+    for (int q = 0; q < kFull; ++q) *reinterpret_cast<bf4*>(&of.d[q][r][n]) = o[q];
+    Op<kFull> m[NC2];
 #pragma unroll
-    for (int i = 0; i < NB; ++i) {
-      st.t[i] = end.t[i];
-#pragma unroll
-      for (int q = 0; q < NC2; ++q) mma<kFull>(st.t[i], split8<kFull>(a[i][q][0], a[i][q][1]), s[q]);
-    }
+    for (int q = 0; q < NC2; ++q) m[q] = split8<kFull>(a[q][0], a[q][1]);
+    const f4 last = st;
+    st = end;
+    // (two places in turn: a wave is at most one segment ahead of another)
+    __syncthreads();
+    keep(k, last);
     if (k + 2 < p.S) fetch(k + 1);
+#pragma unroll
+    for (int q = 0; q < NC2; ++q) mma<kFull>(st, m[q], of.rows(0, 32 * q));
   }
-  st.keep(at(p.S - 1), PB, w);
+  keep(p.S - 1, st);
 }
 
 template <typename T, int W, int NP, bool BACK> hipError_t walk_t(const DeltaParams& p, hipStream_t stream) {
@@ -405,15 +602,16 @@ template <typename T, int W, int NP, bool BACK> hipError_t walk_t(const DeltaPar
     e = allow_lds(delta_walk_kernel<T, W, NP, BACK, false>, lds);
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL((delta_walk_kernel<T, W, NP, BACK, false>), dim3((unsigned)(heads * (p.S - 1) * (p.P + NP) / (16 * W))),
-                       dim3(64 * W), lds, stream, p);
-    hipLaunchKernelGGL((delta_join_kernel<NP, BACK>), dim3((unsigned)(heads * p.P / 16)), dim3(64), 0, stream, p);
+                       dim3(128 * W), lds, stream, p);
+    hipLaunchKernelGGL((delta_join_kernel<NP, BACK>), dim3((unsigned)(heads * p.P / 16)), dim3(4 * NP), 0, stream,
+                       p);
   }
-  hipLaunchKernelGGL((delta_walk_kernel<T, W, NP, BACK, true>), dim3((unsigned)(heads * p.S * p.P / (16 * W))), dim3(64 * W),
+  hipLaunchKernelGGL((delta_walk_kernel<T, W, NP, BACK, true>), dim3((unsigned)(heads * p.S * p.P / (16 * W))), dim3(128 * W),
                      lds, stream, p);
   return hipGetLastError();
 }
 template <typename T, int W, bool BACK> hipError_t width_t(const DeltaParams& p, hipStream_t s) {
-  return p.N <= 32 ? walk_t<T, W, 32, BACK>(p, s) : p.N <= 64 ? walk_t<T, W, 64, BACK>(p, s) : walk_t<T, W, 128, BACK>(p, s);
+  return p.N <= 32 ? walk_t<T, W, 32, BACK>(p, s) : p.N <= 64 ? walk_t<T, W, 64, BACK>(p, s) : walk_t<T, 2, 128, BACK>(p, s);
 }
 template <typename T, bool BACK> hipError_t part_t(const DeltaParams& p, hipStream_t s) {
   return delta_part(p.P) == 64 ? width_t<T, 4, BACK>(p, s) : width_t<T, 2, BACK>(p, s);
