@@ -28,7 +28,7 @@ namespace ttt {
 
 namespace {
 
-template <typename T, int W, int NP, bool BACK> struct WalkShared {
+template <typename T, int W, int NP, bool BACK, bool OUT> struct WalkShared {
   static constexpr int IN = ScanType<T>::IN, MID = ScanType<T>::MID, Q = kDeltaQ<T>, PAIRS = delta_pairs(Q);
   static constexpr int TB = Q / 16, NB = NP / 16, NC2 = NP / 32;
   struct alignas(16) Side {  // a chunk's, in turn
@@ -41,9 +41,10 @@ template <typename T, int W, int NP, bool BACK> struct WalkShared {
   Planes<IN, BACK ? Q : 1, NP> q;
   Planes<IN, BACK ? Q : 1, 16 * W> dO;
   // what is handed over
-  bf8 s[BACK ? 1 : W][BACK ? 1 : MID][BACK ? 1 : NC2][64];
-  f4 x[BACK ? 1 : W][BACK ? 1 : TB][64];
-  f4 md[BACK ? W : 1][BACK ? TB : 1][64], qd[BACK ? W : 1][BACK ? NB : 1][64];
+  static constexpr bool YS = OUT && !BACK;
+  bf8 s[YS ? W : 1][YS ? MID : 1][YS ? NC2 : 1][YS ? 64 : 1];
+  f4 x[YS ? W : 1][YS ? TB : 1][YS ? 64 : 1];
+  f4 md[BACK ? W : 1][BACK ? TB : 1][BACK ? 64 : 1], qd[BACK ? W : 1][BACK ? NB : 1][BACK ? 64 : 1];
 };
 
 // a chunk's blocks of Z on their way from memory to operands in planes
@@ -130,7 +131,7 @@ template <typename T> __device__ __forceinline__ Op<ScanType<T>::IN> row_op(cons
 // OUT: outputs too; else the segments' ends alone
 template <typename T, int W, int NP, bool BACK, bool OUT>
 __global__ __launch_bounds__(128 * W) void delta_walk_kernel(DeltaParams p) {
-  using Sh = WalkShared<T, W, NP, BACK>;
+  using Sh = WalkShared<T, W, NP, BACK, OUT>;
   static_assert(offsetof(Sh, q) % 16 == 0 && offsetof(Sh, dO) % 16 == 0 && offsetof(Sh, s) % 16 == 0 &&
                     offsetof(Sh, x) % 16 == 0 && offsetof(typename Sh::Side, z) % 16 == 0 &&
                     offsetof(typename Sh::Side, tok) % 16 == 0 && offsetof(typename Sh::Side, v) % 16 == 0,
@@ -593,16 +594,16 @@ template <int NP, bool BACK> __global__ __launch_bounds__(4 * NP) void delta_joi
 }
 
 template <typename T, int W, int NP, bool BACK> hipError_t walk_t(const DeltaParams& p, hipStream_t stream) {
-  constexpr size_t lds = sizeof(WalkShared<T, W, NP, BACK>);
+  constexpr size_t lds = sizeof(WalkShared<T, W, NP, BACK, true>), lds1 = sizeof(WalkShared<T, W, NP, BACK, false>);
   static_assert(lds <= 160 * 1024, "LDS of a compute unit");
   hipError_t e = allow_lds(delta_walk_kernel<T, W, NP, BACK, true>, lds);
   if (e != hipSuccess) return e;
   const long long heads = (long long)p.B * p.H;
   if (p.S > 1) {
-    e = allow_lds(delta_walk_kernel<T, W, NP, BACK, false>, lds);
+    e = allow_lds(delta_walk_kernel<T, W, NP, BACK, false>, lds1);
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL((delta_walk_kernel<T, W, NP, BACK, false>), dim3((unsigned)(heads * (p.S - 1) * (p.P + NP) / (16 * W))),
-                       dim3(128 * W), lds, stream, p);
+                       dim3(128 * W), lds1, stream, p);
     hipLaunchKernelGGL((delta_join_kernel<NP, BACK>), dim3((unsigned)(heads * p.P / 16)), dim3(4 * NP), 0, stream,
                        p);
   }
