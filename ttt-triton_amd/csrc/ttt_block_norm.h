@@ -37,7 +37,7 @@ constexpr int kBlockNormMaxD = 8192;
 // res_dtype: the residual's type, or -1 without one
 hipError_t launch_block_norm_fwd(const BlockNormParams& p, int dtype, int res_dtype, hipStream_t stream);
 hipError_t launch_block_norm_bwd(const BlockNormParams& p, int dtype, int res_dtype, hipStream_t stream);
-int block_norm_parts(long long R, int D);
+int block_norm_parts(long long R, int D, int waves = 3);
 
 // lanes to a row
 constexpr int block_lanes(int D) { return D <= 64 ? 8 : D <= 128 ? 16 : D <= 256 ? 32 : D <= 1024 ? 64 : D <= 4096 ? 256 : 512; }

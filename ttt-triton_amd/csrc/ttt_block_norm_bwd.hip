@@ -11,8 +11,17 @@ namespace ttt {
 
 namespace {
 
-template <typename T, typename TR, int LANES, int V, int NCH>
-__global__ __launch_bounds__(block_threads(LANES)) void block_norm_bwd_kernel(BlockNormParams p) {
+// Waves to a SIMD that the registers are cut to: three where a lane has up to 12 values and no gate
+// beside a residual, or fp32 beside one (32,768 rows of 768 in bf16 with an fp32 residual: 114 us, 138 with
+// the two that fit without, the workgroups in one and a half rounds); one where 16 values, a gate and a
+// residual would spill a hundred registers
+template <typename T, typename TR, bool GATE, int LANES, int V, int NCH>
+constexpr int kWaves = V * NCH <= 12 && LANES < 512 && (__is_same(TR, NoResidual) || (!GATE && sizeof(T) == 2)) ? 3
+                       : V * NCH == 16 && GATE && !__is_same(TR, NoResidual) && LANES < 512                   ? 1
+                                                                                                             : 2;
+
+template <typename T, typename TR, bool GATE, int LANES, int V, int NCH>
+__global__ __launch_bounds__(block_threads(LANES), (kWaves<T, TR, GATE, LANES, V, NCH>)) void block_norm_bwd_kernel(BlockNormParams p) {
   constexpr bool RES = !__is_same(TR, NoResidual);
   typedef typename ResidualOf<TR, T>::type R;
   constexpr int NT = block_threads(LANES), ROWS = NT / LANES;
@@ -42,7 +51,7 @@ __global__ __launch_bounds__(block_threads(LANES)) void block_norm_bwd_kernel(Bl
       const int c = V * (LANES * i + l), left = D - c;
       if (left > 0) {
         nx[i].load(static_cast<const T*>(p.x) + outer * p.ldx + in + c, left);
-        if (p.gate != nullptr) nz[i].load(static_cast<const T*>(p.gate) + outer * p.ldg + in + c, left);
+        if (GATE) nz[i].load(static_cast<const T*>(p.gate) + outer * p.ldg + in + c, left);
         if (p.dr != nullptr) nr[i].load(static_cast<const R*>(p.dr) + row * D + c, left);
         if (next) {
           nres[i].load(static_cast<const R*>(p.res) + outer * p.ldr + in + c, left);
@@ -57,8 +66,8 @@ __global__ __launch_bounds__(block_threads(LANES)) void block_norm_bwd_kernel(Bl
   if (row < p.R) fetch(row);
   for (; row < p.R; row += step) {
     const float inv = ni, jnv = nj;
-    // x i, n without w; k = s silu(z), kz = s silu'(z); D
-    float u[NCH][V], k[NCH][V], kz[NCH][V], d[NCH][V], g[NCH][V], q[NCH][V];
+    // x i; silu(z) and n silu'(z); D; and r j, then dn w
+    float u[NCH][V], si[GATE ? NCH : 1][V], dsi[GATE ? NCH : 1][V], d[NCH][V], g[NCH][V];
     float s2 = 0.f;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
@@ -66,35 +75,32 @@ __global__ __launch_bounds__(block_threads(LANES)) void block_norm_bwd_kernel(Bl
       Raw<float, V> w, sc, w2;
       if (left > 0) {
         if (p.w != nullptr) w.load(p.w + c, left);
-        if (p.s != nullptr) sc.load(p.s + c, left);
+        if (p.s != nullptr && next) sc.load(p.s + c, left);
         if (next) w2.load(p.w2 + c, left);
       }
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         u[i][e] = nx[i].f(e) * inv;
-        float si = 1.f, dsi = 0.f;
-        if (p.gate != nullptr) {
+        const float n = u[i][e] * (p.w != nullptr && e < left ? w.v[e] : 1.f);
+        float of = n;  // what the residual is added to
+        if (GATE) {
           const float z = nz[i].f(e), sg = sigmoid_f(z);
-          si = z * sg;
-          dsi = sg * __builtin_fmaf(z, 1.0f - sg, 1.0f);
+          si[i][e] = z * sg;
+          dsi[i][e] = n * sg * __builtin_fmaf(z, 1.0f - sg, 1.0f);
+          of *= si[i][e];
         }
-        const float scale = p.s != nullptr && e < left ? sc.v[e] : 1.f;
-        const float we = p.w != nullptr && e < left ? w.v[e] : 1.f;
-        const float n = u[i][e] * we;
-        k[i][e] = si * scale;
-        kz[i][e] = dsi * scale * n;
         d[i][e] = nr[i].f(e);
-        q[i][e] = n * si;     // what the scale multiplies
         g[i][e] = 0.f;
         if (next) {
-          const float r = nres[i].f(e) + n * k[i][e], dy = ny[i].f(e), rj = r * jnv;
+          if (p.s != nullptr && e < left) of *= sc.v[e];
+          const float dy = ny[i].f(e), rj = (nres[i].f(e) + of) * jnv;
           if (e < left) {
-            g[i][e] = dy * w2.v[e];
+            const float dyw = dy * w2.v[e];
             dw2[i][e] = __builtin_fmaf(dy, rj, dw2[i][e]);
-            s2 = __builtin_fmaf(g[i][e], rj, s2);
+            s2 = __builtin_fmaf(dyw, rj, s2);
+            d[i][e] = __builtin_fmaf(dyw, jnv, d[i][e]);
           }
-          d[i][e] = __builtin_fmaf(g[i][e], jnv, d[i][e]);
-          g[i][e] = rj;       // from here on r j
+          g[i][e] = rj;
         }
       }
     }
@@ -112,22 +118,21 @@ __global__ __launch_bounds__(block_threads(LANES)) void block_norm_bwd_kernel(Bl
       const int c = V * (LANES * i + l), left = D - c;
       if (left > 0) {
         if (RES && p.dres != nullptr) store_row<R, V>(static_cast<R*>(p.dres) + row * D + c, left, d[i]);
-        if (p.gate != nullptr) {
-          float dz[V];
-#pragma unroll
-          for (int e = 0; e < V; ++e) dz[e] = d[i][e] * kz[i][e];
-          store_row<T, V>(static_cast<T*>(p.dgate) + row * D + c, left, dz);
-        }
-        Raw<float, V> w;
+        Raw<float, V> w, sc;
         if (p.w != nullptr) w.load(p.w + c, left);
+        if (p.s != nullptr) sc.load(p.s + c, left);
+        float dz[V];
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          ds[i][e] = __builtin_fmaf(d[i][e], q[i][e], ds[i][e]);
-          const float dn = d[i][e] * k[i][e];
+          const float we = p.w != nullptr && e < left ? w.v[e] : 1.f, gate = GATE ? si[i][e] : 1.f;
+          ds[i][e] = __builtin_fmaf(d[i][e], u[i][e] * we * gate, ds[i][e]);
+          const float dm = p.s != nullptr && e < left ? d[i][e] * sc.v[e] : d[i][e], dn = dm * gate;
+          if (GATE) dz[e] = dm * dsi[i][e];
           dw[i][e] = __builtin_fmaf(dn, u[i][e], dw[i][e]);
-          g[i][e] = p.w != nullptr && e < left ? dn * w.v[e] : dn;
+          g[i][e] = dn * we;
           if (e < left) s1 = __builtin_fmaf(g[i][e], u[i][e], s1);
         }
+        if (GATE) store_row<T, V>(static_cast<T*>(p.dgate) + row * D + c, left, dz);
       }
     }
     const float m1 = p.w != nullptr ? share_sum<LANES>(s1, red) / (float)D : 0.f;
@@ -188,8 +193,14 @@ __global__ __launch_bounds__(256) void block_norm_param_grads_kernel(BlockNormPa
 template <typename T, typename TR> struct Bwd {
   template <int LANES, int V, int NCH> struct Of {
     static hipError_t run(const BlockNormParams& p, hipStream_t stream) {
-      const int parts = block_norm_parts(p.R, p.D);
-      hipLaunchKernelGGL((block_norm_bwd_kernel<T, TR, LANES, V, NCH>), dim3(parts), dim3(block_threads(LANES)), 0, stream, p);
+      const int parts = block_norm_parts(
+          p.R, p.D, p.gate != nullptr ? kWaves<T, TR, true, LANES, V, NCH> : kWaves<T, TR, false, LANES, V, NCH>);
+      if (p.gate != nullptr)
+        hipLaunchKernelGGL((block_norm_bwd_kernel<T, TR, true, LANES, V, NCH>), dim3(parts), dim3(block_threads(LANES)), 0,
+                           stream, p);
+      else
+        hipLaunchKernelGGL((block_norm_bwd_kernel<T, TR, false, LANES, V, NCH>), dim3(parts), dim3(block_threads(LANES)), 0,
+                           stream, p);
       if (p.partial != nullptr)
         hipLaunchKernelGGL(block_norm_param_grads_kernel, dim3(3 * ((p.D + 15) / 16)), dim3(256), 0, stream, p, parts);
       return hipGetLastError();
@@ -208,9 +219,11 @@ template <typename T> hipError_t residual_t(const BlockNormParams& p, int dtype,
 
 }  // namespace
 
-int block_norm_parts(long long R, int D) {
+// Workgroups of the backward: as many as are held at once with `waves` to a SIMD (the partial sums
+// are sized for three, of which there are the most)
+int block_norm_parts(long long R, int D, int waves) {
   const int lanes = block_lanes(D), rows = block_threads(lanes) / lanes;
-  const long long blocks = (R + rows - 1) / rows, most = lanes == 512 ? 512 : 768;
+  const long long blocks = (R + rows - 1) / rows, most = lanes == 512 ? 256 : 256 * waves;
   return (int)std::max(1LL, std::min(blocks, most));
 }
 hipError_t launch_block_norm_bwd(const BlockNormParams& p, int dtype, int res_dtype, hipStream_t s) {
