@@ -9,8 +9,9 @@ gated_delta  S_t = e^{g_t} S_{t-1} + u_t (x) k_t,  u_t = beta_t (v_t - e^{g_t} S
 Activations share one dtype (fp32, bf16 or fp16; g and beta may each be fp32 beside a
 16-bit v); states are fp32.  q, k, v, g and beta may be columns of a wider contiguous
 matrix of rows: they are read in place where q, k and v start on 16 bytes in every row,
-and from a copy elsewhere.  Results do not depend on which, nor on the other sequences of
-a batch.
+and from a copy elsewhere.  Results do not depend on which; nothing of a call depends on
+another sequence of its batch, but its rounding may: the length is cut up by the number of
+sequences and heads.
 
 Sums, states and their products are fp32; in bf16 calls what leads to bf16 results alone
 (the masked products of q and k, the state that an output reads) is rounded to 2^-17 of

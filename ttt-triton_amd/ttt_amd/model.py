@@ -23,6 +23,11 @@ SelectiveSSM is a third layer type beside them, a selective state-space layer on
 same projection GEMM and heads: short causal convolution, scan and gated norm (ssm.py,
 norm.py), with a form for single tokens that goes on from a prompt's state.
 
+GatedDeltaStack is a fourth: `num_layers` blocks of a gated delta-rule mixer (delta.py) and,
+where `ffn_dim` is given, a gated feed-forward (ffn.py), on an fp32 residual, with the norms
+around them, their gate and residual scales in one operator each (norm.block_norm); it goes
+on token by token as well.
+
 Parameter names and shapes of the TTT layers are the reference's (wq ... wu, wo,
 learnable_ttt_lr_weight [H,1,D], learnable_ttt_lr_bias [H,1],
 ttt_norm_weight/bias [H,F], post_norm, W1/b1/W2/b2), so a reference state
@@ -44,11 +49,13 @@ import torch
 import torch.nn.functional as Fn
 from torch import nn
 
+from .delta import gated_delta, gated_delta_step
+from .ffn import gated_linear
 from .layer_io import POST_NORM_EPS, RECON_EPS, PostNormFunction, ProducerFunction, rope_table
 from .linear import TTTLinearFunction
 from .memo import mlp_memo_combine
 from .mlp import LN_EPS, TTTMLPFunction
-from .norm import layer_norm
+from .norm import block_norm, layer_norm
 from .ssm import CONV_WIDTHS, MAX_STATE, causal_conv, causal_conv_step, selective_scan, selective_scan_step
 
 MAX_MODEL_DIM = 1024  # H * F, the widest row the producer / post-norm kernels take
@@ -125,18 +132,21 @@ class ModelConfig:
     latent_width: int = 1
     theta: float = 10000.0
     compressed_num_frames: Optional[int] = None
-    # ssm_layer "selective_scan": the state's width, the groups of heads that share B
-    # and C, and the convolution's width
+    # ssm_layer "selective_scan" and "gated_delta": the state's width, the groups of heads
+    # that share B and C, or q and k, and the convolution's width
     state_dim: int = 64
     num_groups: int = 1
     conv_width: int = 4
+    # "gated_delta": the feed-forward's width, 0 for blocks without one (num_layers blocks)
+    ffn_dim: int = 0
 
     def __post_init__(self):
         if self.compressed_num_frames is None:
             self.compressed_num_frames = self.seq_len
         if self.model_dim % self.num_heads:
             raise ValueError("model_dim must be a multiple of num_heads")
-        mini_batches = self.ssm_layer != "selective_scan"  # which takes any length and has none
+        recurrent = self.ssm_layer in ("selective_scan", "gated_delta")
+        mini_batches = not recurrent  # which take any length and have none
         if mini_batches and self.seq_len % self.mini_batch_size:
             raise ValueError("seq_len must be a multiple of mini_batch_size")
         if (self.model_dim // self.num_heads) % 2:
@@ -151,13 +161,15 @@ class ModelConfig:
             raise ValueError(f"model_dim {self.model_dim} > {MAX_MODEL_DIM}, the widest the layer kernels take")
         if mini_batches and (self.mini_batch_size % 16 or not 16 <= self.mini_batch_size <= 64):
             raise ValueError(f"mini_batch_size {self.mini_batch_size}: a multiple of 16 from 16 to 64 is needed")
-        if self.ssm_layer == "selective_scan":
+        if recurrent:
             if self.state_dim % 16 or not 16 <= self.state_dim <= MAX_STATE:
                 raise ValueError(f"state_dim {self.state_dim}: a multiple of 16 up to {MAX_STATE} is needed")
             if self.num_groups < 1 or self.num_heads % self.num_groups:
                 raise ValueError(f"num_groups {self.num_groups} must divide the {self.num_heads} heads")
             if self.conv_width not in CONV_WIDTHS:
                 raise ValueError(f"conv_width {self.conv_width}: one of {CONV_WIDTHS} is needed")
+        if self.ssm_layer == "gated_delta" and (self.num_layers < 1 or self.ffn_dim < 0):
+            raise ValueError(f"num_layers {self.num_layers} must be 1 or more, ffn_dim {self.ffn_dim} 0 or more")
 
 
 class TTTLayerBase(nn.Module):
@@ -402,9 +414,174 @@ class SelectiveSSM(nn.Module):
         return self._out(y, z)
 
 
+class GatedDelta(nn.Module):
+    """A gated delta-rule mixer: per token one projection to z | q | k | v | b | dt, a short
+    causal convolution with SiLU over q | k | v, the delta rule with q and k at unit length,
+    log-decays -exp(A_log) softplus(dt + dt_bias) and weights sigmoid(b), the heads' root-mean-square
+    norm with the gate silu(z), and the output projection."""
+
+    def __init__(self, config: ModelConfig):
+        super().__init__()
+        self.config = config
+        self.width, self.num_heads = config.model_dim, config.num_heads
+        self.head_dim = config.model_dim // config.num_heads
+        self.groups, self.state_dim = config.num_groups, config.state_dim
+        D, H = self.width, self.num_heads
+        self.conv_channels = D + 2 * self.groups * self.state_dim
+        self.in_proj = nn.Linear(D, D + self.conv_channels + 2 * H, bias=True)
+        self.conv_weight = nn.Parameter(torch.empty(self.conv_channels, config.conv_width))
+        self.conv_bias = nn.Parameter(torch.zeros(self.conv_channels))
+        self.A_log = nn.Parameter(torch.empty(H))
+        self.dt_bias = nn.Parameter(torch.empty(H))
+        self.norm_weight = nn.Parameter(torch.ones(self.head_dim))
+        self.wo = nn.Linear(D, D, bias=True)
+        pad = _padded_width(self.in_proj.out_features) - self.in_proj.out_features
+        self.register_buffer("_proj_pad_w", torch.zeros(pad, D), persistent=False)
+        self.register_buffer("_proj_pad_b", torch.zeros(pad), persistent=False)
+        self.init_weights()
+
+    def init_weights(self):
+        """Rates and steps as the selective state-space layer's."""
+        for lin in (self.in_proj, self.wo):
+            nn.init.normal_(lin.weight, mean=0.0, std=0.02)
+            nn.init.zeros_(lin.bias)
+        bound = self.config.conv_width ** -0.5
+        nn.init.uniform_(self.conv_weight, -bound, bound)
+        nn.init.zeros_(self.conv_bias)
+        nn.init.ones_(self.norm_weight)
+        with torch.no_grad():
+            self.A_log.copy_(torch.log(torch.empty_like(self.A_log).uniform_(1.0, 16.0)))
+            step = torch.exp(torch.empty_like(self.dt_bias).uniform_(math.log(1e-3), math.log(0.1)))
+            self.dt_bias.copy_(torch.log(torch.expm1(step)))
+
+    def _project(self, x: torch.Tensor):
+        w, b = self.in_proj.weight, self.in_proj.bias
+        if self._proj_pad_w.shape[0]:
+            w = torch.cat([w, self._proj_pad_w.to(w.dtype)])
+            b = torch.cat([b, self._proj_pad_b.to(b.dtype)])
+        return self._columns(projection(x, w, b))
+
+    def _columns(self, p: torch.Tensor):
+        """(z [.., D], q | k | v [.., C], the log-decays and weights [.., H] fp32)"""
+        D, C, H = self.width, self.conv_channels, self.num_heads
+        z, qkv, b, dt = p.split([D, C, H, H, p.shape[-1] - D - C - 2 * H], -1)[:4]
+        g = -torch.exp(self.A_log.float()) * Fn.softplus(dt.float() + self.dt_bias.float())
+        return z, qkv, g, torch.sigmoid(b.float())
+
+    def _heads(self, qkv: torch.Tensor):
+        """q and k [.., G, N], v [.., H, F]"""
+        n = self.groups * self.state_dim
+        q, k, v = qkv.split([n, n, self.width], -1)
+        return (*(t.unflatten(-1, (self.groups, self.state_dim)) for t in (q, k)),
+                v.unflatten(-1, (self.num_heads, self.head_dim)))
+
+    def _out(self, o: torch.Tensor, z: torch.Tensor):
+        h = block_norm(o, self.norm_weight, gate=z.unflatten(-1, (self.num_heads, self.head_dim)), eps=POST_NORM_EPS)
+        return self.wo(h.flatten(-2))
+
+    def _run(self, x: torch.Tensor, cache: Optional[SSMCache], keep: bool, last_only: bool):
+        z, qkv, g, beta = self._project(x)
+        first = (None, None) if cache is None else (cache.conv, cache.state)
+        qkv = causal_conv(qkv, self.conv_weight, self.conv_bias, first[0], "silu", keep)
+        qkv, conv = qkv if keep else (qkv, None)
+        o = gated_delta(*self._heads(qkv), g, beta, first[1], return_final_state=keep)
+        o, state = o if keep else (o, None)
+        if last_only:  # the norm and the output projection are by tokens
+            o, z = o[:, -1], z[:, -1]
+        return self._out(o, z), SSMCache(conv, state) if keep else None
+
+    def forward(self, x: torch.Tensor, last_only: bool = False):
+        """[B, L, D], or with last_only the last token's output [B, D]."""
+        return self._run(x, None, False, last_only)[0]
+
+    @torch.no_grad()
+    def step(self, x: torch.Tensor, cache: SSMCache):
+        """One token x [B, D] of every sequence: its output [B, D], the cache moved on in place."""
+        z, qkv, g, beta = self._columns(self.in_proj(x))
+        qkv = causal_conv_step(qkv, cache.conv, self.conv_weight, self.conv_bias, "silu")
+        return self._out(gated_delta_step(*self._heads(qkv), g, beta, cache.state), z)
+
+
+class GatedFeedForward(nn.Module):
+    """down(silu(x Wg^T) * (x Wu^T)), both projections and the gating in one kernel."""
+
+    def __init__(self, width: int, hidden: int):
+        super().__init__()
+        self.w_gate = nn.Parameter(torch.empty(hidden, width))
+        self.w_up = nn.Parameter(torch.empty(hidden, width))
+        self.down = nn.Linear(hidden, width, bias=False)
+        for w in (self.w_gate, self.w_up, self.down.weight):
+            nn.init.normal_(w, mean=0.0, std=0.02)
+
+    def forward(self, x: torch.Tensor):
+        dt = torch.get_autocast_dtype(x.device.type) if torch.is_autocast_enabled(x.device.type) else x.dtype
+        return self.down(gated_linear(x.to(dt), self.w_gate.to(dt), self.w_up.to(dt)))
+
+
+class GatedDeltaStack(nn.Module):
+    """`num_layers` blocks of a GatedDelta mixer and, with ffn_dim, a GatedFeedForward on an fp32
+    residual r: r <- r + s * norm(part(norm(r))), the norms by root mean squares.  What a part
+    gives is normed, scaled, added to r and normed for the next part in one call; the last norm
+    is the stack's output.
+
+    forward takes any sequence length; prompt also returns the caches (one a block) that step
+    goes on from, one token a call.  (`rope` is the other layers' and is not read.)"""
+
+    def __init__(self, config: ModelConfig):
+        super().__init__()
+        self.config = config
+        D = config.model_dim
+        parts = []
+        for _ in range(config.num_layers):
+            parts.append(GatedDelta(config))
+            if config.ffn_dim:
+                parts.append(GatedFeedForward(D, config.ffn_dim))
+        self.parts = nn.ModuleList(parts)
+        self.first_norm = nn.Parameter(torch.ones(D))
+        self.out_norms = nn.Parameter(torch.ones(len(parts), D))    # of what a part gives
+        self.scales = nn.Parameter(torch.full((len(parts), D), len(parts) ** -0.5))
+        self.next_norms = nn.Parameter(torch.ones(len(parts), D))   # before the next part, or the output
+
+    def _join(self, i: int, y: torch.Tensor, r: torch.Tensor):
+        return block_norm(y, self.out_norms[i], r, scale=self.scales[i], next_weight=self.next_norms[i], eps=POST_NORM_EPS)
+
+    def _run(self, x: torch.Tensor, caches, keep: bool, last_only: bool):
+        r, y = x.float(), block_norm(x, self.first_norm, eps=POST_NORM_EPS)
+        last = max(i for i, part in enumerate(self.parts) if isinstance(part, GatedDelta))
+        kept = []
+        for i, part in enumerate(self.parts):
+            if isinstance(part, GatedDelta):
+                only = last_only and i == last  # behind the last mixer everything is by tokens
+                y, cache = part._run(y, None if caches is None else caches[len(kept)], keep, only)
+                kept.append(cache)
+                r = r[:, -1] if only else r
+            else:
+                y = part(y)
+            r, y = self._join(i, y, r)
+        return y, kept
+
+    def forward(self, x: torch.Tensor, rope: Optional[torch.Tensor] = None, last_only: bool = False):
+        """[B, L, D], or with last_only the last token's output [B, D]."""
+        return self._run(x, None, False, last_only)[0]
+
+    def prompt(self, x: torch.Tensor, cache=None, last_only: bool = False):
+        """(forward's output, the caches behind x), from empty caches or given ones (which are
+        left as they are)."""
+        return self._run(x, cache, True, last_only)
+
+    @torch.no_grad()
+    def step(self, x: torch.Tensor, cache):
+        """One token x [B, D] of every sequence: its output [B, D], the caches moved on in place."""
+        r, y = x.float(), block_norm(x, self.first_norm, eps=POST_NORM_EPS)
+        caches = iter(cache)
+        for i, part in enumerate(self.parts):
+            r, y = self._join(i, part.step(y, next(caches)) if isinstance(part, GatedDelta) else part(y), r)
+        return y
+
+
 class TTTWrapper(nn.Module):
     """ttt_layer.py:20-57: the layer and its rotary table.  ssm_layer "selective_scan" is a
-    SelectiveSSM in the same place."""
+    SelectiveSSM and "gated_delta" a GatedDeltaStack in the same place."""
 
     def __init__(self, config: ModelConfig):
         super().__init__()
@@ -415,6 +592,8 @@ class TTTWrapper(nn.Module):
             self.ttt = TTTMLP(config)
         elif config.ssm_layer == "selective_scan":
             self.ttt = SelectiveSSM(config)
+        elif config.ssm_layer == "gated_delta":
+            self.ttt = GatedDeltaStack(config)
         else:
             raise TypeError(f"no ttt layer of type {config.ssm_layer}")
         self.register_buffer("rope", self._rope(), persistent=False)
@@ -450,24 +629,25 @@ class TTTForecaster(nn.Module):
     def _forecast(self, h: torch.Tensor) -> torch.Tensor:
         return self.head(h).view(h.size(0), self.pred_len, self.d_out)
 
-    def _ssm(self) -> SelectiveSSM:
+    def _ssm(self):
         layer = self.ttt.ttt
-        if not isinstance(layer, SelectiveSSM):
-            raise TypeError("a forecast that goes on token by token needs ssm_layer 'selective_scan'")
+        if not isinstance(layer, (SelectiveSSM, GatedDeltaStack)):
+            raise TypeError("a forecast that goes on token by token needs ssm_layer 'selective_scan' or 'gated_delta'")
         return layer
 
-    def prompt(self, seq_x: torch.Tensor, cache: Optional[SSMCache] = None):
+    def prompt(self, seq_x: torch.Tensor, cache=None):
         """(forward's forecast [B, pred_len, d_out] behind seq_x [B, L, d_in], the cache that
-        step goes on from); ssm_layer "selective_scan" only."""
+        step goes on from); ssm_layer "selective_scan" or "gated_delta" only."""
         layer = self._ssm()
         h, cache = layer.prompt(projection(seq_x, self.in_proj.weight, self.in_proj.bias), cache, last_only=True)
         return self._forecast(h), cache
 
     @torch.no_grad()
-    def step(self, x: torch.Tensor, cache: SSMCache):
+    def step(self, x: torch.Tensor, cache):
         """The forecast behind one more observation x [B, d_in] of every series."""
         layer = self._ssm()
         return self._forecast(layer.step(projection(x, self.in_proj.weight, self.in_proj.bias), cache))
 
 
-__all__ = ["ModelConfig", "TTTLinear", "TTTMLP", "SelectiveSSM", "SSMCache", "TTTWrapper", "TTTForecaster"]
+__all__ = ["ModelConfig", "TTTLinear", "TTTMLP", "SelectiveSSM", "GatedDelta", "GatedFeedForward", "GatedDeltaStack",
+           "SSMCache", "TTTWrapper", "TTTForecaster"]

@@ -49,6 +49,8 @@ def _row_stride(t: torch.Tensor, lead: int, width: int):
     if t.is_contiguous():
         return width
     shape, strides = t.shape, t.stride()
+    if lead == 1 and len(shape) == 3 and strides[2] == 1 and strides[1] == shape[2] and strides[0] >= width:
+        return strides[0]  # (the heads of single tokens, columns of a wider matrix)
     inner, ld, step = 1, None, 0
     for i in range(t.dim() - 1, -1, -1):
         n, st = shape[i], strides[i]
