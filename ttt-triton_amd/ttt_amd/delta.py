@@ -33,7 +33,7 @@ from torch.autograd.function import once_differentiable
 from . import _lib
 from ._common import check_device, dtype_code, f32c, on_device
 from .ssm import (_as, _bytes, _empty, _near_rows, _no_grad_through, _opt, _rows, _sizes, _state_in_place, _stream,
-                  _token_rows, _wants_grad, _whole)
+                  _wants_grad, _whole)
 
 MAX_HEAD_DIM = 256  # P, a multiple of 32
 MAX_STATE = 128     # N, a multiple of 16
@@ -77,10 +77,11 @@ def _delta_state(h0, shape):
     return _whole(f32c(h0), 16)
 
 
-def _qk_rows(q, k, g, beta, rows, align, sizes):
+def _qk_rows(q, k, g, beta, sizes):
+    """The four inputs and their row strides as the kernels take them"""
     _, _, H, _, G, N = sizes
-    return (*rows(q, align, G * N), *rows(k, align, G * N), *_rows(g, g.dim() - 1, g.element_size(), H),
-            *_rows(beta, beta.dim() - 1, beta.element_size(), H))
+    return (*_near_rows(q, 16, G * N), *_near_rows(k, 16, G * N), *_rows(g, 2, g.element_size(), H),
+            *_rows(beta, 2, beta.element_size(), H))
 
 
 def _delta_forward(q, k, v, g, beta, h0, scale, unit, want_last, train):
@@ -89,7 +90,7 @@ def _delta_forward(q, k, v, g, beta, h0, scale, unit, want_last, train):
     B, L, H, P, G, N = sizes
     code = codes[0]
     h0 = _delta_state(h0, (B, H, P, N))
-    rows = _qk_rows(q, k, g, beta, _near_rows, 16, sizes)
+    rows = _qk_rows(q, k, g, beta, sizes)
     qr, ldq, kr, ldk, gr, ldg, br, ldb = rows
     vr, ldv = _near_rows(v, 16, H * P)
     o = v.new_empty((B, L, H, P))
@@ -129,7 +130,7 @@ class GatedDeltaFunction(torch.autograd.Function):
         B, L, H, P, G, N = ctx.sizes
         ldq, ldk, ldg, ldb = ctx.lds
         if (q.stride(), k.stride(), g.stride(), beta.stride()) != ctx.strides or (q.data_ptr() | k.data_ptr()) % 16:
-            q, ldq, k, ldk, g, ldg, beta, ldb = _qk_rows(q, k, g, beta, _near_rows, 16, ctx.sizes)
+            q, ldq, k, ldk, g, ldg, beta, ldb = _qk_rows(q, k, g, beta, ctx.sizes)
         saved = _whole(saved, 16)
         dev, act = q.device, q.dtype
         do = torch.zeros((B, L, H, P), device=dev, dtype=act) if do is None else do
@@ -185,8 +186,9 @@ def gated_delta_step(q, k, v, g, beta, state, scale=None, l2_norm: bool = True):
     o = v.new_empty((B, H, P))
     if o.numel() == 0:
         return o
-    qr, ldq, kr, ldk, gr, ldg, br, ldb = _qk_rows(q, k, g, beta, _token_rows, 4 * v.element_size(), sizes)
-    vr, ldv = _token_rows(v, v.element_size(), H * P)
+    es = v.element_size()
+    (qr, ldq), (kr, ldk), (vr, ldv) = _rows(q, 1, 4 * es, G * N), _rows(k, 1, 4 * es, G * N), _rows(v, 1, es, H * P)
+    (gr, ldg), (br, ldb) = _rows(g, 1, g.element_size(), H), _rows(beta, 1, beta.element_size(), H)
     with on_device(dev):
         st = _lib.load().ttt_delta_step(qr.data_ptr(), ldq, kr.data_ptr(), ldk, vr.data_ptr(), ldv, gr.data_ptr(), ldg,
                                         br.data_ptr(), ldb, state.data_ptr(), B, H, P, G, N, scale, int(bool(l2_norm)),

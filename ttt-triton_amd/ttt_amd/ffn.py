@@ -34,12 +34,14 @@ def _ffn_args(x, w_gate, w_up, b_gate, b_up, activation):
             raise ValueError(f"{n} must be [F]=[{F}], got {list(b.shape)}")
     if activation not in _lib.GATE_ACTIVATIONS:
         raise ValueError(f"unknown activation {activation!r} (one of {tuple(_lib.GATE_ACTIVATIONS)})")
-    some = [t for t in (b_gate, b_up) if t is not None]
-    for t in (w_gate, w_up, *some):
-        if t.dtype != act:
-            raise ValueError(f"weights and biases must have x's dtype {act}, got {t.dtype}")
-    code = dtype_code(act)
-    dev = check_device(x, w_gate, w_up, *some)
+    code, dev, near = dtype_code(act), x.device, x.device.type == "cuda"
+    for t in (w_gate, w_up, b_gate, b_up):
+        if t is not None:
+            if t.dtype != act:
+                raise ValueError(f"weights and biases must have x's dtype {act}, got {t.dtype}")
+            near = near and t.device == dev
+    if not near:
+        check_device(x, *[t for t in (w_gate, w_up, b_gate, b_up) if t is not None])
     R = x.numel() // D
     if R >= (1 << 31) - 256:
         raise ValueError(f"gated_linear takes fewer than 2^31 - 256 rows, got {R}")

@@ -132,16 +132,25 @@ def _block_args(x, weight, residual, gate, scale, next_weight, eps):
         raise ValueError("next_weight (the norm before the next block) needs a residual")
     if not 0.0 < eps <= 1.0:
         raise ValueError(f"eps must be in (0, 1], got {eps}")
-    dev = check_device(x, *[t for t in (weight, residual, gate, scale, next_weight) if t is not None])
-    params = [_param(t, (D,), n) for t, n in ((weight, "weight"), (scale, "scale"), (next_weight, "next_weight"))]
-    return dev, code, -1 if residual is None else dtype_code(residual.dtype), params
+    dev = x.device
+    if dev.type != "cuda":
+        check_device(x)
+    for t in (weight, residual, gate, scale, next_weight):
+        if t is not None and t.device != dev:
+            check_device(x, t)
+    of = (D,)
+    return (dev, code, -1 if residual is None else code if residual.dtype == act else dtype_code(residual.dtype),
+            (_param(weight, of, "weight"), _param(scale, of, "scale"), _param(next_weight, of, "next_weight")))
 
 
 def _block_rows(ts):
     """(the tensors as rows, heads, their row strides): as plain rows where all are laid out
     so, else as wider rows of `heads` each, else from copies."""
+    x, *more = ts
+    D, dim = x.shape[-1], x.dim()
+    if x.is_contiguous() and all(t is None or t.is_contiguous() for t in more):
+        return ts, 1, [D if t is not None else 0 for t in ts]
     some = [t for t in ts if t is not None]
-    D, dim = some[0].shape[-1], some[0].dim()
     lds = [_row_stride(t, dim - 1, D) for t in some]
     heads = 1
     if None in lds and dim > 2:
