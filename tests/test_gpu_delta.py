@@ -44,6 +44,15 @@ def test_long_single_sequence(lib, dt, L):
 
 
 @pytest.mark.parametrize("dt", T.DTYPES)
+@pytest.mark.parametrize("N,P", [(16, 64), (32, 128), (32, 96), (48, 64), (128, 64), (96, 32)])
+def test_segments_of_each_width(lib, dt, N, P):
+    """The segments' products, of every width of the state, with more and fewer columns than a
+    workgroup has."""
+    d = T.delta_inputs(1, 1100, 2, 1, N, P, dt, seed=N + P)
+    T.delta_check(d, T.delta_run(T.dev(d)))
+
+
+@pytest.mark.parametrize("dt", T.DTYPES)
 def test_many_chains(lib, dt):
     """More sequences and heads than workgroups are held at once: one segment of each."""
     d = T.delta_inputs(70, 70, 8, 4, 16, 32, dt, seed=10)

@@ -128,6 +128,9 @@ template <typename T> __device__ __forceinline__ Op<ScanType<T>::IN> row_op(cons
   }
 }
 
+// workgroups that have the columns of the identity between them
+constexpr int identity_groups(int W, int NP) { return (NP + 16 * W - 1) / (16 * W); }
+
 // OUT: outputs too; else the segments' ends alone
 template <typename T, int W, int NP, bool BACK, bool OUT>
 __global__ __launch_bounds__(128 * W) void delta_walk_kernel(DeltaParams p) {
@@ -144,7 +147,7 @@ __global__ __launch_bounds__(128 * W) void delta_walk_kernel(DeltaParams p) {
   const int PB = delta_part(p.P), parts = p.P / PB, cols = PB / (16 * W), NC = (p.L + Q - 1) / Q;
   const unsigned at = on_xcd(blockIdx.x, gridDim.x);
   // groups of columns to a head: of its features, and without outputs of the identity behind them
-  const int own = parts * cols, groups = own + (OUT ? 0 : NP / (16 * W)), segs = OUT ? p.S : p.S - 1;
+  const int own = parts * cols, groups = own + (OUT ? 0 : identity_groups(W, NP)), segs = OUT ? p.S : p.S - 1;
   const int grp_c = (int)(at % groups);
   const int s = (int)(at / groups % segs) + (!OUT && BACK ? 1 : 0);
   const long long head = at / groups / segs;  // sequence and head
@@ -243,7 +246,7 @@ __global__ __launch_bounds__(128 * W) void delta_walk_kernel(DeltaParams p) {
         }
         __syncthreads();  // what was handed over has been read
         const int c = chunk_of(k - 1), left = min(Q, p.L - c * Q);
-        // (x is no number from the first token on whose row is not finite: ttt_delta.h)
+        // (x is no number from the first token on whose row is not finite: below)
         const int bad = first_not_finite(x);
         if (__ballot(bad < Q) != 0) {
 #pragma unroll
@@ -535,7 +538,7 @@ __global__ __launch_bounds__(128 * W) void delta_walk_kernel(DeltaParams p) {
   if (!OUT) {
     if (features)
       st.keep(p.seg + (chain * p.S + s) * (NP * PB) + f0, PB, w);
-    else
+    else if (f0 + 16 * w < NP)  // (32 columns leave two of four waves without any)
       st.keep(p.trans + (head * p.S + s) * (NP * NP) + f0, NP, w);
   } else if (p.h_last != nullptr && s == (BACK ? 0 : p.S - 1)) {
     st.store(p.h_last + (chain * PB + f0) * p.N, p.N, p.N, w);
@@ -602,8 +605,8 @@ template <typename T, int W, int NP, bool BACK> hipError_t walk_t(const DeltaPar
   if (p.S > 1) {
     e = allow_lds(delta_walk_kernel<T, W, NP, BACK, false>, lds1);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((delta_walk_kernel<T, W, NP, BACK, false>), dim3((unsigned)(heads * (p.S - 1) * (p.P + NP) / (16 * W))),
-                       dim3(128 * W), lds1, stream, p);
+    const long long groups = heads * (p.S - 1) * (p.P / (16 * W) + identity_groups(W, NP));
+    hipLaunchKernelGGL((delta_walk_kernel<T, W, NP, BACK, false>), dim3((unsigned)groups), dim3(128 * W), lds1, stream, p);
     hipLaunchKernelGGL((delta_join_kernel<NP, BACK>), dim3((unsigned)(heads * p.P / 16)), dim3(4 * NP), 0, stream,
                        p);
   }
