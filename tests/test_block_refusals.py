@@ -53,6 +53,15 @@ def test_delta(lib):
     assert lib.ttt_delta_bwd_workspace_bytes(2, 99, 4, 64, 3, 64, BF16) == 0
 
 
+def test_delta_most_sequences(lib):
+    """A launch has at most 2^32 - 1 threads, 8 to a feature and column of a state (128 at most), or
+    up to 32 to a feature alone: refused past that."""
+    for fn, more in ((lib.ttt_delta_saved_bytes, ()), (lib.ttt_delta_workspace_bytes, ()), (lib.ttt_delta_bwd_workspace_bytes, (1,))):
+        for P, most in ((32, ((1 << 29) - 1) // 160), (64, (1 << 21) - 1), (256, (1 << 19) - 1)):
+            assert fn(most, 1, 1, P, *more, 16, BF16) > 0
+            assert fn(most + 1, 1, 1, P, *more, 16, BF16) == 0
+
+
 def test_delta_segments_and_sizes(lib):
     """Sizes grow with what they are of, and a long prompt of few heads is cut into segments while
     many are not: the workspace beside Z, M and the tokens' numbers is the segments'."""

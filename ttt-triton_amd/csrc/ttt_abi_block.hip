@@ -65,8 +65,10 @@ DeltaPlan delta_plan(int B, int L, int H, int P, int G, int N, int dtype) {
   return s;
 }
 bool delta_grid_ok(const DeltaPlan& s, int B, int H, int P) {
-  // (prep: 256 threads a chunk and head; walk: four for a feature and sequence; gradients: 512 a chunk and head)
-  return (long long)B * H * (P + 128) <= kMaxThreads / 4 / s.S && (long long)B * H <= kMaxThreads / 512 / s.NC;
+  // (prep: 256 threads a chunk and head; walk: eight for a column, a feature or one of the identity's, and segment;
+  // join: up to 32 a feature; gradients: 512 a chunk and head)
+  const long long heads = (long long)B * H;
+  return heads * (P + 128) <= kMaxThreads / 8 / s.S && heads * P <= kMaxThreads / 32 && heads <= kMaxThreads / 512 / s.NC;
 }
 bool delta_plan_ok(int B, int L, int H, int P, int G, int N, int dtype, DeltaPlan& s) {
   if (check_delta(B, L, H, P, G, N, dtype, dtype, dtype) != TTT_OK) return false;
