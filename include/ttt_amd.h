@@ -499,7 +499,7 @@ int ttt_layer_norm_bwd(const void* x, long long ldx, const void* gate, long long
  *   h0       [B][H][P][N], or NULL for zeros
  *   o        [B][L][H][P]                   h_last [B][H][P][N], or NULL
  *   saved    NULL, or ttt_delta_saved_bytes: what ttt_delta_bwd needs of the forward
- *   workspace  ttt_delta_workspace_bytes
+ *   workspace  ttt_delta_workspace_bytes; ttt_delta_bwd reads it again
  * Precision, alignment and rows as with ttt_scan_fwd. */
 size_t ttt_delta_saved_bytes(int B, int L, int H, int P, int N, int dtype);
 size_t ttt_delta_workspace_bytes(int B, int L, int H, int P, int N, int dtype);
@@ -510,14 +510,15 @@ int ttt_delta_fwd(const void* q, long long ldq, const void* k, long long ldk, co
                   void* stream);
 
 /* Its gradients from dO [B*L][lddo] and dh_last (NULL: zeros), given what ttt_delta_fwd
- * saved for the same inputs: dq, dk [B][L][G][N], dv [B][L][H][P], dg, dbeta [B][L][H] in the
+ * saved for the same inputs, and its workspace as it left it (`kept`): dq, dk [B][L][G][N], dv [B][L][H][P], dg, dbeta [B][L][H] in the
  * types of g and beta, dh0 [B][H][P][N] (or NULL). */
 size_t ttt_delta_bwd_workspace_bytes(int B, int L, int H, int P, int G, int N, int dtype);
 int ttt_delta_bwd(const void* q, long long ldq, const void* k, long long ldk, const void* g, long long ldg,
                   const void* beta, long long ldbeta, const void* dO, long long lddo, const float* dh_last,
-                  const void* saved, size_t saved_bytes, int B, int L, int H, int P, int G, int N, float scale,
-                  int unit, int dtype, int g_dtype, int beta_dtype, void* dq, void* dk, void* dv, void* dg,
-                  void* dbeta, float* dh0, void* workspace, size_t workspace_bytes, void* stream);
+                  const void* saved, size_t saved_bytes, const void* kept, size_t kept_bytes, int B, int L, int H,
+                  int P, int G, int N, float scale, int unit, int dtype, int g_dtype, int beta_dtype, void* dq,
+                  void* dk, void* dv, void* dg, void* dbeta, float* dh0, void* workspace, size_t workspace_bytes,
+                  void* stream);
 
 /* One token of every sequence: rows as above with one a sequence, h [B][H][P][N] updated
  * in place, o [B][H][P]. */

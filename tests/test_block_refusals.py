@@ -11,7 +11,7 @@ DIMS = dict(B=2, L=99, H=4, P=64, G=2, N=64)
 HOW = dict(scale=0.125, unit=1, dtype=BF16, gd=F32, bd=BF16)
 DELTA = dict(**DELTA_IN, h0=P, **DIMS, **HOW, o=P, last=P, saved=P, sbytes=1 << 40, ws=P, wbytes=1 << 40, stream=None)
 DELTA_BWD = dict(q=P, ldq=128, k=P, ldk=128, g=P, ldg=4, beta=P, ldb=4, dO=P, lddo=256, dlast=P, saved=P, sbytes=1 << 40,
-                 **DIMS, **HOW, dq=P, dk=P, dv=P, dg=P, db=P, dh0=P, ws=P, wbytes=1 << 40, stream=None)
+                 kept=P, kbytes=1 << 40, **DIMS, **HOW, dq=P, dk=P, dv=P, dg=P, db=P, dh0=P, ws=P, wbytes=1 << 40, stream=None)
 DELTA_STEP = dict(**DELTA_IN, h=P, B=2, H=4, P=64, G=2, N=64, **HOW, o=P, stream=None)
 NORM = dict(x=P, ldx=64, gate=P, ldg=64, res=P, ldr=64, w=P, s=P, w2=P, R=6, D=64, heads=1, eps=1e-6, dtype=BF16, rd=F32,
             r=P, y=P, stats=P, stream=None)
@@ -48,6 +48,7 @@ def test_delta(lib):
     dims = (2, 99, 4, 64, 64, BF16)
     assert f(wbytes=lib.ttt_delta_workspace_bytes(*dims) - 1) == E_WS
     assert f(sbytes=lib.ttt_delta_saved_bytes(*dims) - 1) == E_WS and b(sbytes=lib.ttt_delta_saved_bytes(*dims) - 1) == E_WS
+    assert b(kept=None) == E_NULL and b(kept=Q) == E_ALIGN and b(kbytes=4 * 2 * 4 * 2 * (516 + 2 * 2560) - 1) == E_WS
     assert b(wbytes=lib.ttt_delta_bwd_workspace_bytes(2, 99, 4, 64, 2, 64, BF16) - 1) == E_WS
     assert lib.ttt_delta_saved_bytes(2, 99, 4, 48, 64, BF16) == 0 and lib.ttt_delta_workspace_bytes(2, 99, 4, 64, 8, BF16) == 0
     assert lib.ttt_delta_bwd_workspace_bytes(2, 99, 4, 64, 3, 64, BF16) == 0

@@ -369,7 +369,7 @@ size_t ttt_delta_workspace_bytes(int B, int L, int H, int P, int N, int dtype) {
 }
 size_t ttt_delta_bwd_workspace_bytes(int B, int L, int H, int P, int G, int N, int dtype) {
   DeltaPlan s;
-  return delta_plan_ok(B, L, H, P, G, N, dtype, s) ? s.tok + 2 * s.zm + s.states + s.rows + 2 * s.qk + s.seg + s.trans : 0;
+  return delta_plan_ok(B, L, H, P, G, N, dtype, s) ? s.states + s.rows + 2 * s.qk + s.seg + s.trans : 0;
 }
 
 int ttt_delta_fwd(const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv,
@@ -435,15 +435,15 @@ int ttt_delta_fwd(const void* q, long long ldq, const void* k, long long ldk, co
     p.states = static_cast<float*>(saved);
     p.rows = reinterpret_cast<float*>(static_cast<char*>(saved) + s.states);
   }
-  const hipError_t e = ttt::launch_delta_prep(p, dtype, false, static_cast<hipStream_t>(stream));
+  const hipError_t e = ttt::launch_delta_prep(p, dtype, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_status(e);
   return hip_status(ttt::launch_delta_fwd(p, dtype, static_cast<hipStream_t>(stream)));
 }
 
 int ttt_delta_bwd(const void* q, long long ldq, const void* k, long long ldk, const void* g, long long ldg,
                   const void* beta, long long ldbeta, const void* dO, long long lddo, const float* dh_last,
-                  const void* saved, size_t saved_bytes, int B, int L, int H, int P, int G, int N, float scale,
-                  int unit, int dtype, int g_dtype, int beta_dtype, void* dq, void* dk, void* dv, void* dg,
+                  const void* saved, size_t saved_bytes, const void* kept, size_t kept_bytes, int B, int L, int H,
+                  int P, int G, int N, float scale, int unit, int dtype, int g_dtype, int beta_dtype, void* dq, void* dk, void* dv, void* dg,
                   void* dbeta, float* dh0, void* workspace, size_t workspace_bytes, void* stream) {
   int st = check_delta(B, L, H, P, G, N, dtype, g_dtype, beta_dtype);
   if (st != TTT_OK) return st;
@@ -459,6 +459,7 @@ int ttt_delta_bwd(const void* q, long long ldq, const void* k, long long ldk, co
   REQUIRE(beta, size_of(beta_dtype));
   REQUIRE(dO, 16);
   REQUIRE(saved, 16);
+  REQUIRE(kept, 16);
   REQUIRE(dq, 16);
   REQUIRE(dk, 16);
   REQUIRE(dv, 16);
@@ -466,10 +467,8 @@ int ttt_delta_bwd(const void* q, long long ldq, const void* k, long long ldk, co
   REQUIRE(dbeta, size_of(beta_dtype));
   OPTIONAL(dh_last, 16);
   OPTIONAL(dh0, 16);
-  if (saved_bytes < s.states + s.rows) return TTT_ERR_WORKSPACE;
-  if (workspace == nullptr ||
-      workspace_bytes < s.tok + 2 * s.zm + s.states + s.rows + 2 * s.qk + s.seg + s.trans)
-    return TTT_ERR_WORKSPACE;
+  if (saved_bytes < s.states + s.rows || kept_bytes < s.tok + 2 * s.zm) return TTT_ERR_WORKSPACE;
+  if (workspace == nullptr || workspace_bytes < s.states + s.rows + 2 * s.qk + s.seg + s.trans) return TTT_ERR_WORKSPACE;
   OPTIONAL(workspace, 16);
   ttt::DeltaParams p{};
   p.q = q;
@@ -501,9 +500,10 @@ int ttt_delta_bwd(const void* q, long long ldq, const void* k, long long ldk, co
     ws += n;
     return at;
   };
-  p.tok = reinterpret_cast<float*>(take(s.tok));
-  p.z = reinterpret_cast<float*>(take(s.zm));
-  p.m = reinterpret_cast<float*>(take(s.zm));
+  float* const of = const_cast<float*>(static_cast<const float*>(kept));  // read only
+  p.tok = of;
+  p.z = of + s.tok / 4;
+  p.m = of + (s.tok + s.zm) / 4;
   p.states = reinterpret_cast<float*>(take(s.states));
   p.rows = reinterpret_cast<float*>(take(s.rows));
   p.S = s.S;
@@ -517,9 +517,7 @@ int ttt_delta_bwd(const void* q, long long ldq, const void* k, long long ldk, co
     p.dkp = reinterpret_cast<float*>(take(s.qk));
   }
   const hipStream_t on = static_cast<hipStream_t>(stream);
-  hipError_t e = ttt::launch_delta_prep(p, dtype, true, on);
-  if (e != hipSuccess) return hip_status(e);
-  e = ttt::launch_delta_walk_back(p, dtype, on);
+  const hipError_t e = ttt::launch_delta_walk_back(p, dtype, on);
   if (e != hipSuccess) return hip_status(e);
   p.gstates = p.states;
   p.states = const_cast<float*>(static_cast<const float*>(saved));

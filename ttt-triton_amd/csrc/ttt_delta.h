@@ -39,7 +39,7 @@ struct DeltaParams {
   void* o;                // [B][L][H][P]; backwards dv
   float* h_last;          // [B][H][P][N] (may be null); backwards the gradient of the initial state
   float* tok;             // [B*H][NC] DeltaTok
-  float *z, *m;           // [B*H][NC][tiles][64][4]: Z and M by blocks and lanes
+  float *z, *m;           // [B*H][NC][tiles][64][4]: Z and M by blocks, as tile_at has them
   float* states;          // [B*H*parts][NC][NP][PB]: the states entering the chunks, or walking back the
                           // gradients of those leaving them (may be null)
   float* rows;            // [B*H*parts][NC*Q][PB]: x, or walking back y (may be null)
@@ -58,7 +58,7 @@ struct DeltaParams {
 };
 hipError_t launch_delta_fwd(const DeltaParams& p, int dtype, hipStream_t stream);
 hipError_t launch_delta_walk_back(const DeltaParams& p, int dtype, hipStream_t stream);
-hipError_t launch_delta_prep(const DeltaParams& p, int dtype, bool back, hipStream_t stream);
+hipError_t launch_delta_prep(const DeltaParams& p, int dtype, hipStream_t stream);
 hipError_t launch_delta_bwd(const DeltaParams& p, int dtype, hipStream_t stream);
 struct DeltaStepParams {
   const void *q, *k, *v, *g, *beta;  // [B][ldq], ..
@@ -94,8 +94,17 @@ template <int Q> struct alignas(16) DeltaTok {
   __device__ __forceinline__ static f4 four(const float* a, int t) { return *reinterpret_cast<const f4*>(a + t); }
 };
 
-// A block of Z or M has its free token to a lane (forwards the row, backwards the column) and four
-// contracted ones to a lane's registers.  Two of them are an operand of 32 contracted tokens:
+// Z and M are kept by blocks of 16 x 16 as the forward's operands take them: a row to a lane, four
+// columns to its registers.  Walking back the column is a lane's and the rows are contracted: four
+// reads of 4 bytes each, 16 bytes apart between the lanes.
+template <bool BACK> __device__ __forceinline__ f4 tile_at(const float* p, int t) {
+  const int l = lane_id(), g = l >> 4, r = l & 15;
+  p += t * 256;
+  if constexpr (!BACK) return *reinterpret_cast<const f4*>(p + 4 * l);
+  p += (r >> 2) * 64 + 16 * g + (r & 3);
+  return f4{p[0], p[4], p[8], p[12]};
+}
+// A block has its free token to a lane and four contracted ones to a lane's registers.  Two of them are an operand of 32 contracted tokens:
 // forwards of row block b, columns 32q.. (q <= b / 2), backwards of column block b, rows 32q..
 // (q >= b / 2); the place of an operand among the triangle's:
 __device__ __forceinline__ constexpr int pair_at(bool back, int Q, int b, int q) {
@@ -117,6 +126,13 @@ template <typename T> __device__ __forceinline__ float token_value(const void* p
 // keep their last bits
 __device__ __forceinline__ float bounded_decay(float g) { return g < -1000.f ? -1000.f : g; }
 
+// Whether any value of a wave's tiles is not finite; of large finite ones whose sum is not too
+template <int TB> __device__ __forceinline__ bool any_not_finite(const f4 (&t)[TB]) {
+  f4 s = t[0];
+#pragma unroll
+  for (int b = 1; b < TB; ++b) s += t[b];
+  return __ballot(!(fabsf((s[0] + s[1]) + (s[2] + s[3])) < 3.3895e38f)) != 0;
+}
 // The first of a column's 16 blocks' rows (tile rows 4g + e of TB tiles, a lane group each)
 // whose value is not finite, 16 TB where there is none; the same in the column's four lanes
 template <int TB> __device__ __forceinline__ int first_not_finite(const f4 (&t)[TB]) {

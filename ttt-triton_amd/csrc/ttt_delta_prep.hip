@@ -46,7 +46,7 @@ __device__ __forceinline__ void row_squares(const Stage<T, ROWS, COLS, NT>& s, f
   }
 }
 
-template <typename T, int NP, bool BACK> __global__ __launch_bounds__(256) void delta_prep_kernel(DeltaParams p) {
+template <typename T, int NP> __global__ __launch_bounds__(256) void delta_prep_kernel(DeltaParams p) {
   using Sh = PrepShared<T, NP>;
   constexpr int IN = Sh::IN, Q = Sh::Q, TB = Q / 16, NC2 = NP / 32;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -99,7 +99,7 @@ template <typename T, int NP, bool BACK> __global__ __launch_bounds__(256) void 
   for (int i = threadIdx.x; i < delta_tok_floats(Q) / 4; i += 256)
     reinterpret_cast<f4*>(p.tok + chunk * delta_tok_floats(Q))[i] = reinterpret_cast<const f4*>(&tok)[i];
 
-  // F_ij over a tile's rows (tokens tr..) and its column tc; the rows' tokens i, or j
+  // F_ij over a tile's rows (tokens tr..) and its column tc; the rows are tokens i, or j
   const auto decays = [&](int tr, int tc, bool rows_later) {
     const f4 h4 = tok.four(tok.hi, tr), l4 = tok.four(tok.lo, tr);
     const float hc = tok.hi[tc], lc = tok.lo[tc];
@@ -127,25 +127,18 @@ template <typename T, int NP, bool BACK> __global__ __launch_bounds__(256) void 
 #pragma unroll
     for (int e = 0; e < 4; ++e) at[u][e] = only_if(j < i + e, acc[e]);
   }
-  // M: forwards the free token i and contracted j, backwards the other way
+  // M: rows j, columns i
   float* mp = p.m + chunk * (TILES * 256);
 #pragma unroll
   for (int t = w; t < TILES; t += 4) {
     const int ib = tri_row(t), jb = t - tri(ib, 0);  // blocks of q and of k
     f4 acc = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int q = 0; q < NC2; ++q) {
-      const Op<IN> oq = sh.q.rows(16 * ib, 32 * q), ok = sh.k.rows(16 * jb, 32 * q);
-      if constexpr (BACK)
-        mma<kFull>(acc, oq, ok);
-      else
-        mma<kFull>(acc, ok, oq);
-    }
-    const int tr = 16 * (BACK ? ib : jb) + 4 * g, tc = 16 * (BACK ? jb : ib) + r;
-    const float fc = BACK ? tok.rk[tc] : tok.rq[tc];
-    acc *= decays(tr, tc, BACK) * tok.four(BACK ? tok.rq : tok.rk, tr) * (fc * p.scale);
+    for (int q = 0; q < NC2; ++q) mma<kFull>(acc, sh.k.rows(16 * jb, 32 * q), sh.q.rows(16 * ib, 32 * q));
+    const int j = 16 * jb + 4 * g, i = 16 * ib + r;
+    acc *= decays(j, i, false) * tok.four(tok.rk, j) * (tok.rq[i] * p.scale);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) acc[e] = only_if(BACK ? tc <= tr + e : tr + e <= tc, acc[e]);
+    for (int e = 0; e < 4; ++e) acc[e] = only_if(j + e <= i, acc[e]);
     *reinterpret_cast<f4*>(mp + (t * 64 + l) * 4) = acc;
   }
   __syncthreads();  // the rows have been read
@@ -222,39 +215,30 @@ template <typename T, int NP, bool BACK> __global__ __launch_bounds__(256) void 
 #pragma unroll
   for (int t = w; t < TILES; t += 4) {
     const int ib = tri_row(t), jb = t - tri(ib, 0);
-    f4 v;
-    if constexpr (BACK) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = sh.a[16 * ib + 4 * g + e][16 * jb + r];
-    } else {
-      v = *reinterpret_cast<const f4*>(&sh.a[16 * ib + r][16 * jb + 4 * g]);
-    }
+    const f4 v = *reinterpret_cast<const f4*>(&sh.a[16 * ib + r][16 * jb + 4 * g]);
     *reinterpret_cast<f4*>(zp + (t * 64 + l) * 4) = v;
   }
 }
 
-template <typename T, int NP, bool BACK> hipError_t prep_t(const DeltaParams& p, hipStream_t stream) {
+template <typename T, int NP> hipError_t prep_t(const DeltaParams& p, hipStream_t stream) {
   constexpr size_t lds = sizeof(PrepShared<T, NP>);
   static_assert(lds <= 160 * 1024, "LDS of a compute unit");
   constexpr int Q = kDeltaQ<T>;
-  const hipError_t e = allow_lds(delta_prep_kernel<T, NP, BACK>, lds);
+  const hipError_t e = allow_lds(delta_prep_kernel<T, NP>, lds);
   if (e != hipSuccess) return e;
   const long long blocks = (long long)p.B * p.H * ((p.L + Q - 1) / Q);
-  hipLaunchKernelGGL((delta_prep_kernel<T, NP, BACK>), dim3((unsigned)blocks), dim3(256), lds, stream, p);
+  hipLaunchKernelGGL((delta_prep_kernel<T, NP>), dim3((unsigned)blocks), dim3(256), lds, stream, p);
   return hipGetLastError();
 }
-template <typename T, bool BACK> hipError_t width_t(const DeltaParams& p, hipStream_t s) {
-  return p.N <= 32 ? prep_t<T, 32, BACK>(p, s) : p.N <= 64 ? prep_t<T, 64, BACK>(p, s) : prep_t<T, 128, BACK>(p, s);
-}
-template <typename T> hipError_t way_t(const DeltaParams& p, bool back, hipStream_t s) {
-  return back ? width_t<T, true>(p, s) : width_t<T, false>(p, s);
+template <typename T> hipError_t width_t(const DeltaParams& p, hipStream_t s) {
+  return p.N <= 32 ? prep_t<T, 32>(p, s) : p.N <= 64 ? prep_t<T, 64>(p, s) : prep_t<T, 128>(p, s);
 }
 
 }  // namespace
 
-hipError_t launch_delta_prep(const DeltaParams& p, int dtype, bool back, hipStream_t s) {
-  return dtype == TTT_DTYPE_BF16 ? way_t<__bf16>(p, back, s)
-         : dtype == TTT_DTYPE_F16 ? way_t<_Float16>(p, back, s) : way_t<float>(p, back, s);
+hipError_t launch_delta_prep(const DeltaParams& p, int dtype, hipStream_t s) {
+  return dtype == TTT_DTYPE_BF16 ? width_t<__bf16>(p, s)
+         : dtype == TTT_DTYPE_F16 ? width_t<_Float16>(p, s) : width_t<float>(p, s);
 }
 
 }  // namespace ttt

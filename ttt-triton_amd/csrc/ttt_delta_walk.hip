@@ -40,6 +40,9 @@ template <typename T, int W, int NP, bool BACK, bool OUT> struct WalkShared {
   // backwards the chunk's that the helpers form M^T do and Q^T do of
   Planes<IN, BACK ? Q : 1, NP> q;
   Planes<IN, BACK ? Q : 1, 16 * W> dO;
+  // and its M, which all waves take; of 3 blocks each wave has its own from memory
+  static constexpr bool MS = BACK && Q == 64;
+  bf8 m[MS ? kFull : 1][MS ? PAIRS : 1][MS ? 64 : 1];
   // what is handed over
   static constexpr bool YS = OUT && !BACK;
   bf8 s[YS ? W : 1][YS ? MID : 1][YS ? NC2 : 1][YS ? 64 : 1];
@@ -54,7 +57,7 @@ template <int Q, int W, bool BACK> struct Blocks {
   __device__ __forceinline__ void load(const float* p, int w) {
 #pragma unroll
     for (int i = 0; i < CNT; ++i)
-      if (i * W + w < ALL) v[i] = *reinterpret_cast<const f4*>(p + ((i * W + w) * 64 + lane_id()) * 4);
+      if (i * W + w < ALL) v[i] = tile_at<BACK>(p, i * W + w);
   }
   __device__ __forceinline__ void store(bf8 (*to)[delta_pairs(Q)][64], int w) const {
 #pragma unroll
@@ -75,7 +78,7 @@ template <int Q, bool BACK> struct Masked {
   f4 v[delta_tiles(Q)];
   __device__ __forceinline__ void load(const float* p) {
 #pragma unroll
-    for (int t = 0; t < delta_tiles(Q); ++t) v[t] = *reinterpret_cast<const f4*>(p + (t * 64 + lane_id()) * 4);
+    for (int t = 0; t < delta_tiles(Q); ++t) v[t] = tile_at<BACK>(p, t);
   }
   // of the free block b, contracted blocks 2q and 2q + 1
   template <int PL> __device__ __forceinline__ Op<PL> op(int b, int q) const {
@@ -135,7 +138,7 @@ constexpr int identity_groups(int W, int NP) { return (NP + 16 * W - 1) / (16 * 
 template <typename T, int W, int NP, bool BACK, bool OUT>
 __global__ __launch_bounds__(128 * W) void delta_walk_kernel(DeltaParams p) {
   using Sh = WalkShared<T, W, NP, BACK, OUT>;
-  static_assert(offsetof(Sh, q) % 16 == 0 && offsetof(Sh, dO) % 16 == 0 && offsetof(Sh, s) % 16 == 0 &&
+  static_assert(offsetof(Sh, q) % 16 == 0 && offsetof(Sh, dO) % 16 == 0 && offsetof(Sh, m) % 16 == 0 && offsetof(Sh, s) % 16 == 0 &&
                     offsetof(Sh, x) % 16 == 0 && offsetof(typename Sh::Side, z) % 16 == 0 &&
                     offsetof(typename Sh::Side, tok) % 16 == 0 && offsetof(typename Sh::Side, v) % 16 == 0,
                 "read 16 bytes at a time");
@@ -165,6 +168,8 @@ __global__ __launch_bounds__(128 * W) void delta_walk_kernel(DeltaParams p) {
     const int side = i >= (int)sizeof(Sh::Side::z) / 16, o = i - side * (int)sizeof(Sh::Side::z) / 16;
     reinterpret_cast<f4*>(&sh.side[side].z)[o] = f4{0.f, 0.f, 0.f, 0.f};
   }
+  if constexpr (Sh::MS)
+    for (int i = threadIdx.x; i < (int)sizeof(Sh::m) / 16; i += 2 * NT) reinterpret_cast<f4*>(&sh.m)[i] = f4{0.f, 0.f, 0.f, 0.f};
   __syncthreads();
 
   if (helps) {
@@ -174,7 +179,7 @@ __global__ __launch_bounds__(128 * W) void delta_walk_kernel(DeltaParams p) {
     const T* V = static_cast<const T*>(BACK ? p.dO : p.v) + (features ? (long long)hp * PB + f0 : 0);
     Stage<T, Q, NP, NT> sk, sq;
     Stage<T, Q, 16 * W, NT> sv;
-    Blocks<Q, W, BACK> bz;
+    Blocks<Q, W, BACK> bz, bm;
     Copy<delta_tok_floats(Q), NT> ct;
     Masked<Q, BACK> m;
     sk.place(p.ldk, p.N);
@@ -247,7 +252,7 @@ __global__ __launch_bounds__(128 * W) void delta_walk_kernel(DeltaParams p) {
         __syncthreads();  // what was handed over has been read
         const int c = chunk_of(k - 1), left = min(Q, p.L - c * Q);
         // (x is no number from the first token on whose row is not finite: below)
-        const int bad = first_not_finite(x);
+        const int bad = any_not_finite(x) ? first_not_finite(x) : Q;
         if (__ballot(bad < Q) != 0) {
 #pragma unroll
           for (int ob = 0; ob < TB; ++ob)
@@ -299,10 +304,11 @@ __global__ __launch_bounds__(128 * W) void delta_walk_kernel(DeltaParams p) {
         const int left = min(Q, p.L - c * Q);
         sq.load(Qr + first_row(c) * p.ldq, left);
         sv.load(V + first_row(c) * ldv, features ? left : 0);
+        if constexpr (Sh::MS) bm.load(p.m + (head * NC + c) * (delta_tiles(Q) * 256), w);
       };
       f4 eq[QB][2];
-      const auto fetch_m = [&](int c) {
-        m.load(p.m + (head * NC + c) * (delta_tiles(Q) * 256));
+      const auto fetch_own = [&](int c) {
+        if constexpr (!Sh::MS) m.load(p.m + (head * NC + c) * (delta_tiles(Q) * 256));
         const float* of = p.tok + (head * NC + c) * delta_tok_floats(Q) + 7 * Q + 4 * g;
 #pragma unroll
         for (int q = 0; q < QB; ++q)
@@ -312,6 +318,7 @@ __global__ __launch_bounds__(128 * W) void delta_walk_kernel(DeltaParams p) {
       const auto put_do = [&] {
         sq.store(sh.q);
         sv.store(sh.dO);
+        if constexpr (Sh::MS) bm.store(sh.m, w);
       };
       // M^T do and Q^T do, the latter with its factors
       f4 md[TB], qd[NB];
@@ -324,7 +331,16 @@ __global__ __launch_bounds__(128 * W) void delta_walk_kernel(DeltaParams p) {
           md[ob] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int q = 0; q < QB; ++q)
-            if (meets(true, ob, 2 * q + 1)) mma<kFull>(md[ob], m.template op<kFull>(ob, q), dt[q]);
+            if (meets(true, ob, 2 * q + 1)) {
+              Op<kFull> mo;
+              if constexpr (Sh::MS) {
+#pragma unroll
+                for (int a = 0; a < kFull; ++a) mo.v[a] = sh.m[a][pair_at(true, Q, ob, q)][l];
+              } else {
+                mo = m.template op<kFull>(ob, q);
+              }
+              mma<kFull>(md[ob], mo, dt[q]);
+            }
         }
 #pragma unroll
         for (int i = 0; i < NB; ++i) qd[i] = f4{0.f, 0.f, 0.f, 0.f};
@@ -343,7 +359,7 @@ __global__ __launch_bounds__(128 * W) void delta_walk_kernel(DeltaParams p) {
       };
       fetch(chunk_of(0));
       fetch_do(chunk_of(0));
-      fetch_m(chunk_of(0));
+      fetch_own(chunk_of(0));
       put(sh.side[0]);
       put_do();
       __syncthreads();
@@ -352,7 +368,7 @@ __global__ __launch_bounds__(128 * W) void delta_walk_kernel(DeltaParams p) {
       if (n > 1) {
         fetch(chunk_of(1));
         fetch_do(chunk_of(1));
-        fetch_m(chunk_of(1));
+        fetch_own(chunk_of(1));
       }
       __syncthreads();
       if (n > 1) put_do();
@@ -362,7 +378,7 @@ __global__ __launch_bounds__(128 * W) void delta_walk_kernel(DeltaParams p) {
         if (k + 2 < n) fetch_do(chunk_of(k + 2));
         if (k + 1 < n) {
           form();
-          if (k + 2 < n) fetch_m(chunk_of(k + 2));
+          if (k + 2 < n) fetch_own(chunk_of(k + 2));
         }
         __syncthreads();  // what was handed over has been read, and so have q and do
         if (k + 1 < n) {
@@ -379,6 +395,7 @@ __global__ __launch_bounds__(128 * W) void delta_walk_kernel(DeltaParams p) {
     return;
   }
 
+  if (!OUT) __builtin_amdgcn_s_setprio(2);
   StateTiles<NP> st;
   if (!OUT) {
     st.load(nullptr, 0, 0, w);
@@ -446,7 +463,7 @@ __global__ __launch_bounds__(128 * W) void delta_walk_kernel(DeltaParams p) {
       for (int ob = 0; ob < TB; ++ob) by[ob] = t[ob] * tok.four(tok.beta, 16 * ob + 4 * g);
       if constexpr (!BACK) {
         // A token that is not finite reaches the tokens behind it alone: 0 times it is no 0
-        bad = first_not_finite(by);
+        if (any_not_finite(by)) bad = first_not_finite(by);
         if (__ballot(bad < Q) != 0) {
 #pragma unroll
           for (int ob = 0; ob < TB; ++ob)

@@ -97,7 +97,7 @@ SIGNATURES = {
     "ttt_delta_workspace_bytes": (_S, [_I] * 6),
     "ttt_delta_fwd": (_I, [_P, _L] * 5 + [_P] + [_I] * 6 + [_F] + [_I] * 4 + [_P, _P] + [_P, _S] * 2 + [_P]),
     "ttt_delta_bwd_workspace_bytes": (_S, [_I] * 7),
-    "ttt_delta_bwd": (_I, [_P, _L] * 5 + [_P, _P, _S] + [_I] * 6 + [_F] + [_I] * 4 + [_P] * 6 + [_P, _S, _P]),
+    "ttt_delta_bwd": (_I, [_P, _L] * 5 + [_P, _P, _S, _P, _S] + [_I] * 6 + [_F] + [_I] * 4 + [_P] * 6 + [_P, _S, _P]),
     "ttt_delta_step": (_I, [_P, _L] * 5 + [_P] + [_I] * 5 + [_F] + [_I] * 4 + [_P, _P]),
     "ttt_block_norm_fwd": (_I, [_P, _L] * 3 + [_P] * 3 + [_L, _I, _I, _F, _I, _I] + [_P] * 4),
     "ttt_block_norm_partial_bytes": (_S, [_L, _I]),

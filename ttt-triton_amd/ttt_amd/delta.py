@@ -105,18 +105,19 @@ def _delta_forward(q, k, v, g, beta, h0, scale, unit, want_last, train):
                                br.data_ptr(), ldb, _opt(h0), B, L, H, P, G, N, scale, unit, *codes, o.data_ptr(),
                                _opt(last), _opt(saved), nsv, ws.data_ptr(), nws, _stream(dev))
     _lib.check(st, "ttt_delta_fwd")
-    return o, last, (rows, saved, sizes, codes, scale)
+    return o, last, (rows, saved, ws, sizes, codes, scale)
 
 
 class GatedDeltaFunction(torch.autograd.Function):
     """apply(q, k, v, g, beta, initial_state, scale, l2_norm, want_last) -> (o, last state
     or None); differentiable wrt all tensors.  The forward keeps the states entering its
-    chunks of 64 tokens (32 in fp32 and fp16) and what each token's state missed."""
+    chunks of 64 tokens (32 in fp32 and fp16), what each token's state missed, and its
+    workspace: what the chunks' keys and queries give by themselves."""
 
     @staticmethod
     def forward(ctx, q, k, v, g, beta, h0, scale, unit, want_last):
-        o, last, (rows, saved, sizes, codes, scale) = _delta_forward(q, k, v, g, beta, h0, scale, unit, want_last, True)
-        ctx.save_for_backward(rows[0], rows[2], rows[4], rows[6], saved)
+        o, last, (rows, saved, kept, sizes, codes, scale) = _delta_forward(q, k, v, g, beta, h0, scale, unit, want_last, True)
+        ctx.save_for_backward(rows[0], rows[2], rows[4], rows[6], saved, kept)
         ctx.lds, ctx.strides = rows[1::2], tuple(t.stride() for t in rows[::2])
         ctx.sizes, ctx.codes, ctx.scale, ctx.unit = sizes, codes, scale, unit
         ctx.state_dtype = None if h0 is None else h0.dtype
@@ -126,12 +127,12 @@ class GatedDeltaFunction(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, do, dlast):
-        q, k, g, beta, saved = ctx.saved_tensors
+        q, k, g, beta, saved, kept = ctx.saved_tensors
         B, L, H, P, G, N = ctx.sizes
         ldq, ldk, ldg, ldb = ctx.lds
         if (q.stride(), k.stride(), g.stride(), beta.stride()) != ctx.strides or (q.data_ptr() | k.data_ptr()) % 16:
             q, ldq, k, ldk, g, ldg, beta, ldb = _qk_rows(q, k, g, beta, ctx.sizes)
-        saved = _whole(saved, 16)
+        saved, kept = _whole(saved, 16), _whole(kept, 16)
         dev, act = q.device, q.dtype
         do = torch.zeros((B, L, H, P), device=dev, dtype=act) if do is None else do
         dor, ldo = _near_rows(do if do.dtype == act else do.to(act), 16, H * P)
@@ -145,8 +146,8 @@ class GatedDeltaFunction(torch.autograd.Function):
         ws = saved.new_empty(nws)
         with on_device(dev):
             st = lib.ttt_delta_bwd(q.data_ptr(), ldq, k.data_ptr(), ldk, g.data_ptr(), ldg, beta.data_ptr(), ldb,
-                                   dor.data_ptr(), ldo, _opt(dlast), saved.data_ptr(), saved.numel(), B, L, H, P, G, N,
-                                   ctx.scale, ctx.unit, *ctx.codes, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                                   dor.data_ptr(), ldo, _opt(dlast), saved.data_ptr(), saved.numel(), kept.data_ptr(),
+                                   kept.numel(), B, L, H, P, G, N, ctx.scale, ctx.unit, *ctx.codes, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                                    dg.data_ptr(), db.data_ptr(), _opt(dh0), ws.data_ptr(), nws, _stream(dev))
         _lib.check(st, "ttt_delta_bwd")
         return dq, dk, dv, dg, db, _as(dh0, ctx.state_dtype), None, None, None
