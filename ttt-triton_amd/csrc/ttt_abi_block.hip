@@ -369,7 +369,7 @@ size_t ttt_delta_workspace_bytes(int B, int L, int H, int P, int N, int dtype) {
 }
 size_t ttt_delta_bwd_workspace_bytes(int B, int L, int H, int P, int G, int N, int dtype) {
   DeltaPlan s;
-  return delta_plan_ok(B, L, H, P, G, N, dtype, s) ? s.states + s.rows + 2 * s.qk + s.seg + s.trans : 0;
+  return delta_plan_ok(B, L, H, P, G, N, dtype, s) ? s.states + s.rows + 2 * s.qk + s.seg : 0;
 }
 
 int ttt_delta_fwd(const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv,
@@ -467,8 +467,9 @@ int ttt_delta_bwd(const void* q, long long ldq, const void* k, long long ldk, co
   REQUIRE(dbeta, size_of(beta_dtype));
   OPTIONAL(dh_last, 16);
   OPTIONAL(dh0, 16);
-  if (saved_bytes < s.states + s.rows || kept_bytes < s.tok + 2 * s.zm) return TTT_ERR_WORKSPACE;
-  if (workspace == nullptr || workspace_bytes < s.states + s.rows + 2 * s.qk + s.seg + s.trans) return TTT_ERR_WORKSPACE;
+  if (saved_bytes < s.states + s.rows || kept_bytes < s.tok + 2 * s.zm + s.seg + s.trans)
+    return TTT_ERR_WORKSPACE;
+  if (workspace == nullptr || workspace_bytes < s.states + s.rows + 2 * s.qk + s.seg) return TTT_ERR_WORKSPACE;
   OPTIONAL(workspace, 16);
   ttt::DeltaParams p{};
   p.q = q;
@@ -510,7 +511,7 @@ int ttt_delta_bwd(const void* q, long long ldq, const void* k, long long ldk, co
   p.per = s.per;
   if (s.S > 1) {
     p.seg = reinterpret_cast<float*>(take(s.seg));
-    p.trans = reinterpret_cast<float*>(take(s.trans));
+    p.trans = of + (s.tok + 2 * s.zm + s.seg) / 4;
   }
   if (s.share > 1) {
     p.dqp = reinterpret_cast<float*>(take(s.qk));

@@ -17,9 +17,12 @@
 // the state S that enters it to T S + E, with T = prod e^{g_t} (1 - b_t k_t (x) k_t): a first walk
 // without outputs, of all segments at once, gives E from the state 0 and T from the columns of
 // the identity, as features without values; one launch goes over the segments with their
-// products (delta_join_kernel), and then all segments are walked at once.
+// products (delta_join_kernel), and then all segments are walked at once.  Back, a segment takes
+// the gradient dS' to T^T dS' + E', with the forward's T.
 #include <math.h>
 #include <stddef.h>
+
+#include <type_traits>
 
 #include "ttt_buf.h"
 #include "ttt_delta.h"
@@ -133,6 +136,8 @@ template <typename T> __device__ __forceinline__ Op<ScanType<T>::IN> row_op(cons
 
 // workgroups that have the columns of the identity between them
 constexpr int identity_groups(int W, int NP) { return (NP + 16 * W - 1) / (16 * W); }
+// segments whose products are formed: those before the last, and where a way back follows that too
+__host__ __device__ __forceinline__ int product_segments(const DeltaParams& p) { return p.states != nullptr ? p.S : p.S - 1; }
 
 // OUT: outputs too; else the segments' ends alone
 template <typename T, int W, int NP, bool BACK, bool OUT>
@@ -149,12 +154,14 @@ __global__ __launch_bounds__(128 * W) void delta_walk_kernel(DeltaParams p) {
   const int w = helps ? wave_id() : wave_id() - W, l = lane_id(), g = l >> 4, r = l & 15;
   const int PB = delta_part(p.P), parts = p.P / PB, cols = PB / (16 * W), NC = (p.L + Q - 1) / Q;
   const unsigned at = on_xcd(blockIdx.x, gridDim.x);
-  // groups of columns to a head: of its features, and without outputs of the identity behind them
-  const int own = parts * cols, groups = own + (OUT ? 0 : identity_groups(W, NP)), segs = OUT ? p.S : p.S - 1;
+  // groups of columns to a head: of its features, and for the segments' products of the identity
+  const int own = parts * cols, groups = own + (OUT || BACK ? 0 : identity_groups(W, NP));
+  const int segs = OUT ? p.S : BACK ? p.S - 1 : product_segments(p);
   const int grp_c = (int)(at % groups);
   const int s = (int)(at / groups % segs) + (!OUT && BACK ? 1 : 0);
   const long long head = at / groups / segs;  // sequence and head
-  const bool features = OUT || grp_c < own;
+  const bool features = OUT || BACK || grp_c < own;
+  if (!OUT && !BACK && features && s == p.S - 1) return;  // (the way back takes its product alone)
   const int b = (int)(head / p.H), h = (int)(head - (long long)b * p.H), grp = h / (p.H / p.G);
   const int part = features ? grp_c / cols : 0, f0 = features ? 16 * W * (grp_c % cols) : 16 * W * (grp_c - own);
   const int hp = h * parts + part;
@@ -399,7 +406,7 @@ __global__ __launch_bounds__(128 * W) void delta_walk_kernel(DeltaParams p) {
   StateTiles<NP> st;
   if (!OUT) {
     st.load(nullptr, 0, 0, w);
-    if (!features) {
+    if (!BACK && !features) {
 #pragma unroll
       for (int i = 0; i < NB; ++i)
 #pragma unroll
@@ -553,7 +560,7 @@ __global__ __launch_bounds__(128 * W) void delta_walk_kernel(DeltaParams p) {
     __syncthreads();
   }
   if (!OUT) {
-    if (features)
+    if (BACK || features)
       st.keep(p.seg + (chain * p.S + s) * (NP * PB) + f0, PB, w);
     else if (f0 + 16 * w < NP)  // (32 columns leave two of four waves without any)
       st.keep(p.trans + (head * p.S + s) * (NP * NP) + f0, NP, w);
@@ -564,7 +571,9 @@ __global__ __launch_bounds__(128 * W) void delta_walk_kernel(DeltaParams p) {
 
 // The segments' ends -> the states they start from, in place: a workgroup has 16 features of a
 // part and goes over the segments, a wave to 16 rows of the state, which go from one to the next
-// through LDS; the next segment's product is on its way.
+// through LDS; the products of the next four are on their way (with one: 20 us for 20 segments of 64 x 64).
+constexpr int kAhead = 4;
+static_assert(kAhead % 2 == 0, "two places in turn");
 template <int NP, bool BACK> __global__ __launch_bounds__(4 * NP) void delta_join_kernel(DeltaParams p) {
   constexpr int NB = NP / 16, NC2 = NP / 32;
   __shared__ Planes<kFull, 16, NP> sh[2];  // features by n
@@ -576,40 +585,60 @@ template <int NP, bool BACK> __global__ __launch_bounds__(4 * NP) void delta_joi
   if (p.h0 != nullptr && n < p.N) st = *reinterpret_cast<const f4*>(p.h0 + (chain * PB + f) * p.N + n);
   const auto seg = [&](int k) { return BACK ? p.S - 1 - k : k; };
   const auto at = [&](int k) { return p.seg + (chain * p.S + seg(k)) * (NP * PB) + n * PB + f; };
-  f4 a[NC2][2];  // row 16 w + r, columns 32q + 8g..
-  const auto fetch = [&](int k) {
-    const float* t = p.trans + (head * p.S + seg(k)) * (NP * NP) + (16 * w + r) * NP + 8 * g;
+  struct Segment {
+    f4 a[NC2][2];  // row 16 w + r, columns 32q + 8g.., back of the transposed
+    f4 end;
+  } on[kAhead];
+  // (past the last one that one again: no branches, so that a wait is for the oldest loads alone)
+  const auto fetch = [&](Segment& to, int k) {
+    k = min(k, p.S - 2);
+    const float* t = p.trans + (head * p.S + seg(k)) * (NP * NP) + (BACK ? 8 * g * NP + 16 * w + r : (16 * w + r) * NP + 8 * g);
 #pragma unroll
     for (int q = 0; q < NC2; ++q)
 #pragma unroll
-      for (int o = 0; o < 2; ++o) a[q][o] = *reinterpret_cast<const f4*>(t + 32 * q + 4 * o);
+      for (int o = 0; o < 2; ++o)
+        if constexpr (BACK) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) end[e] = at(k)[e * PB];
+          for (int e = 0; e < 4; ++e) to.a[q][o][e] = t[(32 * q + 4 * o + e) * NP];
+        } else {
+          to.a[q][o] = *reinterpret_cast<const f4*>(t + 32 * q + 4 * o);
+        }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) to.end[e] = at(k)[e * PB];
   };
   const auto keep = [&](int k, f4 v) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) at(k)[e * PB] = v[e];
   };
-  fetch(0);
+#pragma unroll
+  for (int d = 0; d < kAhead; ++d) fetch(on[d], d);
+  const auto go = [&](int k0, auto more) {
+#pragma unroll
+    for (int d = 0; d < kAhead; ++d) {
+      const int k = k0 + d;
+      if (!more && k + 1 >= p.S) break;
+      Planes<kFull, 16, NP>& of = sh[d & 1];
+      bf4 o[kFull];
+      split4<kFull>(st, o);
+#pragma unroll
+      for (int q = 0; q < kFull; ++q) *reinterpret_cast<bf4*>(&of.d[q][r][n]) = o[q];
+      Op<kFull> m[NC2];
+#pragma unroll
+      for (int q = 0; q < NC2; ++q) m[q] = split8<kFull>(on[d].a[q][0], on[d].a[q][1]);
+      const f4 last = st;
+      st = on[d].end;
+      // (two places in turn: a wave is at most one segment ahead of another)
+      __syncthreads();
+      keep(k, last);
+      if constexpr (more) fetch(on[d], k + kAhead);
+#pragma unroll
+      for (int q = 0; q < NC2; ++q) mma<kFull>(st, m[q], of.rows(0, 32 * q));
+    }
+  };
+  int k = 0;
 #pragma unroll 1
-  for (int k = 0; k + 1 < p.S; ++k) {
-    Planes<kFull, 16, NP>& of = sh[k & 1];
-    bf4 o[kFull];
-    split4<kFull>(st, o);
-#pragma unroll
-    for (int q = 0; q < kFull; ++q) *reinterpret_cast<bf4*>(&of.d[q][r][n]) = o[q];
-    Op<kFull> m[NC2];
-#pragma unroll
-    for (int q = 0; q < NC2; ++q) m[q] = split8<kFull>(a[q][0], a[q][1]);
-    const f4 last = st;
-    st = end;
-    // (two places in turn: a wave is at most one segment ahead of another)
-    __syncthreads();
-    keep(k, last);
-    if (k + 2 < p.S) fetch(k + 1);
-#pragma unroll
-    for (int q = 0; q < NC2; ++q) mma<kFull>(st, m[q], of.rows(0, 32 * q));
-  }
+  for (; k + kAhead + 1 < p.S; k += kAhead) go(k, std::true_type{});
+  go(k, std::false_type{});
   keep(p.S - 1, st);
 }
 
@@ -622,7 +651,8 @@ template <typename T, int W, int NP, bool BACK> hipError_t walk_t(const DeltaPar
   if (p.S > 1) {
     e = allow_lds(delta_walk_kernel<T, W, NP, BACK, false>, lds1);
     if (e != hipSuccess) return e;
-    const long long groups = heads * (p.S - 1) * (p.P / (16 * W) + identity_groups(W, NP));
+    const long long groups =
+        BACK ? heads * (p.S - 1) * (p.P / (16 * W)) : heads * product_segments(p) * (p.P / (16 * W) + identity_groups(W, NP));
     hipLaunchKernelGGL((delta_walk_kernel<T, W, NP, BACK, false>), dim3((unsigned)groups), dim3(128 * W), lds1, stream, p);
     hipLaunchKernelGGL((delta_join_kernel<NP, BACK>), dim3((unsigned)(heads * p.P / 16)), dim3(4 * NP), 0, stream,
                        p);
