@@ -27,7 +27,8 @@ struct FfnParams {
   long long lddy;
   int R, D, F, Dp, Fp;        // widths as the user's and padded to 8
   int planes, act;
-  int splits, bias_parts;     // (splits: of the product that is launched)
+  int splits, whole;          // of the product that is launched (FfnCut)
+  int bias_parts;
 };
 // few rows: the operands as the user's, rows of x ldx elements apart
 hipError_t launch_ffn_few(const FfnParams& p, int dtype, hipStream_t stream);
@@ -43,17 +44,20 @@ constexpr int ffn_planes(int dtype) { return dtype == TTT_DTYPE_F32 ? 3 : 1; }
 
 // How a product is cut up: tiles of 256 x 256, a workgroup to a compute unit, or of 128 x 128,
 // two; and the steps of 64 contracted values of a tile into shares, whose sums are joined by
-// another launch.
+// another launch.  Or as many whole rounds of large tiles as there are, and what is left of them,
+// less than a round, in four small ones each by another launch.
 struct FfnCut {
   bool large;
   int splits;
+  int whole;  // large tiles before the small ones, or 0: one size
 };
 // M x N results (the width of both projections together), `steps` of 64 contracted values, joined
-// over `most` shares or fewer.  In units of a step of a large tile (1,024 clocks at the matrix
-// instructions' rate, about 1,500 measured), a small tile's takes 0.6 with another on the compute
-// unit; a tile's start and end take about 5; a join reads and writes its sums at the card's bandwidth.
-inline FfnCut ffn_cut(long long M, long long N, long long steps, int most) {
-  FfnCut best{false, 1};
+// over `most` shares or fewer, `mixed` where two sizes may be.  In units of a step of a large tile
+// (1.7 us at the rate of a large product), a small tile's takes 0.6 with another on the compute unit;
+// a tile's start and end take about 5, another launch 2; a join reads and writes its sums at the
+// card's bandwidth.
+inline FfnCut ffn_cut(long long M, long long N, long long steps, int most, bool mixed) {
+  FfnCut best{false, 1, 0};
   double least = 0.0;
   for (int large = 0; large < 2; ++large) {
     const long long side = large ? 256 : 128, places = large ? 256 : 512;
@@ -64,9 +68,14 @@ inline FfnCut ffn_cut(long long M, long long N, long long steps, int most) {
       const double time = rounds * ((double)((steps + k - 1) / k) * (large ? 1.0 : 0.6) + 5.0) + join;
       if ((large == 0 && k == 1) || time < least) {
         least = time;
-        best = {large != 0, k};
+        best = {large != 0, k, 0};
       }
     }
+  }
+  const long long tiles = ((M + 255) / 256) * ((N + 255) / 256), whole = tiles / 256 * 256;
+  if (mixed && whole > 0 && whole < tiles) {
+    const double small = (double)((4 * (tiles - whole) + 511) / 512);
+    if ((double)(whole / 256) * ((double)steps + 5.0) + small * ((double)steps * 0.6 + 5.0) + 2.0 < least) best = {false, 1, (int)whole};
   }
   return best;
 }
@@ -74,16 +83,19 @@ constexpr int kFfnMostSplits = 16;
 inline long long ffn_steps(long long contracted, int dtype) {
   return (contracted + kFfnStep - 1) / kFfnStep * (dtype == TTT_DTYPE_F32 ? 6 : 1);
 }
-inline FfnCut ffn_cut_up(long long R, int D, int F, int dtype) { return ffn_cut(R, 2LL * F, ffn_steps(ffn_pad(D), dtype), 1); }
+// (one size with sums of rows, which are by a tile's waves)
+inline FfnCut ffn_cut_up(long long R, int D, int F, int dtype, bool sums) {
+  return ffn_cut(R, 2LL * F, ffn_steps(ffn_pad(D), dtype), 1, !sums);
+}
 inline FfnCut ffn_cut_dx(long long R, int D, int F, int dtype) {
-  return ffn_cut(R, D, 2 * ffn_steps(ffn_pad(F), dtype), kFfnMostSplits);
+  return ffn_cut(R, D, 2 * ffn_steps(ffn_pad(F), dtype), kFfnMostSplits, true);
 }
 inline FfnCut ffn_cut_dw(long long R, int D, int F, int dtype) {
-  return ffn_cut(2LL * ffn_pad(F), D, ffn_steps(R, dtype), kFfnMostSplits);
+  return ffn_cut(2LL * ffn_pad(F), D, ffn_steps(R, dtype), kFfnMostSplits, false);
 }
 // rows of partial sums of the bias gradients: one to a wave's rows
 inline int ffn_bias_parts(long long R, int D, int F, int dtype) {
-  const long long side = ffn_cut_up(R, D, F, dtype).large ? 256 : 128;
+  const long long side = ffn_cut_up(R, D, F, dtype, true).large ? 256 : 128;
   return (int)((R + side - 1) / side) * 2;
 }
 

@@ -120,6 +120,25 @@ template <Lies L, Side S, int FREE> __device__ __forceinline__ bf8 take(const un
   }
 }
 
+// The order of a step's reads of LDS and products: the first operands, then a read to every few
+// products, two or more tiles ahead of them.  (By itself the compiler has each pair of reads right
+// before its products, which wait for them.)
+template <int N, int PER> __device__ __forceinline__ void interleave() {
+  if constexpr (N > 0) {
+    __builtin_amdgcn_sched_group_barrier(0x008, PER, 0);  // matrix instructions
+    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);    // reads of LDS
+    interleave<N - 1, PER>();
+  }
+}
+template <int TN, int TM, Lies LN, Lies LM> __device__ __forceinline__ void reads_ahead() {
+  constexpr int rn = LN == Lies::Free ? 2 : 1, rm = LM == Lies::Free ? 2 : 1, K = kFfnStep / 32;
+  constexpr int head = TN * rn + 2 * rm, rest = K * (TN * rn + TM * rm) - head, products = K * TN * TM, per = (products - 2 * TN) / rest;
+  static_assert(per > 0, "a product to a read at least");
+  __builtin_amdgcn_sched_group_barrier(0x100, head, 0);
+  interleave<rest, per>();
+  __builtin_amdgcn_sched_group_barrier(0x008, products - rest * per, 0);
+}
+
 // 4 values of T behind each other from p, of n there are
 template <typename T> __device__ __forceinline__ f4 load_up_to4(const T* p, int n) {
   Raw<T, 4> v;
@@ -155,14 +174,21 @@ __global__ __launch_bounds__(64 * WN * WM) void ffn_kernel(FfnParams p) {
   const int w = wave_id(), l = lane_id(), g = l >> 4, r = l & 15, wn = w % WN, wm = w / WN;
   // rows and columns of all tiles, and contracted values
   const int M = JOB == Job::Dw ? 2 * p.Fp : p.R, N = UP ? p.F : p.D, K = JOB == Job::Dw ? p.R : JOB == Job::Dx ? p.Fp : p.Dp;
-  const int tm = (M + BM - 1) / BM, tn = (N + (UP ? HALF : BN) - 1) / (UP ? HALF : BN);
+  // (behind whole rounds of large tiles: those that are left, in four)
+  constexpr bool SMALL = BM == 128;
+  const int in_four = SMALL && p.whole > 0 ? 2 : 1, HM = in_four * BM, HN = in_four * (UP ? HALF : BN);
+  const int tm = (M + HM - 1) / HM, tn = (N + HN - 1) / HN;
   // Neighbours on a die have eight rows of tiles by all columns, one column after the other
   unsigned id = on_xcd(blockIdx.x, gridDim.x);
+  const unsigned quarter = in_four == 2 ? id & 3 : 0;
+  if (in_four == 2) id = p.whole + id / 4;
   const int split = (int)(id / (unsigned)(tm * tn));
   id -= split * (tm * tn);
   const int band = (int)(id / (8u * tn)), high = min(8, tm - 8 * band);
   id -= band * 8 * tn;
-  const int m0 = (8 * band + (int)(id % high)) * BM, n0 = (int)(id / high) * (UP ? HALF : BN);
+  const int m0 = (8 * band + (int)(id % high)) * HM + (int)(quarter & 1) * BM;
+  const int n0 = (int)(id / high) * HN + (int)(quarter >> 1) * (UP ? HALF : BN);
+  if (m0 >= M || n0 >= N) return;
 
   const int ksteps = (K + kFfnStep - 1) / kFfnStep, pairs = p.planes == 3 ? 6 : 1, segs = JOB == Job::Dx ? 2 : 1;
   const int all = ksteps * pairs * segs, per = UP ? all : (all + p.splits - 1) / p.splits;
@@ -231,6 +257,7 @@ __global__ __launch_bounds__(64 * WN * WM) void ffn_kernel(FfnParams p) {
 #pragma unroll
         for (int i = 0; i < TN; ++i) acc[i][j] = product<E>(pn[i], pm[j], acc[i][j]);
     }
+    reads_ahead<TN, TM, LN, LM>();
   }
 
   // A pair of tiles' columns are eight neighbours in a lane: 8g + 4i + e of 32
@@ -438,7 +465,10 @@ template <typename T, Job JOB, int WN, int WM, int TN, int TM> hipError_t tile_t
   if (e != hipSuccess) return e;
   constexpr bool up = JOB == Job::Fwd || JOB == Job::Grad;
   const long long M = JOB == Job::Dw ? 2LL * p.Fp : p.R, N = up ? 2LL * p.F : p.D;
-  const long long blocks = ((M + BM - 1) / BM) * ((N + BN - 1) / BN) * p.splits;
+  const long long large = ((M + 255) / 256) * ((N + 255) / 256);
+  const long long blocks = p.whole == 0 ? ((M + BM - 1) / BM) * ((N + BN - 1) / BN) * p.splits
+                           : BM == 256  ? p.whole
+                                        : 4 * (large - p.whole);
   hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(64 * WN * WM), lds, s, p);
   if (p.splits > 1) {
     const long long quads = M * p.Dp / 4;
@@ -447,10 +477,15 @@ template <typename T, Job JOB, int WN, int WM, int TN, int TM> hipError_t tile_t
   return hipGetLastError();
 }
 template <typename T, Job JOB> hipError_t job_t(const FfnParams& p, bool large, hipStream_t s) {
+  if (p.whole > 0) {
+    const hipError_t e = tile_t<T, JOB, 4, 2, 4, 8>(p, s);
+    if (e != hipSuccess) return e;
+  }
   return large ? tile_t<T, JOB, 4, 2, 4, 8>(p, s) : tile_t<T, JOB, 2, 2, 4, 4>(p, s);
 }
 template <Job JOB> hipError_t type_t(FfnParams p, FfnCut cut, int dtype, hipStream_t s) {
   p.splits = cut.splits;
+  p.whole = cut.whole;
   return dtype == TTT_DTYPE_BF16 ? job_t<__bf16, JOB>(p, cut.large, s)
          : dtype == TTT_DTYPE_F16 ? job_t<_Float16, JOB>(p, cut.large, s) : job_t<float, JOB>(p, cut.large, s);
 }
@@ -481,9 +516,9 @@ hipError_t planes_t(const void* from, long long ld, int rows, int width, void* t
 hipError_t launch_ffn_few(const FfnParams& p, int dtype, hipStream_t s) {
   return dtype == TTT_DTYPE_BF16 ? few_t<__bf16>(p, s) : dtype == TTT_DTYPE_F16 ? few_t<_Float16>(p, s) : few_t<float>(p, s);
 }
-hipError_t launch_ffn_fwd(const FfnParams& p, int dtype, hipStream_t s) { return type_t<Job::Fwd>(p, ffn_cut_up(p.R, p.D, p.F, dtype), dtype, s); }
+hipError_t launch_ffn_fwd(const FfnParams& p, int dtype, hipStream_t s) { return type_t<Job::Fwd>(p, ffn_cut_up(p.R, p.D, p.F, dtype, false), dtype, s); }
 hipError_t launch_ffn_grad(const FfnParams& p, int dtype, hipStream_t s) {
-  const hipError_t e = type_t<Job::Grad>(p, ffn_cut_up(p.R, p.D, p.F, dtype), dtype, s);
+  const hipError_t e = type_t<Job::Grad>(p, ffn_cut_up(p.R, p.D, p.F, dtype, p.bias_part != nullptr), dtype, s);
   if (e != hipSuccess || p.bias_part == nullptr) return e;
   return dtype == TTT_DTYPE_BF16 ? bias_t<__bf16>(p, s) : dtype == TTT_DTYPE_F16 ? bias_t<_Float16>(p, s) : bias_t<float>(p, s);
 }
