@@ -59,6 +59,17 @@ template <bool GRAD> __device__ __forceinline__ float act_value(int act, float a
   return a * c;
 }
 
+// .. of N values, one branch for all of them: their exponentials and reciprocals overlap
+template <bool GRAD, int N> __device__ __forceinline__ void act_values(int act, const float (&a)[N], float (&f)[N], float (&d)[N]) {
+  if (act == TTT_ACT_SILU) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) f[e] = act_value<GRAD>(TTT_ACT_SILU, a[e], d[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) f[e] = act_value<GRAD>(TTT_ACT_GELU, a[e], d[e]);
+  }
+}
+
 enum class Job { Fwd, Grad, Dx, Dw };
 // how an operand lies: its contracted values side by side, or its free ones
 enum class Lies { Contracted, Free };
@@ -286,19 +297,21 @@ __global__ __launch_bounds__(64 * WN * WM) void ffn_kernel(FfnParams p) {
       for (int j = 0; j < TM; ++j) {
         const int m = m0 + 16 * (wm * TM + j) + r;
         float u[8], v[8];  // y; or da and db
+        float a[8], fa[8], d[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) a[e] = acc[i + e / 4][j][e & 3] + bg.f(e);
+        act_values<JOB == Job::Grad>(p.act, a, fa, d);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float a = acc[i + e / 4][j][e & 3] + bg.f(e), b = acc[TN / 2 + i + e / 4][j][e & 3] + bu.f(e);
+          const float b = acc[TN / 2 + i + e / 4][j][e & 3] + bu.f(e);
           if constexpr (JOB == Job::Fwd) {
-            float d;
-            u[e] = act_value<false>(p.act, a, d) * b;
+            u[e] = fa[e] * b;
           } else {
             // (0 past the last row and column: nothing from there reaches the sums)
-            float d;
-            const float y = dy[j].f(e), f = act_value<true>(p.act, a, d);
+            const float y = dy[j].f(e);
             const bool in = m < M && e < left;
-            v[e] = in ? y * f : 0.f;
-            u[e] = in ? y * b * d : 0.f;
+            v[e] = in ? y * fa[e] : 0.f;
+            u[e] = in ? y * b * d[e] : 0.f;
             sg[e] += u[e];
             su[e] += v[e];
           }
