@@ -173,6 +173,21 @@ def test_not_finite(lib, dt, which, bad):
             assert torch.isnan(o[t:, 0]).all() and torch.isnan(got["last"][1, 0]).all()
 
 
+def test_largest_values(lib):
+    """A value above what the products' planes hold, 3.39e38, counts as infinite whatever stands
+    beside it: no earlier output sees it."""
+    d = T.dev(T.delta_inputs(2, 100, 1, 1, 32, 32, F32, seed=13))
+    d["beta"][:] = 1.0
+    ref = T.delta_run(d, grads=False)
+    for t in (5, 30, 70):
+        for other in (-3.3e38, 3.3e38):
+            e = {**d, "v": d["v"].clone()}
+            e["v"][1, t, 0, 0], e["v"][1, t + 1, 0, 0] = 3.4e38, other
+            got = T.delta_run(e, grads=False)
+            assert torch.equal(got["o"][0], ref["o"][0]) and torch.equal(got["o"][1, :t], ref["o"][1, :t]), (t, other)
+            assert torch.isnan(got["o"][1, t:, 0, 0]).all() and torch.equal(got["o"][1, :, :, 1:], ref["o"][1, :, :, 1:])
+
+
 def test_empty(lib):
     from ttt_amd.delta import gated_delta, gated_delta_step
     for B, L in ((2, 0), (0, 5)):

@@ -178,3 +178,12 @@ def test_in_a_graph_and_on_the_cpu(lib):
                 want = gated_linear(*a)
                 torch.cuda.synchronize()
                 assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("dt", T.DTYPES)
+@pytest.mark.parametrize("R,D,F,bias", [(4099, 400, 2100, False), (4099, 4200, 200, True)])
+def test_rounds_of_large_tiles_and_what_is_left(lib, dt, R, D, F, bias):
+    """More than a round of large tiles and less than two, of both projections' columns and of dx:
+    what is left of them is cut in four."""
+    d = inputs(R, D, F, dt, bias=bias, seed=R + D)
+    check(d, run(T.dev(d)))

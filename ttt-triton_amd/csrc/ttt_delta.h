@@ -126,12 +126,15 @@ template <typename T> __device__ __forceinline__ float token_value(const void* p
 // keep their last bits
 __device__ __forceinline__ float bounded_decay(float g) { return g < -1000.f ? -1000.f : g; }
 
-// Whether any value of a wave's tiles is not finite; of large finite ones whose sum is not too
+// Whether any value of a wave's tiles is not finite, or so large that their sum is not: no value
+// that first_not_finite finds is missed (|.|, so that none takes another's place)
 template <int TB> __device__ __forceinline__ bool any_not_finite(const f4 (&t)[TB]) {
-  f4 s = t[0];
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int b = 1; b < TB; ++b) s += t[b];
-  return __ballot(!(fabsf((s[0] + s[1]) + (s[2] + s[3])) < 3.3895e38f)) != 0;
+  for (int b = 0; b < TB; ++b)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[e] += fabsf(t[b][e]);
+  return __ballot(!((s[0] + s[1]) + (s[2] + s[3]) < 3.3895e38f)) != 0;
 }
 // The first of a column's 16 blocks' rows (tile rows 4g + e of TB tiles, a lane group each)
 // whose value is not finite, 16 TB where there is none; the same in the column's four lanes
