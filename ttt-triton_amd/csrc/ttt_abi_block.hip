@@ -27,10 +27,10 @@ struct DeltaPlan {
   size_t tok, zm, states, rows, qk, seg, trans;
 };
 // Segments that the tokens are cut into: as many as make the walk quickest.  In units of a chunk's
-// walk with outputs (3.6 to 4.6 us with 64 tokens, 2.2 to 3.8 with 32), one without takes 0.7, a
+// walk with outputs (3.6 to 5.9 us with 64 tokens, 2.2 to 3.8 with 32), one without takes 0.7, a
 // segment's join 0.3 and two more launches 2; a compute unit holds one workgroup of 64 features or
 // of states over 64 wide, else two.  (Kernels of 16,384 tokens of 12 heads of 64 x 64 in bf16: 930 us
-// with one, 190 with 20.)
+// with one, 160 with 20; 32,768 tokens of 16 x 12 heads fill the compute units with one.)
 int delta_segments(long long heads, int P, int NP, int NC) {
   const int wide = P % 64 == 0 && NP < 128 ? 64 : 32, places = wide == 64 || NP == 128 ? 256 : 512;
   const auto rounds = [&](long long columns) { return (double)((heads * columns / wide + places - 1) / places); };

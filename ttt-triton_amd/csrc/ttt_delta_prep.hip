@@ -8,6 +8,12 @@
 //                                       a wave to a column of blocks, in fp32 products
 //   M_ij = s F_ij (q_i . k_j), j <= i
 // Z and M are written in fp32 by blocks, as the walks' operands take them.
+//
+// 32,768 tokens of 12 heads of 64 x 64 in bf16: 64 us for 100 MB of q and k read and 138 MB written,
+// 3.8 TB/s; bound by memory and by the solve's plain instructions (half of the time each).  A in the
+// place of the rows makes that seven workgroups to a compute unit: 76 us with both side by side.
+// The backward takes the forward's Z and M (walk back 20 us dearer by reads of 4 bytes, 3 with
+// M's planes shared in LDS) in place of another launch of this kernel with transposed blocks (63 us).
 #include <math.h>
 
 #include "ttt_delta.h"

@@ -217,9 +217,14 @@ class BlockNormFunction(torch.autograd.Function):
         rdt = torch.float32 if rcode == _lib.DTYPE_F32 else dt
         dr, dy = None if dr is None else as_act(dr, rdt), None if dy is None else as_act(dy, dt)
         needs = ctx.needs_input_grad
+        # without the next norm r's gradient passes to the residual as it is, and to an x that is
+        # neither normed, gated nor scaled
+        same = dr if w2 is None and rcode >= 0 else None
+        if same is not None and rdt == dt and w is None and s is None and gate is None:
+            return same, None, same, None, None, None, None
         dx = x.new_empty(shape)
         dg = x.new_empty(shape) if gate is not None else None
-        dres = x.new_empty(shape, dtype=rdt) if rcode >= 0 and needs[2] else None
+        dres = x.new_empty(shape, dtype=rdt) if rcode >= 0 and needs[2] and same is None else None
         want = [t is not None and needs[i] for t, i in ((w, 1), (s, 4), (w2, 5))]
         dp, part, n = [None] * 3, None, 0
         if any(want):
@@ -233,7 +238,7 @@ class BlockNormFunction(torch.autograd.Function):
                                                 _stream(dev))
         _lib.check(st, "ttt_block_norm_bwd")
         dw, ds, dw2 = (None if t is None else _as(t, q) for t, q in zip(dp, ctx.dtypes))
-        return dx, dw, dres, dg, ds, dw2, None
+        return dx, dw, dres if same is None else same, dg, ds, dw2, None
 
 
 def block_norm(x, weight=None, residual=None, gate=None, scale=None, next_weight=None, eps: float = LAYER_NORM_EPS):
