@@ -200,3 +200,21 @@ def test_in_a_graph_and_on_the_cpu(lib):
             wr, wy = block_norm(*a)
             torch.cuda.synchronize()
             assert torch.equal(r, wr) and torch.equal(y, wy)
+
+
+@pytest.mark.parametrize("parts,res_dt", [("r", BF16), ("r", F32), ("wr", BF16)])
+def test_gradient_that_passes_as_it_is(lib, parts, res_dt):
+    """The residual's gradient, and a plain x's, may be the result's; the leaves' gradients are each
+    its own memory all the same, from one backward to the next."""
+    from ttt_amd.norm import block_norm
+    d = T.dev(inputs((37, 96), BF16, parts, res_dt, seed=21))
+    x, res = (d[k].detach().requires_grad_(True) for k in ("x", "residual"))
+    dr = d["dr"].clone()
+    for n in (1, 2):
+        block_norm(x, d["weight"], res).backward(dr)
+        assert torch.equal(dr, d["dr"]) and torch.equal(res.grad, n * dr)
+        if parts == "r":
+            assert torch.equal(x.grad, n * dr.to(BF16))
+    assert len({x.grad.data_ptr(), res.grad.data_ptr(), dr.data_ptr()}) == 3
+    x.grad.zero_()
+    assert torch.equal(res.grad, 2 * dr) and torch.equal(dr, d["dr"])
