@@ -90,12 +90,13 @@ template <Lies L, Side S, int FREE> struct Panel {
   static constexpr int ROWS = L == Lies::Contracted ? FREE : kFfnStep;
   static constexpr int BYTES = FREE * kFfnStep * 2;
   // the rows that are read at once: 0..7 of eight, or of the first operand 0..3 and 8..11 of
-  // sixteen; of free values the four of a transposing read, whose lanes have 32 or 64 bytes of each
+  // sixteen; of free values rows 0..3 and 8..11 too, whose lanes have 32 bytes of each, or every other
+  // 8 of 64: the first operand's take two turns in any order
   __device__ __forceinline__ static int place(int row, int piece) {
     if constexpr (L == Lies::Contracted)
       return piece ^ (S == Side::First ? (row & 3) | ((row >> 1) & 4) : row & 7);
     else
-      return piece ^ (S == Side::First ? (row & 3) << 2 : (row & 7) << 1);
+      return piece ^ (S == Side::First ? (row & 3) << 2 : ((row & 3) | ((row >> 1) & 4)) << 1);
   }
 };
 
