@@ -12,7 +12,7 @@
 // in place of reading the r that was stored, rounded: the bytes are the same.
 //
 // Both are bound by HBM (32,768 rows of 768 in bf16 with an fp32 residual and both norms: 60 us forward,
-// 5.0 TB/s, and 113 back, 4.0 TB/s; with a gate, by heads of 64: 29 and 62, 5.2 and 4.0).  A row is read once and held in registers over its reductions, by
+// 5.0 TB/s, and 95 back, 4.8 TB/s; with a gate, by heads of 64: 29 and 44, 5.2 and 5.7).  A row is read once and held in registers over its reductions, by
 // 8 to 64 lanes of a wave or by 4 or 8 waves, so that few lanes' places are empty; a lane has
 // 4, 8, 12 or 16 values of it.  Heads are rows side by side in a wider row.
 #pragma once

@@ -11,12 +11,12 @@ namespace ttt {
 
 namespace {
 
-// Waves to a SIMD that the registers are cut to: three where a lane has up to 12 values and no gate
-// beside a residual, or fp32 beside one (32,768 rows of 768 in bf16 with an fp32 residual: 114 us, 138 with
-// the two that fit without, the workgroups in one and a half rounds); one where 16 values, a gate and a
-// residual would spill a hundred registers
+// Waves to a SIMD that the registers are cut to: three where a lane has up to 12 values and no
+// residual (32,768 rows of 12 heads of 64 in bf16 with a gate: 44 us), else two (32,768 rows of 768 in
+// bf16 with an fp32 residual: 95 us; 115 with three, which spill 18 registers); one where 16 values, a gate
+// and a residual would spill a hundred
 template <typename T, typename TR, bool GATE, int LANES, int V, int NCH>
-constexpr int kWaves = V * NCH <= 12 && LANES < 512 && (__is_same(TR, NoResidual) || (!GATE && sizeof(T) == 2)) ? 3
+constexpr int kWaves = V * NCH <= 12 && LANES < 512 && __is_same(TR, NoResidual) ? 3
                        : V * NCH == 16 && GATE && !__is_same(TR, NoResidual) && LANES < 512                   ? 1
                                                                                                              : 2;
 
@@ -60,6 +60,24 @@ __global__ __launch_bounds__(block_threads(LANES), (kWaves<T, TR, GATE, LANES, V
       }
     }
   };
+  // The parameters are in LDS, 1 where there is none: read from memory behind the next row's loads, they
+  // would wait for those
+  constexpr int COLS = LANES * V * NCH;
+  extern __shared__ __attribute__((aligned(16))) float par[];
+  for (int c = threadIdx.x; c < COLS; c += NT) {
+    par[c] = p.w != nullptr && c < D ? p.w[c] : 1.f;
+    par[COLS + c] = p.s != nullptr && c < D ? p.s[c] : 1.f;
+    par[2 * COLS + c] = next && c < D ? p.w2[c] : 1.f;
+  }
+  __syncthreads();
+  const auto params = [&](int which, int c, float (&v)[V]) {
+#pragma unroll
+    for (int q = 0; q < V; q += 4) {
+      const f4 a = *reinterpret_cast<const f4*>(par + which * COLS + c + q);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[q + e] = a[e];
+    }
+  };
   const long long step = (long long)gridDim.x * ROWS;
   // (rows of a wave's lanes: each group ends by itself; of more waves: together)
   long long row = (long long)blockIdx.x * ROWS + threadIdx.x / LANES;
@@ -72,16 +90,16 @@ __global__ __launch_bounds__(block_threads(LANES), (kWaves<T, TR, GATE, LANES, V
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
       const int c = V * (LANES * i + l), left = D - c;
-      Raw<float, V> w, sc, w2;
-      if (left > 0) {
-        if (p.w != nullptr) w.load(p.w + c, left);
-        if (p.s != nullptr && next) sc.load(p.s + c, left);
-        if (next) w2.load(p.w2 + c, left);
+      float w[V], sc[V], w2[V];
+      params(0, c, w);
+      if (next) {
+        params(1, c, sc);
+        params(2, c, w2);
       }
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         u[i][e] = nx[i].f(e) * inv;
-        const float n = u[i][e] * (p.w != nullptr && e < left ? w.v[e] : 1.f);
+        const float n = u[i][e] * w[e];
         float of = n;  // what the residual is added to
         if (GATE) {
           const float z = nz[i].f(e), sg = sigmoid_f(z);
@@ -92,10 +110,10 @@ __global__ __launch_bounds__(block_threads(LANES), (kWaves<T, TR, GATE, LANES, V
         d[i][e] = nr[i].f(e);
         g[i][e] = 0.f;
         if (next) {
-          if (p.s != nullptr && e < left) of *= sc.v[e];
+          of *= sc[e];
           const float dy = ny[i].f(e), rj = (nres[i].f(e) + of) * jnv;
           if (e < left) {
-            const float dyw = dy * w2.v[e];
+            const float dyw = dy * w2[e];
             dw2[i][e] = __builtin_fmaf(dy, rj, dw2[i][e]);
             s2 = __builtin_fmaf(dyw, rj, s2);
             d[i][e] = __builtin_fmaf(dyw, jnv, d[i][e]);
@@ -118,15 +136,14 @@ __global__ __launch_bounds__(block_threads(LANES), (kWaves<T, TR, GATE, LANES, V
       const int c = V * (LANES * i + l), left = D - c;
       if (left > 0) {
         if (RES && p.dres != nullptr) store_row<R, V>(static_cast<R*>(p.dres) + row * D + c, left, d[i]);
-        Raw<float, V> w, sc;
-        if (p.w != nullptr) w.load(p.w + c, left);
-        if (p.s != nullptr) sc.load(p.s + c, left);
-        float dz[V];
+        float w[V], sc[V], dz[V];
+        params(0, c, w);
+        params(1, c, sc);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          const float we = p.w != nullptr && e < left ? w.v[e] : 1.f, gate = GATE ? si[i][e] : 1.f;
+          const float we = w[e], gate = GATE ? si[i][e] : 1.f;
           ds[i][e] = __builtin_fmaf(d[i][e], u[i][e] * we * gate, ds[i][e]);
-          const float dm = p.s != nullptr && e < left ? d[i][e] * sc.v[e] : d[i][e], dn = dm * gate;
+          const float dm = d[i][e] * sc[e], dn = dm * gate;
           if (GATE) dz[e] = dm * dsi[i][e];
           dw[i][e] = __builtin_fmaf(dn, u[i][e], dw[i][e]);
           g[i][e] = dn * we;
@@ -192,15 +209,22 @@ __global__ __launch_bounds__(256) void block_norm_param_grads_kernel(BlockNormPa
 
 template <typename T, typename TR> struct Bwd {
   template <int LANES, int V, int NCH> struct Of {
+    template <bool GATE> static hipError_t launch(const BlockNormParams& p, int parts, hipStream_t stream) {
+      constexpr int lds = 3 * LANES * V * NCH * 4;
+      const auto kernel = block_norm_bwd_kernel<T, TR, GATE, LANES, V, NCH>;
+      if (lds > 65536) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                                 hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        if (e != hipSuccess) return e;
+      }
+      hipLaunchKernelGGL(kernel, dim3(parts), dim3(block_threads(LANES)), lds, stream, p);
+      return hipGetLastError();
+    }
     static hipError_t run(const BlockNormParams& p, hipStream_t stream) {
       const int parts = block_norm_parts(
           p.R, p.D, p.gate != nullptr ? kWaves<T, TR, true, LANES, V, NCH> : kWaves<T, TR, false, LANES, V, NCH>);
-      if (p.gate != nullptr)
-        hipLaunchKernelGGL((block_norm_bwd_kernel<T, TR, true, LANES, V, NCH>), dim3(parts), dim3(block_threads(LANES)), 0,
-                           stream, p);
-      else
-        hipLaunchKernelGGL((block_norm_bwd_kernel<T, TR, false, LANES, V, NCH>), dim3(parts), dim3(block_threads(LANES)), 0,
-                           stream, p);
+      const hipError_t e = p.gate != nullptr ? launch<true>(p, parts, stream) : launch<false>(p, parts, stream);
+      if (e != hipSuccess) return e;
       if (p.partial != nullptr)
         hipLaunchKernelGGL(block_norm_param_grads_kernel, dim3(3 * ((p.D + 15) / 16)), dim3(256), 0, stream, p, parts);
       return hipGetLastError();
