@@ -13,8 +13,9 @@
 // LDS.  A barrier ends a chunk; another one, in its course, lets what was handed over be written
 // again.
 //
-// 32,768 tokens in 16 sequences of 12 heads of 64 x 64 in bf16: 190 us each way, 192 workgroups at
-// once with 32 chunks each, 5.9 us (12,600 clocks) a chunk and 2.8 TB/s.  A chunk's chain bounds it:
+// 32,768 tokens in 16 sequences of 12 heads of 64 x 64 in bf16: 190 us forward and 177 back (190 with
+// branches around its loads, which waits then count as none), 192 workgroups at once with 32
+// chunks each, 5.9 us (12,600 clocks) a chunk and 2.8 TB/s.  A chunk's chain bounds it:
 // 84 matrix instructions and 550 plain ones with 45 waits in a wave that has the state, 34 and 500 in
 // the wave beside it on the SIMD; together they fill half of the issue slots.
 //
@@ -117,6 +118,14 @@ template <int FLOATS, int NT> struct Copy {
     }
   }
 };
+
+// (dropped past the buffer's range)
+template <typename E> __device__ __forceinline__ void bstore_one(rsrc_t r, int voff, int soff, E v) {
+  if constexpr (sizeof(E) == 2)
+    __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(short, v), r, voff, soff, 0);
+  else
+    bstore_f32(r, voff, soff, v);
+}
 
 // what StateTiles::keep wrote
 template <int NP> __device__ __forceinline__ void take_kept(StateTiles<NP>& st, const float* __restrict__ s, int ld, int w) {
@@ -377,30 +386,24 @@ __global__ __launch_bounds__(128 * W) void delta_walk_kernel(DeltaParams p) {
       __syncthreads();
       form();
       hand();
-      if (n > 1) {
-        fetch(chunk_of(1));
-        fetch_do(chunk_of(1));
-        fetch_own(chunk_of(1));
-      }
+      // (past the last chunk it is the last one again, as forwards)
+      const auto ask = [&](int k, const auto& f) { f(chunk_of(min(k, n - 1))); };
+      ask(1, fetch);
+      ask(1, fetch_do);
+      ask(1, fetch_own);
       __syncthreads();
-      if (n > 1) put_do();
+      put_do();
       __syncthreads();
 #pragma unroll 1
       for (int k = 0; k < n; ++k) {
-        if (k + 2 < n) fetch_do(chunk_of(k + 2));
-        if (k + 1 < n) {
-          form();
-          if (k + 2 < n) fetch_own(chunk_of(k + 2));
-        }
+        ask(k + 2, fetch_do);
+        form();
+        ask(k + 2, fetch_own);
         __syncthreads();  // what was handed over has been read, and so have q and do
-        if (k + 1 < n) {
-          hand();
-          put(sh.side[(k + 1) & 1]);
-          if (k + 2 < n) {
-            fetch(chunk_of(k + 2));
-            put_do();
-          }
-        }
+        hand();
+        put(sh.side[(k + 1) & 1]);
+        ask(k + 2, fetch);
+        put_do();
         __syncthreads();
       }
     }
@@ -519,17 +522,18 @@ __global__ __launch_bounds__(128 * W) void delta_walk_kernel(DeltaParams p) {
     if constexpr (BACK) {
       __syncthreads();
       if constexpr (OUT) {
-        float* rows = p.rows + ((chain * NC + c) * Q) * PB + f0 + 16 * w + r;
-        const int left = p.L - c * Q;
-        T* to = static_cast<T*>(p.o) + first_row(c) * ldo + (long long)hp * PB + f0 + 16 * w + r;
+        const int left = min(Q, p.L - c * Q), es = (int)sizeof(T);
+        const rsrc_t rows = make_rsrc(p.rows + ((chain * NC + c) * Q) * PB + f0 + 16 * w, (unsigned)(Q * PB * 4));
+        const rsrc_t out = make_rsrc(static_cast<T*>(p.o) + first_row(c) * ldo + (long long)hp * PB + f0 + 16 * w,
+                                     (unsigned)left * (unsigned)ldo * (unsigned)es);
+        const int at_row = (4 * g * PB + r) * 4, at_o = (4 * g * (int)ldo + r) * es;
 #pragma unroll
         for (int ob = 0; ob < TB; ++ob) {
           const auto d = to_frag<T>(u[ob]).v;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int i = 16 * ob + 4 * g + e;
-            rows[i * PB] = t[ob][e];
-            if (i < left) to[i * ldo] = d[e];
+            bstore_f32(rows, at_row + (16 * ob + e) * PB * 4, 0, t[ob][e]);
+            bstore_one(out, at_o + (16 * ob + e) * (int)ldo * es, 0, d[e]);
           }
         }
       }
