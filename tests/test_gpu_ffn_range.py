@@ -1,0 +1,71 @@
+"""The gated feed-forward projections' backward in fp16 where what it forms on the way is past
+fp16's largest number and the gradients are not."""
+
+import pytest
+import torch
+
+from tests import _block as T
+from tests.test_gpu_ffn import ARGS, check, run
+
+pytestmark = pytest.mark.gpu
+
+F16 = torch.float16
+
+
+def far_inputs(R, D, F, rows, seed):
+    """Gradients of the gate's projection of a few 10^5 in `rows` of the rows (dy b f'(a), with b of about
+    2^-8 2^10 sqrt(D) and dy of 2^15 / sqrt(D)), of 2^-10 of that in the others, and dx, dWg and
+    dWu within fp16: dx by the gate's weights of 2^-10, dWg by x of 2^-8."""
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(s, generator=g)  # noqa: E731
+    of = torch.full((R, 1), 2.0 ** -10)
+    of[rows] = 1.0
+    return dict(x=(2.0 ** -8 * r(R, D)).half(), w_gate=(2.0 ** -10 * r(F, D)).half(), w_up=(2.0 ** 10 * r(F, D)).half(),
+                b_gate=None, b_up=None, dy=(2.0 ** 15 / D ** 0.5 * of * (1 + r(R, F).abs())).clamp(max=6e4).half())
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("R,D,F,rows", [
+    (2, 64, 16, [0]), (33, 40, 17, [32]), (65, 24, 33, [0, 64]), (130, 64, 72, [63, 64, 129]), (300, 57, 100, slice(0, 64)),
+    (700, 96, 40, [699]), (4099, 400, 2100, [0, 1000, 4098]), (4099, 4200, 200, [17, 2048]), (6200, 40, 1030, slice(3000, 3030))])
+def test_formed_gradients_past_the_largest_number(lib, act, R, D, F, rows):
+    """Small, large and mixed tiles, some waves' rows past it and others not, shares of the sums."""
+    d = far_inputs(R, D, F, rows, seed=R + F)
+    a, b = (d["x"].double() @ d[k].double().T for k in ("w_gate", "w_up"))
+    assert float((d["dy"].double() * b * 0.5).abs().max()) > 1e5  # (f'(a) is 1/2 in both within a thousandth)
+    check(d, run(T.dev(d), act), act)
+
+
+def test_far_gradients_and_no_weight(lib):
+    """As large as they can be, they come to nothing where the gate's weights are 0."""
+    d = dict(x=torch.full((100, 64), 6e4), w_gate=torch.zeros(40, 64), w_up=torch.full((40, 64), 6e4), dy=torch.full((100, 40), 6e4))
+    got = run({**T.dev({k: t.half() for k, t in d.items()}), "b_gate": None, "b_up": None})
+    assert (got["dx"] == 0).all() and (got["y"] == 0).all() and (got["dw_up"] == 0).all() and torch.isinf(got["dw_gate"]).all()
+
+
+@pytest.mark.parametrize("R,D,F", [(130, 64, 72), (4099, 400, 2100)])
+def test_no_trace_of_an_earlier_call(lib, R, D, F):
+    """Calls without such values, before and after one with them and in a graph that sees both: the same bits."""
+    far = T.dev(far_inputs(R, D, F, [5, R - 1], 1))
+    near = {**far, "dy": far["dy"] * 2.0 ** -12}
+    want, large = run(near), run(far)
+    for d, ref in ((near, want), (far, large), (near, want)):
+        for k, t in run(d).items():
+            assert torch.equal(t, ref[k]), k
+    from ttt_amd.ffn import gated_linear
+    leaves = [far[k].clone().requires_grad_(True) for k in ARGS if far[k] is not None]
+    dy = near["dy"].clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.autograd.grad(gated_linear(*leaves), leaves, dy)
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        grads = torch.autograd.grad(gated_linear(*leaves), leaves, dy)
+    for d, ref in ((near, want), (far, large), (near, want), (far, large)):
+        dy.copy_(d["dy"])
+        g.replay()
+        torch.cuda.synchronize()
+        for k, t in zip(("dx", "dw_gate", "dw_up"), grads):
+            assert torch.equal(t, ref[k]), k

@@ -103,7 +103,8 @@ int check_ffn(int R, int D, int F, int act, int dtype) {
 }
 struct FfnPlan {
   bool in_place;
-  size_t x, w, grad, part, bias;
+  size_t x, w, grad, part, bias, far;
+  size_t backward() const { return x + 2 * w + grad + part + bias + far; }
 };
 FfnPlan ffn_plan(int R, int D, int F, int dtype) {
   FfnPlan s;
@@ -111,11 +112,12 @@ FfnPlan ffn_plan(int R, int D, int F, int dtype) {
   s.in_place = planes == 1 && D % 8 == 0;
   s.x = s.in_place ? 0 : up256(planes * R * Dp * 2);
   s.w = s.in_place ? 0 : up256(planes * F * Dp * 2);
-  s.grad = up256(planes * R * 2 * Fp * 2);
+  s.grad = up256((size_t)ttt::ffn_grad_planes(dtype) * R * 2 * Fp * 2);
   const int of_dx = ttt::ffn_cut_dx(R, D, F, dtype).splits, of_dw = ttt::ffn_cut_dw(R, D, F, dtype).splits;
   const size_t dx = of_dx > 1 ? (size_t)of_dx * R * Dp * 4 : 0, dw = of_dw > 1 ? (size_t)of_dw * 2 * Fp * Dp * 4 : 0;
   s.part = up256(std::max(dx, dw));  // (one after the other)
   s.bias = up256((size_t)ttt::ffn_bias_parts(R, D, F, dtype) * 2 * Fp * 4);
+  s.far = dtype == TTT_DTYPE_F16 ? 256 + up256((size_t)ttt::ffn_far_blocks(R, F)) : 0;
   return s;
 }
 // x, wg and wu as the products read them: in place, or as planes in the workspace
@@ -160,7 +162,7 @@ size_t ttt_ffn_workspace_bytes(int R, int D, int F, int dtype) {
 size_t ttt_ffn_bwd_workspace_bytes(int R, int D, int F, int dtype) {
   if (check_ffn(R, D, F, TTT_ACT_SILU, dtype) != TTT_OK) return 0;
   const FfnPlan s = ffn_plan(R, D, F, dtype);
-  return s.x + 2 * s.w + s.grad + s.part + s.bias;
+  return s.backward();
 }
 
 int ttt_ffn_fwd(const void* x, long long ldx, const void* wg, const void* wu, const void* bg, const void* bu, int R,
@@ -223,7 +225,7 @@ int ttt_ffn_bwd(const void* x, long long ldx, const void* wg, const void* wu, co
   OPTIONAL(dbg, n);
   OPTIONAL(dbu, n);
   if ((dwg == nullptr) != (dwu == nullptr)) return TTT_ERR_ARG;
-  if (workspace == nullptr || workspace_bytes < s.x + 2 * s.w + s.grad + s.part + s.bias) return TTT_ERR_WORKSPACE;
+  if (workspace == nullptr || workspace_bytes < s.backward()) return TTT_ERR_WORKSPACE;
   if (!aligned(workspace, 16)) return TTT_ERR_ALIGN;
   ttt::FfnParams p{};
   p.bg = bg;
@@ -252,6 +254,11 @@ int ttt_ffn_bwd(const void* x, long long ldx, const void* wg, const void* wu, co
   if (s.part > 0) p.part = reinterpret_cast<float*>(ws);
   ws += s.part;
   if (dbg != nullptr || dbu != nullptr) p.bias_part = reinterpret_cast<float*>(ws);
+  ws += s.bias;
+  if (s.far > 0) {
+    p.far = reinterpret_cast<int*>(ws);
+    p.over = reinterpret_cast<unsigned char*>(ws + 256);
+  }
   e = ttt::launch_ffn_grad(p, dtype, on);
   if (e == hipSuccess && dx != nullptr) e = ttt::launch_ffn_dx(p, dtype, on);
   if (e == hipSuccess && dwg != nullptr) e = ttt::launch_ffn_dw(p, dtype, on);

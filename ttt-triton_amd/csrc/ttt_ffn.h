@@ -24,6 +24,10 @@ struct FfnParams {
   void *dbg, *dbu;            // [F], or null
   float* part;                // [splits][R or 2 Fp][Dp] of dx, or dwg and dwu, where their steps are split
   float* bias_part;           // [bias_parts][2 Fp], or null
+  // fp16: whether a value of da or db is past its largest number, in blocks of 16 rows by 32 columns of both
+  // and anywhere; `grad` has a second plane for those, read where there are any
+  unsigned char* over;
+  int* far;
   long long lddy;
   int R, D, F, Dp, Fp;        // widths as the user's and padded to 8
   int planes, act;
@@ -33,7 +37,7 @@ struct FfnParams {
 // few rows: the operands as the user's, rows of x ldx elements apart
 hipError_t launch_ffn_few(const FfnParams& p, int dtype, hipStream_t stream);
 hipError_t launch_ffn_fwd(const FfnParams& p, int dtype, hipStream_t stream);
-hipError_t launch_ffn_grad(const FfnParams& p, int dtype, hipStream_t stream);  // writes `grad`, dbg, dbu
+hipError_t launch_ffn_grad(const FfnParams& p, int dtype, hipStream_t stream);  // writes `grad`, `over`, `far`, dbg, dbu
 hipError_t launch_ffn_dx(const FfnParams& p, int dtype, hipStream_t stream);
 hipError_t launch_ffn_dw(const FfnParams& p, int dtype, hipStream_t stream);
 // rows of `width` values `ld` elements apart -> planes of rows padded with zeros to a multiple of 8
@@ -41,6 +45,10 @@ hipError_t launch_ffn_planes(const void* from, long long ld, int rows, int width
 
 constexpr int ffn_pad(int n) { return (n + 7) / 8 * 8; }
 constexpr int ffn_planes(int dtype) { return dtype == TTT_DTYPE_F32 ? 3 : 1; }
+constexpr int ffn_grad_planes(int dtype) { return dtype == TTT_DTYPE_F16 ? 2 : ffn_planes(dtype); }
+constexpr int kFfnFarRows = 16, kFfnFarCols = 32;  // of a block of `over`: what a wave stores at once
+constexpr int ffn_far_cols(int F) { return (F + kFfnFarCols - 1) / kFfnFarCols; }
+constexpr long long ffn_far_blocks(long long R, int F) { return (R + kFfnFarRows - 1) / kFfnFarRows * ffn_far_cols(F); }
 
 // How a product is cut up: tiles of 256 x 256, a workgroup to a compute unit, or of 128 x 128,
 // two; and the steps of 64 contracted values of a tile into shares, whose sums are joined by

@@ -19,7 +19,10 @@
 // the rate of bf16 (the fp32 matrix instructions have a sixteenth).  da and db of 16-bit calls
 // are rounded to the activations' type where dx and dW read them, as a layer that formed them
 // one after the other would hand them on: their rounding adds to that at the store, each
-// half a step (1.4 times the store's alone); two planes would double the two products.
+// half a step (1.4 times the store's alone); two planes would double the two products.  In fp16 they
+// may be past its largest number where dx and dW are not: such values go, 2^-30 times themselves, to
+// a second plane, whose products are formed (first, and then brought to scale) only if there is one.
+// Blocks with one are marked; one more launch puts zeros in the plane's other blocks, or finds no mark.
 //
 // 32,768 rows, 768 by 2,048, bf16: y 235 us (877 TFLOP/s), da and db 269, dx 262 in one round of large
 // tiles and one of small, dW 247 and a join of 12 (294 and 257 before that and before the reads' order).
@@ -179,6 +182,21 @@ template <typename T> __device__ __forceinline__ void store_grad(const FfnMatrix
     store_row<T, 8>(reinterpret_cast<T*>(to), 8, v);
   }
 }
+// fp16: where some are past its largest number, those that are finite go, scaled, to the second plane.
+// (Beyond that one's range any product but with 0 is past the results' too.)
+constexpr float kMostF16 = 65520.f;   // rounds to infinity
+constexpr float kFar = 1073741824.f;  // 2^30: 2^16 is 2^-14 of it, a normal number, and 2^46 its largest
+__device__ __forceinline__ void store_far(const FfnMatrix& m, long long row, int col, const float (&v)[8]) {
+  float near[8], far[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const bool past = fabsf(v[e]) >= kMostF16 && fabsf(v[e]) < __builtin_inff();
+    near[e] = past ? 0.f : v[e];
+    far[e] = past ? fminf(fmaxf(v[e] * (1.f / kFar), -65504.f), 65504.f) : 0.f;
+  }
+  store_grad<_Float16>(m, row, col, near);
+  store_grad<_Float16>({static_cast<const char*>(m.p) + m.plane, m.ld, 0}, row, col, far);
+}
 
 // Tiles of WN TN 16 columns (the first operand's free values, four to a lane's registers) by
 // WM TM 16 rows (the second's, a lane each)
@@ -209,15 +227,17 @@ __global__ __launch_bounds__(64 * WN * WM) void ffn_kernel(FfnParams p) {
   const int n0 = (int)(id / high) * HN + (int)(quarter >> 1) * (UP ? HALF : BN);
   if (m0 >= M || n0 >= N) return;
 
-  const int ksteps = (K + kFfnStep - 1) / kFfnStep, pairs = p.planes == 3 ? 6 : 1, segs = JOB == Job::Dx ? 2 : 1;
+  constexpr bool WIDE = __is_same(T, _Float16) && !UP;  // where `grad` may have a second plane
+  const int ksteps = (K + kFfnStep - 1) / kFfnStep, segs = JOB == Job::Dx ? 2 : 1;
+  const int pairs = p.planes == 3 ? 6 : WIDE && *p.far != 0 ? 2 : 1;
   const int all = ksteps * pairs * segs, per = UP ? all : (all + p.splits - 1) / p.splits;
   const int first = split * per, steps = min(all, first + per) - first;
 
   // the step that is sent next: its contracted values, of which weights, and the planes
   int sk = first % ksteps, ss = first / ksteps % segs, sp = first / (ksteps * segs);
   const auto next = [&](int buf) {
-    // planes a of the first operand and b of the second: (2,0) (1,1) (0,2) (1,0) (0,1) (0,0)
-    const int pa = pairs == 1 ? 0 : (0x001012 >> (4 * sp)) & 15, pb = pairs == 1 ? 0 : (0x010210 >> (4 * sp)) & 15;
+    // planes a of the first operand and b of the second: (2,0) (1,1) (0,2) (1,0) (0,1) (0,0), or (0,1) (0,0)
+    const int pa = pairs < 6 ? 0 : (0x001012 >> (4 * sp)) & 15, pb = pairs < 6 ? pairs - 1 - sp : (0x010210 >> (4 * sp)) & 15;
     const int k = sk * kFfnStep, left = K - k;
     unsigned char* to = smem + buf * STEP;
     if constexpr (UP) {
@@ -257,26 +277,41 @@ __global__ __launch_bounds__(64 * WN * WM) void ffn_kernel(FfnParams p) {
   // a wave's tiles of columns: of both halves where a tile has both projections
   const auto tile_n = [&](int i) { return UP ? (i < TN / 2 ? wn * (TN / 2) + i : HALF / 16 + wn * (TN / 2) + i - TN / 2) : wn * TN + i; };
   if (steps > 0) next(0);
+  const auto go = [&](int from, int to) {
 #pragma unroll 1
-  for (int s = 0; s < steps; ++s) {
-    // the step is here, in all waves, and the one before it has been read
-    __builtin_amdgcn_s_waitcnt(0x0F70);  // (vmcnt(0))
-    __syncthreads();
-    if (s + 1 < steps) next((s + 1) & 1);
-    const unsigned char* at = smem + (s & 1) * STEP;
+    for (int s = from; s < to; ++s) {
+      // the step is here, in all waves, and the one before it has been read
+      __builtin_amdgcn_s_waitcnt(0x0F70);  // (vmcnt(0))
+      __syncthreads();
+      if (s + 1 < steps) next((s + 1) & 1);
+      const unsigned char* at = smem + (s & 1) * STEP;
 #pragma unroll
-    for (int k = 0; k < kFfnStep / 32; ++k) {
-      bf8 pn[TN], pm[TM];
+      for (int k = 0; k < kFfnStep / 32; ++k) {
+        bf8 pn[TN], pm[TM];
 #pragma unroll
-      for (int i = 0; i < TN; ++i) pn[i] = take<LN, Side::First, BN>(at, tile_n(i), k);
+        for (int i = 0; i < TN; ++i) pn[i] = take<LN, Side::First, BN>(at, tile_n(i), k);
 #pragma unroll
-      for (int j = 0; j < TM; ++j) pm[j] = take<LM, Side::Second, BM>(at + Panel<LN, Side::First, BN>::BYTES, wm * TM + j, k);
+        for (int j = 0; j < TM; ++j) pm[j] = take<LM, Side::Second, BM>(at + Panel<LN, Side::First, BN>::BYTES, wm * TM + j, k);
 #pragma unroll
-      for (int j = 0; j < TM; ++j)
+        for (int j = 0; j < TM; ++j)
 #pragma unroll
-        for (int i = 0; i < TN; ++i) acc[i][j] = product<E>(pn[i], pm[j], acc[i][j]);
+          for (int i = 0; i < TN; ++i) acc[i][j] = product<E>(pn[i], pm[j], acc[i][j]);
+      }
+      reads_ahead<TN, TM, LN, LM>();
     }
-    reads_ahead<TN, TM, LN, LM>();
+  };
+  if constexpr (WIDE) {
+    const int wide = pairs == 2 ? max(0, min(steps, ksteps * segs - first)) : 0;  // steps of the second plane
+    if (wide > 0) {
+      go(0, wide);
+#pragma unroll
+      for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int j = 0; j < TM; ++j) acc[i][j] *= kFar;
+    }
+    go(wide, steps);
+  } else {
+    go(0, steps);
   }
 
   // A pair of tiles' columns are eight neighbours in a lane: 8g + 4i + e of 32
@@ -326,9 +361,27 @@ __global__ __launch_bounds__(64 * WN * WM) void ffn_kernel(FfnParams p) {
         }
         if constexpr (JOB == Job::Fwd) {
           if (m < M && left > 0) store_row<T, 8>(static_cast<T*>(p.y) + (long long)m * p.F + f, left, u);
-        } else if (m < M && f < p.Fp) {
-          store_grad<T>(p.grad, m, f, u);
-          store_grad<T>(p.grad, m, p.Fp + f, v);
+        } else {
+          bool any = false;
+          if constexpr (__is_same(T, _Float16)) {
+            float most = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) most = fmaxf(most, fmaxf(fabsf(u[e]), fabsf(v[e])));
+            any = __ballot(most >= kMostF16) != 0;
+          }
+          if (m < M && f < p.Fp) {
+            if (any) {
+              store_far(p.grad, m, f, u);
+              store_far(p.grad, m, p.Fp + f, v);
+            } else {
+              store_grad<T>(p.grad, m, f, u);
+              store_grad<T>(p.grad, m, p.Fp + f, v);
+            }
+          }
+          if constexpr (__is_same(T, _Float16)) {
+            const int rows = m0 + 16 * (wm * TM + j), cols = n0 + 16 * (wn * (TN / 2) + i);  // the block's first
+            if (l == 0 && rows < M && cols < N) p.over[(long long)(rows / kFfnFarRows) * ffn_far_cols(p.F) + cols / kFfnFarCols] = any;
+          }
         }
       }
       if (JOB == Job::Grad && p.bias_part != nullptr) {
@@ -381,6 +434,33 @@ template <typename T, Job JOB> __global__ __launch_bounds__(256) void ffn_join_k
   for (int k = 1; k < p.splits; ++k) v += *reinterpret_cast<const f4*>(s + 4 * k * quads);
   T* to = static_cast<T*>(JOB == Job::Dx ? p.dx : m < p.Fp ? p.dwg : p.dwu);
   store_up_to4(to + (long long)f * p.D + n, p.D - n, v);
+}
+// fp16: whether any block has a mark, and if so zeros to the second plane's blocks without one.  (32,768
+// rows by 2,048: 5 us without a mark.)
+__global__ __launch_bounds__(256) void ffn_far_kernel(FfnParams p, long long blocks) {
+  unsigned any = 0;
+  const long long whole = blocks / 16;
+#pragma unroll 8
+  for (long long i = threadIdx.x; i < whole; i += 256) {
+    const u4v v = reinterpret_cast<const u4v*>(p.over)[i];
+    any |= v[0] | v[1] | v[2] | v[3];
+  }
+  if (16 * whole + threadIdx.x < blocks) any |= p.over[16 * whole + threadIdx.x];
+  const bool far = __syncthreads_or(any != 0) != 0;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *p.far = far;
+  if (!far) return;
+  const int cols = ffn_far_cols(p.F);
+  constexpr int PIECES = kFfnFarCols / 8, EACH = kFfnFarRows * PIECES;  // of 16 bytes, to a row and block
+  for (long long k = (long long)blockIdx.x * (256 / EACH) + threadIdx.x / EACH; k < blocks; k += (long long)gridDim.x * (256 / EACH)) {
+    if (p.over[k] != 0) continue;
+    const int at = threadIdx.x % EACH;
+    const long long rb = k / cols, row = kFfnFarRows * rb + at / PIECES;
+    const int c = kFfnFarCols * (int)(k - rb * cols) + 8 * (at % PIECES);
+    if (row >= p.R || c >= p.Fp) continue;
+    char* to = static_cast<char*>(const_cast<void*>(p.grad.p)) + p.grad.plane + row * p.grad.ld;
+    *reinterpret_cast<u4v*>(to + c * 2) = u4v{0, 0, 0, 0};
+    *reinterpret_cast<u4v*>(to + (p.Fp + c) * 2) = u4v{0, 0, 0, 0};
+  }
 }
 template <typename T> __global__ __launch_bounds__(256) void ffn_bias_kernel(FfnParams p) {
   const int n = 2 * p.Fp, c = blockIdx.x * 16 + (threadIdx.x & 15);
@@ -539,7 +619,12 @@ hipError_t launch_ffn_few(const FfnParams& p, int dtype, hipStream_t s) {
 }
 hipError_t launch_ffn_fwd(const FfnParams& p, int dtype, hipStream_t s) { return type_t<Job::Fwd>(p, ffn_cut_up(p.R, p.D, p.F, dtype, false), dtype, s); }
 hipError_t launch_ffn_grad(const FfnParams& p, int dtype, hipStream_t s) {
-  const hipError_t e = type_t<Job::Grad>(p, ffn_cut_up(p.R, p.D, p.F, dtype, p.bias_part != nullptr), dtype, s);
+  hipError_t e = type_t<Job::Grad>(p, ffn_cut_up(p.R, p.D, p.F, dtype, p.bias_part != nullptr), dtype, s);
+  if (e == hipSuccess && dtype == TTT_DTYPE_F16) {
+    const long long blocks = ffn_far_blocks(p.R, p.F);
+    hipLaunchKernelGGL(ffn_far_kernel, dim3((unsigned)std::min(blocks, 256LL)), dim3(256), 0, s, p, blocks);
+    e = hipGetLastError();
+  }
   if (e != hipSuccess || p.bias_part == nullptr) return e;
   return dtype == TTT_DTYPE_BF16 ? bias_t<__bf16>(p, s) : dtype == TTT_DTYPE_F16 ? bias_t<_Float16>(p, s) : bias_t<float>(p, s);
 }
