@@ -69,3 +69,22 @@ def test_no_trace_of_an_earlier_call(lib, R, D, F):
         torch.cuda.synchronize()
         for k, t in zip(("dx", "dw_gate", "dw_up"), grads):
             assert torch.equal(t, ref[k]), k
+
+
+@pytest.mark.parametrize("R,D,F,bias", [(65, 24, 1100, False), (700, 96, 40, False), (2043, 501, 333, True)])
+def test_rows_beside_such_values_keep_their_bits(lib, R, D, F, bias):
+    """Whatever the shares that the sums are cut into: dx of the other rows, and the weights' gradients of
+    the other columns."""
+    from tests.test_gpu_ffn import inputs
+    d = T.dev(inputs(R, D, F, F16, bias=bias, seed=R))
+    ref = run(d)
+    e = {**d, "dy": d["dy"].clone(), "w_up": d["w_up"].clone()}
+    e["dy"][R // 2, 5] = 6e4
+    e["w_up"][5] *= 60
+    got = run(e)
+    rows, cols = ([i for i in range(n) if i != k] for n, k in ((R, R // 2), (F, 5)))
+    q = run({**d, "w_up": e["w_up"]})  # (column 5's weights reach every row)
+    assert torch.equal(got["dx"][rows], q["dx"][rows])
+    for k in ("dw_gate", "dw_up"):
+        assert torch.equal(got[k][cols], ref[k][cols]), k
+    assert float((e["dy"][R // 2, 5].double() * (e["x"][R // 2].double() @ e["w_up"][5].double())).abs()) > 2e5

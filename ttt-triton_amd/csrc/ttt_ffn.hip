@@ -227,17 +227,21 @@ __global__ __launch_bounds__(64 * WN * WM) void ffn_kernel(FfnParams p) {
   const int n0 = (int)(id / high) * HN + (int)(quarter >> 1) * (UP ? HALF : BN);
   if (m0 >= M || n0 >= N) return;
 
-  constexpr bool WIDE = __is_same(T, _Float16) && !UP;  // where `grad` may have a second plane
-  const int ksteps = (K + kFfnStep - 1) / kFfnStep, segs = JOB == Job::Dx ? 2 : 1;
-  const int pairs = p.planes == 3 ? 6 : WIDE && *p.far != 0 ? 2 : 1;
+  const int ksteps = (K + kFfnStep - 1) / kFfnStep, pairs = p.planes == 3 ? 6 : 1, segs = JOB == Job::Dx ? 2 : 1;
   const int all = ksteps * pairs * segs, per = UP ? all : (all + p.splits - 1) / p.splits;
-  const int first = split * per, steps = min(all, first + per) - first;
+  const int first = split * per, own = min(all, first + per) - first;
+  // (the second plane's steps are those of the first again, before them: a share has the same values)
+  constexpr bool WIDE = __is_same(T, _Float16) && !UP;
+  const bool far = WIDE && *p.far != 0;
+  const int steps = far ? 2 * own : own;
 
   // the step that is sent next: its contracted values, of which weights, and the planes
-  int sk = first % ksteps, ss = first / ksteps % segs, sp = first / (ksteps * segs);
+  int sk = first % ksteps, ss = first / ksteps % segs, sp = first / (ksteps * segs), sent = 0;
+  long long beside = far ? p.grad.plane : 0;  // to the plane of `grad`
   const auto next = [&](int buf) {
-    // planes a of the first operand and b of the second: (2,0) (1,1) (0,2) (1,0) (0,1) (0,0), or (0,1) (0,0)
-    const int pa = pairs < 6 ? 0 : (0x001012 >> (4 * sp)) & 15, pb = pairs < 6 ? pairs - 1 - sp : (0x010210 >> (4 * sp)) & 15;
+    // planes a of the first operand and b of the second: (2,0) (1,1) (0,2) (1,0) (0,1) (0,0)
+    const int pa = pairs == 1 ? 0 : (0x001012 >> (4 * sp)) & 15;
+    const int pb = pairs == 1 ? 0 : (0x010210 >> (4 * sp)) & 15;
     const int k = sk * kFfnStep, left = K - k;
     unsigned char* to = smem + buf * STEP;
     if constexpr (UP) {
@@ -251,13 +255,13 @@ __global__ __launch_bounds__(64 * WN * WM) void ffn_kernel(FfnParams p) {
       const FfnMatrix& wt = ss == 0 ? p.wg : p.wu;
       send<LN, Side::First, BN, NW>(static_cast<const char*>(wt.p) + pa * wt.plane + (long long)k * wt.ld + n0 * 2, wt.ld, p.F - k,
                        (p.Dp - n0) / 8, to, w);
-      send<LM, Side::Second, BM, NW>(static_cast<const char*>(p.grad.p) + pb * p.grad.plane + (long long)m0 * p.grad.ld +
+      send<LM, Side::Second, BM, NW>(static_cast<const char*>(p.grad.p) + (WIDE ? beside : pb * p.grad.plane) + (long long)m0 * p.grad.ld +
                            ((long long)ss * p.Fp + k) * 2,
                        p.grad.ld, M - m0, left / 8, to + Panel<LN, Side::First, BN>::BYTES, w);
     } else {
       send<LN, Side::First, BN, NW>(static_cast<const char*>(p.x.p) + pa * p.x.plane + (long long)k * p.x.ld + n0 * 2, p.x.ld, left,
                        (p.Dp - n0) / 8, to, w);
-      send<LM, Side::Second, BM, NW>(static_cast<const char*>(p.grad.p) + pb * p.grad.plane + (long long)k * p.grad.ld + m0 * 2, p.grad.ld,
+      send<LM, Side::Second, BM, NW>(static_cast<const char*>(p.grad.p) + (WIDE ? beside : pb * p.grad.plane) + (long long)k * p.grad.ld + m0 * 2, p.grad.ld,
                        left, (M - m0) / 8, to + Panel<LN, Side::First, BN>::BYTES, w);
     }
     if (++sk == ksteps) {
@@ -266,6 +270,12 @@ __global__ __launch_bounds__(64 * WN * WM) void ffn_kernel(FfnParams p) {
         ss = 0;
         ++sp;
       }
+    }
+    if constexpr (WIDE) {  // (no branch: a step's reads and products stay in one block)
+      const bool again = ++sent == own;
+      sk = again ? first % ksteps : sk;
+      ss = again ? first / ksteps : ss;
+      beside = again ? 0 : beside;
     }
   };
 
@@ -301,15 +311,14 @@ __global__ __launch_bounds__(64 * WN * WM) void ffn_kernel(FfnParams p) {
     }
   };
   if constexpr (WIDE) {
-    const int wide = pairs == 2 ? max(0, min(steps, ksteps * segs - first)) : 0;  // steps of the second plane
-    if (wide > 0) {
-      go(0, wide);
+    if (far) {
+      go(0, own);
 #pragma unroll
       for (int i = 0; i < TN; ++i)
 #pragma unroll
         for (int j = 0; j < TM; ++j) acc[i][j] *= kFar;
     }
-    go(wide, steps);
+    go(steps - own, steps);
   } else {
     go(0, steps);
   }

@@ -4,7 +4,8 @@ both products, the activation and the gating in one kernel, with its backward.
 fp32, bf16 or fp16, weights and biases in x's type.  Sums are fp32.  The backward forms
 both projections again in place of keeping them; in 16 bits it rounds their gradients to
 that type where the gradients of x and of the weights read them (those of the biases are
-their sums before)."""
+their sums before).  In fp16 those past its largest number are kept apart, scaled, with as
+many bits: a gradient is infinite only where it is itself past it."""
 
 from __future__ import annotations
 
