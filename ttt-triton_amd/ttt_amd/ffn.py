@@ -5,7 +5,11 @@ fp32, bf16 or fp16, weights and biases in x's type.  Sums are fp32.  The backwar
 both projections again in place of keeping them; in 16 bits it rounds their gradients to
 that type where the gradients of x and of the weights read them (those of the biases are
 their sums before).  In fp16 those past its largest number are kept apart, scaled, with as
-many bits: a gradient is infinite only where it is itself past it."""
+many bits: a gradient is infinite only where it is itself past it.
+
+A value that is not finite reaches what is formed of it and no other row of x or of the weights.
+In fp32, whose values are multiplied in bf16 planes, one above 3.39e38 counts as infinite, and
+what an infinite one reaches is NaN."""
 
 from __future__ import annotations
 
