@@ -1,0 +1,33 @@
+"""The sizes that the gated delta rule takes, by the threads of its launches (no GPU: the C entry points
+return their status, and the size functions 0, before any launch)."""
+
+import pytest
+
+from tests.test_block_refusals import BF16, DELTA, DELTA_BWD, E_NULL, E_SHAPE, F32, _call
+
+CHUNK = {BF16: 64, F32: 32}
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from ttt_amd import _lib
+    return _lib.load()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("B,H", [(1, 16), (8, 2), (3, 5)])
+def test_chunks(lib, dtype, B, H):
+    """Fewer than 2^32 threads in a launch: 256 to a chunk and head forwards, 512 in the backward and in a
+    forward that it follows."""
+    fwd, train = (((1 << 32) - 1) // n // (B * H) * CHUNK[dtype] for n in (256, 512))
+    kw = dict(B=B, H=H, G=H, P=32, N=16, dtype=dtype, ldq=16 * H, ldk=16 * H, ldv=32 * H, ldg=H, ldb=H, bd=F32)
+    for L, alone, trains in ((train, True, True), (train + 1, True, False), (fwd, True, False), (fwd + 1, False, False)):
+        dims = (B, L, H, 32, 16, dtype)
+        assert (lib.ttt_delta_workspace_bytes(*dims) > 0) == alone, L
+        assert (lib.ttt_delta_saved_bytes(*dims) > 0) == trains, L
+        assert (lib.ttt_delta_bwd_workspace_bytes(B, L, H, 32, H, 16, dtype) > 0) == trains, L
+        # (a call that is taken goes on to its missing tensor)
+        assert _call(lib.ttt_delta_fwd, DELTA, **kw, L=L, saved=None, v=None) == (E_NULL if alone else E_SHAPE), L
+        assert _call(lib.ttt_delta_fwd, DELTA, **kw, L=L, v=None) == (E_NULL if trains else E_SHAPE), L
+        bwd = {k: v for k, v in kw.items() if k != "ldv"}
+        assert _call(lib.ttt_delta_bwd, DELTA_BWD, **bwd, L=L, lddo=32 * H, dq=None) == (E_NULL if trains else E_SHAPE), L

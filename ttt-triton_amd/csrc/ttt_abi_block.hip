@@ -64,16 +64,17 @@ DeltaPlan delta_plan(int B, int L, int H, int P, int G, int N, int dtype) {
   s.trans = s.S > 1 ? (size_t)B * H * s.S * NP * NP * 4 : 0;
   return s;
 }
-bool delta_grid_ok(const DeltaPlan& s, int B, int H, int P) {
-  // (prep: 256 threads a chunk and head; walk: eight for a column, a feature or one of the identity's, and segment;
-  // join: up to 32 a feature; gradients: 512 a chunk and head)
+// (forwards, prep: 256 threads a chunk and head; walk: eight for a column, a feature or one of the identity's, and
+// segment; join: up to 32 a feature; where a backward follows its gradients: 512 a chunk and head)
+bool delta_grid_ok(const DeltaPlan& s, int B, int H, int P, bool train) {
   const long long heads = (long long)B * H;
-  return heads * (P + 128) <= kMaxThreads / 8 / s.S && heads * P <= kMaxThreads / 32 && heads <= kMaxThreads / 512 / s.NC;
+  return heads * (P + 128) <= kMaxThreads / 8 / s.S && heads * P <= kMaxThreads / 32 &&
+         heads <= kMaxThreads / (train ? 512 : 256) / s.NC;
 }
-bool delta_plan_ok(int B, int L, int H, int P, int G, int N, int dtype, DeltaPlan& s) {
+bool delta_plan_ok(int B, int L, int H, int P, int G, int N, int dtype, bool train, DeltaPlan& s) {
   if (check_delta(B, L, H, P, G, N, dtype, dtype, dtype) != TTT_OK) return false;
   s = delta_plan(B, L, H, P, G, N, dtype);
-  return delta_grid_ok(s, B, H, P);
+  return delta_grid_ok(s, B, H, P, train);
 }
 
 // ---- norms around a block
@@ -368,15 +369,15 @@ int ttt_block_norm_bwd(const void* x, long long ldx, const void* gate, long long
 
 size_t ttt_delta_saved_bytes(int B, int L, int H, int P, int N, int dtype) {
   DeltaPlan s;
-  return delta_plan_ok(B, L, H, P, 1, N, dtype, s) ? s.states + s.rows : 0;
+  return delta_plan_ok(B, L, H, P, 1, N, dtype, true, s) ? s.states + s.rows : 0;
 }
 size_t ttt_delta_workspace_bytes(int B, int L, int H, int P, int N, int dtype) {
   DeltaPlan s;
-  return delta_plan_ok(B, L, H, P, 1, N, dtype, s) ? s.tok + 2 * s.zm + s.seg + s.trans : 0;
+  return delta_plan_ok(B, L, H, P, 1, N, dtype, false, s) ? s.tok + 2 * s.zm + s.seg + s.trans : 0;
 }
 size_t ttt_delta_bwd_workspace_bytes(int B, int L, int H, int P, int G, int N, int dtype) {
   DeltaPlan s;
-  return delta_plan_ok(B, L, H, P, G, N, dtype, s) ? s.states + s.rows + 2 * s.qk + s.seg : 0;
+  return delta_plan_ok(B, L, H, P, G, N, dtype, true, s) ? s.states + s.rows + 2 * s.qk + s.seg : 0;
 }
 
 int ttt_delta_fwd(const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv,
@@ -387,7 +388,7 @@ int ttt_delta_fwd(const void* q, long long ldq, const void* k, long long ldk, co
   int st = check_delta(B, L, H, P, G, N, dtype, g_dtype, beta_dtype);
   if (st != TTT_OK) return st;
   const DeltaPlan s = delta_plan(B, L, H, P, G, N, dtype);
-  if (!delta_grid_ok(s, B, H, P)) return TTT_ERR_SHAPE;
+  if (!delta_grid_ok(s, B, H, P, saved != nullptr)) return TTT_ERR_SHAPE;
   if (ldg < H || ldbeta < H) return TTT_ERR_SHAPE;
   if ((st = check_row(ldq, (long long)G * N, L, dtype)) != TTT_OK) return st;
   if ((st = check_row(ldk, (long long)G * N, L, dtype)) != TTT_OK) return st;
@@ -455,7 +456,7 @@ int ttt_delta_bwd(const void* q, long long ldq, const void* k, long long ldk, co
   int st = check_delta(B, L, H, P, G, N, dtype, g_dtype, beta_dtype);
   if (st != TTT_OK) return st;
   const DeltaPlan s = delta_plan(B, L, H, P, G, N, dtype);
-  if (!delta_grid_ok(s, B, H, P)) return TTT_ERR_SHAPE;
+  if (!delta_grid_ok(s, B, H, P, true)) return TTT_ERR_SHAPE;
   if (ldg < H || ldbeta < H) return TTT_ERR_SHAPE;
   if ((st = check_row(ldq, (long long)G * N, L, dtype)) != TTT_OK) return st;
   if ((st = check_row(ldk, (long long)G * N, L, dtype)) != TTT_OK) return st;
