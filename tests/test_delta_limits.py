@@ -31,3 +31,18 @@ def test_chunks(lib, dtype, B, H):
         assert _call(lib.ttt_delta_fwd, DELTA, **kw, L=L, v=None) == (E_NULL if trains else E_SHAPE), L
         bwd = {k: v for k, v in kw.items() if k != "ldv"}
         assert _call(lib.ttt_delta_bwd, DELTA_BWD, **bwd, L=L, lddo=32 * H, dq=None) == (E_NULL if trains else E_SHAPE), L
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_sums_of_the_heads_that_share(lib, dtype):
+    """Their launch has a thread for four values of dq and of dk: B L G N / 2 of them, below 2^32, where heads share
+    q and k; each has its own in the call that has as many groups as heads."""
+    for G in (8, 4):
+        H, most = 2 * G, ((1 << 32) - 256) * 2 // 128 // G
+        kw = dict(B=1, H=H, G=G, P=32, N=128, dtype=dtype, ldq=128 * G, ldk=128 * G, ldv=32 * H, ldg=H, ldb=H, bd=F32, v=None)
+        for n, ok in ((most, True), (most + 1, False)):
+            assert (lib.ttt_delta_bwd_workspace_bytes(1, n, H, 32, G, 128, dtype) > 0) == ok, (G, n)
+            assert _call(lib.ttt_delta_fwd, DELTA, **kw, L=n) == (E_NULL if ok else E_SHAPE), (G, n)
+        assert _call(lib.ttt_delta_fwd, DELTA, **kw, L=most + 1, saved=None) == E_NULL
+    n = ((1 << 32) - 256) * 2 // 128 // 16 + 1
+    assert lib.ttt_delta_bwd_workspace_bytes(1, n, 16, 32, 16, 128, dtype) > 0

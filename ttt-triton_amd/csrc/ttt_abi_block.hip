@@ -65,16 +65,18 @@ DeltaPlan delta_plan(int B, int L, int H, int P, int G, int N, int dtype) {
   return s;
 }
 // (forwards, prep: 256 threads a chunk and head; walk: eight for a column, a feature or one of the identity's, and
-// segment; join: up to 32 a feature; where a backward follows its gradients: 512 a chunk and head)
-bool delta_grid_ok(const DeltaPlan& s, int B, int H, int P, bool train) {
+// segment; join: up to 32 a feature; where a backward follows its gradients: 512 a chunk and head, and the sums of
+// the heads that share q and k: one for four values of both)
+bool delta_grid_ok(const DeltaPlan& s, int B, int L, int H, int P, int G, int N, bool train) {
   const long long heads = (long long)B * H;
-  return heads * (P + 128) <= kMaxThreads / 8 / s.S && heads * P <= kMaxThreads / 32 &&
-         heads <= kMaxThreads / (train ? 512 : 256) / s.NC;
+  if (heads * (P + 128) > kMaxThreads / 8 / s.S || heads * P > kMaxThreads / 32 || heads > kMaxThreads / (train ? 512 : 256) / s.NC)
+    return false;
+  return !train || s.share == 1 || (long long)B * L * G <= (kMaxThreads - 255) * 2 / N;
 }
 bool delta_plan_ok(int B, int L, int H, int P, int G, int N, int dtype, bool train, DeltaPlan& s) {
   if (check_delta(B, L, H, P, G, N, dtype, dtype, dtype) != TTT_OK) return false;
   s = delta_plan(B, L, H, P, G, N, dtype);
-  return delta_grid_ok(s, B, H, P, train);
+  return delta_grid_ok(s, B, L, H, P, G, N, train);
 }
 
 // ---- norms around a block
@@ -388,7 +390,7 @@ int ttt_delta_fwd(const void* q, long long ldq, const void* k, long long ldk, co
   int st = check_delta(B, L, H, P, G, N, dtype, g_dtype, beta_dtype);
   if (st != TTT_OK) return st;
   const DeltaPlan s = delta_plan(B, L, H, P, G, N, dtype);
-  if (!delta_grid_ok(s, B, H, P, saved != nullptr)) return TTT_ERR_SHAPE;
+  if (!delta_grid_ok(s, B, L, H, P, G, N, saved != nullptr)) return TTT_ERR_SHAPE;
   if (ldg < H || ldbeta < H) return TTT_ERR_SHAPE;
   if ((st = check_row(ldq, (long long)G * N, L, dtype)) != TTT_OK) return st;
   if ((st = check_row(ldk, (long long)G * N, L, dtype)) != TTT_OK) return st;
@@ -456,7 +458,7 @@ int ttt_delta_bwd(const void* q, long long ldq, const void* k, long long ldk, co
   int st = check_delta(B, L, H, P, G, N, dtype, g_dtype, beta_dtype);
   if (st != TTT_OK) return st;
   const DeltaPlan s = delta_plan(B, L, H, P, G, N, dtype);
-  if (!delta_grid_ok(s, B, H, P, true)) return TTT_ERR_SHAPE;
+  if (!delta_grid_ok(s, B, L, H, P, G, N, true)) return TTT_ERR_SHAPE;
   if (ldg < H || ldbeta < H) return TTT_ERR_SHAPE;
   if ((st = check_row(ldq, (long long)G * N, L, dtype)) != TTT_OK) return st;
   if ((st = check_row(ldk, (long long)G * N, L, dtype)) != TTT_OK) return st;
