@@ -49,13 +49,13 @@ import torch
 import torch.nn.functional as Fn
 from torch import nn
 
-from .delta import gated_delta, gated_delta_step
+from .delta import MAX_HEAD_DIM, gated_delta, gated_delta_step
 from .ffn import gated_linear
 from .layer_io import POST_NORM_EPS, RECON_EPS, PostNormFunction, ProducerFunction, rope_table
 from .linear import TTTLinearFunction
 from .memo import mlp_memo_combine
 from .mlp import LN_EPS, TTTMLPFunction
-from .norm import block_norm, layer_norm
+from .norm import MAX_BLOCK_WIDTH, block_norm, layer_norm
 from .ssm import CONV_WIDTHS, MAX_STATE, causal_conv, causal_conv_step, selective_scan, selective_scan_step
 
 MAX_MODEL_DIM = 1024  # H * F, the widest row the producer / post-norm kernels take
@@ -155,9 +155,14 @@ class ModelConfig:
         # take head dims 32 and 64 and model widths up to 1024; the inner loop
         # takes mini-batches of 16 to 64 tokens in steps of 16
         F = self.model_dim // self.num_heads
-        if F not in (32, 64):
+        if self.ssm_layer == "gated_delta":  # which has operators of its own
+            if F % 32 or F > MAX_HEAD_DIM:
+                raise ValueError(f"head dim model_dim/num_heads = {F}: a multiple of 32 up to {MAX_HEAD_DIM} is needed")
+            if self.model_dim > MAX_BLOCK_WIDTH:
+                raise ValueError(f"model_dim {self.model_dim} > {MAX_BLOCK_WIDTH}, the widest rows of block_norm")
+        elif F not in (32, 64):
             raise ValueError(f"head dim model_dim/num_heads = {F}: this build's layer kernels take 32 or 64")
-        if self.model_dim > MAX_MODEL_DIM:
+        elif self.model_dim > MAX_MODEL_DIM:
             raise ValueError(f"model_dim {self.model_dim} > {MAX_MODEL_DIM}, the widest the layer kernels take")
         if mini_batches and (self.mini_batch_size % 16 or not 16 <= self.mini_batch_size <= 64):
             raise ValueError(f"mini_batch_size {self.mini_batch_size}: a multiple of 16 from 16 to 64 is needed")
