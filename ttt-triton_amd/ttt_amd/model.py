@@ -550,7 +550,15 @@ class GatedDeltaStack(nn.Module):
     def _join(self, i: int, y: torch.Tensor, r: torch.Tensor):
         return block_norm(y, self.out_norms[i], r, scale=self.scales[i], next_weight=self.next_norms[i], eps=POST_NORM_EPS)
 
+    def _of(self, caches):
+        """The caches, one a block, before anything is moved on"""
+        blocks = self.config.num_layers
+        if not (isinstance(caches, (list, tuple)) and len(caches) == blocks and all(isinstance(c, SSMCache) for c in caches)):
+            raise ValueError(f"a stack of {blocks} blocks goes on from a list of {blocks} caches, as prompt returns it")
+        return caches
+
     def _run(self, x: torch.Tensor, caches, keep: bool, last_only: bool):
+        caches = None if caches is None else self._of(caches)
         r, y = x.float(), block_norm(x, self.first_norm, eps=POST_NORM_EPS)
         last = max(i for i, part in enumerate(self.parts) if isinstance(part, GatedDelta))
         kept = []
@@ -577,8 +585,8 @@ class GatedDeltaStack(nn.Module):
     @torch.no_grad()
     def step(self, x: torch.Tensor, cache):
         """One token x [B, D] of every sequence: its output [B, D], the caches moved on in place."""
+        caches = iter(self._of(cache))
         r, y = x.float(), block_norm(x, self.first_norm, eps=POST_NORM_EPS)
-        caches = iter(cache)
         for i, part in enumerate(self.parts):
             r, y = self._join(i, part.step(y, next(caches)) if isinstance(part, GatedDelta) else part(y), r)
         return y
