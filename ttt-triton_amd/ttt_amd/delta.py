@@ -167,7 +167,7 @@ def gated_delta(q, k, v, g, beta, initial_state=None, scale=None, l2_norm: bool 
     if v.dim() == 4 and v.numel() == 0:
         dev, (B, _, H, P, _, N), *_ = _delta_args(q, k, v, g, beta, initial_state, scale, 2)
         _delta_state(initial_state, (B, H, P, N))
-        first = torch.zeros(B, H, P, N, device=dev) if initial_state is None else initial_state.float().clone()
+        first = torch.zeros(B, H, P, N, device=dev) if initial_state is None else initial_state.float().clone(memory_format=torch.contiguous_format)
         o = _empty(v, q, k, g, beta)
         return (o, first) if return_final_state else o
     if _wants_grad(q, k, v, g, beta, initial_state):
