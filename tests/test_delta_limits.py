@@ -2,7 +2,9 @@
 return their status, and the size functions 0, before any launch)."""
 
 import pytest
+import torch
 
+from tests._stubs import launches  # noqa: F401
 from tests.test_block_refusals import BF16, DELTA, DELTA_BWD, E_NULL, E_SHAPE, F32, _call
 
 CHUNK = {BF16: 64, F32: 32}
@@ -46,3 +48,16 @@ def test_sums_of_the_heads_that_share(lib, dtype):
         assert _call(lib.ttt_delta_fwd, DELTA, **kw, L=most + 1, saved=None) == E_NULL
     n = ((1 << 32) - 256) * 2 // 128 // 16 + 1
     assert lib.ttt_delta_bwd_workspace_bytes(1, n, 16, 32, 16, 128, dtype) > 0
+
+
+@pytest.mark.parametrize("train", [True, False])
+def test_refused_before_a_launch(launches, monkeypatch, train):  # noqa: F811
+    """Where a size function gives 0, the call raises: a forward that trains does not go on without `saved`."""
+    from ttt_amd import delta
+    monkeypatch.setattr(delta, "check_device", lambda *ts: ts[0].device)
+    name = f"ttt_delta_{'saved' if train else 'workspace'}_bytes"
+    monkeypatch.setattr(delta, "_bytes", lambda n, *a: 0 if n == name else 1024)
+    z = lambda *s: torch.zeros(s, requires_grad=train)  # noqa: E731
+    with pytest.raises(ValueError, match="too many"):
+        delta.gated_delta(z(1, 3, 1, 16), z(1, 3, 1, 16), z(1, 3, 2, 32), z(1, 3, 2), z(1, 3, 2))
+    assert not launches.calls

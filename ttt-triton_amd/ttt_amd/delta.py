@@ -98,6 +98,8 @@ def _delta_forward(q, k, v, g, beta, h0, scale, unit, want_last, train):
     lib = _lib.load()
     nsv = _bytes("ttt_delta_saved_bytes", B, L, H, P, N, code) if train else 0
     nws = _bytes("ttt_delta_workspace_bytes", B, L, H, P, N, code)
+    if not nws or train and not nsv:  # (0 for what a launch has no threads for)
+        raise ValueError(f"gated_delta{' with gradients' if nws else ''} has too many tokens and heads: {list(v.shape)}")
     saved = torch.empty(nsv, device=dev, dtype=torch.uint8) if train else None
     ws = torch.empty(nws, device=dev, dtype=torch.uint8)
     with on_device(dev):
@@ -158,7 +160,7 @@ def gated_delta(q, k, v, g, beta, initial_state=None, scale=None, l2_norm: bool 
     """The gated delta rule over v [B,L,H,P] with keys and queries k and q [B,L,G,N],
     log-decays g [B,L,H] (<= 0; -inf forgets the state) and weights beta [B,L,H], from
     zeros or initial_state [B,H,P,N] fp32.  l2_norm: q and k are taken at unit length,
-    x / sqrt(|x|^2 + 1e-6) (without it they are used as they are: the state grows without
+    x / sqrt(|x|^2 + 1e-6), |x|^2 in fp32, for |x| below 1e19 (without it they are used as they are: the state grows without
     bound where beta |k|^2 > 2).  scale: N^-1/2 where none is given.  P is a multiple of 32
     up to 256, N of 16 up to 128.  Returns o [B,L,H,P] in v's dtype, and with
     return_final_state the last state [B,H,P,N] fp32 as well, which gated_delta_step and a
