@@ -511,7 +511,8 @@ int ttt_delta_fwd(const void* q, long long ldq, const void* k, long long ldk, co
 
 /* Its gradients from dO [B*L][lddo] and dh_last (NULL: zeros), given what ttt_delta_fwd
  * saved for the same inputs, and its workspace as it left it (`kept`): dq, dk [B][L][G][N], dv [B][L][H][P], dg, dbeta [B][L][H] in the
- * types of g and beta, dh0 [B][H][P][N] (or NULL). */
+ * types of g and beta, dh0 [B][H][P][N] (or NULL).  (A size function gives 0 for sizes that the calls refuse; a
+ * forward without `saved` takes twice the chunks and heads of one that a backward follows.) */
 size_t ttt_delta_bwd_workspace_bytes(int B, int L, int H, int P, int G, int N, int dtype);
 int ttt_delta_bwd(const void* q, long long ldq, const void* k, long long ldk, const void* g, long long ldg,
                   const void* beta, long long ldbeta, const void* dO, long long lddo, const float* dh_last,
@@ -560,7 +561,8 @@ int ttt_ffn_fwd(const void* x, long long ldx, const void* wg, const void* wu, co
                 int D, int F, int activation, int dtype, void* y, void* workspace, size_t workspace_bytes,
                 void* stream);
 
-/* Its gradients from dy [R][lddy], any alignment: dx [R][D] (or NULL), dwg and dwu [F][D] (both
+/* Its gradients from dy [R][lddy], any alignment (in 16 bits formed of da and db rounded to the type; in
+ * fp16 with those past its largest number kept apart): dx [R][D] (or NULL), dwg and dwu [F][D] (both
  * or neither), dbg and dbu [F] (each may be NULL).  Alignment as above, whatever R is. */
 size_t ttt_ffn_bwd_workspace_bytes(int R, int D, int F, int dtype);
 int ttt_ffn_bwd(const void* x, long long ldx, const void* wg, const void* wu, const void* bg, const void* bu,

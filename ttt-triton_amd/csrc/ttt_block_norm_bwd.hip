@@ -14,7 +14,9 @@ namespace {
 // Waves to a SIMD that the registers are cut to: three where a lane has up to 12 values and no
 // residual (32,768 rows of 12 heads of 64 in bf16 with a gate: 44 us), else two (32,768 rows of 768 in
 // bf16 with an fp32 residual: 95 us; 115 with three, which spill 18 registers); one where 16 values, a gate
-// and a residual would spill a hundred
+// and a residual would spill a hundred, but for rows of 512 lanes, whose eight waves are two to a SIMD
+// whatever is asked for: above 6,144 columns with a gate and a residual 36 to 86 registers spill (4,096 rows
+// of 8,192 in bf16 with an fp32 residual, forward and backward: 333 us, 195 without the gate; of 6,144 181 and 170)
 template <typename T, typename TR, bool GATE, int LANES, int V, int NCH>
 constexpr int kWaves = V * NCH <= 12 && LANES < 512 && __is_same(TR, NoResidual) ? 3
                        : V * NCH == 16 && GATE && !__is_same(TR, NoResidual) && LANES < 512                   ? 1

@@ -10,7 +10,8 @@
 // turn.  An operand whose contracted values are neighbours in memory is read 16 bytes a lane;
 // one whose free values are (the weights for dx, both operands of dW) by the transposing
 // read, so that nothing is transposed in memory.  The 16-byte pieces of a row lie in LDS
-// permuted by the row's number, for reads without bank conflicts; pieces outside a matrix read 0.
+// permuted by the row's number, so that reads meet in no bank, but for the first operand's transposing
+// ones (dx's weights, dW's x), which take two turns; pieces outside a matrix read 0.
 // The gate's and the other projection's columns of a tile meet in one wave, which forms y, or
 // da and db, from its accumulators.
 //
@@ -25,15 +26,17 @@
 // Blocks with one are marked; one more launch puts zeros in the plane's other blocks, or finds no mark.
 //
 // 32,768 rows, 768 by 2,048, bf16: y 235 us (877 TFLOP/s), da and db 269, dx 262 in one round of large
-// tiles and one of small, dW 247 and a join of 12 (294 and 257 before that and before the reads' order).
+// tiles and one of small, dW 241 and a join of 12 (294 and 257 before that and before the reads' order);
+// in fp16 y 217, da and db 264, dx 254, dW 232 and 12.
 // A step of a large tile is 64 KB to LDS by 1 KB loads, 192 KB of reads from it and 2,048 clocks of
 // matrix instructions on each SIMD; it takes about 3,600.  Without the loads to LDS the products
 // alone take 86% of the time, the loads alone 70%: they overlap in part, with a barrier a step.
 // Steps of 32 with three on their way wait for less and meet twice as many barriers: 15 to 20% slower.
 //
-// Few rows (up to 64, a token of each sequence): the weights are read once, by as many
-// workgroups as have 16 columns, the contraction shared out over eight waves; nothing goes
-// through LDS but the waves' sums.  (64 rows, 768 by 2,048: 6.1 us, 6.7 MB: a launch and its latency.)
+// Few rows (up to 64, a token of each sequence): a workgroup has 16 columns and up to 32 rows, the
+// contraction shared out over eight waves; nothing goes through LDS but the waves' sums.  The weights
+// are read once for 32 rows, twice for 33 to 64, the second time from a cache.  (768 by 2,048, 6.7 MB,
+// in a graph: 4.4 us for 16 rows, 5.2 for 32, 5.3 for 64: a launch and its latency.)
 #include <math.h>
 
 #include <algorithm>
@@ -499,7 +502,7 @@ template <typename T> __global__ __launch_bounds__(256) void ffn_planes_kernel(c
   }
 }
 
-// Few rows: a workgroup has 16 columns of both projections and up to 64 rows, a wave every
+// Few rows: a workgroup has 16 columns of both projections and 16 or 32 rows, a wave every
 // eighth 32 contracted values
 constexpr int kFewWaves = 8;
 template <typename T> struct FewOp { typedef Op<3> type; };
