@@ -258,13 +258,14 @@ __global__ __launch_bounds__(64 * WN * WM) void ffn_kernel(FfnParams p) {
       const FfnMatrix& wt = ss == 0 ? p.wg : p.wu;
       send<LN, Side::First, BN, NW>(static_cast<const char*>(wt.p) + pa * wt.plane + (long long)k * wt.ld + n0 * 2, wt.ld, p.F - k,
                        (p.Dp - n0) / 8, to, w);
-      send<LM, Side::Second, BM, NW>(static_cast<const char*>(p.grad.p) + (WIDE ? beside : pb * p.grad.plane) + (long long)m0 * p.grad.ld +
-                           ((long long)ss * p.Fp + k) * 2,
+      send<LM, Side::Second, BM, NW>(static_cast<const char*>(p.grad.p) + (WIDE ? beside : pb * p.grad.plane) +
+                           (long long)m0 * p.grad.ld + ((long long)ss * p.Fp + k) * 2,
                        p.grad.ld, M - m0, left / 8, to + Panel<LN, Side::First, BN>::BYTES, w);
     } else {
       send<LN, Side::First, BN, NW>(static_cast<const char*>(p.x.p) + pa * p.x.plane + (long long)k * p.x.ld + n0 * 2, p.x.ld, left,
                        (p.Dp - n0) / 8, to, w);
-      send<LM, Side::Second, BM, NW>(static_cast<const char*>(p.grad.p) + (WIDE ? beside : pb * p.grad.plane) + (long long)k * p.grad.ld + m0 * 2, p.grad.ld,
+      send<LM, Side::Second, BM, NW>(static_cast<const char*>(p.grad.p) + (WIDE ? beside : pb * p.grad.plane) +
+                           (long long)k * p.grad.ld + m0 * 2, p.grad.ld,
                        left, (M - m0) / 8, to + Panel<LN, Side::First, BN>::BYTES, w);
     }
     if (++sk == ksteps) {

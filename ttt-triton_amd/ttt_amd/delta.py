@@ -32,7 +32,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._common import check_device, dtype_code, f32c, on_device
-from .ssm import (_as, _bytes, _empty, _near_rows, _no_grad_through, _opt, _rows, _sizes, _state_in_place, _stream,
+from .ssm import (_as, _bytes, _empty, _fresh, _near_rows, _no_grad_through, _opt, _rows, _sizes, _state_in_place, _stream,
                   _wants_grad, _whole)
 
 MAX_HEAD_DIM = 256  # P, a multiple of 32
@@ -169,7 +169,7 @@ def gated_delta(q, k, v, g, beta, initial_state=None, scale=None, l2_norm: bool 
     if v.dim() == 4 and v.numel() == 0:
         dev, (B, _, H, P, _, N), *_ = _delta_args(q, k, v, g, beta, initial_state, scale, 2)
         _delta_state(initial_state, (B, H, P, N))
-        first = torch.zeros(B, H, P, N, device=dev) if initial_state is None else initial_state.float().clone(memory_format=torch.contiguous_format)
+        first = torch.zeros(B, H, P, N, device=dev) if initial_state is None else _fresh(initial_state.float())
         o = _empty(v, q, k, g, beta)
         return (o, first) if return_final_state else o
     if _wants_grad(q, k, v, g, beta, initial_state):

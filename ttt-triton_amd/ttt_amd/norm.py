@@ -250,8 +250,8 @@ def block_norm(x, weight=None, residual=None, gate=None, scale=None, next_weight
     a residual, (r, y) with y = r / sqrt(mean r^2 + eps) * next_weight, what the next block
     reads.  gate has x's shape and dtype, the residual x's shape in x's dtype or fp32, which r
     has as well (x's without one); weight, scale and next_weight are [D].  y is normed from r
-    before it is rounded; squares are summed in fp32 (rows of a length below 1e19).  x, gate and residual may be columns of a wider matrix, by heads
-    too ([.., H, D])."""
+    before it is rounded; squares are summed in fp32 (rows of a length below 1e19).  x, gate
+    and residual may be columns of a wider matrix, by heads too ([.., H, D])."""
     if x.dim() and x.numel() == 0 and x.shape[-1]:
         _block_args(x, weight, residual, gate, scale, next_weight, eps)
         r = _empty(x if residual is None else residual, x, weight, residual, gate, scale, next_weight)

@@ -105,7 +105,12 @@ def _whole(t, align: int = 1):
     """t as one contiguous block on `align` bytes"""
     if t is None or t.is_contiguous() and t.data_ptr() % align == 0:
         return t
-    return t.detach().clone(memory_format=torch.contiguous_format)
+    return _fresh(t.detach())
+
+
+def _fresh(t):
+    """A contiguous copy, whatever t's strides"""
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _stream(dev: torch.device) -> int:
@@ -268,7 +273,7 @@ def causal_conv(x, weight, bias=None, initial_state=None, activation=None, retur
         _, _, C, W, _, _ = _conv_args(x, weight, bias, initial_state, activation, 2)
         shape = (x.shape[0], W - 1, C)
         _conv_state(initial_state, shape, x.dtype)
-        first = x.new_zeros(shape) if initial_state is None else initial_state.to(x.dtype).clone(memory_format=torch.contiguous_format)
+        first = x.new_zeros(shape) if initial_state is None else _fresh(initial_state.to(x.dtype))
         y = _empty(x, weight, bias)
         return (y, first) if return_final_state else y
     if _wants_grad(x, weight, bias, initial_state):
@@ -435,7 +440,7 @@ def selective_scan(x, dt, A, Bm, Cm, D=None, dt_bias=None, initial_state=None, d
     if x.dim() == 4 and x.numel() == 0:
         dev, (B, _, H, P, _, N), *_ = _scan_args(x, dt, A, Bm, Cm, D, dt_bias, initial_state, 2)
         _scan_state(initial_state, (B, H, P, N))
-        first = torch.zeros(B, H, P, N, device=dev) if initial_state is None else initial_state.float().clone(memory_format=torch.contiguous_format)
+        first = torch.zeros(B, H, P, N, device=dev) if initial_state is None else _fresh(initial_state.float())
         y = _empty(x, dt, A, Bm, Cm, D, dt_bias)
         return (y, first) if return_final_state else y
     if _wants_grad(x, dt, A, Bm, Cm, D, dt_bias, initial_state):
